@@ -661,6 +661,134 @@ int tmnn_debug_philox_uniform(tmnn_context *ctx, uint64_t seed,
                               uint32_t counter_base, uint32_t count, float low,
                               float high, float *out);
 
+/* ---- class logits --------------------------------------------------------------- */
+/* Operators over rows of class logits: what a field (or any model) with class
+ * outputs needs beside the losses above, for callers with a loss of their own
+ * (tmnn_forward_for_training, tmnn_backward_accumulate) and for reading its
+ * answers. No counterpart in the reference.
+ *
+ * logits [rows][classes], unit stride within a row and row_stride elements
+ * (>= classes) from row to row, at any alignment of an element. All sums are
+ * held in fp32. -inf masks a class. Class ids are int32 or int64.
+ *
+ * Rows that leave nothing (every class -inf): log-probabilities -inf, entropy 0,
+ * rank -1, alternatives -1, loss 0, gradient 0. Rows with a NaN or +inf: NaN
+ * (rank and alternatives -1).
+ *
+ * A tmnn_logits holds the workspace of its calls (few rows are split over
+ * several blocks); nothing is allocated by the *_device calls, which only
+ * enqueue on `stream` (a hipStream_t of the context's device, NULL being the null
+ * stream, or TMNN_STREAM_CONTEXT). Calls through one handle on several streams
+ * are ordered where they share the workspace; a handle of its own lets a stream
+ * run freely, and is needed for a stream that is being captured into a graph. The
+ * host-pointer calls copy in and out, on the context's stream, and return when the
+ * results are there. */
+#define TMNN_STREAM_CONTEXT ((void *)(intptr_t)-1) /* the context's own stream */
+#define TMNN_DTYPE_F32 0
+#define TMNN_DTYPE_F16 1
+#define TMNN_DTYPE_BF16 2
+#define TMNN_INDEX_I32 0
+#define TMNN_INDEX_I64 1
+/* Largest `classes`, `top_k` and `teacher_k`. */
+#define TMNN_LOGITS_MAX_CLASSES (1 << 24)
+#define TMNN_LOGITS_MAX_TOP 128
+#define TMNN_LOGITS_MAX_TEACHER 256
+
+typedef struct tmnn_logits tmnn_logits;
+int tmnn_logits_create(tmnn_context *ctx, tmnn_logits **out);
+int tmnn_logits_destroy(tmnn_logits *h);
+
+/* Of each row, p = softmax(logits / temperature):
+ *   logprob[row]     ln p of class tokens[row]; 0 for a negative token (a row
+ *                    without one), NaN for a token >= classes
+ *   rank[row]        classes that come before it (larger logit, or equal and of a
+ *                    lower index); -1 without a token
+ *   entropy[row]     -sum p ln p
+ *   top_ids[row][j], top_logprobs[row][j]
+ *                    the top_k best classes in that order and their ln p; masked
+ *                    classes are none (-1, -inf)
+ *   stats[row][2]    the largest logit m, sum exp((logits - m) / temperature)
+ * Null outputs are left out (top_ids and top_logprobs both or neither). The
+ * backward call reads entropy (where d_entropy is not null), stats and top_ids
+ * (where d_top_logprobs is not null) and writes d_logits, the gradient of
+ *   sum_row d_logprob logprob + d_entropy entropy + sum_j d_top_logprobs[j] top_logprobs[j]
+ * (null: 0). Entries of top_ids outside the classes are not used, and a class
+ * that is listed twice counts by its first entry. Rows whose upstream gradients are
+ * all 0 get 0. d_logits has the type of the logits and may be the logits. */
+typedef struct tmnn_token_logprobs_args {
+  uint32_t struct_size;       /* sizeof(tmnn_token_logprobs_args) */
+  int32_t dtype;              /* TMNN_DTYPE_* of logits and d_logits */
+  int32_t index_dtype;        /* TMNN_INDEX_* of tokens */
+  int32_t top_k;              /* 0..TMNN_LOGITS_MAX_TOP */
+  int64_t rows;
+  int64_t classes;
+  int64_t row_stride;
+  int64_t d_row_stride;       /* of d_logits */
+  const void *logits;
+  const void *tokens;         /* [rows], nullable: no row has a token */
+  float *logprob;             /* [rows] */
+  float *entropy;             /* [rows] */
+  int32_t *rank;              /* [rows] */
+  float *stats;               /* [rows][2] */
+  int32_t *top_ids;           /* [rows][top_k] */
+  float *top_logprobs;        /* [rows][top_k] */
+  const float *d_logprob;     /* [rows] */
+  const float *d_entropy;     /* [rows] */
+  const float *d_top_logprobs; /* [rows][top_k] */
+  void *d_logits;             /* [rows][classes] */
+  float temperature;          /* > 0 */
+  int32_t reserved;           /* 0 */
+} tmnn_token_logprobs_args;
+
+int tmnn_token_logprobs(tmnn_logits *h, const tmnn_token_logprobs_args *args);
+int tmnn_token_logprobs_device(tmnn_logits *h, const tmnn_token_logprobs_args *args, void *stream);
+int tmnn_token_logprobs_backward(tmnn_logits *h, const tmnn_token_logprobs_args *args);
+int tmnn_token_logprobs_backward_device(tmnn_logits *h, const tmnn_token_logprobs_args *args,
+                                        void *stream);
+
+/* What the teacher's values are. LOGITS: its logits; its distribution over the
+ * listed classes is their softmax at the temperature. LOGPROBS: natural
+ * logarithms of its probabilities (at the temperature already); the classes that
+ * are not listed form one class of mass 1 - sum exp(value) (dropped where no class is
+ * left). */
+#define TMNN_TEACHER_LOGITS 0
+#define TMNN_TEACHER_LOGPROBS 1
+
+/* Distillation from a teacher's top values, q against p = softmax(logits / T):
+ *   loss[row] = row_weights[row] T^2 KL(q || p)
+ *   d_logits  = the gradient of sum_row loss[row]
+ * in one call (d_logits null: the loss alone). stats[row][4] is what the backward
+ * call needs: it writes d_logits = d_loss[row] T^2 dKL/dlogits, with d_loss passed as
+ * row_weights (stats of a call without weights, or with weights that are not 0).
+ * Negative teacher_ids mark unused entries; an id that is listed twice counts by its
+ * first entry; an id >= classes or a NaN value makes its row NaN. Rows of weight 0
+ * are not read: loss and gradient 0. A row without entries: loss and gradient 0.
+ * d_logits has the type of the logits and may be the logits. */
+typedef struct tmnn_distill_args {
+  uint32_t struct_size;       /* sizeof(tmnn_distill_args) */
+  int32_t dtype;              /* TMNN_DTYPE_* of logits and d_logits */
+  int32_t index_dtype;        /* TMNN_INDEX_* of teacher_ids */
+  int32_t teacher_kind;       /* TMNN_TEACHER_* */
+  int64_t rows;
+  int64_t classes;
+  int64_t row_stride;
+  int64_t d_row_stride;       /* of d_logits */
+  const void *logits;
+  const void *teacher_ids;    /* [rows][teacher_k] */
+  const float *teacher;       /* [rows][teacher_k] */
+  const float *row_weights;   /* [rows], nullable: 1 (backward: d_loss, not null) */
+  float *loss;                /* [rows], nullable */
+  float *stats;               /* [rows][4], 16-byte aligned, nullable (backward: read) */
+  void *d_logits;             /* [rows][classes], nullable */
+  int32_t teacher_k;          /* 1..TMNN_LOGITS_MAX_TEACHER */
+  float temperature;          /* T > 0 */
+} tmnn_distill_args;
+
+int tmnn_distill(tmnn_logits *h, const tmnn_distill_args *args);
+int tmnn_distill_device(tmnn_logits *h, const tmnn_distill_args *args, void *stream);
+int tmnn_distill_backward(tmnn_logits *h, const tmnn_distill_args *args);
+int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

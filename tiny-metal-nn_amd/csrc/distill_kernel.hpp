@@ -1,0 +1,550 @@
+// distill_kernel.hpp -- distillation of rows of logits from a teacher's listed
+// values: loss and gradient.
+//
+//   loss = w T^2 [ sum_j q_j (ln q_j - ln p_j) + q_r (ln q_r - ln p_r) ]
+//   d z_v = w T [ Q p_v - q_v [v listed] - q_r p_v / p_r [v not listed] ],  Q = sum_j q_j + q_r
+//
+// with p = softmax(z / T). Kind 0 (teacher logits): q = softmax(t / T) over the
+// listed classes, q_r = 0. Kind 1 (teacher log-probabilities): q = exp(t), and
+// the classes that are not listed form one class of mass q_r = 1 - sum q.
+//
+// Kind 1 sums up the classes that are not listed by themselves, relative to their
+// own maximum m_d, and lets the listed ones join: ln p_r and p_v / p_r keep their
+// precision however little the rest weighs. Either way the gradient of the
+// classes that are not listed is one exponential,
+//   w T a_d 2^(c (z_v - m_d)),
+// and that of listed class j is w T (a_a 2^(c (z_j - m_a)) - q_j); (m_d, a_d, m_a,
+// a_a) are the row's statistics. m_a = -inf marks a row whose classes are all
+// masked: loss and gradient 0.
+#pragma once
+
+#include "logprob_kernel.hpp"
+
+namespace tmnn_hip {
+
+constexpr int kMaxTeacher = 256;
+constexpr int kMaxPartLen = 1 << 17;  // classes of a block: its bits of listed classes in LDS
+
+struct DistillArgs {
+  const void *logits;
+  int64_t row_stride;
+  const void *ids;
+  const float *teacher;
+  const float *weights;  // null: 1; backward: the loss's gradient
+  int32_t wide_index, kind;
+  int32_t rows, classes, k;
+  int32_t parts, part_len;
+  float c, t, inv_t;  // log2(e) / T, T, 1 / T
+  float *loss;
+  float *stats;  // [rows][4]
+  void *d_logits;
+  int64_t d_row_stride;
+  float2 *part_sum;  // [rows][parts]: m, r
+  float *list_z;     // [rows][k]: logits of the listed classes
+};
+
+// What the loss and the gradient need of a row beyond its listed classes.
+struct DistillRow {
+  float m_d, a_d, m_a, a_a;
+};
+
+// A listed class's ln q - ln p, the differences of its logits in 64 bits: the loss is
+// small against both.
+__device__ __forceinline__ float log_ratio(const DistillArgs &a, float t, float top, float log_z,
+                                           float z, float m, float log_s) {
+  const double inv_t = 1.0 / static_cast<double>(a.t);
+  const double lq = a.kind == 0 ? (static_cast<double>(t) - top) * inv_t - log_z : t;
+  return static_cast<float>(lq - (static_cast<double>(z) - m) * inv_t + log_s);
+}
+// q of a teacher value: relative to `top` over 1 / inv_z (kind 0), or itself.
+__device__ __forceinline__ float teacher_mass(const DistillArgs &a, float t, float top, float inv_z) {
+  return a.kind == 0 ? exp2_raw((t - top) * a.c) * inv_z : expf(t);
+}
+
+// sum q over G lanes' listed classes, each lane's by `each(f)`: (sum q, 1 - sum q).
+// Kind 1 takes the mass that the teacher left out from 64-bit sums: 1 - sum q in 32 bits
+// is off by 2^-24 of the whole, which is all of a small rest.
+struct TeacherMass {
+  float all, left;
+};
+template <int G, class Each>
+__device__ __forceinline__ TeacherMass teacher_total(const DistillArgs &a, float top, Each each) {
+  TeacherMass m{0.0f, 0.0f};
+  if (a.kind == 0) {
+    each([&](float t) { m.all += exp2_raw((t - top) * a.c); });
+    m.all = lanes_sum<G>(m.all);
+    return m;
+  }
+  double total = 0.0;
+  each([&](float t) { total += exp(static_cast<double>(t)); });
+  total = lanes_sum<G>(total);
+  m.all = static_cast<float>(total);
+  m.left = fmaxf(static_cast<float>(1.0 - total), 0.0f);
+  return m;
+}
+
+// The row's statistics and the part of its loss that the listed classes do not
+// bring: dense = settled sums of all classes (kind 0) or of the unlisted ones
+// (kind 1); all = of all classes; mass = sum q, left = 1 - mass (kind 1).
+__device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const Soft &dense,
+                                                  const Soft &all, float mass, float left,
+                                                  float *rest_loss) {
+  DistillRow r;
+  r.m_a = all.m;
+  *rest_loss = 0.0f;
+  if (a.kind == 0) {
+    r.a_a = mass / all.S;
+    r.m_d = r.m_a;
+    r.a_d = r.a_a;
+    return r;
+  }
+  const bool rest = dense.S != 0.0f;
+  const float qr = rest ? left : 0.0f;
+  const float q = mass + qr;
+  r.a_a = q / all.S;
+  r.m_d = rest ? dense.m : 0.0f;
+  // (no rest: 0, or the NaN of the listed classes)
+  r.a_d = rest ? exp2_raw((dense.m - all.m) * a.c) * r.a_a - qr / dense.S : 0.0f * r.a_a;
+  if (qr > 0.0f) {
+    const float log_pr = (dense.m - all.m) * a.inv_t + (log1pf(dense.r) - log1pf(all.r));
+    *rest_loss = qr * (logf(qr) - log_pr);
+  }
+  return r;
+}
+
+// ---- short rows -----------------------------------------------------------------
+
+// BACK: statistics are given and only the gradient is written.
+template <class T, int G, bool BACK>
+__global__ __launch_bounds__(kGroupThreads) void distill_group_kernel(DistillArgs a) {
+  constexpr int N = Row<T>::n;
+  __shared__ int owner[kGroupThreads * N];    // the first entry that lists a class
+  __shared__ float listed[kGroupThreads * N];  // its q
+  const float inf = __builtin_inff();
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kGroupThreads / G) + threadIdx.x / G;
+  const float w = row < a.rows ? (a.weights ? a.weights[row] : 1.0f) : 0.0f;
+  const bool live = row < a.rows && w != 0.0f;
+  const T *z = static_cast<const T *>(a.logits) + (live ? row : 0) * a.row_stride;
+  float v[N];
+  load_vec<T>(z, lane * N, live ? a.classes : 0, v);
+  int *own = owner + (threadIdx.x - lane) * N;
+  float *q_of = listed + (threadIdx.x - lane) * N;
+  const int k = live ? a.k : 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    own[lane * N + j] = 0x7fffffff;
+    q_of[lane * N + j] = 0.0f;
+  }
+  wave_fence();
+  float wrong = 0.0f;
+  for (int j = lane; j < k; j += G) {
+    const int64_t id = load_index(a.ids, row * a.k + j, a.wide_index);
+    if (id >= a.classes)
+      wrong = 1.0f;
+    else if (id >= 0)
+      atomicMin(&own[id], j);
+  }
+  wave_fence();
+  auto entries = [&](auto f) {
+    for (int j = lane; j < k; j += G) {
+      const int64_t id = load_index(a.ids, row * a.k + j, a.wide_index);
+      if (id >= 0 && id < a.classes && own[id] == j)
+        f(static_cast<int>(id), a.teacher[row * a.k + j]);
+    }
+  };
+  float top = -inf;
+  entries([&](int, float t) {
+    top = fmaxf(top, t);
+    if (t != t) wrong = 1.0f;
+  });
+  top = lanes_max<G>(top);
+  wrong = lanes_max<G>(wrong);
+  const TeacherMass tm =
+      teacher_total<G>(a, top, [&](auto f) { entries([&](int, float t) { f(t); }); });
+  const float total = tm.all;
+  // no mass at all: nothing is listed, or only values of -inf
+  const bool none = a.kind == 0 && top == -inf;
+  const float inv_z = a.kind == 0 ? 1.0f / total : 1.0f, log_z = logf(total);
+  float mass = a.kind != 0 ? total : none ? 0.0f : total * inv_z;
+  if (wrong != 0.0f) mass = __builtin_nanf("");
+
+  DistillRow r{};
+  if (!BACK) {
+    Soft all, dense;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      all.m = fmaxf(all.m, v[j]);
+      if (own[lane * N + j] == 0x7fffffff) dense.m = fmaxf(dense.m, v[j]);
+    }
+    all.m = lanes_max<G>(all.m);
+    dense.m = lanes_max<G>(dense.m);
+    const float shift = all.m == -inf ? 0.0f : all.m, rest = dense.m == -inf ? 0.0f : dense.m;
+    // classes of the largest logit, whose terms are 1, by number
+    int all_n = 0, dense_n = 0;
+    all.r = dense.r = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float e = exp2_raw((v[j] - shift) * a.c);
+      all.r += v[j] == all.m ? 0.0f : e;
+      all_n += v[j] == all.m;
+      if (a.kind != 0 && own[lane * N + j] == 0x7fffffff) {
+        const float f = exp2_raw((v[j] - rest) * a.c);
+        dense.r += v[j] == dense.m ? 0.0f : f;
+        dense_n += v[j] == dense.m;
+      }
+    }
+    all.r = lanes_sum<G>(all.r) + static_cast<float>((all.m == -inf ? 0 : lanes_isum<G>(all_n)) - 1);
+    if (all.m == inf) all.r = __builtin_nanf("");
+    all.S = 1.0f + all.r;
+    if (a.kind != 0) {
+      dense.r = lanes_sum<G>(dense.r) +
+                static_cast<float>((dense.m == -inf ? 0 : lanes_isum<G>(dense_n)) - 1);
+      if (dense.m == inf) dense.r = __builtin_nanf("");
+      dense.S = 1.0f + dense.r;
+    }
+    float loss = 0.0f, rest_loss;
+    r = distill_row(a, dense, all, mass, tm.left, &rest_loss);
+    const float log_s = log1pf(all.r);
+    entries([&](int id, float t) {
+      const float q = none ? 0.0f : teacher_mass(a, t, top, inv_z);
+      q_of[id] = q;
+      if (q != 0.0f)
+        loss += q * log_ratio(a, t, top, log_z, Row<T>::up(z[id]), all.m, log_s);
+    });
+    loss = lanes_sum<G>(loss) + rest_loss;
+    if (wrong != 0.0f) loss = __builtin_nanf("");
+    const bool empty = all.m == -inf && all.S == 0.0f;
+    if (empty) r.m_a = -inf;
+    if (lane == 0 && row < a.rows) {
+      if (a.loss) a.loss[row] = !live || empty ? 0.0f : loss * a.t * a.t * w;
+      if (a.stats)
+        reinterpret_cast<float4 *>(a.stats)[row] =
+            live ? make_float4(r.m_d, r.a_d, r.m_a, r.a_a) : make_float4(0.0f, 0.0f, -inf, 0.0f);
+    }
+    if (!a.d_logits) return;
+  } else {
+    if (live) {
+      const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
+      r = DistillRow{s.x, s.y, s.z, s.w};
+    }
+    entries([&](int id, float t) { q_of[id] = none ? 0.0f : teacher_mass(a, t, top, inv_z); });
+  }
+  wave_fence();
+  if (row >= a.rows) return;
+  const bool zero = !live || (r.m_a == -inf && r.a_a == r.a_a);
+  const float scale = w * a.t;
+  float d[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const bool in = own[lane * N + j] != 0x7fffffff;
+    const float e = exp2_raw((v[j] - (in ? r.m_a : r.m_d)) * a.c);
+    const float g = (in ? r.a_a : r.a_d) * e - q_of[lane * N + j];
+    d[j] = zero ? 0.0f : scale * g;
+  }
+  store_vec<T>(static_cast<T *>(a.d_logits) + row * a.d_row_stride, lane * N, a.classes, d);
+}
+
+// ---- long rows ---------------------------------------------------------------------
+
+struct ListLds {
+  int id[kMaxTeacher];
+  float z[kMaxTeacher], t[kMaxTeacher], q[kMaxTeacher];
+  float wrong;
+  DistillRow row;
+  float scale;
+};
+
+// The listed classes: -1 for unused entries and for classes listed before (the
+// first entry counts). An entry beyond the classes makes the row NaN.
+template <int NT>
+__device__ __forceinline__ int read_list(const DistillArgs &a, ListLds &l, int64_t row) {
+  static_assert(NT >= kMaxTeacher, "a thread for each listed class");
+  const int tid = threadIdx.x;
+  if (tid == 0) l.wrong = 0.0f;
+  __syncthreads();
+  int id = -1;
+  if (tid < a.k) {
+    const int64_t i = load_index(a.ids, row * a.k + tid, a.wide_index);
+    if (i >= a.classes) l.wrong = 1.0f;  // every writer writes the same
+    id = i >= 0 && i < a.classes ? static_cast<int>(i) : -1;
+    l.id[tid] = id;
+    l.t[tid] = a.teacher[row * a.k + tid];
+  }
+  __syncthreads();
+  if (id >= 0)
+    for (int j = 0; j < tid; ++j)
+      if (l.id[j] == id) {
+        id = -1;
+        break;
+      }
+  __syncthreads();
+  if (tid < a.k) l.id[tid] = id;
+  return id;
+}
+
+// One wave: q of the listed classes into l.q; returns their mass. `top` and `log_z`
+// as log_ratio takes them.
+__device__ __forceinline__ TeacherMass teacher_sums(const DistillArgs &a, ListLds &l, float *top,
+                                                    float *log_z) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const float inf = __builtin_inff();
+  float t_max = -inf;
+  float wrong = l.wrong;
+  for (int j = lane; j < a.k; j += kWave)
+    if (l.id[j] >= 0) {
+      t_max = fmaxf(t_max, l.t[j]);
+      if (l.t[j] != l.t[j]) wrong = 1.0f;
+    }
+  t_max = lanes_max<kWave>(t_max);
+  wrong = lanes_max<kWave>(wrong);
+  TeacherMass m = teacher_total<kWave>(a, t_max, [&](auto f) {
+    for (int j = lane; j < a.k; j += kWave)
+      if (l.id[j] >= 0) f(l.t[j]);
+  });
+  const float total = m.all;
+  const bool none = a.kind == 0 && t_max == -inf;
+  const float inv_z = a.kind == 0 ? 1.0f / total : 1.0f;
+  for (int j = lane; j < a.k; j += kWave)
+    l.q[j] = l.id[j] >= 0 && !none ? teacher_mass(a, l.t[j], t_max, inv_z) : 0.0f;
+  *top = t_max;
+  *log_z = logf(total);
+  // sum q is 1 for kind 0 (a sum of NaN stays one)
+  m.all = wrong != 0.0f ? __builtin_nanf("") : a.kind != 0 ? total : none ? 0.0f : total * inv_z;
+  return m;
+}
+
+// Writes the gradient of a part: all classes as unlisted ones, then the listed.
+// The caller has read the listed logits and synchronised since.
+template <class T, int NT>
+__device__ __forceinline__ void distill_gradient(const DistillArgs &a, const T *z, T *out,
+                                                 int begin, int end, const DistillRow &r,
+                                                 float scale, int id, float zj, float q) {
+  if (r.m_a == -__builtin_inff() && r.a_a == r.a_a) {  // every class is masked
+    zero_part<T, NT>(out, begin, end);
+    return;
+  }
+  const ExpAt e(r.m_d, a.c);
+  const float f = scale * r.a_d * e.fix;
+  if (e.huge)
+    map_part<T, NT>(z, out, begin, end, [&](float v) { return f * exp2_raw(e.x_huge(v)); });
+  else
+    map_part<T, NT>(z, out, begin, end, [&](float v) { return f * exp2_raw(e.x_plain(v)); });
+  __syncthreads();
+  if (id >= begin && id < end)
+    out[id] = Row<T>::down(scale * (r.a_a * exp2_raw((zj - r.m_a) * a.c) - q));
+}
+
+// From the sums of a row: its loss, statistics and gradient (of one part).
+template <class T, int NT>
+__device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l, int64_t row,
+                                               int part, const T *z, int begin, int end,
+                                               const Soft &dense, int id, float zj, float w) {
+  const int tid = threadIdx.x;
+  if (tid < a.k) l.z[tid] = zj;
+  __syncthreads();
+  if (tid < kWave) {
+    float top, log_z, rest_loss, loss = 0.0f;
+    const TeacherMass mass = teacher_sums(a, l, &top, &log_z);
+    Soft all = dense;
+    if (a.kind != 0) {
+      for (int j = tid; j < a.k; j += kWave)
+        if (l.id[j] >= 0) all.m = fmaxf(all.m, l.z[j]);
+      all.m = lanes_max<kWave>(all.m);
+      const float shift = all.m == -__builtin_inff() ? 0.0f : all.m;
+      // the 1 that r leaves out is the rest's, or of the first listed class that has it
+      bool first = true;
+      all.r = 0.0f;
+      soft_join(all, dense, a.c, first);
+      float one = -1e9f, s = 0.0f;
+      for (int j = tid; j < a.k; j += kWave)
+        if (l.id[j] >= 0 && l.z[j] == all.m) one = fmaxf(one, -static_cast<float>(j));
+      one = first ? -lanes_max<kWave>(one) : -1.0f;
+      for (int j = tid; j < a.k; j += kWave)
+        if (l.id[j] >= 0 && static_cast<float>(j) != one) s += exp2_raw((l.z[j] - shift) * a.c);
+      all.r += lanes_sum<kWave>(s);
+      if (all.m == -__builtin_inff()) all.r -= 1.0f;  // no class: S = 0 (or NaN)
+      if (all.m == __builtin_inff()) all.r = __builtin_nanf("");
+      all.S = 1.0f + all.r;
+    }
+    const DistillRow r = distill_row(a, dense, all, mass.all, mass.left, &rest_loss);
+    const float log_s = log1pf(all.r);
+    for (int j = tid; j < a.k; j += kWave) {
+      const float q = l.q[j];
+      if (l.id[j] >= 0 && q != 0.0f)
+        loss += q * log_ratio(a, l.t[j], top, log_z, l.z[j], all.m, log_s);
+    }
+    loss = lanes_sum<kWave>(loss) + rest_loss;
+    if (l.wrong != 0.0f) loss = __builtin_nanf("");
+    if (tid == 0) {
+      const bool empty = all.m == -__builtin_inff() && all.S == 0.0f;
+      DistillRow o = r;
+      if (empty) o = DistillRow{0.0f, 0.0f, -__builtin_inff(), 0.0f};
+      l.row = o;
+      if (part == 0) {
+        if (a.loss) a.loss[row] = empty ? 0.0f : loss * a.t * a.t * w;
+        if (a.stats)
+          reinterpret_cast<float4 *>(a.stats)[row] = make_float4(o.m_d, o.a_d, o.m_a, o.a_a);
+      }
+    }
+  }
+  __syncthreads();
+  if (!a.d_logits) return;
+  T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
+  distill_gradient<T, NT>(a, z, out, begin, end, l.row, w * a.t, id, zj,
+                          tid < a.k ? l.q[tid] : 0.0f);
+}
+
+// A row of weight 0 is not read.
+template <class T, int NT>
+__device__ __forceinline__ void distill_no_weight(const DistillArgs &a, int64_t row, int part,
+                                                  int begin, int end) {
+  if (part == 0 && threadIdx.x == 0) {
+    if (a.loss) a.loss[row] = 0.0f;
+    if (a.stats)
+      reinterpret_cast<float4 *>(a.stats)[row] =
+          make_float4(0.0f, 0.0f, -__builtin_inff(), 0.0f);
+  }
+  if (a.d_logits)
+    zero_part<T, NT>(static_cast<T *>(a.d_logits) + row * a.d_row_stride, begin, end);
+}
+
+template <class T, int NT, bool TAIL>
+__global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
+  constexpr int N = Row<T>::n, U = kLogitVecs;
+  extern __shared__ uint32_t listed[];  // TAIL: a bit for each class of the part
+  __shared__ BlockLds<NT> lds;
+  __shared__ ListLds list;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+  const int begin = part * a.part_len;
+  const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+  const float w = a.weights ? a.weights[row] : 1.0f;
+  if (w == 0.0f) {
+    if (a.parts == 1) distill_no_weight<T, NT>(a, row, part, begin, end);
+    return;
+  }
+  if (TAIL)
+    for (int i = tid; i * 32 < end - begin; i += NT) listed[i] = 0u;
+  const int id = read_list<NT>(a, list, row);
+  float zj = 0.0f;
+  if (id >= begin && id < end) {
+    zj = Row<T>::up(z[id]);
+    if (TAIL) atomicOr(&listed[(id - begin) >> 5], 1u << ((id - begin) & 31));
+  }
+  if (TAIL) __syncthreads();
+  // a listed class counts apart from the rest
+  auto hide = [&](int i, float *v) {
+    if (!TAIL) return;
+    const int o = i - begin;
+    if (i >= end) return;
+    const uint32_t bits = (listed[o >> 5] >> (o & 31)) & ((1u << N) - 1u);
+    if (bits == 0) return;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (bits >> j & 1u) v[j] = -__builtin_inff();
+  };
+  Soft s;
+  auto take = [&](int i, float(&v)[U][N]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) hide(i + u * NT * N, v[u]);
+    float cm = v[0][0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < N; ++j) cm = fmaxf(cm, v[u][j]);
+    soft_add<U * N, false>(s, &v[0][0], cm, a.c);
+  };
+  int at = begin;
+  for (; at + NT * N * U <= end; at += NT * N * U) {
+    const int i = at + tid * N;
+    float v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) widen<T>(load_raw(z + i + u * NT * N), v[u]);
+    take(i, v);
+  }
+  if (at < end) {
+    const int i = at + tid * N;
+    float v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_vec<T>(z, i + u * NT * N, end, v[u]);
+    take(i, v);
+  }
+  int n = 0;
+  s = soft_finish<T, NT, false>(lds, s, z, begin, end, a.c, n, hide);
+  if (a.parts > 1) {
+    if (tid == 0) a.part_sum[blockIdx.x] = make_float2(s.m, s.r);
+    if (id >= begin && id < end) a.list_z[row * a.k + tid] = zj;
+    return;
+  }
+  distill_finish<T, NT>(a, list, row, 0, z, begin, end, s, id, zj, w);
+}
+
+// Joins the sums of a row's parts (in their order), and finishes one part.
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
+  __shared__ float2 sum[kMaxParts];
+  __shared__ ListLds list;
+  const int tid = threadIdx.x;
+  const int blocks = a.d_logits ? a.parts : 1;
+  const int64_t row = blockIdx.x / blocks;
+  const int part = blockIdx.x % blocks;
+  const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+  const int begin = part * a.part_len;
+  const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+  const float w = a.weights ? a.weights[row] : 1.0f;
+  if (w == 0.0f) {
+    distill_no_weight<T, NT>(a, row, part, begin, end);
+    return;
+  }
+  for (int p = tid; p < a.parts; p += NT) sum[p] = a.part_sum[row * a.parts + p];
+  const int id = read_list<NT>(a, list, row);
+  const float zj = id >= 0 ? a.list_z[row * a.k + tid] : 0.0f;
+  Soft s;
+  for (int p = 0; p < a.parts; ++p) s.m = fmaxf(s.m, sum[p].x);
+  bool first = true;
+  s.r = 0.0f;
+  for (int p = 0; p < a.parts; ++p) {
+    Soft b;
+    b.m = sum[p].x;
+    b.r = sum[p].y;
+    b.S = 1.0f + b.r;
+    soft_join(s, b, a.c, first);
+  }
+  if (s.m == -__builtin_inff()) s.r -= 1.0f;  // no class: S = 0 (or NaN)
+  s.S = 1.0f + s.r;
+  distill_finish<T, NT>(a, list, row, part, z, begin, end, s, id, zj, w);
+}
+
+// The gradient alone, from the statistics.
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void distill_grad_block_kernel(DistillArgs a) {
+  __shared__ ListLds list;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+  T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
+  const int begin = part * a.part_len;
+  const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+  const float w = a.weights ? a.weights[row] : 1.0f;
+  if (w == 0.0f) {
+    zero_part<T, NT>(out, begin, end);
+    return;
+  }
+  const int id = read_list<NT>(a, list, row);
+  const float zj = id >= begin && id < end ? Row<T>::up(z[id]) : 0.0f;
+  const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
+  __syncthreads();
+  if (tid < kWave) {
+    float top, log_z;
+    (void)teacher_sums(a, list, &top, &log_z);
+  }
+  __syncthreads();
+  distill_gradient<T, NT>(a, z, out, begin, end, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, id, zj,
+                          tid < a.k ? list.q[tid] : 0.0f);
+}
+
+}  // namespace tmnn_hip

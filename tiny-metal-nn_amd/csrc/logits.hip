@@ -1,0 +1,645 @@
+// logits.hip -- host side of the class-logit operators (include/tmnn_hip.h):
+// argument checks, the choice of kernel and split, the workspace, and the
+// host-pointer forms.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <mutex>
+#include <new>
+#include <vector>
+
+#include "context.hpp"
+#include "distill_kernel.hpp"
+#include "logprob_kernel.hpp"
+#include "tmnn_hip.h"
+
+using namespace tmnn_hip;
+
+namespace {
+
+// Workspace of the calls that split rows: at most kMaxSplit parts at a time.
+constexpr int kMaxSplit = 4096;
+constexpr size_t kSumBytes = kMaxSplit * sizeof(float4);
+constexpr size_t kKeyBytes = static_cast<size_t>(kMaxSplit) * kMaxTop * sizeof(uint64_t);
+constexpr size_t kListBytes = static_cast<size_t>(kMaxSplit) * kMaxTeacher * sizeof(float);
+
+}  // namespace
+
+struct tmnn_logits {
+  tmnn_context *ctx = nullptr;
+  DevBuf work;              // part sums, part keys, listed logits
+  DevBuf arena;             // arrays of the host-pointer calls
+  std::mutex host_mu;       // the arena belongs to one host-pointer call
+  std::mutex mu;            // the fields below, and the order of calls that share `work`
+  bool used = false;        // `last` has taken the workspace
+  hipStream_t last = nullptr;
+  hipEvent_t moved = nullptr;
+};
+
+namespace {
+
+size_t dtype_size(int32_t dtype) { return dtype == TMNN_DTYPE_F32 ? 4 : 2; }
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+template <class A>
+int check_matrix(const A *a, const char *what) {
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (a->struct_size != sizeof(A)) return bad("struct_size mismatch");
+  if (a->dtype < TMNN_DTYPE_F32 || a->dtype > TMNN_DTYPE_BF16) return bad("invalid dtype");
+  if (a->index_dtype != TMNN_INDEX_I32 && a->index_dtype != TMNN_INDEX_I64)
+    return bad("invalid index_dtype");
+  if (a->rows < 0 || a->rows > INT32_MAX) return bad("rows must be in [0, 2^31)");
+  if (a->classes < 1 || a->classes > TMNN_LOGITS_MAX_CLASSES)
+    return bad("classes must be in [1, 2^24]");
+  if (a->row_stride < a->classes) return bad("row_stride must be at least classes");
+  if (a->d_logits && a->d_row_stride < a->classes)
+    return bad("d_row_stride must be at least classes");
+  // c = log2(e) / T stays an ordinary number
+  if (!(a->temperature >= 1e-6f && a->temperature <= 1e6f))
+    return bad("temperature must be in [1e-6, 1e6]");
+  if (a->rows == 0) return TMNN_OK;
+  if (!a->logits) return bad("logits is null");
+  const size_t size = dtype_size(a->dtype);
+  if (!aligned(a->logits, size) || !aligned(a->d_logits, size))
+    return bad("logits and d_logits must be aligned to their type");
+  return TMNN_OK;
+}
+
+int check_logprobs(const tmnn_token_logprobs_args *a, bool back) {
+  const char *what = back ? "token_logprobs_backward" : "token_logprobs";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (!a) return bad("args is null");
+  const int rc = check_matrix(a, what);
+  if (rc != TMNN_OK) return rc;
+  if (a->top_k < 0 || a->top_k > TMNN_LOGITS_MAX_TOP) return bad("top_k must be in [0, 128]");
+  if (a->rows == 0) return TMNN_OK;
+  if (!aligned(a->tokens, a->index_dtype == TMNN_INDEX_I64 ? 8 : 4))
+    return bad("tokens must be aligned to their type");
+  for (const void *p : {static_cast<const void *>(a->logprob), static_cast<const void *>(a->entropy),
+                        static_cast<const void *>(a->rank), static_cast<const void *>(a->stats),
+                        static_cast<const void *>(a->top_ids),
+                        static_cast<const void *>(a->top_logprobs),
+                        static_cast<const void *>(a->d_logprob),
+                        static_cast<const void *>(a->d_entropy),
+                        static_cast<const void *>(a->d_top_logprobs)})
+    if (!aligned(p, 4)) return bad("arrays of 32-bit values must be 4-byte aligned");
+  if (back) {
+    if (!a->d_logits) return bad("d_logits is null");
+    if (!a->stats) return bad("stats is null");
+    if (a->d_logprob && !a->tokens) return bad("d_logprob needs tokens");
+    if (a->d_entropy && !a->entropy) return bad("d_entropy needs entropy");
+    if (a->d_top_logprobs && a->top_k > 0 && !a->top_ids) return bad("d_top_logprobs needs top_ids");
+    return TMNN_OK;
+  }
+  if (!a->top_ids != !a->top_logprobs) return bad("top_ids and top_logprobs go together");
+  if (a->top_k > 0 && !a->top_ids) return bad("top_k > 0 needs top_ids and top_logprobs");
+  return TMNN_OK;
+}
+
+int check_distill(const tmnn_distill_args *a, bool back) {
+  const char *what = back ? "distill_backward" : "distill";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (!a) return bad("args is null");
+  const int rc = check_matrix(a, what);
+  if (rc != TMNN_OK) return rc;
+  if (a->teacher_kind != TMNN_TEACHER_LOGITS && a->teacher_kind != TMNN_TEACHER_LOGPROBS)
+    return bad("invalid teacher_kind");
+  if (a->teacher_k < 1 || a->teacher_k > TMNN_LOGITS_MAX_TEACHER)
+    return bad("teacher_k must be in [1, 256]");
+  if (a->rows == 0) return TMNN_OK;
+  if (!a->teacher_ids || !a->teacher) return bad("teacher_ids and teacher must not be null");
+  if (!aligned(a->teacher_ids, a->index_dtype == TMNN_INDEX_I64 ? 8 : 4))
+    return bad("teacher_ids must be aligned to their type");
+  if (!aligned(a->teacher, 4) || !aligned(a->row_weights, 4) || !aligned(a->loss, 4))
+    return bad("arrays of 32-bit values must be 4-byte aligned");
+  if (!aligned(a->stats, 16)) return bad("stats must be 16-byte aligned");
+  if (back) {
+    if (!a->d_logits) return bad("d_logits is null");
+    if (!a->stats) return bad("stats is null");
+    if (!a->row_weights) return bad("row_weights (the loss's gradient) is null");
+  } else if (!a->loss && !a->stats && !a->d_logits) {
+    return bad("nothing to compute");
+  }
+  return TMNN_OK;
+}
+
+// Takes the workspace for `st`: where the last call that used it went to another
+// stream, `st` waits for that one's work.
+int take_workspace(tmnn_logits *h, hipStream_t st) {
+  if (h->used && h->last != st) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TMNN_HIP_TRY(hipStreamIsCapturing(st, &cap));
+    if (cap != hipStreamCaptureStatusNone)
+      return fail(TMNN_ERR_UNSUPPORTED,
+                  "a captured stream needs a logits handle of its own (another stream used this one)");
+    if (hipEventRecord(h->moved, h->last) == hipSuccess) {
+      TMNN_HIP_TRY(hipStreamWaitEvent(st, h->moved, 0));
+    } else {  // the last stream is gone
+      (void)hipGetLastError();
+      TMNN_HIP_TRY(hipDeviceSynchronize());
+    }
+  }
+  h->used = true;
+  h->last = st;
+  return TMNN_OK;
+}
+
+// ---- kernels by size ---------------------------------------------------------------
+
+// Rows of up to 64 vectors go to as many lanes as they have vectors (a power of two).
+int group_lanes(int64_t classes, int n) {
+  const int64_t vecs = (classes + n - 1) / n;
+  int g = 1;
+  while (g < vecs) g *= 2;
+  return g <= kWave ? g : 0;
+}
+
+struct Split {
+  int threads, parts, part_len;
+};
+
+// Threads of a block, and blocks of a row.
+Split split_of(int64_t rows, int64_t classes, int n, int min_threads, int64_t blocks) {
+  Split s;
+  const int64_t vecs = (classes + n - 1) / n;
+  int64_t parts = 1;
+  if (rows < blocks) parts = std::min<int64_t>(blocks / rows, vecs / (4 * 256));
+  parts = std::max<int64_t>(parts, (classes + kMaxPartLen - 1) / kMaxPartLen);
+  parts = std::min<int64_t>(std::max<int64_t>(parts, 1), kMaxParts);
+  int64_t len = (classes + parts - 1) / parts;
+  if (parts > 1) len = (len + 255) / 256 * 256;
+  s.part_len = static_cast<int>(len);
+  s.parts = static_cast<int>((classes + len - 1) / len);
+  s.threads = len / n >= 4 * 1024 ? 1024 : len / n >= 4 * 512 ? 512 : 256;
+  s.threads = std::max(s.threads, min_threads);
+  return s;
+}
+
+constexpr int64_t kSplitBlocks = 512;
+
+// Rows of one launch: at most 2^31 threads, and the workspace of its parts.
+template <class F>
+int in_slices(int64_t rows, int64_t threads_per_row, int parts, F launch) {
+  int64_t step = std::max<int64_t>(1, (1ll << 31) / threads_per_row - 1);
+  if (parts > 1) step = std::min<int64_t>(step, kMaxSplit / parts);
+  for (int64_t at = 0; at < rows; at += step) {
+    launch(at, static_cast<int32_t>(std::min(step, rows - at)));
+    TMNN_HIP_TRY(hipGetLastError());
+  }
+  return TMNN_OK;
+}
+
+dim3 group_grid(int rows, int g) {
+  const int per = kGroupThreads / g;
+  return dim3((rows + per - 1) / per);
+}
+
+#define TMNN_BY_GROUP(g, CALL) \
+  switch (g) {                 \
+    case 1: CALL(1); break;    \
+    case 2: CALL(2); break;    \
+    case 4: CALL(4); break;    \
+    case 8: CALL(8); break;    \
+    case 16: CALL(16); break;  \
+    case 32: CALL(32); break;  \
+    default: CALL(64); break;  \
+  }
+#define TMNN_BY_THREADS(nt, CALL) \
+  switch (nt) {                   \
+    case 256: CALL(256); break;   \
+    case 512: CALL(512); break;   \
+    default: CALL(1024); break;   \
+  }
+
+template <class T>
+LogprobArgs logprob_slice(const LogprobArgs &a, int64_t at, int32_t rows) {
+  LogprobArgs s = a;
+  auto move = [&](auto *&p, int64_t n) {
+    if (p) p += at * n;
+  };
+  s.rows = rows;
+  s.logits = static_cast<const T *>(a.logits) + at * a.row_stride;
+  if (a.tokens) s.tokens = static_cast<const char *>(a.tokens) + at * (a.wide_index ? 8 : 4);
+  move(s.logprob, 1);
+  move(s.entropy, 1);
+  move(s.rank, 1);
+  move(s.stats, 2);
+  move(s.top_ids, a.top_k);
+  move(s.top_logprobs, a.top_k);
+  move(s.d_logprob, 1);
+  move(s.d_entropy, 1);
+  move(s.d_top, a.top_k);
+  move(s.entropy_in, 1);
+  move(s.stats_in, 2);
+  move(s.top_in, a.top_k);
+  if (a.d_logits) s.d_logits = static_cast<T *>(a.d_logits) + at * a.d_row_stride;
+  return s;
+}
+
+template <class T>
+int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
+  constexpr int n = Row<T>::n;
+  if (const int g = group_lanes(a.classes, n)) {
+    return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
+      const LogprobArgs s = logprob_slice<T>(a, at, r);
+#define CALL(G) \
+  hipLaunchKernelGGL((logprob_group_kernel<T, G>), group_grid(r, G), dim3(kGroupThreads), 0, st, s)
+      TMNN_BY_GROUP(g, CALL)
+#undef CALL
+    });
+  }
+  // four threads to an alternative, so that the threads' maxima bound them well
+  const Split sp = split_of(rows, a.classes, n, a.top_k > 64 ? 512 : 256, kSplitBlocks);
+  a.parts = sp.parts;
+  a.part_len = sp.part_len;
+  a.part_sum = static_cast<float4 *>(h->work.ptr);
+  a.part_key = reinterpret_cast<uint64_t *>(static_cast<char *>(h->work.ptr) + kSumBytes);
+  if (a.parts > 1) {
+    const int rc = take_workspace(h, st);
+    if (rc != TMNN_OK) return rc;
+  }
+  return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, a.parts,
+                   [&](int64_t at, int32_t r) {
+                     const LogprobArgs s = logprob_slice<T>(a, at, r);
+#define CALL(NT) \
+  hipLaunchKernelGGL((logprob_block_kernel<T, NT>), dim3(r * a.parts), dim3(NT), 0, st, s)
+                     TMNN_BY_THREADS(sp.threads, CALL)
+#undef CALL
+                     if (a.parts > 1)
+                       hipLaunchKernelGGL((logprob_join_kernel<T>), dim3(r), dim3(kJoinThreads), 0,
+                                          st, s);
+                   });
+}
+
+template <class T>
+int run_logprobs_grad(LogprobArgs a, int64_t rows, hipStream_t st) {
+  constexpr int n = Row<T>::n;
+  if (const int g = group_lanes(a.classes, n)) {
+    return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
+      const LogprobArgs s = logprob_slice<T>(a, at, r);
+#define CALL(G)                                                                              \
+  hipLaunchKernelGGL((logprob_grad_group_kernel<T, G>), group_grid(r, G), dim3(kGroupThreads), 0, \
+                     st, s)
+      TMNN_BY_GROUP(g, CALL)
+#undef CALL
+    });
+  }
+  const Split sp = split_of(rows, a.classes, n, 256, kSplitBlocks);
+  a.parts = sp.parts;
+  a.part_len = sp.part_len;
+  return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1, [&](int64_t at, int32_t r) {
+    const LogprobArgs s = logprob_slice<T>(a, at, r);
+#define CALL(NT) \
+  hipLaunchKernelGGL((logprob_grad_block_kernel<T, NT>), dim3(r * a.parts), dim3(NT), 0, st, s)
+    TMNN_BY_THREADS(sp.threads, CALL)
+#undef CALL
+  });
+}
+
+template <class T>
+DistillArgs distill_slice(const DistillArgs &a, int64_t at, int32_t rows) {
+  DistillArgs s = a;
+  s.rows = rows;
+  s.logits = static_cast<const T *>(a.logits) + at * a.row_stride;
+  s.ids = static_cast<const char *>(a.ids) + at * a.k * (a.wide_index ? 8 : 4);
+  s.teacher = a.teacher + at * a.k;
+  if (a.weights) s.weights = a.weights + at;
+  if (a.loss) s.loss = a.loss + at;
+  if (a.stats) s.stats = a.stats + at * 4;
+  if (a.d_logits) s.d_logits = static_cast<T *>(a.d_logits) + at * a.d_row_stride;
+  return s;
+}
+
+template <class T>
+int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStream_t st) {
+  constexpr int n = Row<T>::n;
+  if (const int g = group_lanes(a.classes, n)) {
+    return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
+      const DistillArgs s = distill_slice<T>(a, at, r);
+#define CALL(G)                                                                           \
+  if (back)                                                                               \
+    hipLaunchKernelGGL((distill_group_kernel<T, G, true>), group_grid(r, G),              \
+                       dim3(kGroupThreads), 0, st, s);                                    \
+  else                                                                                    \
+    hipLaunchKernelGGL((distill_group_kernel<T, G, false>), group_grid(r, G),             \
+                       dim3(kGroupThreads), 0, st, s)
+      TMNN_BY_GROUP(g, CALL)
+#undef CALL
+    });
+  }
+  const Split sp = split_of(rows, a.classes, n, 256, kSplitBlocks);
+  a.parts = sp.parts;
+  a.part_len = sp.part_len;
+  if (back)
+    return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1,
+                     [&](int64_t at, int32_t r) {
+                       const DistillArgs s = distill_slice<T>(a, at, r);
+#define CALL(NT) \
+  hipLaunchKernelGGL((distill_grad_block_kernel<T, NT>), dim3(r * a.parts), dim3(NT), 0, st, s)
+                       TMNN_BY_THREADS(sp.threads, CALL)
+#undef CALL
+                     });
+  a.part_sum = static_cast<float2 *>(h->work.ptr);
+  a.list_z = reinterpret_cast<float *>(static_cast<char *>(h->work.ptr) + kSumBytes + kKeyBytes);
+  if (a.parts > 1) {
+    const int rc = take_workspace(h, st);
+    if (rc != TMNN_OK) return rc;
+  }
+  return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, a.parts,
+                   [&](int64_t at, int32_t r) {
+                     const DistillArgs s = distill_slice<T>(a, at, r);
+                     const size_t bits = (static_cast<size_t>(sp.part_len) + 31) / 32 * 4;
+#define CALL(NT)                                                                                   \
+  if (a.kind == TMNN_TEACHER_LOGPROBS)                                                             \
+    hipLaunchKernelGGL((distill_block_kernel<T, NT, true>), dim3(r * a.parts), dim3(NT), bits, st, \
+                       s);                                                                         \
+  else                                                                                             \
+    hipLaunchKernelGGL((distill_block_kernel<T, NT, false>), dim3(r * a.parts), dim3(NT), 0, st, s)
+                     TMNN_BY_THREADS(sp.threads, CALL)
+#undef CALL
+                     if (a.parts > 1) {
+                       const dim3 grid(r * (a.d_logits ? a.parts : 1));
+#define CALL(NT) hipLaunchKernelGGL((distill_join_kernel<T, NT>), grid, dim3(NT), 0, st, s)
+                       TMNN_BY_THREADS(sp.threads, CALL)
+#undef CALL
+                     }
+                   });
+}
+
+// ---- calls on device memory -----------------------------------------------------------
+
+int logprobs_device(tmnn_logits *h, const tmnn_token_logprobs_args &u, bool back, hipStream_t st) {
+  LogprobArgs a{};
+  a.logits = u.logits;
+  a.row_stride = u.row_stride;
+  a.tokens = u.tokens;
+  a.wide_index = u.index_dtype == TMNN_INDEX_I64;
+  a.classes = static_cast<int32_t>(u.classes);
+  a.top_k = u.top_k;
+  a.parts = 1;
+  a.inv_t = static_cast<float>(1.0 / u.temperature);
+  a.c = static_cast<float>(1.4426950408889634 / u.temperature);
+  if (back) {
+    a.d_logprob = u.d_logprob;
+    a.d_entropy = u.d_entropy;
+    a.d_top = u.top_k > 0 ? u.d_top_logprobs : nullptr;
+    a.entropy_in = u.entropy;
+    a.stats_in = u.stats;
+    a.top_in = u.top_ids;
+    a.d_logits = u.d_logits;
+    a.d_row_stride = u.d_row_stride;
+  } else {
+    a.logprob = u.logprob;
+    a.entropy = u.entropy;
+    a.rank = u.rank;
+    a.stats = u.stats;
+    a.top_ids = u.top_ids;
+    a.top_logprobs = u.top_logprobs;
+  }
+  std::lock_guard<std::mutex> lock(h->mu);
+  switch (u.dtype) {
+    case TMNN_DTYPE_F32:
+      return back ? run_logprobs_grad<float>(a, u.rows, st) : run_logprobs<float>(h, a, u.rows, st);
+    case TMNN_DTYPE_F16:
+      return back ? run_logprobs_grad<_Float16>(a, u.rows, st)
+                  : run_logprobs<_Float16>(h, a, u.rows, st);
+    default:
+      return back ? run_logprobs_grad<__bf16>(a, u.rows, st) : run_logprobs<__bf16>(h, a, u.rows, st);
+  }
+}
+
+int distill_device(tmnn_logits *h, const tmnn_distill_args &u, bool back, hipStream_t st) {
+  DistillArgs a{};
+  a.logits = u.logits;
+  a.row_stride = u.row_stride;
+  a.ids = u.teacher_ids;
+  a.teacher = u.teacher;
+  a.weights = u.row_weights;
+  a.wide_index = u.index_dtype == TMNN_INDEX_I64;
+  a.kind = u.teacher_kind;
+  a.classes = static_cast<int32_t>(u.classes);
+  a.k = u.teacher_k;
+  a.parts = 1;
+  a.t = u.temperature;
+  a.inv_t = static_cast<float>(1.0 / u.temperature);
+  a.c = static_cast<float>(1.4426950408889634 / u.temperature);
+  a.loss = back ? nullptr : u.loss;
+  a.stats = u.stats;
+  a.d_logits = u.d_logits;
+  a.d_row_stride = u.d_row_stride;
+  std::lock_guard<std::mutex> lock(h->mu);
+  switch (u.dtype) {
+    case TMNN_DTYPE_F32:
+      return run_distill<float>(h, a, u.rows, back, st);
+    case TMNN_DTYPE_F16:
+      return run_distill<_Float16>(h, a, u.rows, back, st);
+    default:
+      return run_distill<__bf16>(h, a, u.rows, back, st);
+  }
+}
+
+hipStream_t stream_of(tmnn_logits *h, void *stream) {
+  return stream == TMNN_STREAM_CONTEXT ? h->ctx->stream : static_cast<hipStream_t>(stream);
+}
+
+// ---- calls on host memory ---------------------------------------------------------------
+
+// The host arrays of a call and their places in the handle's arena.
+class HostArrays {
+ public:
+  enum Dir { kIn, kOut };
+  // `rows` x `width` bytes, `pitch` bytes from row to row on the host; packed on the device
+  template <class P>
+  void add(P *&slot, Dir dir, int64_t rows, size_t width, size_t pitch) {
+    if (!slot || rows == 0 || width == 0) return;
+    items_.push_back({const_cast<void *>(static_cast<const void *>(slot)),
+                      const_cast<void **>(reinterpret_cast<const void *const *>(&slot)), dir, rows,
+                      width, pitch, bytes_});
+    bytes_ += (static_cast<size_t>(rows) * width + 255) / 256 * 256;
+  }
+  template <class P>
+  void add(P *&slot, Dir dir, int64_t rows, size_t width) {
+    add(slot, dir, rows, width, width);
+  }
+  int enter(tmnn_logits *h) {
+    TMNN_HIP_TRY(h->arena.ensure(std::max<size_t>(bytes_, 256)));
+    for (const Item &i : items_) {
+      char *d = h->arena.as<char>() + i.at;
+      *i.slot = d;
+      if (i.dir == kIn)
+        TMNN_HIP_TRY(hipMemcpy2DAsync(d, i.width, i.host, i.pitch, i.width, i.rows,
+                                      hipMemcpyHostToDevice, h->ctx->stream));
+    }
+    return TMNN_OK;
+  }
+  int leave(tmnn_logits *h) {
+    for (const Item &i : items_)
+      if (i.dir == kOut)
+        TMNN_HIP_TRY(hipMemcpy2DAsync(i.host, i.pitch, h->arena.as<char>() + i.at, i.width, i.width,
+                                      i.rows, hipMemcpyDeviceToHost, h->ctx->stream));
+    return TMNN_OK;
+  }
+
+ private:
+  struct Item {
+    void *host;
+    void **slot;
+    Dir dir;
+    int64_t rows;
+    size_t width, pitch, at;
+  };
+  std::vector<Item> items_;
+  size_t bytes_ = 0;
+};
+
+template <class Run>
+int on_host(tmnn_logits *h, HostArrays &arrays, Run run) {
+  std::lock_guard<std::mutex> lock(h->host_mu);
+  int rc = arrays.enter(h);
+  if (rc == TMNN_OK) rc = run();
+  if (rc == TMNN_OK) rc = arrays.leave(h);
+  const hipError_t e = hipStreamSynchronize(h->ctx->stream);
+  if (rc == TMNN_OK && e != hipSuccess)
+    rc = fail(TMNN_ERR_GPU, std::string("hipStreamSynchronize: ") + hipGetErrorString(e));
+  return rc;
+}
+
+int logprobs_host(tmnn_logits *h, tmnn_token_logprobs_args u, bool back) {
+  const size_t size = dtype_size(u.dtype), index = u.index_dtype == TMNN_INDEX_I64 ? 8 : 4;
+  const size_t k = static_cast<size_t>(u.top_k);
+  const auto out = back ? HostArrays::kIn : HostArrays::kOut;
+  HostArrays m;
+  m.add(u.logits, HostArrays::kIn, u.rows, u.classes * size, u.row_stride * size);
+  m.add(u.tokens, HostArrays::kIn, u.rows, index);
+  m.add(u.entropy, out, u.rows, 4);
+  m.add(u.stats, out, u.rows, 8);
+  m.add(u.top_ids, out, u.rows, 4 * k);
+  if (back) {
+    m.add(u.d_logprob, HostArrays::kIn, u.rows, 4);
+    m.add(u.d_entropy, HostArrays::kIn, u.rows, 4);
+    m.add(u.d_top_logprobs, HostArrays::kIn, u.rows, 4 * k);
+    m.add(u.d_logits, HostArrays::kOut, u.rows, u.classes * size, u.d_row_stride * size);
+  } else {
+    m.add(u.logprob, HostArrays::kOut, u.rows, 4);
+    m.add(u.rank, HostArrays::kOut, u.rows, 4);
+    m.add(u.top_logprobs, HostArrays::kOut, u.rows, 4 * k);
+    u.d_logits = nullptr;
+  }
+  u.row_stride = u.d_row_stride = u.classes;
+  return on_host(h, m, [&] { return logprobs_device(h, u, back, h->ctx->stream); });
+}
+
+int distill_host(tmnn_logits *h, tmnn_distill_args u, bool back) {
+  const size_t size = dtype_size(u.dtype), index = u.index_dtype == TMNN_INDEX_I64 ? 8 : 4;
+  const size_t k = static_cast<size_t>(u.teacher_k);
+  HostArrays m;
+  m.add(u.logits, HostArrays::kIn, u.rows, u.classes * size, u.row_stride * size);
+  m.add(u.teacher_ids, HostArrays::kIn, u.rows, index * k);
+  m.add(u.teacher, HostArrays::kIn, u.rows, 4 * k);
+  m.add(u.row_weights, HostArrays::kIn, u.rows, 4);
+  m.add(u.stats, back ? HostArrays::kIn : HostArrays::kOut, u.rows, 16);
+  if (back)
+    u.loss = nullptr;
+  else
+    m.add(u.loss, HostArrays::kOut, u.rows, 4);
+  m.add(u.d_logits, HostArrays::kOut, u.rows, u.classes * size, u.d_row_stride * size);
+  u.row_stride = u.d_row_stride = u.classes;
+  return on_host(h, m, [&] { return distill_device(h, u, back, h->ctx->stream); });
+}
+
+// No exception leaves a C entry point.
+template <class F>
+int entry(tmnn_logits *h, F f) {
+  if (!h) return fail(TMNN_ERR_INVALID_ARGUMENT, "logits handle is null");
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return fail(TMNN_ERR_RUNTIME, "out of host memory");
+  } catch (const std::exception &e) {
+    return fail(TMNN_ERR_RUNTIME, e.what());
+  }
+}
+
+int token_logprobs(tmnn_logits *h, const tmnn_token_logprobs_args *args, bool back, bool host,
+                   void *stream) {
+  return entry(h, [&] {
+    const int rc = check_logprobs(args, back);
+    if (rc != TMNN_OK || args->rows == 0) return rc;
+    TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
+    return host ? logprobs_host(h, *args, back)
+                : logprobs_device(h, *args, back, stream_of(h, stream));
+  });
+}
+
+int distill(tmnn_logits *h, const tmnn_distill_args *args, bool back, bool host, void *stream) {
+  return entry(h, [&] {
+    const int rc = check_distill(args, back);
+    if (rc != TMNN_OK || args->rows == 0) return rc;
+    TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
+    return host ? distill_host(h, *args, back) : distill_device(h, *args, back, stream_of(h, stream));
+  });
+}
+
+}  // namespace
+
+extern "C" {
+
+int tmnn_logits_create(tmnn_context *ctx, tmnn_logits **out) {
+  if (!out) return fail(TMNN_ERR_INVALID_ARGUMENT, "out is null");
+  *out = nullptr;
+  if (!ctx) return fail(TMNN_ERR_INVALID_ARGUMENT, "context is null");
+  TMNN_HIP_TRY(hipSetDevice(ctx->device));
+  std::unique_ptr<tmnn_logits> h(new (std::nothrow) tmnn_logits());
+  if (!h) return fail(TMNN_ERR_RUNTIME, "out of host memory");
+  h->ctx = ctx;
+  TMNN_HIP_TRY(h->work.ensure(kSumBytes + kKeyBytes + kListBytes));
+  TMNN_HIP_TRY(hipEventCreateWithFlags(&h->moved, hipEventDisableTiming));
+  *out = h.release();
+  return TMNN_OK;
+}
+
+int tmnn_logits_destroy(tmnn_logits *h) {
+  if (!h) return TMNN_OK;
+  (void)hipSetDevice(h->ctx->device);
+  if (h->used && hipStreamSynchronize(h->last) != hipSuccess) (void)hipGetLastError();
+  if (h->moved) (void)hipEventDestroy(h->moved);
+  delete h;
+  return TMNN_OK;
+}
+
+int tmnn_token_logprobs(tmnn_logits *h, const tmnn_token_logprobs_args *args) {
+  return token_logprobs(h, args, false, true, nullptr);
+}
+int tmnn_token_logprobs_device(tmnn_logits *h, const tmnn_token_logprobs_args *args, void *stream) {
+  return token_logprobs(h, args, false, false, stream);
+}
+int tmnn_token_logprobs_backward(tmnn_logits *h, const tmnn_token_logprobs_args *args) {
+  return token_logprobs(h, args, true, true, nullptr);
+}
+int tmnn_token_logprobs_backward_device(tmnn_logits *h, const tmnn_token_logprobs_args *args,
+                                        void *stream) {
+  return token_logprobs(h, args, true, false, stream);
+}
+int tmnn_distill(tmnn_logits *h, const tmnn_distill_args *args) {
+  return distill(h, args, false, true, nullptr);
+}
+int tmnn_distill_device(tmnn_logits *h, const tmnn_distill_args *args, void *stream) {
+  return distill(h, args, false, false, stream);
+}
+int tmnn_distill_backward(tmnn_logits *h, const tmnn_distill_args *args) {
+  return distill(h, args, true, true, nullptr);
+}
+int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, void *stream) {
+  return distill(h, args, true, false, stream);
+}
+
+}  // extern "C"

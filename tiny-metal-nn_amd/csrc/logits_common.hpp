@@ -1,0 +1,392 @@
+// logits_common.hpp -- what the class-logit kernels share: typed vector
+// access to rows of any alignment, sums over lanes, the online softmax and the
+// selection of the k largest keys of a block.
+//
+// A row of logits z with scale c = log2(e) / T is summed up as (m, S, E):
+//   m = max z,  S = sum 2^(c (z - m)),  E = sum 2^(c (z - m)) c (z - m)
+// in one pass. Inside the pass the exponent is one fma, x = z c - R with
+// R = fl(m c); at its end rho = m c - R (exact) takes the rounding of R out
+// again, so that S belongs to m itself and not to R. A finished sum also has
+// r = S - 1, the sum without the maximum's own term, to the precision of a sum that
+// never met that 1: the logarithm of a probability near 1 is -ln(1 + r).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace tmnn_hip {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNoShift = -1e37f;   // R of a sum without terms; every other R is larger
+constexpr float kPlainShift = 1e30f; // |m c| up to which z c - R cannot overflow
+constexpr int kWave = 64;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+
+// 16 bytes of a row at a time, at the alignment of one element: the hardware
+// takes unaligned global vectors, so rows of odd strides need no other path.
+template <class T>
+struct Row;
+
+template <>
+struct Row<float> {
+  static constexpr int n = 4;
+  typedef f32x4v V __attribute__((aligned(4)));
+  static __device__ __forceinline__ float up(float x) { return x; }
+  static __device__ __forceinline__ float down(float x) { return x; }
+};
+template <>
+struct Row<_Float16> {
+  static constexpr int n = 8;
+  typedef f16x8v V __attribute__((aligned(2)));
+  static __device__ __forceinline__ float up(_Float16 x) { return static_cast<float>(x); }
+  static __device__ __forceinline__ _Float16 down(float x) { return static_cast<_Float16>(x); }
+};
+template <>
+struct Row<__bf16> {
+  static constexpr int n = 8;
+  typedef bf16x8v V __attribute__((aligned(2)));
+  static __device__ __forceinline__ float up(__bf16 x) { return static_cast<float>(x); }
+  static __device__ __forceinline__ __bf16 down(float x) { return static_cast<__bf16>(x); }
+};
+
+template <class T>
+__device__ __forceinline__ typename Row<T>::V load_raw(const T *p) {
+  return *reinterpret_cast<const typename Row<T>::V *>(p);
+}
+
+template <class T>
+__device__ __forceinline__ void widen(const typename Row<T>::V &v, float *out) {
+#pragma unroll
+  for (int j = 0; j < Row<T>::n; ++j) out[j] = Row<T>::up(v[j]);
+}
+
+// Elements i .. i + n of a row that ends at `end`; -inf past the end.
+template <class T>
+__device__ __forceinline__ void load_vec(const T *row, int i, int end, float *out) {
+  if (i + Row<T>::n <= end) {
+    widen<T>(load_raw(row + i), out);
+  } else {
+#pragma unroll
+    for (int j = 0; j < Row<T>::n; ++j)
+      out[j] = i + j < end ? Row<T>::up(row[i + j]) : -__builtin_inff();
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store_vec(T *row, int i, int end, const float *v) {
+  if (i + Row<T>::n <= end) {
+    typename Row<T>::V o;
+#pragma unroll
+    for (int j = 0; j < Row<T>::n; ++j) o[j] = Row<T>::down(v[j]);
+    *reinterpret_cast<typename Row<T>::V *>(row + i) = o;
+  } else {
+#pragma unroll
+    for (int j = 0; j < Row<T>::n; ++j)
+      if (i + j < end) row[i + j] = Row<T>::down(v[j]);
+  }
+}
+
+__device__ __forceinline__ int64_t load_index(const void *p, int64_t i, bool wide) {
+  return wide ? static_cast<const int64_t *>(p)[i]
+              : static_cast<int64_t>(static_cast<const int32_t *>(p)[i]);
+}
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---- sums over G consecutive lanes (all lanes get the result) ----------------
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  const int v = __float_as_int(x);
+  return __int_as_float(__builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false));
+}
+
+// Lanes 1, 2, 4, 8 apart by DPP (quad permutations, then the mirror of 8 and of
+// 16 lanes, whose quads already agree), 16 and 32 apart through the LDS
+// crossbar. Both partners add the same two numbers: every lane ends with the
+// same bits.
+template <int G, class Op>
+__device__ __forceinline__ float over_lanes(float x, Op op) {
+  if (G >= 2) x = op(x, dpp<0xB1>(x));
+  if (G >= 4) x = op(x, dpp<0x4E>(x));
+  if (G >= 8) x = op(x, dpp<0x141>(x));
+  if (G >= 16) x = op(x, dpp<0x140>(x));
+  if (G >= 32)
+    x = op(x, __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), 0x401F)));
+  if (G >= 64) x = op(x, __shfl_xor(x, 32));
+  return x;
+}
+template <int G>
+__device__ __forceinline__ float lanes_max(float x) {
+  return over_lanes<G>(x, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int G>
+__device__ __forceinline__ float lanes_sum(float x) {
+  return over_lanes<G>(x, [](float a, float b) { return a + b; });
+}
+template <int G>
+__device__ __forceinline__ double lanes_sum(double x) {
+  for (int off = 1; off < G; off *= 2) x += __shfl_xor(x, off, kWave);
+  return x;
+}
+template <int G>
+__device__ __forceinline__ int lanes_isum(int x) {
+  return __float_as_int(over_lanes<G>(__int_as_float(x), [](float a, float b) {
+    return __int_as_float(__float_as_int(a) + __float_as_int(b));
+  }));
+}
+template <int G>
+__device__ __forceinline__ uint64_t lanes_key_max(uint64_t k) {
+  for (int off = G / 2; off > 0; off >>= 1) {
+    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(k), off, kWave);
+    k = o > k ? o : k;
+  }
+  return k;
+}
+
+// Orders the LDS accesses of one wave's lanes (lockstep: a compiler fence).
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// ---- the online softmax -------------------------------------------------------
+
+struct Soft {
+  float m = -__builtin_inff();
+  float R = kNoShift;
+  float S = 0.0f;
+  float E = 0.0f;
+  float r = -1.0f;  // of a finished sum: S - 1
+};
+
+// Below this, S - 1 of an fp32 sum has lost too many bits.
+constexpr float kPeaked = 1.125f;
+
+// Takes the terms z[0..N) into a running sum. A new maximum rescales the sum,
+// which happens about ln(length) times a thread. Masked terms (-inf) add 0: their
+// exponent is held at -200 where it is multiplied. NaN terms make S NaN.
+template <int N, bool ENT>
+__device__ __forceinline__ void soft_add(Soft &s, const float *z, float zmax, float c) {
+  if (zmax > s.m) {
+    const float R = fmaxf(zmax * c, kNoShift);
+    const float d = s.R - R, r = exp2_raw(d);
+    if (ENT) s.E = r * __builtin_fmaf(s.S, d, s.E);
+    s.S *= r;
+    s.m = zmax;
+    s.R = R;
+  }
+  float e[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float x = __builtin_fmaf(z[j], c, -s.R);
+    e[j] = exp2_raw(x);
+    if (ENT) s.E = __builtin_fmaf(e[j], fmaxf(x, -200.0f), s.E);
+  }
+#pragma unroll
+  for (int w = 1; w < N; w *= 2)
+#pragma unroll
+    for (int j = 0; j + w < N; j += 2 * w) e[j] += e[j + w];
+  s.S += e[0];
+}
+
+// The sum over G lanes, in the lanes' common shift.
+template <int G, bool ENT>
+__device__ __forceinline__ void soft_lanes(Soft &s) {
+  const float R = lanes_max<G>(s.R), d = s.R - R, r = exp2_raw(d);
+  if (ENT) s.E = lanes_sum<G>(r * __builtin_fmaf(s.S, d, s.E));
+  s.S = lanes_sum<G>(s.S * r);
+  s.R = R;
+  s.m = lanes_max<G>(s.m);
+}
+
+// m c is too large for the fma form, or not a number that can be a shift.
+__device__ __forceinline__ bool soft_is_huge(float m, float c) {
+  return !(fabsf(m * c) <= kPlainShift) && m != -__builtin_inff();
+}
+
+// Takes the rounding of R out of S and E (see the head of the file).
+__device__ __forceinline__ void soft_settle(Soft &s, float c) {
+  if (s.m != -__builtin_inff()) {  // else no terms; S is 0, or NaN from NaN terms
+    const float rho = __builtin_fmaf(s.m, c, -s.R), f = exp2f(-rho);
+    s.E = f * __builtin_fmaf(s.S, -rho, s.E);
+    s.S *= f;
+  }
+  s.r = s.S - 1.0f;
+}
+
+// Finished sums: S and E of `b` in the shift of m >= b.m.
+__device__ __forceinline__ void soft_shift(Soft &b, float m, float c) {
+  if (b.S == 0.0f) {
+    b.E = 0.0f;
+    return;
+  }
+  const float d = (b.m - m) * c, r = exp2_raw(d);
+  b.E = r == 0.0f ? 0.0f : r * __builtin_fmaf(b.S, d, b.E);
+  b.S *= r;
+}
+
+// Adds a finished sum `b` to `s`, whose m is the largest of all that will be added.
+// The first sum that attains m brings the 1 that r leaves out (`first`).
+__device__ __forceinline__ void soft_join(Soft &s, Soft b, float c, bool &first) {
+  const bool one = b.m == s.m && first && b.m != -__builtin_inff();
+  const float r = b.r;
+  soft_shift(b, s.m, c);
+  s.r += one ? r : b.S;
+  s.E += b.E;
+  if (one) first = false;
+}
+
+// 2^(c (z - m)) as the gradients need it: the same fma form with the rounding of
+// R in a factor of its own, or, for huge m, the difference first.
+struct ExpAt {
+  float c, R, m, fix;
+  bool huge;
+  __device__ __forceinline__ ExpAt(float m_, float c_) : c(c_), m(m_) {
+    huge = soft_is_huge(m, c);
+    R = m * c;
+    fix = huge ? 1.0f : exp2f(-__builtin_fmaf(m, c, -R));
+  }
+  __device__ __forceinline__ float x_plain(float z) const { return __builtin_fmaf(z, c, -R); }
+  __device__ __forceinline__ float x_huge(float z) const { return (z - m) * c; }
+  // c (z - m), once a row or class rather than in the dense loops
+  __device__ __forceinline__ float x(float z) const { return (z - m) * c; }
+};
+
+// ---- order of classes: by value, then by the lowest index -------------------------
+
+__device__ __forceinline__ uint32_t order_of(float z) {
+  const uint32_t b = __float_as_uint(z + 0.0f);  // -0 and +0 are equal
+  return b ^ (static_cast<int32_t>(b) < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return __uint_as_float(o ^ (o & 0x80000000u ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t key_of(float z, int i) {
+  return static_cast<uint64_t>(order_of(z)) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
+}
+__device__ __forceinline__ int key_index(uint64_t k) {
+  return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
+}
+// The smallest float above z (z finite or -inf).
+__device__ __forceinline__ float next_above(float z) {
+  const int32_t b = __float_as_int(z + 0.0f);
+  return __int_as_float(b >= 0 ? b + 1 : b - 1);
+}
+
+// ---- the k largest keys of a block ---------------------------------------------
+
+constexpr int kCandidates = 1024;
+
+template <int NT>
+struct SelectLds {
+  uint64_t key[NT];
+  uint64_t cand[kCandidates];
+  uint64_t tau;
+  int count;
+};
+
+// A key that at least k of the NT thread keys reach, as high as its search
+// finds: bit by bit over the values, then over the indices of an equal value,
+// ending as soon as exactly k keys reach it. Run by one wave.
+template <int NT>
+__device__ __forceinline__ uint64_t kth_key(const uint64_t *key, int k) {
+  constexpr int W = NT / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  uint32_t hi[W], lo[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const uint64_t q = key[lane + kWave * i];
+    hi[i] = static_cast<uint32_t>(q >> 32);
+    lo[i] = static_cast<uint32_t>(q);
+  }
+  uint32_t p = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = p | 1u << b;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) n += __popcll(__ballot(hi[i] >= t));
+    if (n >= k) p = t;
+    if (n == k) return static_cast<uint64_t>(p) << 32;
+  }
+  int above = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) above += __popcll(__ballot(hi[i] > p));
+  uint32_t q = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = q | 1u << b;
+    int n = above;
+#pragma unroll
+    for (int i = 0; i < W; ++i) n += __popcll(__ballot(hi[i] == p && lo[i] >= t));
+    if (n >= k) q = t;
+    if (n == k) break;
+  }
+  return static_cast<uint64_t>(p) << 32 | q;
+}
+
+// The k largest keys of the block's elements, in order, to put(j, key) for j up
+// to the returned count (fewer than k where the block has fewer). `mine` is a key
+// that one of the thread's elements reaches (0: it has none) and whose high word
+// no element of the thread exceeds. scan(f) calls f(key) for each
+// of the thread's elements. No element costs anything beyond the running maximum
+// of the first pass: the k-th largest of the threads' maxima bounds the answer from
+// below, and only the threads that reach it look at their elements again. Where
+// more than kCandidates elements reach that bound, the bound is made exact by counting.
+template <int NT, class Scan, class Put>
+__device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int k, Scan scan,
+                                            Put put) {
+  const int tid = threadIdx.x;
+  s.key[tid] = mine;
+  if (tid == 0) s.count = 0;
+  __syncthreads();
+  if (tid < kWave) {
+    const uint64_t t = kth_key<NT>(s.key, k);
+    if (tid == 0) s.tau = t;
+  }
+  __syncthreads();
+  uint64_t tau = s.tau;
+  auto gather = [&](uint64_t q) {
+    if (q >= tau) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kCandidates) s.cand[at] = q;
+    }
+  };
+  if (mine != 0 && (mine | 0xffffffffu) >= tau) scan(gather);
+  __syncthreads();
+  int n = s.count;
+  if (n > kCandidates) {
+    uint64_t t = 0;
+    for (int b = 63; b >= 0; --b) {
+      const uint64_t test = t | 1ull << b;
+      __syncthreads();
+      if (tid == 0) s.count = 0;
+      __syncthreads();
+      int c = 0;
+      if (mine != 0 && (mine | 0xffffffffu) >= test) scan([&](uint64_t q) { c += q >= test; });
+      if (c) atomicAdd(&s.count, c);
+      __syncthreads();
+      if (s.count >= k) t = test;
+    }
+    __syncthreads();
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    tau = t;
+    if (mine != 0 && (mine | 0xffffffffu) >= tau) scan(gather);
+    __syncthreads();
+    n = s.count;
+  }
+  // the place of a candidate is the number of larger ones
+  for (int i = tid; i < n; i += NT) {
+    const uint64_t q = s.cand[i];
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += s.cand[j] > q;
+    if (place < k) put(place, q);
+  }
+  return n < k ? n : k;
+}
+
+}  // namespace tmnn_hip

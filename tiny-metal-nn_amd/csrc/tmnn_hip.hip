@@ -24,6 +24,7 @@
 
 #include "tmnn_hip.h"
 #include "aux_kernels.hpp"
+#include "context.hpp"
 #include "encode_kernel.hpp"
 #include "field_kernel.hpp"
 #include "grad_kernel.hpp"
@@ -72,18 +73,6 @@ struct ScratchDevice {
 };
 std::mutex g_scratch_mu;
 std::vector<ScratchDevice> g_scratch;
-
-int fail(int code, const std::string &msg) {
-  g_last_error = msg;
-  return code;
-}
-
-#define TMNN_HIP_TRY(expr)                                                   \
-  do {                                                                       \
-    hipError_t e_ = (expr);                                                  \
-    if (e_ != hipSuccess)                                                    \
-      return fail(TMNN_ERR_GPU, std::string(#expr) + ": " + hipGetErrorString(e_)); \
-  } while (0)
 
 // "%.6f" baked constants (mlp_kernel_emitter.cpp:91-92), read back as float.
 float baked6(float v) {
@@ -217,38 +206,6 @@ KernelChoice select_kernel(int HP, int INP, bool f16, bool train, int D, int F, 
   return {};
 }
 
-struct DevBuf {
-  void *ptr = nullptr;
-  size_t bytes = 0;
-  bool borrowed = false;  // ptr is a region of the device scratch (never freed or grown)
-  DevBuf() = default;
-  DevBuf(const DevBuf &) = delete;
-  DevBuf &operator=(const DevBuf &) = delete;
-  ~DevBuf() {
-    if (ptr && !borrowed) (void)hipFree(ptr);
-  }
-  hipError_t ensure(size_t want) {
-    if (want <= bytes) return hipSuccess;
-    if (borrowed) return hipErrorInvalidValue;  // a scratch region never grows
-    if (ptr) {
-      (void)hipFree(ptr);
-      ptr = nullptr;
-      bytes = 0;
-    }
-    const size_t rounded = (want + 255) / 256 * 256;
-    hipError_t e = hipMalloc(&ptr, rounded);
-    if (e == hipSuccess)
-      bytes = rounded;
-    else
-      (void)hipGetLastError();  // returned here; the next launch's check must not find it
-    return e;
-  }
-  template <class T>
-  T *as() const {
-    return static_cast<T *>(ptr);
-  }
-};
-
 struct KernelPlan {
   FieldKernel fn = nullptr;
   bool f16 = false, train = false;
@@ -269,20 +226,6 @@ struct KernelPlan {
 };
 
 }  // namespace
-
-struct tmnn_context {
-  int device = 0;
-  hipStream_t stream = nullptr;
-  int cu_count = 0;
-  uint64_t mem_bytes = 0;
-  std::string name;
-  unsigned char *scratch = nullptr;  // this device's copy of the step scratch (device address)
-  // Pinned host memory of the host-pointer calls whose arrays fit (stage_in /
-  // stage_out): inputs, then outputs, then the step's loss (kStageTotal
-  // bytes, freed with the context). One call at a time holds it (StageLease).
-  unsigned char *stage = nullptr;
-  std::mutex stage_mu;
-};
 
 struct tmnn_trainer {
   tmnn_context *ctx = nullptr;
@@ -2160,6 +2103,11 @@ int host_training_step(tmnn_trainer *tr, const float *input, const float *target
 }
 
 }  // namespace
+
+int tmnn_hip::fail(int code, const std::string &msg) {
+  g_last_error = msg;
+  return code;
+}
 
 extern "C" {
 

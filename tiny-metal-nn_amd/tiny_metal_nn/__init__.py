@@ -8,6 +8,7 @@ Same module name and Trainer surface as the reference's Python package
 from __future__ import annotations
 
 from .config import ConfigError, canonicalize_model_config
+from .logits import LogitOps
 from .trainer import (ClosedError, ConcurrentTrainingStepError, DTypeError,
                       OptimizerStateBlob, Trainer, philox_uniform, plan_network)
 
@@ -18,6 +19,7 @@ __all__ = [
     "ConcurrentTrainingStepError",
     "ConfigError",
     "DTypeError",
+    "LogitOps",
     "OptimizerStateBlob",
     "Trainer",
     "canonicalize_model_config",

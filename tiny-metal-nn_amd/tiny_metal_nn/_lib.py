@@ -227,6 +227,32 @@ class StoragePolicy(ctypes.Structure):
         "step_targets", "step_reduction", "requires_staging_uploads")]
 
 
+# TMNN_DTYPE_*, TMNN_INDEX_*, TMNN_TEACHER_* of the class-logit operators
+DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+INDEX_DTYPES = {"int32": 0, "int64": 1}
+TEACHER_KINDS = {"logits": 0, "logprobs": 1}
+LOGITS_MAX_CLASSES, LOGITS_MAX_TOP, LOGITS_MAX_TEACHER = 1 << 24, 128, 256
+
+
+class TokenLogprobsArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(k, ctypes.c_int32) for k in (
+        "dtype", "index_dtype", "top_k")] + [(k, ctypes.c_int64) for k in (
+            "rows", "classes", "row_stride", "d_row_stride")] + [
+        (k, ctypes.c_void_p) for k in (
+            "logits", "tokens", "logprob", "entropy", "rank", "stats", "top_ids", "top_logprobs",
+            "d_logprob", "d_entropy", "d_top_logprobs", "d_logits")] + [
+        ("temperature", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class DistillArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(k, ctypes.c_int32) for k in (
+        "dtype", "index_dtype", "teacher_kind")] + [(k, ctypes.c_int64) for k in (
+            "rows", "classes", "row_stride", "d_row_stride")] + [
+        (k, ctypes.c_void_p) for k in (
+            "logits", "teacher_ids", "teacher", "row_weights", "loss", "stats", "d_logits")] + [
+        ("teacher_k", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
 _V = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _U32 = ctypes.c_uint32
@@ -297,6 +323,17 @@ SIGNATURES = {
     "tmnn_debug_morton_sort": (ctypes.c_int, [_V, _V, _I32, _V, _V]),
     "tmnn_debug_get_resolutions": (ctypes.c_int, [_V, _V, _I32]),
     "tmnn_debug_train_image": (ctypes.c_int, [_V, _V, _V, ctypes.POINTER(ctypes.c_uint64)]),
+    "tmnn_logits_create": (ctypes.c_int, [_V, ctypes.POINTER(_V)]),
+    "tmnn_logits_destroy": (ctypes.c_int, [_V]),
+    # the arguments as the packed bytes of TokenLogprobsArgs / DistillArgs
+    "tmnn_token_logprobs": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_token_logprobs_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_token_logprobs_backward": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_token_logprobs_backward_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_distill": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_distill_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_distill_backward": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_distill_backward_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
     "tmnn_debug_philox_uniform": (ctypes.c_int, [_V, ctypes.c_uint64, _U32, _U32, _F, _F, _V]),
 }
 
