@@ -256,10 +256,9 @@ struct ListLds {
 };
 
 // The listed classes: -1 for unused entries and for classes listed before (the
-// first entry counts). An entry beyond the classes makes the row NaN.
+// first entry counts). An entry beyond the classes makes the row NaN. NT >= k.
 template <int NT>
 __device__ __forceinline__ int read_list(const DistillArgs &a, ListLds &l, int64_t row) {
-  static_assert(NT >= kMaxTeacher, "a thread for each listed class");
   const int tid = threadIdx.x;
   if (tid == 0) l.wrong = 0.0f;
   __syncthreads();
@@ -353,9 +352,9 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
       all.m = lanes_max<kWave>(all.m);
       const float shift = all.m == -__builtin_inff() ? 0.0f : all.m;
       // the 1 that r leaves out is the rest's, or of the first listed class that has it
-      bool first = true;
+      const bool first = dense.m != all.m || dense.m == -__builtin_inff();
       all.r = 0.0f;
-      soft_join(all, dense, a.c, first);
+      soft_join(all, dense, a.c, !first);
       float one = -1e9f, s = 0.0f;
       for (int j = tid; j < a.k; j += kWave)
         if (l.id[j] >= 0 && l.z[j] == all.m) one = fmaxf(one, -static_cast<float>(j));
@@ -411,7 +410,7 @@ __device__ __forceinline__ void distill_no_weight(const DistillArgs &a, int64_t 
 
 template <class T, int NT, bool TAIL>
 __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
-  constexpr int N = Row<T>::n, U = kLogitVecs;
+  constexpr int N = Row<T>::n;
   extern __shared__ uint32_t listed[];  // TAIL: a bit for each class of the part
   __shared__ BlockLds<NT> lds;
   __shared__ ListLds list;
@@ -447,31 +446,17 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
       if (bits >> j & 1u) v[j] = -__builtin_inff();
   };
   Soft s;
-  auto take = [&](int i, float(&v)[U][N]) {
+  scan_part<T, NT>(z, begin, end, [&](int at, auto &v) {
+    constexpr int W = sizeof(v) / sizeof(v[0]);
+    float cm = -__builtin_inff();
 #pragma unroll
-    for (int u = 0; u < U; ++u) hide(i + u * NT * N, v[u]);
-    float cm = v[0][0];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < W; ++u) {
+      hide(at + tid * N + u * NT * N, v[u]);
 #pragma unroll
       for (int j = 0; j < N; ++j) cm = fmaxf(cm, v[u][j]);
-    soft_add<U * N, false>(s, &v[0][0], cm, a.c);
-  };
-  int at = begin;
-  for (; at + NT * N * U <= end; at += NT * N * U) {
-    const int i = at + tid * N;
-    float v[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u) widen<T>(load_raw(z + i + u * NT * N), v[u]);
-    take(i, v);
-  }
-  if (at < end) {
-    const int i = at + tid * N;
-    float v[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load_vec<T>(z, i + u * NT * N, end, v[u]);
-    take(i, v);
-  }
+    }
+    soft_add<W * N, false>(s, &v[0][0], cm, a.c);
+  });
   int n = 0;
   s = soft_finish<T, NT, false>(lds, s, z, begin, end, a.c, n, hide);
   if (a.parts > 1) {
@@ -485,7 +470,6 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
 // Joins the sums of a row's parts (in their order), and finishes one part.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
-  __shared__ float2 sum[kMaxParts];
   __shared__ ListLds list;
   const int tid = threadIdx.x;
   const int blocks = a.d_logits ? a.parts : 1;
@@ -499,22 +483,16 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
     distill_no_weight<T, NT>(a, row, part, begin, end);
     return;
   }
-  for (int p = tid; p < a.parts; p += NT) sum[p] = a.part_sum[row * a.parts + p];
   const int id = read_list<NT>(a, list, row);
   const float zj = id >= 0 ? a.list_z[row * a.k + tid] : 0.0f;
-  Soft s;
-  for (int p = 0; p < a.parts; ++p) s.m = fmaxf(s.m, sum[p].x);
-  bool first = true;
-  s.r = 0.0f;
-  for (int p = 0; p < a.parts; ++p) {
+  int n = 0;
+  const Soft s = soft_join_parts(a.parts, a.c, n, [&](int p, int &) {
+    const float2 q = a.part_sum[row * a.parts + p];
     Soft b;
-    b.m = sum[p].x;
-    b.r = sum[p].y;
-    b.S = 1.0f + b.r;
-    soft_join(s, b, a.c, first);
-  }
-  if (s.m == -__builtin_inff()) s.r -= 1.0f;  // no class: S = 0 (or NaN)
-  s.S = 1.0f + s.r;
+    b.m = q.x;
+    b.r = q.y;
+    return b;
+  });
   distill_finish<T, NT>(a, list, row, part, z, begin, end, s, id, zj, w);
 }
 

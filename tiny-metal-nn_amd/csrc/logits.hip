@@ -103,7 +103,7 @@ int check_logprobs(const tmnn_token_logprobs_args *a, bool back) {
   return TMNN_OK;
 }
 
-int check_distill(const tmnn_distill_args *a, bool back) {
+int check_distill(const tmnn_distill_args *a, bool back, bool host) {
   const char *what = back ? "distill_backward" : "distill";
   auto bad = [&](const char *m) {
     return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
@@ -121,7 +121,7 @@ int check_distill(const tmnn_distill_args *a, bool back) {
     return bad("teacher_ids must be aligned to their type");
   if (!aligned(a->teacher, 4) || !aligned(a->row_weights, 4) || !aligned(a->loss, 4))
     return bad("arrays of 32-bit values must be 4-byte aligned");
-  if (!aligned(a->stats, 16)) return bad("stats must be 16-byte aligned");
+  if (!host && !aligned(a->stats, 16)) return bad("stats must be 16-byte aligned");
   if (back) {
     if (!a->d_logits) return bad("d_logits is null");
     if (!a->stats) return bad("stats is null");
@@ -168,7 +168,7 @@ struct Split {
 };
 
 // Threads of a block, and blocks of a row.
-Split split_of(int64_t rows, int64_t classes, int n, int min_threads, int64_t blocks) {
+Split split_of(int64_t rows, int64_t classes, int n, int at_least, int64_t blocks) {
   Split s;
   const int64_t vecs = (classes + n - 1) / n;
   int64_t parts = 1;
@@ -179,8 +179,9 @@ Split split_of(int64_t rows, int64_t classes, int n, int min_threads, int64_t bl
   if (parts > 1) len = (len + 255) / 256 * 256;
   s.part_len = static_cast<int>(len);
   s.parts = static_cast<int>((classes + len - 1) / len);
-  s.threads = len / n >= 4 * 1024 ? 1024 : len / n >= 4 * 512 ? 512 : 256;
-  s.threads = std::max(s.threads, min_threads);
+  const int64_t mine = len / n;
+  s.threads = mine >= 8192 ? 512 : mine >= 1024 ? 256 : mine >= 512 ? 128 : 64;
+  while (s.threads < at_least) s.threads *= 2;
   return s;
 }
 
@@ -215,6 +216,8 @@ dim3 group_grid(int rows, int g) {
   }
 #define TMNN_BY_THREADS(nt, CALL) \
   switch (nt) {                   \
+    case 64: CALL(64); break;     \
+    case 128: CALL(128); break;   \
     case 256: CALL(256); break;   \
     case 512: CALL(512); break;   \
     default: CALL(1024); break;   \
@@ -257,8 +260,7 @@ int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
 #undef CALL
     });
   }
-  // four threads to an alternative, so that the threads' maxima bound them well
-  const Split sp = split_of(rows, a.classes, n, a.top_k > 64 ? 512 : 256, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, 2 * a.top_k, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   a.part_sum = static_cast<float4 *>(h->work.ptr);
@@ -293,7 +295,7 @@ int run_logprobs_grad(LogprobArgs a, int64_t rows, hipStream_t st) {
 #undef CALL
     });
   }
-  const Split sp = split_of(rows, a.classes, n, 256, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, a.d_top ? a.top_k + 1 : 1, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1, [&](int64_t at, int32_t r) {
@@ -336,7 +338,7 @@ int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStrea
 #undef CALL
     });
   }
-  const Split sp = split_of(rows, a.classes, n, 256, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, a.k, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   if (back)
@@ -582,7 +584,7 @@ int token_logprobs(tmnn_logits *h, const tmnn_token_logprobs_args *args, bool ba
 
 int distill(tmnn_logits *h, const tmnn_distill_args *args, bool back, bool host, void *stream) {
   return entry(h, [&] {
-    const int rc = check_distill(args, back);
+    const int rc = check_distill(args, back, host);
     if (rc != TMNN_OK || args->rows == 0) return rc;
     TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
     return host ? distill_host(h, *args, back) : distill_device(h, *args, back, stream_of(h, stream));

@@ -106,18 +106,25 @@ __device__ __forceinline__ float dpp(float x) {
 }
 
 // Lanes 1, 2, 4, 8 apart by DPP (quad permutations, then the mirror of 8 and of
-// 16 lanes, whose quads already agree), 16 and 32 apart through the LDS
-// crossbar. Both partners add the same two numbers: every lane ends with the
-// same bits.
+// 16 lanes, whose quads already agree), 16 and 32 apart by swapping rows and halves
+// of two copies. Both partners combine the same two numbers: every lane ends with
+// the same bits.
 template <int G, class Op>
 __device__ __forceinline__ float over_lanes(float x, Op op) {
   if (G >= 2) x = op(x, dpp<0xB1>(x));
   if (G >= 4) x = op(x, dpp<0x4E>(x));
   if (G >= 8) x = op(x, dpp<0x141>(x));
   if (G >= 16) x = op(x, dpp<0x140>(x));
-  if (G >= 32)
-    x = op(x, __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), 0x401F)));
-  if (G >= 64) x = op(x, __shfl_xor(x, 32));
+  if (G >= 32) {
+    const uint32_t v = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  if (G >= 64) {
+    const uint32_t v = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
   return x;
 }
 template <int G>
@@ -196,12 +203,12 @@ __device__ __forceinline__ void soft_add(Soft &s, const float *z, float zmax, fl
 
 // The sum over G lanes, in the lanes' common shift.
 template <int G, bool ENT>
-__device__ __forceinline__ void soft_lanes(Soft &s) {
-  const float R = lanes_max<G>(s.R), d = s.R - R, r = exp2_raw(d);
+__device__ __forceinline__ void soft_lanes(Soft &s, float c) {
+  s.m = lanes_max<G>(s.m);
+  const float R = fmaxf(s.m * c, kNoShift), d = s.R - R, r = exp2_raw(d);
   if (ENT) s.E = lanes_sum<G>(r * __builtin_fmaf(s.S, d, s.E));
   s.S = lanes_sum<G>(s.S * r);
   s.R = R;
-  s.m = lanes_max<G>(s.m);
 }
 
 // m c is too large for the fma form, or not a number that can be a shift.
@@ -231,14 +238,41 @@ __device__ __forceinline__ void soft_shift(Soft &b, float m, float c) {
 }
 
 // Adds a finished sum `b` to `s`, whose m is the largest of all that will be added.
-// The first sum that attains m brings the 1 that r leaves out (`first`).
-__device__ __forceinline__ void soft_join(Soft &s, Soft b, float c, bool &first) {
-  const bool one = b.m == s.m && first && b.m != -__builtin_inff();
+// `one`: b is the first sum that attains m, which brings the 1 that r leaves out.
+__device__ __forceinline__ void soft_join(Soft &s, Soft b, float c, bool one) {
   const float r = b.r;
   soft_shift(b, s.m, c);
   s.r += one ? r : b.S;
   s.E += b.E;
-  if (one) first = false;
+}
+
+// Joins up to 128 finished sums, load(p) the p-th, in every lane of a wave: a fixed
+// tree. `n` adds up each sum's n.
+template <class Load>
+__device__ __forceinline__ Soft soft_join_parts(int parts, float c, int &n, Load load) {
+  const int lane = threadIdx.x & (kWave - 1);
+  Soft b[2], s;
+  int k[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + kWave * i < parts) b[i] = load(lane + kWave * i, k[i]);
+  s.m = lanes_max<kWave>(fmaxf(b[0].m, b[1].m));
+  s.r = 0.0f;
+  const float inf = __builtin_inff();
+  const uint64_t low = __ballot(b[0].m == s.m && s.m != -inf);
+  const uint64_t high = __ballot(b[1].m == s.m && s.m != -inf);
+  const int first = low ? __builtin_ctzll(low) : high ? kWave + __builtin_ctzll(high) : -1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    b[i].S = 1.0f + b[i].r;
+    soft_join(s, b[i], c, lane + kWave * i == first);
+  }
+  s.r = lanes_sum<kWave>(s.r);
+  s.E = lanes_sum<kWave>(s.E);
+  n = lanes_isum<kWave>(k[0] + k[1]);
+  if (s.m == -inf) s.r -= 1.0f;  // no class: S = 0 (or NaN)
+  s.S = 1.0f + s.r;
+  return s;
 }
 
 // 2^(c (z - m)) as the gradients need it: the same fma form with the rounding of
@@ -281,33 +315,56 @@ __device__ __forceinline__ float next_above(float z) {
 // ---- the k largest keys of a block ---------------------------------------------
 
 constexpr int kCandidates = 1024;
+// The threads' keys in groups: 256, or one a thread (at least k either way).
+constexpr int key_groups(int threads) { return threads < 256 ? threads : 256; }
 
 template <int NT>
 struct SelectLds {
   uint64_t key[NT];
   uint64_t cand[kCandidates];
   uint64_t tau;
-  int count;
+  int count, threads;
+  uint16_t thread[NT];
 };
 
-// A key that at least k of the NT thread keys reach, as high as its search
-// finds: bit by bit over the values, then over the indices of an equal value,
-// ending as soon as exactly k keys reach it. Run by one wave.
+// A key that at least k of the groups' keys reach (the largest of their
+// threads'), as high as its search finds: bit by bit below the bits
+// that all keys share, then over the indices of an equal value, ending as soon
+// as exactly k keys reach it. 0 where fewer than k groups have a key. Run by one wave.
 template <int NT>
 __device__ __forceinline__ uint64_t kth_key(const uint64_t *key, int k) {
-  constexpr int W = NT / kWave;
+  constexpr int groups = key_groups(NT), W = groups / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   uint32_t hi[W], lo[W];
+  uint32_t lowest = 0xffffffffu, highest = 0;
+  int n = 0;
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const uint64_t q = key[lane + kWave * i];
+    uint64_t q = key[lane + kWave * i];
+#pragma unroll
+    for (int t = 1; t < NT / groups; ++t) {
+      const uint64_t o = key[lane + kWave * i + groups * t];
+      q = o > q ? o : q;
+    }
     hi[i] = static_cast<uint32_t>(q >> 32);
     lo[i] = static_cast<uint32_t>(q);
+    n += __popcll(__ballot(hi[i] != 0));
+    if (hi[i] != 0) lowest = hi[i] < lowest ? hi[i] : lowest;
+    highest = hi[i] > highest ? hi[i] : highest;
   }
-  uint32_t p = 0;
-  for (int b = 31; b >= 0; --b) {
+  if (n < k) return 0;
+  for (int off = 1; off < kWave; off *= 2) {
+    const uint32_t a = __shfl_xor(lowest, off), b = __shfl_xor(highest, off);
+    lowest = a < lowest ? a : lowest;
+    highest = b > highest ? b : highest;
+  }
+  lowest = __builtin_amdgcn_readfirstlane(lowest);
+  highest = __builtin_amdgcn_readfirstlane(highest);
+  int b = lowest == highest ? -1 : 31 - __builtin_clz(lowest ^ highest);
+  uint32_t p = b < 0 ? highest : b == 31 ? 0u : highest & ~((2u << b) - 1u);
+  for (; b >= 0; --b) {
     const uint32_t t = p | 1u << b;
-    int n = 0;
+    n = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) n += __popcll(__ballot(hi[i] >= t));
     if (n >= k) p = t;
@@ -317,9 +374,9 @@ __device__ __forceinline__ uint64_t kth_key(const uint64_t *key, int k) {
 #pragma unroll
   for (int i = 0; i < W; ++i) above += __popcll(__ballot(hi[i] > p));
   uint32_t q = 0;
-  for (int b = 31; b >= 0; --b) {
+  for (b = 31; b >= 0; --b) {
     const uint32_t t = q | 1u << b;
-    int n = above;
+    n = above;
 #pragma unroll
     for (int i = 0; i < W; ++i) n += __popcll(__ballot(hi[i] == p && lo[i] >= t));
     if (n >= k) q = t;
@@ -329,19 +386,25 @@ __device__ __forceinline__ uint64_t kth_key(const uint64_t *key, int k) {
 }
 
 // The k largest keys of the block's elements, in order, to put(j, key) for j up
-// to the returned count (fewer than k where the block has fewer). `mine` is a key
-// that one of the thread's elements reaches (0: it has none) and whose high word
-// no element of the thread exceeds. scan(f) calls f(key) for each
-// of the thread's elements. No element costs anything beyond the running maximum
-// of the first pass: the k-th largest of the threads' maxima bounds the answer from
-// below, and only the threads that reach it look at their elements again. Where
-// more than kCandidates elements reach that bound, the bound is made exact by counting.
-template <int NT, class Scan, class Put>
-__device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int k, Scan scan,
-                                            Put put) {
+// to the returned count (fewer than k where the block has fewer). Every thread owns
+// `vectors` groups of elements; visit(thread, i, f) calls f(key) for those of a
+// thread's i-th. `mine` is a key that one of the thread's elements reaches (0: it
+// has none) and whose high word none of them exceeds.
+//
+// No element costs anything beyond the running maximum of the first pass: the k-th
+// largest of the groups' maxima bounds the answer from below, and the block looks
+// again only at the elements of the threads that reach it (about k threads, and about
+// k (1 + k / 512) elements that reach it, in no special order). Where more
+// than kCandidates elements do, the bound is made exact by counting.
+template <int NT, class Visit, class Put>
+__device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int k, int vectors,
+                                            Visit visit, Put put) {
   const int tid = threadIdx.x;
   s.key[tid] = mine;
-  if (tid == 0) s.count = 0;
+  if (tid == 0) {
+    s.count = 0;
+    s.threads = 0;
+  }
   __syncthreads();
   if (tid < kWave) {
     const uint64_t t = kth_key<NT>(s.key, k);
@@ -355,10 +418,17 @@ __device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int
       if (at < kCandidates) s.cand[at] = q;
     }
   };
-  if (mine != 0 && (mine | 0xffffffffu) >= tau) scan(gather);
+  if (mine != 0 && (mine | 0xffffffffu) >= tau) s.thread[atomicAdd(&s.threads, 1)] = tid;
+  __syncthreads();
+  const int threads = s.threads;
+  for (int i = tid; i < threads * vectors; i += NT) visit(s.thread[i % threads], i / threads, gather);
   __syncthreads();
   int n = s.count;
   if (n > kCandidates) {
+    auto all_mine = [&](auto f) {
+      if (mine != 0)
+        for (int i = 0; i < vectors; ++i) visit(tid, i, f);
+    };
     uint64_t t = 0;
     for (int b = 63; b >= 0; --b) {
       const uint64_t test = t | 1ull << b;
@@ -366,7 +436,7 @@ __device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int
       if (tid == 0) s.count = 0;
       __syncthreads();
       int c = 0;
-      if (mine != 0 && (mine | 0xffffffffu) >= test) scan([&](uint64_t q) { c += q >= test; });
+      all_mine([&](uint64_t q) { c += q >= test; });
       if (c) atomicAdd(&s.count, c);
       __syncthreads();
       if (s.count >= k) t = test;
@@ -375,7 +445,7 @@ __device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int
     if (tid == 0) s.count = 0;
     __syncthreads();
     tau = t;
-    if (mine != 0 && (mine | 0xffffffffu) >= tau) scan(gather);
+    all_mine(gather);
     __syncthreads();
     n = s.count;
   }

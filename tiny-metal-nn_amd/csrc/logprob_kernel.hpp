@@ -155,10 +155,10 @@ struct BlockLds {
 
 // The block's sum from its threads', in every thread, and the total of `n`.
 template <int NT, bool ENT>
-__device__ __forceinline__ Soft soft_block(BlockLds<NT> &l, Soft s, int &n) {
+__device__ __forceinline__ Soft soft_block(BlockLds<NT> &l, Soft s, float c, int &n) {
   constexpr int W = NT / kWave;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  soft_lanes<kWave, ENT>(s);
+  soft_lanes<kWave, ENT>(s, c);
   n = lanes_isum<kWave>(n);
   if (W == 1) return s;
   if (lane == 0) {
@@ -176,18 +176,51 @@ __device__ __forceinline__ Soft soft_block(BlockLds<NT> &l, Soft s, int &n) {
   o.S = l.S[i];
   o.E = l.E[i];
   n = lanes_isum<W>(l.n[i]);
-  soft_lanes<W, ENT>(o);
+  soft_lanes<W, ENT>(o, c);
   return o;
+}
+
+// Calls take(at, v) for the classes begin .. end of a row: v[W][N] are W vectors of
+// the thread, NT N classes apart, the block's first at `at`. U vectors are in flight;
+// what does not fill them is loaded at once too, and taken one by one.
+template <class T, int NT, class Take>
+__device__ __forceinline__ void scan_part(const T *z, int begin, int end, Take take) {
+  constexpr int N = Row<T>::n, U = kLogitVecs;
+  const int mine = static_cast<int>(threadIdx.x) * N;
+  int at = begin;
+  for (; at + NT * N * U <= end; at += NT * N * U) {
+    float v[U][N];
+#pragma unroll
+    for (int u = 0; u < U; ++u) widen<T>(load_raw(z + at + mine + u * NT * N), v[u]);
+    take(at, v);
+  }
+  if (at >= end) return;
+  float v[U][1][N];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (at + u * NT * N < end) load_vec<T>(z, at + mine + u * NT * N, end, v[u][0]);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (at + u * NT * N < end) take(at + u * NT * N, v[u]);
+}
+
+// The block's sum of x, in every thread.
+template <int NT>
+__device__ __forceinline__ float block_sum(BlockLds<NT> &l, float x) {
+  x = lanes_sum<kWave>(x);
+  if (NT == kWave) return x;
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) l.S[threadIdx.x / kWave] = x;
+  __syncthreads();
+  return lanes_sum<NT / kWave>(l.S[threadIdx.x & (NT / kWave - 1)]);
 }
 
 // Sums of huge logits (|m c| above kPlainShift) again, differences first.
 template <class T, int NT, bool ENT, class Hide>
 __device__ __forceinline__ Soft soft_huge(BlockLds<NT> &l, const T *z, int begin, int end, float m,
-                                       float c, Hide hide) {
+                                          float c, Hide hide) {
   constexpr int N = Row<T>::n;
   Soft s;
-  s.m = m;
-  s.R = 0.0f;
   for (int i = begin + static_cast<int>(threadIdx.x) * N; i < end; i += NT * N) {
     float v[N];
     load_vec<T>(z, i, end, v);
@@ -199,10 +232,9 @@ __device__ __forceinline__ Soft soft_huge(BlockLds<NT> &l, const T *z, int begin
       if (ENT) s.E = __builtin_fmaf(e, fmaxf(x, -200.0f), s.E);
     }
   }
-  if (m == __builtin_inff()) s.S = __builtin_nanf("");
-  __syncthreads();
-  int n = 0;
-  s = soft_block<NT, ENT>(l, s, n);
+  s.m = m;
+  s.S = m == __builtin_inff() ? __builtin_nanf("") : block_sum<NT>(l, s.S);
+  s.E = ENT ? block_sum<NT>(l, s.E) : 0.0f;
   s.r = s.S - 1.0f;
   return s;
 }
@@ -213,7 +245,7 @@ template <class T, int NT, bool ENT, class Hide>
 __device__ __forceinline__ Soft soft_finish(BlockLds<NT> &l, const Soft &mine, const T *z,
                                             int begin, int end, float c, int &n, Hide hide) {
   constexpr int N = Row<T>::n;
-  Soft s = soft_block<NT, ENT>(l, mine, n);
+  Soft s = soft_block<NT, ENT>(l, mine, c, n);
   if (soft_is_huge(s.m, c)) return soft_huge<T, NT, ENT>(l, z, begin, end, s.m, c, hide);
   const float R = s.R;
   soft_settle(s, c);
@@ -232,13 +264,7 @@ __device__ __forceinline__ Soft soft_finish(BlockLds<NT> &l, const Soft &mine, c
   } else {
     r = mine.S * exp2_raw(mine.R - R) * exp2f(-__builtin_fmaf(s.m, c, -R));
   }
-  r = lanes_sum<kWave>(r);
-  if (NT > kWave) {
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) l.S[threadIdx.x / kWave] = r;
-    __syncthreads();
-    r = lanes_sum<NT / kWave>(l.S[threadIdx.x & (NT / kWave - 1)]);
-  }
+  r = block_sum<NT>(l, r);
   s.r = r;
   s.S = 1.0f + r;
   return s;
@@ -248,7 +274,7 @@ __device__ __forceinline__ Soft soft_finish(BlockLds<NT> &l, const Soft &mine, c
 // its best classes. `parts` == 1: the row's outputs; else to the workspace.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
-  constexpr int N = Row<T>::n, U = kLogitVecs;
+  constexpr int N = Row<T>::n;
   __shared__ BlockLds<NT> lds;
   __shared__ SelectLds<NT> sel;
   const int tid = threadIdx.x;
@@ -267,55 +293,46 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
 
   Soft s;
   int rank = 0, first = begin;  // `first`: the vector of the first maximum
-  // a vector in which a class may come before the token
-  auto count = [&](int i, const float *v) {
-    if (i + N <= tok || i > tok) {
-      const float t = i > tok ? above : zt;
+  // W vectors of the thread, the first at i, NT N classes apart. Classes that come
+  // before the token's: at least its logit up to its own place, above it from there
+  // on (`at`: the first class of the block's W vectors).
+  auto take = [&](int at, auto &v) {
+    constexpr int W = sizeof(v) / sizeof(v[0]);
+    const int i = at + tid * N;
+    float vm[W], cm;
 #pragma unroll
-      for (int j = 0; j < N; ++j) rank += v[j] >= t;
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) rank += v[j] >= (i + j < tok ? zt : above);
-    }
-  };
-  auto take = [&](int i, float(&v)[U][N]) {
-    float vm[U], cm;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < W; ++u) {
       vm[u] = v[u][0];
 #pragma unroll
       for (int j = 1; j < N; ++j) vm[u] = fmaxf(vm[u], v[u][j]);
     }
     cm = vm[0];
 #pragma unroll
-    for (int u = 1; u < U; ++u) cm = fmaxf(cm, vm[u]);
+    for (int u = 1; u < W; ++u) cm = fmaxf(cm, vm[u]);
     if (cm > s.m) {
 #pragma unroll
-      for (int u = U - 1; u >= 0; --u)
+      for (int u = W - 1; u >= 0; --u)
         if (vm[u] == cm) first = i + u * NT * N;
     }
-    soft_add<U * N, true>(s, &v[0][0], cm, a.c);
+    soft_add<W * N, true>(s, &v[0][0], cm, a.c);
     if (cm >= zt) {
+      if (at + W * NT * N <= tok || at > tok) {
+        const float t = at > tok ? above : zt;
 #pragma unroll
-      for (int u = 0; u < U; ++u) count(i + u * NT * N, v[u]);
+        for (int u = 0; u < W; ++u)
+#pragma unroll
+          for (int j = 0; j < N; ++j) rank += v[u][j] >= t;
+      } else {
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+          const int before = tok - i - u * NT * N;
+#pragma unroll
+          for (int j = 0; j < N; ++j) rank += v[u][j] >= (j < before ? zt : above);
+        }
+      }
     }
   };
-  const int tile = NT * N * U;
-  int at = begin;
-  for (; at + tile <= end; at += tile) {
-    const int i = at + tid * N;
-    float v[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u) widen<T>(load_raw(z + i + u * NT * N), v[u]);
-    take(i, v);
-  }
-  if (at < end) {
-    const int i = at + tid * N;
-    float v[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u) load_vec<T>(z, i + u * NT * N, end, v[u]);
-    take(i, v);
-  }
+  scan_part<T, NT>(z, begin, end, take);
   const float mine = s.m;
   s = soft_finish<T, NT, true>(lds, s, z, begin, end, a.c, rank, [](int, float *) {});
 
@@ -335,17 +352,16 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
         mine > -__builtin_inff()
             ? static_cast<uint64_t>(order_of(mine)) << 32 | (0xffffffffu - static_cast<uint32_t>(first + N - 1))
             : 0;
-    auto scan = [&](auto f) {
-#pragma unroll 4
-      for (int i = begin + tid * N; i < end; i += NT * N) {
-        float v[N];
-        load_vec<T>(z, i, end, v);
+    const int vectors = (end - begin + NT * N - 1) / (NT * N);
+    auto visit = [&](int thread, int it, auto f) {
+      const int i = begin + (it * NT + thread) * N;
+      float v[N];
+      load_vec<T>(z, i, end, v);
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (v[j] > -__builtin_inff()) f(key_of(v[j], i + j));
-      }
+      for (int j = 0; j < N; ++j)
+        if (v[j] > -__builtin_inff()) f(key_of(v[j], i + j));
     };
-    got = block_select<NT>(sel, key, a.top_k, scan, [&](int j, uint64_t q) {
+    got = block_select<NT>(sel, key, a.top_k, vectors, visit, [&](int j, uint64_t q) {
       if (whole)
         put_top(a, row, j, value_of(static_cast<uint32_t>(q >> 32)), key_index(q), s.m, log_s);
       else
@@ -360,34 +376,25 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
   }
 }
 
-// Joins the parts of a row, in the order of the parts.
+// Joins the parts of a row.
 constexpr int kJoinThreads = 512;
 constexpr int kMaxParts = 128;
 
 template <class T>
 __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs a) {
-  __shared__ float4 sum[kMaxParts];
   __shared__ SelectLds<kJoinThreads> sel;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
-  for (int p = tid; p < a.parts; p += kJoinThreads) sum[p] = a.part_sum[row * a.parts + p];
-  __syncthreads();
-  Soft s;
-  for (int p = 0; p < a.parts; ++p) s.m = fmaxf(s.m, sum[p].x);
   int rank = 0;
-  bool first = true;
-  s.r = 0.0f;
-  for (int p = 0; p < a.parts; ++p) {
+  const Soft s = soft_join_parts(a.parts, a.c, rank, [&](int p, int &n) {
+    const float4 q = a.part_sum[row * a.parts + p];
     Soft b;
-    b.m = sum[p].x;
-    b.r = sum[p].y;
-    b.S = 1.0f + b.r;
-    b.E = sum[p].z;
-    soft_join(s, b, a.c, first);
-    rank += __float_as_int(sum[p].w);
-  }
-  if (s.m == -__builtin_inff()) s.r -= 1.0f;  // no class: S = 0 (or NaN)
-  s.S = 1.0f + s.r;
+    b.m = q.x;
+    b.r = q.y;
+    b.E = q.z;
+    n = __float_as_int(q.w);
+    return b;
+  });
   const bool bad = !(s.S < __builtin_inff()) || s.m == __builtin_inff();
   if (tid == 0) {
     const int64_t token = a.tokens ? load_index(a.tokens, row, a.wide_index) : -1;
@@ -403,13 +410,12 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
     const int n = a.parts * a.top_k;
     uint64_t best = 0;
     for (int i = tid; i < n; i += kJoinThreads) best = keys[i] > best ? keys[i] : best;
-    auto scan = [&](auto f) {
-      for (int i = tid; i < n; i += kJoinThreads) {
-        const uint64_t q = keys[i];
-        if (q != 0) f(q);
-      }
+    auto visit = [&](int thread, int it, auto f) {
+      const int i = it * kJoinThreads + thread;
+      if (i < n && keys[i] != 0) f(keys[i]);
     };
-    got = block_select<kJoinThreads>(sel, best, a.top_k, scan, [&](int j, uint64_t q) {
+    const int vectors = (n + kJoinThreads - 1) / kJoinThreads;
+    got = block_select<kJoinThreads>(sel, best, a.top_k, vectors, visit, [&](int j, uint64_t q) {
       put_top(a, row, j, value_of(static_cast<uint32_t>(q >> 32)), key_index(q), m, log_s);
     });
   }
@@ -553,10 +559,10 @@ __device__ __forceinline__ void zero_part(T *out, int begin, int end) {
 
 // One part of a row. The listed classes and the token are written after all
 // others; their logits are read before the block writes anything, so that the
-// gradient may take the place of the logits.
+// gradient may take the place of the logits. NT > top_k: a thread for each listed class
+// and one for the token.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
-  static_assert(NT >= kMaxTop + 1, "a thread for each listed class and one for the token");
   __shared__ int list[kMaxTop];
   __shared__ float term[kMaxTop];
   __shared__ float sums[2];

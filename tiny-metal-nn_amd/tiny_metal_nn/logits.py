@@ -3,12 +3,11 @@ logits): log-probabilities of given classes with rank, entropy and the best
 alternatives, their gradient, and distillation from a teacher's top values.
 
 Arrays are numpy arrays (copied in and out; the results are there on return) or
-device tensors (anything with data_ptr(), shape, stride() and dtype, as torch's;
-the call is only enqueued, on the tensors' current torch stream unless `stream`
-says otherwise). All arrays of a call are of one sort. Logits are float32,
-float16 or (device) bfloat16, [rows, classes] with unit stride within a row;
-class ids int32 or int64; everything else float32 / int32 and contiguous.
-No counterpart in the reference.
+torch tensors of the operators' device (the call is only enqueued, on torch's
+current stream unless `stream` says otherwise). All arrays of a call are of one
+sort. Logits are float32, float16 or (tensors) bfloat16, [rows, classes] with unit
+stride within a row; class ids int32 or int64; everything else float32 / int32 and
+contiguous. No counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -21,127 +20,141 @@ import numpy as np
 from . import _lib
 from .trainer import ClosedError, DTypeError, _Context
 
+# tmnn_token_logprobs_args, tmnn_distill_args
 _PACK_LOGPROBS = struct.Struct("=Iiii4q12Qfi")
 _PACK_DISTILL = struct.Struct("=Iiii4q7Qif")
 _SIZE_LOGPROBS, _SIZE_DISTILL = _PACK_LOGPROBS.size, _PACK_DISTILL.size
-_DTYPE_NAMES: dict = {}  # dtype object -> its name
 
 
-def _name(dtype) -> str:
-    """'float32' of numpy's and torch's float32 alike."""
-    got = _DTYPE_NAMES.get(dtype)
-    if got is None:
-        got = _DTYPE_NAMES[dtype] = str(dtype).replace("torch.", "")
-    return got
+class _Arrays:
+    """How the arrays of a call are looked at: numpy's, or torch's on a device.
+    Small calls are bound by this host work, so what is right passes in one
+    expression and only what is not is looked at closely."""
 
+    def __init__(self, lib, sort: str):
+        self.sort = sort
+        self.f32, self.i32 = getattr(lib, "float32"), getattr(lib, "int32")
 
-def _on_device(x) -> bool:
-    return hasattr(x, "data_ptr")
+    def name_of(self, dtype) -> str:
+        return str(dtype).replace("torch.", "")
 
-
-class _Call:
-    """The arrays of one call: all on the host or all on one device."""
-
-    __slots__ = ("device", "ordinal", "shape", "dtype", "stride")
-
-    def __init__(self, logits, name: str, ordinal: int):
-        self.device = _on_device(logits)
-        self.ordinal = ordinal
-        if not self.device and not isinstance(logits, np.ndarray):
-            raise TypeError(f"{name} must be a numpy array or a device tensor")
-        dtype = _name(logits.dtype)
-        if dtype not in _lib.DTYPES:
-            raise DTypeError(f"{name} must be float32, float16 or bfloat16, got {dtype}")
-        self.dtype = dtype
-        self.shape = shape = tuple(logits.shape)
-        if len(shape) != 2:
-            raise ValueError(f"{name} must be 2D (rows, classes)")
-        if shape[1] < 1:
-            raise ValueError(f"{name} must have at least one class")
-        self.stride = self._row_stride(logits, name)
-
-    def _row_stride(self, x, name: str) -> int:
-        rows, classes = self.shape
-        if self.device:
-            self._check_place(x, name)
-            row, col = x.stride()
-        else:
-            size = x.itemsize
-            row, col = (s // size if s % size == 0 else -1 for s in x.strides)
-        if rows == 0:
-            return classes
-        if col != 1 and classes > 1:
-            raise ValueError(f"{name} must have unit stride within a row")
-        if rows == 1:
-            return max(row, classes)
-        if row < classes:
-            raise ValueError(f"{name} must have rows that do not overlap")
-        return row
-
-    def _check_place(self, x, name: str) -> None:
-        d = x.device
-        if d.type != "cuda" or (d.index or 0) != self.ordinal:
-            raise ValueError(f"{name} must be on device {self.ordinal}, is on {d}")
-
-    def address(self, x) -> int:
-        return x.data_ptr() if self.device else x.ctypes.data
-
-    def array(self, x, name: str, shape: tuple, dtypes) -> int:
-        """The address of a contiguous array of this shape and one of these types."""
-        if _on_device(x) != self.device or not (self.device or isinstance(x, np.ndarray)):
-            raise TypeError(f"{name} must be {'a device tensor' if self.device else 'a numpy array'}"
-                            ", as the logits are")
-        if _name(x.dtype) not in dtypes:
-            raise DTypeError(f"{name} must be {' or '.join(dtypes)}, got {_name(x.dtype)}")
+    def refuse(self, x, name: str, shape: tuple, want: str):
+        if not self.ours(x):
+            raise TypeError(f"{name} must be {self.sort}, as the logits are, got {type(x).__name__}")
+        if self.name_of(x.dtype) not in want.split(" or "):
+            raise DTypeError(f"{name} must be {want}, got {self.name_of(x.dtype)}")
         if tuple(x.shape) != shape:
             raise ValueError(f"{name} must have shape {shape}, got {tuple(x.shape)}")
-        if self.device:
-            if x.device.type != "cuda" or (x.device.index or 0) != self.ordinal:
-                self._check_place(x, name)
-            if not x.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
-            return x.data_ptr()
-        if not x.flags["C_CONTIGUOUS"]:
-            raise ValueError(f"{name} must be contiguous")
-        return x.ctypes.data
 
-    def matrix(self, x, name: str) -> tuple[int, int]:
+    def logits(self, x, name: str, shape: tuple | None = None, dtype=None) -> tuple:
+        """(address, row stride, rows, classes, type code) of a matrix; of this shape
+        and type where they are given."""
+        code = self.float_codes.get(x.dtype)
+        if code is None or (dtype is not None and x.dtype != dtype):
+            want = "float32, float16 or bfloat16" if dtype is None else f"{self.name_of(dtype)} as the logits"
+            raise DTypeError(f"{name} must be {want}, got {self.name_of(x.dtype)}")
+        if len(x.shape) != 2:
+            raise ValueError(f"{name} must be 2D (rows, classes)")
+        if shape is not None and x.shape != shape:
+            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+        rows, classes = x.shape
+        at, row, col = self.layout(x, name)
+        if classes < 1:
+            raise ValueError(f"{name} must have at least one class")
+        if rows <= 1:
+            row = max(row, classes)
+        if col != 1 and classes > 1 and rows > 0:
+            raise ValueError(f"{name} must have unit stride within a row")
+        if row < classes:
+            raise ValueError(f"{name} must have rows that do not overlap")
+        return at, row, rows, classes, code
+
+    def like(self, x, name: str, logits) -> tuple[int, int]:
         """Address and row stride of a second matrix like the logits."""
-        if _on_device(x) != self.device or not (self.device or isinstance(x, np.ndarray)):
-            raise TypeError(f"{name} must be {'a device tensor' if self.device else 'a numpy array'}"
-                            ", as the logits are")
-        if _name(x.dtype) != self.dtype:
-            raise DTypeError(f"{name} must be {self.dtype} as the logits, got {_name(x.dtype)}")
-        if tuple(x.shape) != self.shape:
-            raise ValueError(f"{name} must have shape {self.shape}, got {tuple(x.shape)}")
-        return self.address(x), self._row_stride(x, name)
+        if not self.ours(x):
+            raise TypeError(f"{name} must be {self.sort}, as the logits are, got {type(x).__name__}")
+        return self.logits(x, name, logits.shape, logits.dtype)[:2]
 
-    def empty(self, shape: tuple, dtype: str):
-        if not self.device:
-            return np.empty(shape, dtype)
-        torch = sys.modules["torch"]
-        return torch.empty(shape, dtype=getattr(torch, dtype), device=f"cuda:{self.ordinal}")
+    def ids(self, x, name: str, shape: tuple) -> tuple[int, int]:
+        """Address and type code of class ids."""
+        if self.ours(x):
+            code = self.index_codes.get(x.dtype)
+            if code is not None:
+                return self.array(x, name, shape, x.dtype), code
+        self.refuse(x, name, shape, "int32 or int64")
 
-    def output(self, out: dict, key: str, shape: tuple, dtype: str, align: int = 1) -> int:
+    def output(self, out: dict, key: str, shape: tuple, dtype) -> int:
         x = out.get(key)
         if x is None:
             x = out[key] = self.empty(shape, dtype)
-        at = self.array(x, f"out[{key!r}]", shape, (dtype,))
-        if at % align:
-            raise ValueError(f"out[{key!r}] must be {align}-byte aligned")
-        return at
-
-    def d_logits(self, out) -> tuple:
-        if out is None:
-            out = self.empty(self.shape, self.dtype)
-        return (out, *self.matrix(out, "d_logits"))
+        return self.array(x, key, shape, dtype)
 
 
-_F32, _I32, _IDS = ("float32",), ("int32",), ("int32", "int64")
+class _HostArrays(_Arrays):
+    device = None
+
+    def __init__(self):
+        super().__init__(np, "a numpy array")
+        self.float_codes = {np.dtype(k): c for k, c in _lib.DTYPES.items() if k != "bfloat16"}
+        self.index_codes = {np.dtype(k): c for k, c in _lib.INDEX_DTYPES.items()}
+
+    @staticmethod
+    def ours(x) -> bool:
+        return isinstance(x, np.ndarray)
+
+    def array(self, x, name: str, shape: tuple, dtype) -> int:
+        if not (self.ours(x) and x.dtype == dtype and x.shape == shape):
+            self.refuse(x, name, shape, np.dtype(dtype).name)
+        if not x.flags.c_contiguous:
+            raise ValueError(f"{name} must be contiguous")
+        return x.ctypes.data
+
+    @staticmethod
+    def layout(x, name: str) -> tuple[int, int, int]:
+        size = x.itemsize
+        row, col = (s // size if s % size == 0 else -1 for s in x.strides)
+        return x.ctypes.data, row, col
+
+    @staticmethod
+    def empty(shape: tuple, dtype):
+        return np.empty(shape, dtype)
 
 
-def _optional(call: _Call, x, name: str, shape: tuple, dtypes=_F32) -> int:
-    return 0 if x is None else call.array(x, name, shape, dtypes)
+class _DeviceArrays(_Arrays):
+    def __init__(self, torch, device: int):
+        super().__init__(torch, "a torch tensor")
+        self.torch, self.device = torch, device
+        self.float_codes = {getattr(torch, k): c for k, c in _lib.DTYPES.items()}
+        self.index_codes = {getattr(torch, k): c for k, c in _lib.INDEX_DTYPES.items()}
+        self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+    @staticmethod
+    def ours(x) -> bool:
+        return hasattr(x, "data_ptr")
+
+    def place(self, x, name: str) -> None:
+        if x.get_device() != self.device:
+            raise ValueError(f"{name} must be on device {self.device}, is on {x.device}")
+
+    def array(self, x, name: str, shape: tuple, dtype) -> int:
+        try:
+            if (x.dtype is dtype and x.shape == shape and x.get_device() == self.device
+                    and x.is_contiguous()):
+                return x.data_ptr()
+        except AttributeError:
+            pass
+        self.refuse(x, name, shape, self.name_of(dtype))
+        self.place(x, name)
+        raise ValueError(f"{name} must be contiguous")
+
+    def layout(self, x, name: str) -> tuple[int, int, int]:
+        if x.get_device() != self.device:
+            self.place(x, name)
+        return (x.data_ptr(), *x.stride())
+
+    def empty(self, shape: tuple, dtype):
+        return self.torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
 
 
 class LogitOps:
@@ -152,12 +165,14 @@ class LogitOps:
     own for a stream that is captured into a graph."""
 
     def __init__(self, device: int = 0):
-        self._lib = _lib.load()
+        lib = self._lib = _lib.load()
         self._ctx = _Context.get(device)
         self._ordinal = device
         h = ctypes.c_void_p()
-        _lib.check(self._lib.tmnn_logits_create(self._ctx.handle, ctypes.byref(h)))
+        _lib.check(lib.tmnn_logits_create(self._ctx.handle, ctypes.byref(h)))
         self._h = h
+        self._host = _HostArrays()
+        self._device: _DeviceArrays | None = None
 
     def close(self) -> None:
         if self._h is not None:
@@ -180,23 +195,33 @@ class LogitOps:
         except Exception:
             pass
 
-    def _run(self, name: str, call: _Call, packed: bytes, stream) -> None:
-        if not call.device:
-            if stream is not None:
-                raise ValueError("stream goes with device tensors")
-            _lib.check(getattr(self._lib, name)(self._h, packed))
-            return
-        if stream is None:
-            stream = sys.modules["torch"].cuda.current_stream(self._ordinal).cuda_stream
-        elif not isinstance(stream, int):
-            stream = stream.cuda_stream
-        rc = getattr(self._lib, name + "_device")(self._h, packed, stream)
-        if rc:
-            _lib.check(rc)
-
-    def _open(self) -> None:
+    def _arrays(self, logits) -> _Arrays:
         if self._h is None:
             raise ClosedError("LogitOps is closed")
+        if isinstance(logits, np.ndarray):
+            return self._host
+        if self._device is None:
+            torch = sys.modules.get("torch")
+            if torch is None or not isinstance(logits, torch.Tensor):
+                raise TypeError(f"logits must be a numpy array or a torch tensor, got {type(logits).__name__}")
+            self._device = _DeviceArrays(torch, self._ordinal)
+        elif not hasattr(logits, "data_ptr"):
+            raise TypeError(f"logits must be a numpy array or a torch tensor, got {type(logits).__name__}")
+        return self._device
+
+    def _run(self, a: _Arrays, on_host, on_device, packed: bytes, stream) -> None:
+        if a.device is None:
+            if stream is not None:
+                raise ValueError("stream goes with torch tensors")
+            rc = on_host(self._h, packed)
+        else:
+            if stream is None:
+                stream = a.raw_stream(a.device)
+            elif not isinstance(stream, int):
+                stream = stream.cuda_stream
+            rc = on_device(self._h, packed, stream)
+        if rc:
+            _lib.check(rc)
 
     # ---- log-probabilities ------------------------------------------------------
     def token_logprobs(self, logits, tokens=None, *, top_k: int = 0, temperature: float = 1.0,
@@ -211,23 +236,25 @@ class LogitOps:
         `out`: arrays to write to, by these names; it gets those that it lacks, and
         is returned. -inf masks a class; a row whose classes are all masked has log p
         -inf and entropy 0, a row with NaN or +inf gives NaN."""
-        self._open()
-        c = _Call(logits, "logits", self._ordinal)
-        n, v = c.shape
+        a = self._arrays(logits)
+        at, stride, n, v, code = a.logits(logits, "logits")
         if not 0 <= top_k <= _lib.LOGITS_MAX_TOP:
             raise ValueError(f"top_k must be in [0, {_lib.LOGITS_MAX_TOP}], got {top_k}")
-        out = {} if out is None else out
-        tok = _optional(c, tokens, "tokens", (n,), _IDS)
-        packed = _PACK_LOGPROBS.pack(
-            _SIZE_LOGPROBS, _lib.DTYPES[c.dtype],
-            0 if tokens is None else _lib.INDEX_DTYPES[_name(tokens.dtype)], top_k, n, v, c.stride, v,
-            c.address(logits), tok, c.output(out, "logprob", (n,), "float32"),
-            c.output(out, "entropy", (n,), "float32"), c.output(out, "rank", (n,), "int32"),
-            c.output(out, "stats", (n, 2), "float32"),
-            c.output(out, "top_ids", (n, top_k), "int32") if top_k else 0,
-            c.output(out, "top_logprobs", (n, top_k), "float32") if top_k else 0,
-            0, 0, 0, 0, temperature, 0)
-        self._run("tmnn_token_logprobs", c, packed, stream)
+        if out is None:
+            out = {}
+        rows = (n,)
+        tok, index = (0, 0) if tokens is None else a.ids(tokens, "tokens", rows)
+        f32, i32 = a.f32, a.i32
+        ids = best = 0
+        if top_k:
+            ids = a.output(out, "top_ids", (n, top_k), i32)
+            best = a.output(out, "top_logprobs", (n, top_k), f32)
+        self._run(a, self._lib.tmnn_token_logprobs, self._lib.tmnn_token_logprobs_device,
+                  _PACK_LOGPROBS.pack(
+                      _SIZE_LOGPROBS, code, index, top_k, n, v, stride, v, at, tok,
+                      a.output(out, "logprob", rows, f32), a.output(out, "entropy", rows, f32),
+                      a.output(out, "rank", rows, i32), a.output(out, "stats", (n, 2), f32),
+                      ids, best, 0, 0, 0, 0, temperature, 0), stream)
         return out
 
     def token_logprobs_backward(self, logits, tokens, forward: dict, *, d_logprob=None,
@@ -236,40 +263,47 @@ class LogitOps:
         """The gradient, in the logits' type, of sum(d_logprob * logprob + d_entropy *
         entropy) + sum(d_top_logprobs * top_logprobs). `forward`: what token_logprobs
         returned for these logits. `out` may be the logits."""
-        self._open()
-        c = _Call(logits, "logits", self._ordinal)
-        n, v = c.shape
-        d, d_at, d_stride = c.d_logits(out)
-        k = 0
+        a = self._arrays(logits)
+        at, stride, n, v, code = a.logits(logits, "logits")
+        if out is None:
+            out = a.empty(logits.shape, logits.dtype)
+        d_at, d_stride = a.like(out, "d_logits", logits)
+        rows, f32 = (n,), a.f32
+        tok, index = (0, 0) if tokens is None else a.ids(tokens, "tokens", rows)
+        k = ids = g_token = g_entropy = entropy = g_top = 0
+        if d_logprob is not None:
+            if tokens is None:
+                raise ValueError("d_logprob needs tokens")
+            g_token = a.array(d_logprob, "d_logprob", rows, f32)
+        if d_entropy is not None:
+            g_entropy = a.array(d_entropy, "d_entropy", rows, f32)
+            entropy = a.array(forward["entropy"], "entropy", rows, f32)
         if d_top_logprobs is not None:
             if len(d_top_logprobs.shape) != 2:
                 raise ValueError("d_top_logprobs must be 2D (rows, top_k)")
             k = int(d_top_logprobs.shape[1])
-        if d_logprob is not None and tokens is None:
-            raise ValueError("d_logprob needs tokens")
-        packed = _PACK_LOGPROBS.pack(
-            _SIZE_LOGPROBS, _lib.DTYPES[c.dtype],
-            0 if tokens is None else _lib.INDEX_DTYPES.get(_name(tokens.dtype), 0), k, n, v, c.stride,
-            d_stride, c.address(logits), _optional(c, tokens, "tokens", (n,), _IDS), 0,
-            0 if d_entropy is None else c.array(forward["entropy"], "entropy", (n,), _F32), 0,
-            c.array(forward["stats"], "stats", (n, 2), _F32),
-            c.array(forward["top_ids"], "top_ids", (n, k), _I32) if k else 0, 0,
-            _optional(c, d_logprob, "d_logprob", (n,)), _optional(c, d_entropy, "d_entropy", (n,)),
-            _optional(c, d_top_logprobs, "d_top_logprobs", (n, k)), d_at, temperature, 0)
-        self._run("tmnn_token_logprobs_backward", c, packed, stream)
-        return d
+            if k:
+                g_top = a.array(d_top_logprobs, "d_top_logprobs", (n, k), f32)
+                ids = a.array(forward["top_ids"], "top_ids", (n, k), a.i32)
+        self._run(a, self._lib.tmnn_token_logprobs_backward,
+                  self._lib.tmnn_token_logprobs_backward_device,
+                  _PACK_LOGPROBS.pack(
+                      _SIZE_LOGPROBS, code, index, k, n, v, stride, d_stride, at, tok, 0, entropy, 0,
+                      a.array(forward["stats"], "stats", (n, 2), f32), ids, 0, g_token, g_entropy,
+                      g_top, d_at, temperature, 0), stream)
+        return out
 
     # ---- distillation --------------------------------------------------------------
     @staticmethod
-    def _teacher(c: _Call, ids, teacher, kind: str) -> tuple[int, int, int]:
-        if kind not in _lib.TEACHER_KINDS:
+    def _teacher(a: _Arrays, n: int, ids, teacher, kind: str) -> tuple[int, int, int, int, int]:
+        code = _lib.TEACHER_KINDS.get(kind)
+        if code is None:
             raise ValueError(f"kind must be 'logits' or 'logprobs', got {kind!r}")
         if len(ids.shape) != 2:
             raise ValueError("teacher_ids must be 2D (rows, entries)")
         k = int(ids.shape[1])
-        n = c.shape[0]
-        return (k, c.array(ids, "teacher_ids", (n, k), _IDS),
-                c.array(teacher, "teacher", (n, k), _F32))
+        at, index = a.ids(ids, "teacher_ids", (n, k))
+        return code, k, at, index, a.array(teacher, "teacher", (n, k), a.f32)
 
     def distill(self, logits, teacher_ids, teacher, *, kind: str = "logits",
                 temperature: float = 1.0, row_weights=None, gradient: bool = True,
@@ -284,37 +318,39 @@ class LogitOps:
 
         `out`: arrays to write to, by these names; it gets those that it lacks, and is
         returned. out["d_logits"] may be the logits."""
-        self._open()
-        c = _Call(logits, "logits", self._ordinal)
-        n, v = c.shape
-        out = {} if out is None else out
-        k, ids_at, teacher_at = self._teacher(c, teacher_ids, teacher, kind)
+        a = self._arrays(logits)
+        at, stride, n, v, code = a.logits(logits, "logits")
+        if out is None:
+            out = {}
+        kind_code, k, ids, index, values = self._teacher(a, n, teacher_ids, teacher, kind)
         d_at, d_stride = 0, v
         if gradient:
-            out["d_logits"], d_at, d_stride = c.d_logits(out.get("d_logits"))
-        packed = _PACK_DISTILL.pack(
-            _SIZE_DISTILL, _lib.DTYPES[c.dtype], _lib.INDEX_DTYPES[_name(teacher_ids.dtype)],
-            _lib.TEACHER_KINDS[kind], n, v, c.stride, d_stride, c.address(logits), ids_at, teacher_at,
-            _optional(c, row_weights, "row_weights", (n,)), c.output(out, "loss", (n,), "float32"),
-            c.output(out, "stats", (n, 4), "float32", 16), d_at, k, temperature)
-        self._run("tmnn_distill", c, packed, stream)
+            d = out.get("d_logits")
+            if d is None:
+                d = out["d_logits"] = a.empty(logits.shape, logits.dtype)
+            d_at, d_stride = a.like(d, "d_logits", logits)
+        f32 = a.f32
+        self._run(a, self._lib.tmnn_distill, self._lib.tmnn_distill_device,
+                  _PACK_DISTILL.pack(
+                      _SIZE_DISTILL, code, index, kind_code, n, v, stride, d_stride, at, ids, values,
+                      0 if row_weights is None else a.array(row_weights, "row_weights", (n,), f32),
+                      a.output(out, "loss", (n,), f32), a.output(out, "stats", (n, 4), f32), d_at, k,
+                      temperature), stream)
         return out
 
     def distill_backward(self, logits, teacher_ids, teacher, stats, d_loss, *, kind: str = "logits",
                          temperature: float = 1.0, out=None, stream=None):
         """The gradient, in the logits' type, of sum(d_loss * loss) of an unweighted
         distill call, from its `stats`. `out` may be the logits."""
-        self._open()
-        c = _Call(logits, "logits", self._ordinal)
-        n, v = c.shape
-        k, ids_at, teacher_at = self._teacher(c, teacher_ids, teacher, kind)
-        d, d_at, d_stride = c.d_logits(out)
-        stats_at = c.array(stats, "stats", (n, 4), _F32)
-        if stats_at % 16:
-            raise ValueError("stats must be 16-byte aligned")
-        packed = _PACK_DISTILL.pack(
-            _SIZE_DISTILL, _lib.DTYPES[c.dtype], _lib.INDEX_DTYPES[_name(teacher_ids.dtype)],
-            _lib.TEACHER_KINDS[kind], n, v, c.stride, d_stride, c.address(logits), ids_at, teacher_at,
-            c.array(d_loss, "d_loss", (n,), _F32), 0, stats_at, d_at, k, temperature)
-        self._run("tmnn_distill_backward", c, packed, stream)
-        return d
+        a = self._arrays(logits)
+        at, stride, n, v, code = a.logits(logits, "logits")
+        kind_code, k, ids, index, values = self._teacher(a, n, teacher_ids, teacher, kind)
+        if out is None:
+            out = a.empty(logits.shape, logits.dtype)
+        d_at, d_stride = a.like(out, "d_logits", logits)
+        self._run(a, self._lib.tmnn_distill_backward, self._lib.tmnn_distill_backward_device,
+                  _PACK_DISTILL.pack(
+                      _SIZE_DISTILL, code, index, kind_code, n, v, stride, d_stride, at, ids, values,
+                      a.array(d_loss, "d_loss", (n,), a.f32), 0, a.array(stats, "stats", (n, 4), a.f32),
+                      d_at, k, temperature), stream)
+        return out
