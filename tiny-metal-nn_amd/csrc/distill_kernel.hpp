@@ -35,6 +35,7 @@ struct DistillArgs {
   int32_t rows, classes, k;
   int32_t parts, part_len;
   float c, t, inv_t;  // log2(e) / T, T, 1 / T
+  double inv_t64;
   float *loss;
   float *stats;  // [rows][4]
   void *d_logits;
@@ -50,15 +51,16 @@ struct DistillRow {
 
 // A listed class's ln q - ln p, the differences of its logits in 64 bits: the loss is
 // small against both.
+template <bool TAIL>
 __device__ __forceinline__ float log_ratio(const DistillArgs &a, float t, float top, float log_z,
                                            float z, float m, float log_s) {
-  const double inv_t = 1.0 / static_cast<double>(a.t);
-  const double lq = a.kind == 0 ? (static_cast<double>(t) - top) * inv_t - log_z : t;
-  return static_cast<float>(lq - (static_cast<double>(z) - m) * inv_t + log_s);
+  const double lq = TAIL ? t : (static_cast<double>(t) - top) * a.inv_t64 - log_z;
+  return static_cast<float>(lq - (static_cast<double>(z) - m) * a.inv_t64 + log_s);
 }
 // q of a teacher value: relative to `top` over 1 / inv_z (kind 0), or itself.
+template <bool TAIL>
 __device__ __forceinline__ float teacher_mass(const DistillArgs &a, float t, float top, float inv_z) {
-  return a.kind == 0 ? exp2_raw((t - top) * a.c) * inv_z : expf(t);
+  return TAIL ? exp_of(t) : exp2_raw((t - top) * a.c) * inv_z;
 }
 
 // sum q over G lanes' listed classes, each lane's by `each(f)`: (sum q, 1 - sum q).
@@ -66,11 +68,13 @@ __device__ __forceinline__ float teacher_mass(const DistillArgs &a, float t, flo
 // is off by 2^-24 of the whole, which is all of a small rest.
 struct TeacherMass {
   float all, left;
+  float poison;  // 0, or NaN where one of the lanes' is
 };
-template <int G, class Each>
-__device__ __forceinline__ TeacherMass teacher_total(const DistillArgs &a, float top, Each each) {
-  TeacherMass m{0.0f, 0.0f};
-  if (a.kind == 0) {
+template <bool TAIL, int G, class Each>
+__device__ __forceinline__ TeacherMass teacher_total(const DistillArgs &a, float top, float poison,
+                                                     Each each) {
+  TeacherMass m{0.0f, 0.0f, lanes_any<G>(poison != 0.0f) ? __builtin_nanf("") : 0.0f};
+  if (!TAIL) {
     each([&](float t) { m.all += exp2_raw((t - top) * a.c); });
     m.all = lanes_sum<G>(m.all);
     return m;
@@ -86,14 +90,15 @@ __device__ __forceinline__ TeacherMass teacher_total(const DistillArgs &a, float
 // The row's statistics and the part of its loss that the listed classes do not
 // bring: dense = settled sums of all classes (kind 0) or of the unlisted ones
 // (kind 1); all = of all classes; mass = sum q, left = 1 - mass (kind 1).
+template <bool TAIL>
 __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const Soft &dense,
                                                   const Soft &all, float mass, float left,
                                                   float *rest_loss) {
   DistillRow r;
   r.m_a = all.m;
   *rest_loss = 0.0f;
-  if (a.kind == 0) {
-    r.a_a = mass / all.S;
+  if (!TAIL) {
+    r.a_a = quotient(mass, all.S);
     r.m_d = r.m_a;
     r.a_d = r.a_a;
     return r;
@@ -101,148 +106,179 @@ __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const So
   const bool rest = dense.S != 0.0f;
   const float qr = rest ? left : 0.0f;
   const float q = mass + qr;
-  r.a_a = q / all.S;
+  r.a_a = quotient(q, all.S);
   r.m_d = rest ? dense.m : 0.0f;
   // (no rest: 0, or the NaN of the listed classes)
-  r.a_d = rest ? exp2_raw((dense.m - all.m) * a.c) * r.a_a - qr / dense.S : 0.0f * r.a_a;
+  r.a_d = rest ? exp2_raw((dense.m - all.m) * a.c) * r.a_a - quotient(qr, dense.S) : 0.0f * r.a_a;
   if (qr > 0.0f) {
-    const float log_pr = (dense.m - all.m) * a.inv_t + (log1pf(dense.r) - log1pf(all.r));
-    *rest_loss = qr * (logf(qr) - log_pr);
+    const float log_pr = (dense.m - all.m) * a.inv_t + (log1p_of(dense.r) - log1p_of(all.r));
+    *rest_loss = qr * (log_of(qr) - log_pr);
   }
   return r;
 }
 
 // ---- short rows -----------------------------------------------------------------
 
-// BACK: statistics are given and only the gradient is written.
-template <class T, int G, bool BACK>
+// TAIL: kind 1. BACK: statistics are given and only the gradient is written. Else, with TAIL,
+// the listed classes are left out of the sums over the lanes' classes, and join them one
+// by one.
+template <class T, int G, int NV, bool TAIL, bool BACK>
 __global__ __launch_bounds__(kGroupThreads) void distill_group_kernel(DistillArgs a) {
-  constexpr int N = Row<T>::n;
-  __shared__ int owner[kGroupThreads * N];    // the first entry that lists a class
-  __shared__ float listed[kGroupThreads * N];  // its q
+  constexpr int N = Row<T>::n, E = N * NV;
+  __shared__ GroupWords<T, G, NV> words;  // the first entry that lists a class, then its gradient
   const float inf = __builtin_inff();
-  const int lane = threadIdx.x & (G - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kGroupThreads / G) + threadIdx.x / G;
+  const Group<T, G, NV> g;
+  const int64_t row = g.row;
   const float w = row < a.rows ? (a.weights ? a.weights[row] : 1.0f) : 0.0f;
   const bool live = row < a.rows && w != 0.0f;
   const T *z = static_cast<const T *>(a.logits) + (live ? row : 0) * a.row_stride;
-  float v[N];
-  load_vec<T>(z, lane * N, live ? a.classes : 0, v);
-  int *own = owner + (threadIdx.x - lane) * N;
-  float *q_of = listed + (threadIdx.x - lane) * N;
   const int k = live ? a.k : 0;
+  // The lane's entries lane, lane + G, ...: the first kKept in registers. NaN values
+  // and ids beyond the classes make `poison` NaN.
+  constexpr int kKept = G <= 4 ? 8 / G : 1;
+  int id[kKept];
+  float value[kKept], logit[kKept], poison = 0.0f;
+  auto entry = [&](int j, int &i, float &t) {
+    const int64_t at = load_index(a.ids, row * a.k + j, a.wide_index);
+    i = at >= 0 && at < a.classes ? static_cast<int>(at) : -1;
+    t = a.teacher[row * a.k + j];
+    if (at >= a.classes || (at >= 0 && t != t)) poison = __builtin_nanf("");
+  };
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    own[lane * N + j] = 0x7fffffff;
-    q_of[lane * N + j] = 0.0f;
+  for (int e = 0; e < kKept; ++e) {
+    id[e] = -1;
+    value[e] = 0.0f;
+    if (g.lane + e * G < k) entry(g.lane + e * G, id[e], value[e]);
   }
+  float v[E];
+  g.load_rows(a.logits, a.row_stride, a.rows, a.classes, live, words.word, v);
+  int *mine = words.lane();
+#pragma unroll
+  for (int e = 0; e < E; ++e) mine[e] = kUnlisted;
   wave_fence();
-  float wrong = 0.0f;
-  for (int j = lane; j < k; j += G) {
-    const int64_t id = load_index(a.ids, row * a.k + j, a.wide_index);
-    if (id >= a.classes)
-      wrong = 1.0f;
-    else if (id >= 0)
-      atomicMin(&own[id], j);
-  }
-  wave_fence();
-  auto entries = [&](auto f) {
-    for (int j = lane; j < k; j += G) {
-      const int64_t id = load_index(a.ids, row * a.k + j, a.wide_index);
-      if (id >= 0 && id < a.classes && own[id] == j)
-        f(static_cast<int>(id), a.teacher[row * a.k + j]);
+#pragma unroll
+  for (int e = 0; e < kKept; ++e)
+    if (id[e] >= 0) {
+      atomicMin(&words.of(id[e]), g.lane + e * G);
+      logit[e] = Row<T>::up(z[id[e]]);
     }
+  for (int j = g.lane + kKept * G; j < k; j += G) {
+    int i;
+    float t;
+    entry(j, i, t);
+    if (i >= 0) atomicMin(&words.of(i), j);
+  }
+  wave_fence();
+#pragma unroll
+  for (int e = 0; e < kKept; ++e)
+    if (id[e] >= 0 && words.of(id[e]) != g.lane + e * G) id[e] = -1;
+  // f(class, value, logit) for the lane's entries that count: first the others, which may
+  // find a class's word taken by another's gradient, whose bits are no entry's number
+  auto entries = [&](auto f) {
+    for (int j = g.lane + kKept * G; j < k; j += G) {
+      int i;
+      float t;
+      entry(j, i, t);
+      if (i >= 0 && words.of(i) == j) f(i, t, Row<T>::up(z[i]));
+    }
+#pragma unroll
+    for (int e = 0; e < kKept; ++e)
+      if (id[e] >= 0) f(id[e], value[e], logit[e]);
   };
   float top = -inf;
-  entries([&](int, float t) {
-    top = fmaxf(top, t);
-    if (t != t) wrong = 1.0f;
-  });
-  top = lanes_max<G>(top);
-  wrong = lanes_max<G>(wrong);
-  const TeacherMass tm =
-      teacher_total<G>(a, top, [&](auto f) { entries([&](int, float t) { f(t); }); });
+  if (!TAIL) {
+    entries([&](int, float t, float) { top = fmaxf(top, t); });
+    top = lanes_max<G>(top);
+  }
+  const TeacherMass tm = teacher_total<TAIL, G>(
+      a, top, poison, [&](auto f) { entries([&](int, float t, float) { f(t); }); });
   const float total = tm.all;
   // no mass at all: nothing is listed, or only values of -inf
-  const bool none = a.kind == 0 && top == -inf;
-  const float inv_z = a.kind == 0 ? 1.0f / total : 1.0f, log_z = logf(total);
-  float mass = a.kind != 0 ? total : none ? 0.0f : total * inv_z;
-  if (wrong != 0.0f) mass = __builtin_nanf("");
+  const bool none = !TAIL && top == -inf && tm.poison == 0.0f;
+  const float inv_z = TAIL ? 1.0f : quotient(1.0f, total), log_z = TAIL ? 0.0f : log_of(total);
+  const float mass = (TAIL ? total : none ? 0.0f : total * inv_z) + tm.poison;
 
   DistillRow r{};
-  if (!BACK) {
-    Soft all, dense;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      all.m = fmaxf(all.m, v[j]);
-      if (own[lane * N + j] == 0x7fffffff) dense.m = fmaxf(dense.m, v[j]);
+  float loss = 0.0f, rest_loss = 0.0f;
+  Soft all;
+  if (BACK) {
+    if (live) {
+      const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
+      r = DistillRow{s.x, s.y, s.z, s.w};
     }
-    all.m = lanes_max<G>(all.m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = exp2_raw((v[e] - r.m_d) * a.c);
+  } else {
+    Soft dense;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (TAIL && mine[e] != kUnlisted) v[e] = -inf;
+      dense.m = fmaxf(dense.m, v[e]);
+    }
     dense.m = lanes_max<G>(dense.m);
-    const float shift = all.m == -inf ? 0.0f : all.m, rest = dense.m == -inf ? 0.0f : dense.m;
-    // classes of the largest logit, whose terms are 1, by number
-    int all_n = 0, dense_n = 0;
-    all.r = dense.r = 0.0f;
+    const float shift = dense.m == -inf ? 0.0f : dense.m;
+    int best_n = 0;  // classes of the largest logit, whose terms are 1
+    dense.r = 0.0f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float e = exp2_raw((v[j] - shift) * a.c);
-      all.r += v[j] == all.m ? 0.0f : e;
-      all_n += v[j] == all.m;
-      if (a.kind != 0 && own[lane * N + j] == 0x7fffffff) {
-        const float f = exp2_raw((v[j] - rest) * a.c);
-        dense.r += v[j] == dense.m ? 0.0f : f;
-        dense_n += v[j] == dense.m;
-      }
+    for (int e = 0; e < E; ++e) {
+      const bool best = v[e] == dense.m;
+      v[e] = exp2_raw((v[e] - shift) * a.c);
+      dense.r += best ? 0.0f : v[e];
+      best_n += best;
     }
-    all.r = lanes_sum<G>(all.r) + static_cast<float>((all.m == -inf ? 0 : lanes_isum<G>(all_n)) - 1);
-    if (all.m == inf) all.r = __builtin_nanf("");
-    all.S = 1.0f + all.r;
-    if (a.kind != 0) {
-      dense.r = lanes_sum<G>(dense.r) +
-                static_cast<float>((dense.m == -inf ? 0 : lanes_isum<G>(dense_n)) - 1);
-      if (dense.m == inf) dense.r = __builtin_nanf("");
-      dense.S = 1.0f + dense.r;
+    best_n = lanes_isum<G>(best_n);
+    dense.r = lanes_sum<G>(dense.r) + static_cast<float>((dense.m == -inf ? 0 : best_n) - 1);
+    if (dense.m == inf) dense.r = __builtin_nanf("");
+    dense.S = 1.0f + dense.r;
+    all = dense;
+    if (TAIL) {
+      entries([&](int, float, float y) { all.m = fmaxf(all.m, y); });
+      all.m = lanes_max<G>(all.m);
+      const float up = all.m == -inf ? 0.0f : all.m;
+      float p = 0.0f;
+      int n = 0;  // listed classes of the largest logit
+      entries([&](int, float, float y) {
+        p += y == all.m ? 0.0f : exp2_raw((y - up) * a.c);
+        n += y == all.m;
+      });
+      n = lanes_isum<G>(n);
+      const bool one = dense.m == all.m;  // the 1 that r leaves out is the rest's, or a listed class's
+      all.r = 0.0f;
+      soft_join(all, dense, a.c, one && dense.m != -inf);
+      all.r += lanes_sum<G>(p) + static_cast<float>(all.m == -inf ? -1 : one ? n : n - 1);
+      if (all.m == inf) all.r = __builtin_nanf("");
+      all.S = 1.0f + all.r;
     }
-    float loss = 0.0f, rest_loss;
-    r = distill_row(a, dense, all, mass, tm.left, &rest_loss);
-    const float log_s = log1pf(all.r);
-    entries([&](int id, float t) {
-      const float q = none ? 0.0f : teacher_mass(a, t, top, inv_z);
-      q_of[id] = q;
-      if (q != 0.0f)
-        loss += q * log_ratio(a, t, top, log_z, Row<T>::up(z[id]), all.m, log_s);
-    });
-    loss = lanes_sum<G>(loss) + rest_loss;
-    if (wrong != 0.0f) loss = __builtin_nanf("");
+    r = distill_row<TAIL>(a, dense, all, mass, tm.left, &rest_loss);
+    if (all.m == -inf && all.S == 0.0f) r.m_a = -inf;
+  }
+  const bool zero = !live || (r.m_a == -inf && r.a_a == r.a_a);
+  const float scale = w * a.t, log_s = log1p_of(all.r);
+  entries([&](int i, float t, float y) {
+    const float q = none ? 0.0f : teacher_mass<TAIL>(a, t, top, inv_z);
+    if (!BACK && q != 0.0f) loss += q * log_ratio<TAIL>(a, t, top, log_z, y, all.m, log_s);
+    const float d = scale * (r.a_a * exp2_raw((y - r.m_a) * a.c) - q);
+    words.of(i) = fabsf(d) < 1.2e-38f ? 0 : __float_as_int(d);
+  });
+  if (!BACK) {
+    loss = lanes_sum<G>(loss) + rest_loss + tm.poison;
     const bool empty = all.m == -inf && all.S == 0.0f;
-    if (empty) r.m_a = -inf;
-    if (lane == 0 && row < a.rows) {
+    if (g.lane == 0 && row < a.rows) {
       if (a.loss) a.loss[row] = !live || empty ? 0.0f : loss * a.t * a.t * w;
       if (a.stats)
         reinterpret_cast<float4 *>(a.stats)[row] =
             live ? make_float4(r.m_d, r.a_d, r.m_a, r.a_a) : make_float4(0.0f, 0.0f, -inf, 0.0f);
     }
     if (!a.d_logits) return;
-  } else {
-    if (live) {
-      const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
-      r = DistillRow{s.x, s.y, s.z, s.w};
-    }
-    entries([&](int id, float t) { q_of[id] = none ? 0.0f : teacher_mass(a, t, top, inv_z); });
   }
   wave_fence();
-  if (row >= a.rows) return;
-  const bool zero = !live || (r.m_a == -inf && r.a_a == r.a_a);
-  const float scale = w * a.t;
-  float d[N];
+  const float dense_scale = scale * r.a_d;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const bool in = own[lane * N + j] != 0x7fffffff;
-    const float e = exp2_raw((v[j] - (in ? r.m_a : r.m_d)) * a.c);
-    const float g = (in ? r.a_a : r.a_d) * e - q_of[lane * N + j];
-    d[j] = zero ? 0.0f : scale * g;
+  for (int e = 0; e < E; ++e) {
+    const float d = mine[e] == kUnlisted ? dense_scale * v[e] : __int_as_float(mine[e]);
+    v[e] = zero ? 0.0f : d;
   }
-  store_vec<T>(static_cast<T *>(a.d_logits) + row * a.d_row_stride, lane * N, a.classes, d);
+  g.store_rows(a.d_logits, a.d_row_stride, a.rows, a.classes, words.word, v);
 }
 
 // ---- long rows ---------------------------------------------------------------------
@@ -265,7 +301,7 @@ __device__ __forceinline__ int read_list(const DistillArgs &a, ListLds &l, int64
   int id = -1;
   if (tid < a.k) {
     const int64_t i = load_index(a.ids, row * a.k + tid, a.wide_index);
-    if (i >= a.classes) l.wrong = 1.0f;  // every writer writes the same
+    if (i >= a.classes) l.wrong = __builtin_nanf("");  // every writer writes the same
     id = i >= 0 && i < a.classes ? static_cast<int>(i) : -1;
     l.id[tid] = id;
     l.t[tid] = a.teacher[row * a.k + tid];
@@ -284,32 +320,31 @@ __device__ __forceinline__ int read_list(const DistillArgs &a, ListLds &l, int64
 
 // One wave: q of the listed classes into l.q; returns their mass. `top` and `log_z`
 // as log_ratio takes them.
+template <bool TAIL>
 __device__ __forceinline__ TeacherMass teacher_sums(const DistillArgs &a, ListLds &l, float *top,
                                                     float *log_z) {
   const int lane = threadIdx.x & (kWave - 1);
   const float inf = __builtin_inff();
-  float t_max = -inf;
-  float wrong = l.wrong;
+  float t_max = -inf, poison = l.wrong;
   for (int j = lane; j < a.k; j += kWave)
     if (l.id[j] >= 0) {
       t_max = fmaxf(t_max, l.t[j]);
-      if (l.t[j] != l.t[j]) wrong = 1.0f;
+      if (l.t[j] != l.t[j]) poison = __builtin_nanf("");
     }
-  t_max = lanes_max<kWave>(t_max);
-  wrong = lanes_max<kWave>(wrong);
-  TeacherMass m = teacher_total<kWave>(a, t_max, [&](auto f) {
+  if (!TAIL) t_max = lanes_max<kWave>(t_max);
+  TeacherMass m = teacher_total<TAIL, kWave>(a, t_max, poison, [&](auto f) {
     for (int j = lane; j < a.k; j += kWave)
       if (l.id[j] >= 0) f(l.t[j]);
   });
   const float total = m.all;
-  const bool none = a.kind == 0 && t_max == -inf;
-  const float inv_z = a.kind == 0 ? 1.0f / total : 1.0f;
+  const bool none = !TAIL && t_max == -inf && m.poison == 0.0f;
+  const float inv_z = TAIL ? 1.0f : quotient(1.0f, total);
   for (int j = lane; j < a.k; j += kWave)
-    l.q[j] = l.id[j] >= 0 && !none ? teacher_mass(a, l.t[j], t_max, inv_z) : 0.0f;
+    l.q[j] = l.id[j] >= 0 && !none ? teacher_mass<TAIL>(a, l.t[j], t_max, inv_z) : 0.0f;
   *top = t_max;
-  *log_z = logf(total);
+  *log_z = TAIL ? 0.0f : log_of(total);
   // sum q is 1 for kind 0 (a sum of NaN stays one)
-  m.all = wrong != 0.0f ? __builtin_nanf("") : a.kind != 0 ? total : none ? 0.0f : total * inv_z;
+  m.all = (TAIL ? total : none ? 0.0f : total * inv_z) + m.poison;
   return m;
 }
 
@@ -335,7 +370,7 @@ __device__ __forceinline__ void distill_gradient(const DistillArgs &a, const T *
 }
 
 // From the sums of a row: its loss, statistics and gradient (of one part).
-template <class T, int NT>
+template <class T, int NT, bool TAIL>
 __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l, int64_t row,
                                                int part, const T *z, int begin, int end,
                                                const Soft &dense, int id, float zj, float w) {
@@ -344,9 +379,9 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
   __syncthreads();
   if (tid < kWave) {
     float top, log_z, rest_loss, loss = 0.0f;
-    const TeacherMass mass = teacher_sums(a, l, &top, &log_z);
+    const TeacherMass mass = teacher_sums<TAIL>(a, l, &top, &log_z);
     Soft all = dense;
-    if (a.kind != 0) {
+    if (TAIL) {
       for (int j = tid; j < a.k; j += kWave)
         if (l.id[j] >= 0) all.m = fmaxf(all.m, l.z[j]);
       all.m = lanes_max<kWave>(all.m);
@@ -355,26 +390,28 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
       const bool first = dense.m != all.m || dense.m == -__builtin_inff();
       all.r = 0.0f;
       soft_join(all, dense, a.c, !first);
-      float one = -1e9f, s = 0.0f;
+      int one = -1;
+      for (int j = 0; first && one < 0 && j < a.k; j += kWave) {
+        const uint64_t at = __ballot(j + tid < a.k && l.id[j + tid] >= 0 && l.z[j + tid] == all.m);
+        if (at) one = j + __builtin_ctzll(at);
+      }
+      float s = 0.0f;
       for (int j = tid; j < a.k; j += kWave)
-        if (l.id[j] >= 0 && l.z[j] == all.m) one = fmaxf(one, -static_cast<float>(j));
-      one = first ? -lanes_max<kWave>(one) : -1.0f;
-      for (int j = tid; j < a.k; j += kWave)
-        if (l.id[j] >= 0 && static_cast<float>(j) != one) s += exp2_raw((l.z[j] - shift) * a.c);
+        if (l.id[j] >= 0 && j != one) s += exp2_raw((l.z[j] - shift) * a.c);
       all.r += lanes_sum<kWave>(s);
       if (all.m == -__builtin_inff()) all.r -= 1.0f;  // no class: S = 0 (or NaN)
       if (all.m == __builtin_inff()) all.r = __builtin_nanf("");
       all.S = 1.0f + all.r;
     }
-    const DistillRow r = distill_row(a, dense, all, mass.all, mass.left, &rest_loss);
-    const float log_s = log1pf(all.r);
+    const DistillRow r = distill_row<TAIL>(a, dense, all, mass.all, mass.left, &rest_loss);
+    const float log_s = log1p_of(all.r);
     for (int j = tid; j < a.k; j += kWave) {
       const float q = l.q[j];
       if (l.id[j] >= 0 && q != 0.0f)
-        loss += q * log_ratio(a, l.t[j], top, log_z, l.z[j], all.m, log_s);
+        loss += q * log_ratio<TAIL>(a, l.t[j], top, log_z, l.z[j], all.m, log_s);
     }
     loss = lanes_sum<kWave>(loss) + rest_loss;
-    if (l.wrong != 0.0f) loss = __builtin_nanf("");
+    loss += mass.poison;
     if (tid == 0) {
       const bool empty = all.m == -__builtin_inff() && all.S == 0.0f;
       DistillRow o = r;
@@ -464,11 +501,11 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
     if (id >= begin && id < end) a.list_z[row * a.k + tid] = zj;
     return;
   }
-  distill_finish<T, NT>(a, list, row, 0, z, begin, end, s, id, zj, w);
+  distill_finish<T, NT, TAIL>(a, list, row, 0, z, begin, end, s, id, zj, w);
 }
 
 // Joins the sums of a row's parts (in their order), and finishes one part.
-template <class T, int NT>
+template <class T, int NT, bool TAIL>
 __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
   __shared__ ListLds list;
   const int tid = threadIdx.x;
@@ -493,11 +530,11 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
     b.r = q.y;
     return b;
   });
-  distill_finish<T, NT>(a, list, row, part, z, begin, end, s, id, zj, w);
+  distill_finish<T, NT, TAIL>(a, list, row, part, z, begin, end, s, id, zj, w);
 }
 
 // The gradient alone, from the statistics.
-template <class T, int NT>
+template <class T, int NT, bool TAIL>
 __global__ __launch_bounds__(NT) void distill_grad_block_kernel(DistillArgs a) {
   __shared__ ListLds list;
   const int tid = threadIdx.x;
@@ -518,7 +555,7 @@ __global__ __launch_bounds__(NT) void distill_grad_block_kernel(DistillArgs a) {
   __syncthreads();
   if (tid < kWave) {
     float top, log_z;
-    (void)teacher_sums(a, list, &top, &log_z);
+    (void)teacher_sums<TAIL>(a, list, &top, &log_z);
   }
   __syncthreads();
   distill_gradient<T, NT>(a, z, out, begin, end, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, id, zj,

@@ -155,20 +155,40 @@ int take_workspace(tmnn_logits *h, hipStream_t st) {
 
 // ---- kernels by size ---------------------------------------------------------------
 
-// Rows of up to 64 vectors go to as many lanes as they have vectors (a power of two).
-int group_lanes(int64_t classes, int n) {
-  const int64_t vecs = (classes + n - 1) / n;
+// Lanes of a row in registers, 16 classes a lane (fewer where one lane holds all); 0: the
+// row is too long.
+int group_lanes(int64_t classes) {
   int g = 1;
-  while (g < vecs) g *= 2;
+  while (g <= kWave && static_cast<int64_t>(g) * 16 < classes) g *= 2;
   return g <= kWave ? g : 0;
+}
+
+// Threads of a block by the vectors of its part. A block's sums and selection cost the
+// same whatever they end, so short parts go to few threads; a long part goes to
+// many, which finish together. us at 64 / 128 / 256 / 512 / 1024 threads: log-probabilities
+// with 20 alternatives of 16384 x 5003 bf16 (625 vectors) 82 / 70 / 106 / 200 / 335, 8192 x
+// 20011 (2501) 137 / 110 / 99 / 134 / 221, 4096 x 131072 (16384) 506 / 388 / 268 / 218 / 209.
+int sum_threads(int64_t vecs) {
+  return vecs < 512 ? 64 : vecs < 1536 ? 128 : vecs < 5000 ? 256 : vecs < 12288 ? 512 : 1024;
+}
+// A block that only writes a gradient: four vectors a thread (16384 x 5003 bf16 75 / 69 / 77 /
+// 98 / 137, 4096 x 131072 431 / 435 / 420 / 407 / 385).
+int map_threads(int64_t vecs) {
+  return vecs < 512 ? 64 : vecs < 1024 ? 128 : vecs < 2048 ? 256 : vecs < 4096 ? 512 : 1024;
+}
+// Sums and gradient in one block (16384 x 5003 bf16 114 / 111 / 137 / 193 / 306, 8192 x 20011 233 /
+// 223 / 198 / 212 / 266, 4096 x 131072 841 / 703 / 650 / 586 / 490).
+int both_threads(int64_t vecs) {
+  return vecs < 512 ? 64 : vecs < 1024 ? 128 : vecs < 4096 ? 256 : vecs < 8192 ? 512 : 1024;
 }
 
 struct Split {
   int threads, parts, part_len;
 };
 
-// Threads of a block, and blocks of a row.
-Split split_of(int64_t rows, int64_t classes, int n, int at_least, int64_t blocks) {
+// Threads of a block, at least so many, and blocks of a row.
+Split split_of(int64_t rows, int64_t classes, int n, int (*threads)(int64_t), int at_least,
+               int64_t blocks) {
   Split s;
   const int64_t vecs = (classes + n - 1) / n;
   int64_t parts = 1;
@@ -179,13 +199,13 @@ Split split_of(int64_t rows, int64_t classes, int n, int at_least, int64_t block
   if (parts > 1) len = (len + 255) / 256 * 256;
   s.part_len = static_cast<int>(len);
   s.parts = static_cast<int>((classes + len - 1) / len);
-  const int64_t mine = len / n;
-  s.threads = mine >= 8192 ? 512 : mine >= 1024 ? 256 : mine >= 512 ? 128 : 64;
+  s.threads = threads((len + n - 1) / n);
   while (s.threads < at_least) s.threads *= 2;
   return s;
 }
 
 constexpr int64_t kSplitBlocks = 512;
+constexpr int kGroupTop = 4;
 
 // Rows of one launch: at most 2^31 threads, and the workspace of its parts.
 template <class F>
@@ -204,15 +224,23 @@ dim3 group_grid(int rows, int g) {
   return dim3((rows + per - 1) / per);
 }
 
-#define TMNN_BY_GROUP(g, CALL) \
-  switch (g) {                 \
-    case 1: CALL(1); break;    \
-    case 2: CALL(2); break;    \
-    case 4: CALL(4); break;    \
-    case 8: CALL(8); break;    \
-    case 16: CALL(16); break;  \
-    case 32: CALL(32); break;  \
-    default: CALL(64); break;  \
+#define TMNN_BY_GROUP(g, CALL)                          \
+  switch (g) {                                          \
+    case 1:                                             \
+      if (a.classes <= n) {                             \
+        CALL(1, 1);                                     \
+      } else if (a.classes <= 8) {                      \
+        CALL(1, 8 / n);                                 \
+      } else {                                          \
+        CALL(1, 16 / n);                                \
+      }                                                 \
+      break;                                            \
+    case 2: CALL(2, 16 / n); break;                     \
+    case 4: CALL(4, 16 / n); break;                     \
+    case 8: CALL(8, 16 / n); break;                     \
+    case 16: CALL(16, 16 / n); break;                   \
+    case 32: CALL(32, 16 / n); break;                   \
+    default: CALL(64, 16 / n); break;                   \
   }
 #define TMNN_BY_THREADS(nt, CALL) \
   switch (nt) {                   \
@@ -251,16 +279,18 @@ LogprobArgs logprob_slice(const LogprobArgs &a, int64_t at, int32_t rows) {
 template <class T>
 int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
   constexpr int n = Row<T>::n;
-  if (const int g = group_lanes(a.classes, n)) {
+  // in registers an alternative costs a round over the lane's classes
+  const int g = group_lanes(a.classes);
+  if (g != 0 && (g <= 16 || a.top_k <= kGroupTop)) {
     return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
       const LogprobArgs s = logprob_slice<T>(a, at, r);
-#define CALL(G) \
-  hipLaunchKernelGGL((logprob_group_kernel<T, G>), group_grid(r, G), dim3(kGroupThreads), 0, st, s)
+#define CALL(G, NV) \
+  hipLaunchKernelGGL((logprob_group_kernel<T, G, NV>), group_grid(r, G), dim3(kGroupThreads), 0, st, s)
       TMNN_BY_GROUP(g, CALL)
 #undef CALL
     });
   }
-  const Split sp = split_of(rows, a.classes, n, 2 * a.top_k, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, sum_threads, 2 * a.top_k, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   a.part_sum = static_cast<float4 *>(h->work.ptr);
@@ -285,17 +315,17 @@ int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
 template <class T>
 int run_logprobs_grad(LogprobArgs a, int64_t rows, hipStream_t st) {
   constexpr int n = Row<T>::n;
-  if (const int g = group_lanes(a.classes, n)) {
+  if (const int g = group_lanes(a.classes)) {
     return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
       const LogprobArgs s = logprob_slice<T>(a, at, r);
-#define CALL(G)                                                                              \
-  hipLaunchKernelGGL((logprob_grad_group_kernel<T, G>), group_grid(r, G), dim3(kGroupThreads), 0, \
+#define CALL(G, NV)                                                                          \
+  hipLaunchKernelGGL((logprob_grad_group_kernel<T, G, NV>), group_grid(r, G), dim3(kGroupThreads), 0, \
                      st, s)
       TMNN_BY_GROUP(g, CALL)
 #undef CALL
     });
   }
-  const Split sp = split_of(rows, a.classes, n, a.d_top ? a.top_k + 1 : 1, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, map_threads, a.d_top ? a.top_k + 1 : 1, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1, [&](int64_t at, int32_t r) {
@@ -324,29 +354,38 @@ DistillArgs distill_slice(const DistillArgs &a, int64_t at, int32_t rows) {
 template <class T>
 int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStream_t st) {
   constexpr int n = Row<T>::n;
-  if (const int g = group_lanes(a.classes, n)) {
+  const bool tail = a.kind == TMNN_TEACHER_LOGPROBS;
+  if (const int g = group_lanes(a.classes)) {
     return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
       const DistillArgs s = distill_slice<T>(a, at, r);
-#define CALL(G)                                                                           \
-  if (back)                                                                               \
-    hipLaunchKernelGGL((distill_group_kernel<T, G, true>), group_grid(r, G),              \
-                       dim3(kGroupThreads), 0, st, s);                                    \
-  else                                                                                    \
-    hipLaunchKernelGGL((distill_group_kernel<T, G, false>), group_grid(r, G),             \
-                       dim3(kGroupThreads), 0, st, s)
+#define LAUNCH(G, NV, TAIL, BACK)                                                            \
+  hipLaunchKernelGGL((distill_group_kernel<T, G, NV, TAIL, BACK>), group_grid(r, G),         \
+                     dim3(kGroupThreads), 0, st, s)
+#define CALL(G, NV)                                                                          \
+  if (tail && back) LAUNCH(G, NV, true, true);                                               \
+  else if (tail) LAUNCH(G, NV, true, false);                                                 \
+  else if (back) LAUNCH(G, NV, false, true);                                                 \
+  else LAUNCH(G, NV, false, false)
       TMNN_BY_GROUP(g, CALL)
 #undef CALL
+#undef LAUNCH
     });
   }
-  const Split sp = split_of(rows, a.classes, n, a.k, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, back ? map_threads : a.d_logits ? both_threads : sum_threads,
+                            a.k, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   if (back)
     return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1,
                      [&](int64_t at, int32_t r) {
                        const DistillArgs s = distill_slice<T>(a, at, r);
-#define CALL(NT) \
-  hipLaunchKernelGGL((distill_grad_block_kernel<T, NT>), dim3(r * a.parts), dim3(NT), 0, st, s)
+#define CALL(NT)                                                                                    \
+  if (tail)                                                                                         \
+    hipLaunchKernelGGL((distill_grad_block_kernel<T, NT, true>), dim3(r * a.parts), dim3(NT), 0, st, \
+                       s);                                                                          \
+  else                                                                                              \
+    hipLaunchKernelGGL((distill_grad_block_kernel<T, NT, false>), dim3(r * a.parts), dim3(NT), 0,   \
+                       st, s)
                        TMNN_BY_THREADS(sp.threads, CALL)
 #undef CALL
                      });
@@ -361,7 +400,7 @@ int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStrea
                      const DistillArgs s = distill_slice<T>(a, at, r);
                      const size_t bits = (static_cast<size_t>(sp.part_len) + 31) / 32 * 4;
 #define CALL(NT)                                                                                   \
-  if (a.kind == TMNN_TEACHER_LOGPROBS)                                                             \
+  if (tail)                                                                                        \
     hipLaunchKernelGGL((distill_block_kernel<T, NT, true>), dim3(r * a.parts), dim3(NT), bits, st, \
                        s);                                                                         \
   else                                                                                             \
@@ -370,7 +409,11 @@ int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStrea
 #undef CALL
                      if (a.parts > 1) {
                        const dim3 grid(r * (a.d_logits ? a.parts : 1));
-#define CALL(NT) hipLaunchKernelGGL((distill_join_kernel<T, NT>), grid, dim3(NT), 0, st, s)
+#define CALL(NT)                                                                            \
+  if (tail)                                                                                 \
+    hipLaunchKernelGGL((distill_join_kernel<T, NT, true>), grid, dim3(NT), 0, st, s);       \
+  else                                                                                      \
+    hipLaunchKernelGGL((distill_join_kernel<T, NT, false>), grid, dim3(NT), 0, st, s)
                        TMNN_BY_THREADS(sp.threads, CALL)
 #undef CALL
                      }
@@ -432,7 +475,8 @@ int distill_device(tmnn_logits *h, const tmnn_distill_args &u, bool back, hipStr
   a.k = u.teacher_k;
   a.parts = 1;
   a.t = u.temperature;
-  a.inv_t = static_cast<float>(1.0 / u.temperature);
+  a.inv_t64 = 1.0 / static_cast<double>(u.temperature);
+  a.inv_t = static_cast<float>(a.inv_t64);
   a.c = static_cast<float>(1.4426950408889634 / u.temperature);
   a.loss = back ? nullptr : u.loss;
   a.stats = u.stats;

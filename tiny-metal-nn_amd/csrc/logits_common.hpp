@@ -34,6 +34,7 @@ struct Row;
 template <>
 struct Row<float> {
   static constexpr int n = 4;
+  typedef f32x4v A;  // aligned to itself, as in LDS
   typedef f32x4v V __attribute__((aligned(4)));
   static __device__ __forceinline__ float up(float x) { return x; }
   static __device__ __forceinline__ float down(float x) { return x; }
@@ -41,6 +42,7 @@ struct Row<float> {
 template <>
 struct Row<_Float16> {
   static constexpr int n = 8;
+  typedef f16x8v A;
   typedef f16x8v V __attribute__((aligned(2)));
   static __device__ __forceinline__ float up(_Float16 x) { return static_cast<float>(x); }
   static __device__ __forceinline__ _Float16 down(float x) { return static_cast<_Float16>(x); }
@@ -48,6 +50,7 @@ struct Row<_Float16> {
 template <>
 struct Row<__bf16> {
   static constexpr int n = 8;
+  typedef bf16x8v A;
   typedef bf16x8v V __attribute__((aligned(2)));
   static __device__ __forceinline__ float up(__bf16 x) { return static_cast<float>(x); }
   static __device__ __forceinline__ __bf16 down(float x) { return static_cast<__bf16>(x); }
@@ -97,12 +100,35 @@ __device__ __forceinline__ int64_t load_index(const void *p, int64_t i, bool wid
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// a / b and ln x to an ulp or two, without the steps that make them exact.
+__device__ __forceinline__ float quotient(float a, float b) { return a * __builtin_amdgcn_rcpf(b); }
+__device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * kLn2; }
+
+// e^t: the product t log2(e) in two parts, so that its rounding does not grow with t.
+__device__ __forceinline__ float exp_of(float t) {
+  constexpr float l = 1.44269504f, l_rest = 1.925963033e-8f;  // log2(e)
+  const float x = t * l;
+  const float rest = __builtin_fmaf(t, l_rest, __builtin_fmaf(t, l, -x));
+  return x > -150.0f ? exp2_raw(x) * __builtin_fmaf(rest, kLn2, 1.0f) : 0.0f;
+}
+
+// ln(1 + r), r >= -1, by what rounding 1 + r leaves out: ln u + (r - (u - 1)) / u. The
+// hardware's log2 is good to an ulp of its result.
+__device__ __forceinline__ float log1p_of(float r) {
+  const float u = 1.0f + r;
+  const float rest = (r - (u - 1.0f)) * __builtin_amdgcn_rcpf(u);
+  const float l = __builtin_amdgcn_logf(u);
+  // u = 0, inf and NaN leave no rest
+  return u > 0.0f && u < __builtin_inff() ? __builtin_fmaf(l, kLn2, rest) : l;
+}
+
 // ---- sums over G consecutive lanes (all lanes get the result) ----------------
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
-  const int v = __float_as_int(x);
-  return __int_as_float(__builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false));
+  // (every lane's source lane exists: no old value, so that the step is part of the
+  // instruction that takes it)
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
 
 // Lanes 1, 2, 4, 8 apart by DPP (quad permutations, then the mirror of 8 and of
@@ -135,24 +161,68 @@ template <int G>
 __device__ __forceinline__ float lanes_sum(float x) {
   return over_lanes<G>(x, [](float a, float b) { return a + b; });
 }
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t v = __double_as_longlong(x);
+  const uint32_t lo = static_cast<uint32_t>(v), hi = static_cast<uint32_t>(v >> 32);
+  const uint32_t l = __builtin_amdgcn_update_dpp(0, lo, CTRL, 0xf, 0xf, true);
+  const uint32_t h = __builtin_amdgcn_update_dpp(0, hi, CTRL, 0xf, 0xf, true);
+  return __longlong_as_double(static_cast<uint64_t>(h) << 32 | l);
+}
 template <int G>
 __device__ __forceinline__ double lanes_sum(double x) {
-  for (int off = 1; off < G; off *= 2) x += __shfl_xor(x, off, kWave);
+  if (G >= 2) x += dpp<0xB1>(x);
+  if (G >= 4) x += dpp<0x4E>(x);
+  if (G >= 8) x += dpp<0x141>(x);
+  if (G >= 16) x += dpp<0x140>(x);
+  if (G >= 32) x += __shfl_xor(x, 16);
+  if (G >= 64) x += __shfl_xor(x, 32);
   return x;
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
 }
 template <int G>
 __device__ __forceinline__ int lanes_isum(int x) {
-  return __float_as_int(over_lanes<G>(__int_as_float(x), [](float a, float b) {
-    return __int_as_float(__float_as_int(a) + __float_as_int(b));
-  }));
+  uint32_t v = static_cast<uint32_t>(x);
+  if (G >= 2) v += dpp<0xB1>(v);
+  if (G >= 4) v += dpp<0x4E>(v);
+  if (G >= 8) v += dpp<0x141>(v);
+  if (G >= 16) v += dpp<0x140>(v);
+  if (G >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = r[0] + r[1];
+  }
+  if (G >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = r[0] + r[1];
+  }
+  return static_cast<int>(v);
 }
 template <int G>
 __device__ __forceinline__ uint64_t lanes_key_max(uint64_t k) {
-  for (int off = G / 2; off > 0; off >>= 1) {
-    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(k), off, kWave);
-    k = o > k ? o : k;
-  }
-  return k;
+  uint32_t hi = static_cast<uint32_t>(k >> 32), lo = static_cast<uint32_t>(k);
+  auto take = [&](uint32_t h, uint32_t l) {
+    const bool more = h > hi || (h == hi && l > lo);
+    hi = more ? h : hi;
+    lo = more ? l : lo;
+  };
+  if (G >= 2) take(dpp<0xB1>(hi), dpp<0xB1>(lo));
+  if (G >= 4) take(dpp<0x4E>(hi), dpp<0x4E>(lo));
+  if (G >= 8) take(dpp<0x141>(hi), dpp<0x141>(lo));
+  if (G >= 16) take(dpp<0x140>(hi), dpp<0x140>(lo));
+  if (G >= 32) take(__shfl_xor(hi, 16), __shfl_xor(lo, 16));
+  if (G >= 64) take(__shfl_xor(hi, 32), __shfl_xor(lo, 32));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// Whether `c` holds in one of the G lanes.
+template <int G>
+__device__ __forceinline__ bool lanes_any(bool c) {
+  const uint64_t all = __ballot(c);
+  if (G == kWave) return all != 0;
+  const int lane = threadIdx.x & (kWave - 1) & ~(G - 1);
+  return (all >> lane & ((1ull << (G & 63)) - 1ull)) != 0;
 }
 
 // Orders the LDS accesses of one wave's lanes (lockstep: a compiler fence).

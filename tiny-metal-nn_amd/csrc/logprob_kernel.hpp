@@ -50,8 +50,8 @@ __device__ __forceinline__ void put_row(const LogprobArgs &a, int64_t row, const
   const float nan = __builtin_nanf(""), inf = __builtin_inff();
   const float m = s.m, S = s.S, E = s.E;
   const bool empty = S == 0.0f, bad = !(S < inf) || m == inf;
-  const float log_s = log1pf(s.r);
-  if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.0f : log_s - kLn2 * (E / S);
+  const float log_s = log1p_of(s.r);
+  if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.0f : log_s - kLn2 * quotient(E, S);
   if (a.stats) {
     a.stats[2 * row] = m;
     a.stats[2 * row + 1] = bad ? nan : S;
@@ -82,63 +82,205 @@ __device__ __forceinline__ void put_no_top(const LogprobArgs &a, int64_t row, in
 
 constexpr int kGroupThreads = 256;
 
-template <class T, int G>
+// A row in the registers of G lanes, NV vectors each: vector u of a lane holds the
+// classes from (u G + lane) N on. Few lanes a row keep what a row costs beyond its
+// classes (sums over lanes, logarithms) in few instructions: 2^18 rows of 16 fp32
+// classes take 16.6 us (distillation) on four lanes a row, and 18.9 us on one lane
+// whose 16-byte accesses lie 64 bytes apart. One lane a row therefore takes its wave's
+// rows, where they are adjacent, through LDS.
+template <class T, int G, int NV>
+struct Group {
+  static constexpr int N = Row<T>::n, E = N * NV;
+  static constexpr int rows = kGroupThreads / G;
+  // LDS words a lane, so that 16 lanes' 16-byte accesses meet different banks
+  static constexpr int pitch = E % 8 == 0 ? E + 4 : E;
+  static constexpr int words = kGroupThreads * pitch;
+  int lane;
+  int64_t row;
+  __device__ __forceinline__ Group()
+      : lane(threadIdx.x & (G - 1)),
+        row(static_cast<int64_t>(blockIdx.x) * rows + threadIdx.x / G) {}
+  __device__ __forceinline__ int at(int u) const { return (u * G + lane) * N; }
+  __device__ __forceinline__ int index(int e) const { return at(e / N) + e % N; }
+
+  // The rows of the wave as one run of elements in LDS; a free vector after every
+  // fourth keeps rows of four from meeting in the same banks.
+  static __device__ __forceinline__ int slot(int element) {
+    const int q = element / N;
+    return (q + q / 4) * N + element % N;
+  }
+  struct Run {
+    T *lds;
+    int64_t first;  // element of the run's start
+    int n, lane;
+  };
+  __device__ __forceinline__ Run run_of(int *word, int64_t all_rows, int classes) const {
+    const int wave = threadIdx.x / kWave;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * rows + wave * kWave;
+    const int64_t left = all_rows - first;
+    Run r;
+    r.lds = reinterpret_cast<T *>(word + wave * kWave * pitch);
+    r.first = first * classes;
+    r.n = left <= 0 ? 0 : static_cast<int>(left < kWave ? left : kWave) * classes;
+    r.lane = threadIdx.x & (kWave - 1);
+    return r;
+  }
+  static constexpr int kSteps = (E + N - 1) / N;  // vectors a lane moves of a full run
+
+  // The row's classes (-inf where it is not `live` and past its end).
+  __device__ __forceinline__ void load_rows(const void *logits, int64_t stride, int64_t all_rows,
+                                            int classes, bool live, int *word, float *v) const {
+    if (G == 1 && NV > 1 && stride == classes) {
+      const Run r = run_of(word, all_rows, classes);
+      const T *z = static_cast<const T *>(logits) + r.first;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int o = (i * kWave + r.lane) * N;
+        if (o + N <= r.n)
+          *reinterpret_cast<typename Row<T>::A *>(r.lds + slot(o)) = load_raw(z + o);
+        else
+          for (int j = o; j < r.n; ++j) r.lds[slot(j)] = z[j];
+      }
+      wave_fence();
+      const int mine = r.lane * classes;
+      if (classes % N == 0) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          if (live && u * N < classes) {
+            const typename Row<T>::A raw = *reinterpret_cast<const typename Row<T>::A *>(r.lds + slot(mine + u * N));
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u * N + j] = Row<T>::up(raw[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u * N + j] = -__builtin_inff();
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          v[e] = live && e < classes ? Row<T>::up(r.lds[slot(mine + e)]) : -__builtin_inff();
+      }
+      wave_fence();
+      return;
+    }
+    const T *z = static_cast<const T *>(logits) + (live ? row : 0) * stride;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) load_vec<T>(z, at(u), live ? classes : 0, v + u * N);
+  }
+  // Every lane of the wave calls it; what the LDS words held is gone.
+  __device__ __forceinline__ void store_rows(void *out, int64_t stride, int64_t all_rows,
+                                             int classes, int *word, const float *v) const {
+    if (G == 1 && NV > 1 && stride == classes) {
+      const Run r = run_of(word, all_rows, classes);
+      T *z = static_cast<T *>(out) + r.first;
+      const int mine = r.lane * classes;
+      wave_fence();
+      if (classes % N == 0) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+          if (u * N < classes) {
+            typename Row<T>::A raw;
+#pragma unroll
+            for (int j = 0; j < N; ++j) raw[j] = Row<T>::down(v[u * N + j]);
+            *reinterpret_cast<typename Row<T>::A *>(r.lds + slot(mine + u * N)) = raw;
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (e < classes) r.lds[slot(mine + e)] = Row<T>::down(v[e]);
+      }
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int o = (i * kWave + r.lane) * N;
+        if (o + N <= r.n)
+          *reinterpret_cast<typename Row<T>::V *>(z + o) =
+              *reinterpret_cast<const typename Row<T>::A *>(r.lds + slot(o));
+        else
+          for (int j = o; j < r.n; ++j) z[j] = r.lds[slot(j)];
+      }
+      return;
+    }
+    if (row >= all_rows) return;
+    T *z = static_cast<T *>(out) + row * stride;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) store_vec<T>(z, at(u), classes, v + u * N);
+  }
+};
+
+template <class T, int G, int NV>
 __global__ __launch_bounds__(kGroupThreads) void logprob_group_kernel(LogprobArgs a) {
-  constexpr int N = Row<T>::n;
-  const int lane = threadIdx.x & (G - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kGroupThreads / G) + threadIdx.x / G;
+  constexpr int N = Row<T>::n, E = N * NV;
+  __shared__ __attribute__((aligned(16))) int words[G == 1 ? Group<T, G, NV>::words : 1];
+  const Group<T, G, NV> g;
+  const int64_t row = g.row;
   const bool live = row < a.rows;
-  const T *z = static_cast<const T *>(a.logits) + (live ? row : 0) * a.row_stride;
-  float v[N];
-  load_vec<T>(z, lane * N, live ? a.classes : 0, v);
   int64_t token = -1;
   if (live && a.tokens) token = load_index(a.tokens, row, a.wide_index);
-  const bool known = token >= 0 && token < a.classes;
-  const float zt = known ? Row<T>::up(z[token]) : 0.0f;
+  float v[E];
+  g.load_rows(a.logits, a.row_stride, a.rows, a.classes, live, words, v);
   float m = v[0];
 #pragma unroll
-  for (int j = 1; j < N; ++j) m = fmaxf(m, v[j]);
+  for (int e = 1; e < E; ++e) m = fmaxf(m, v[e]);
   m = lanes_max<G>(m);
+  // the token's logit, from the lane that holds it
+  float zt = 0.0f;
+  const int tok = token >= 0 && token < a.classes ? static_cast<int>(token) : 0;
+  if (a.tokens) {
+    float mine = v[0];
+    const int which = tok / (G * N) * N + (tok & (N - 1));
+#pragma unroll
+    for (int e = 1; e < E; ++e) mine = which == e ? v[e] : mine;
+    zt = G == 1 ? mine : __shfl(mine, tok / N & (G - 1), G);
+  }
   const float shift = m == -__builtin_inff() ? 0.0f : m;
   Soft s;
   s.m = m;
   s.r = 0.0f;
   int rank = 0, best_n = 0;  // best_n: classes of the largest logit, whose terms are 1
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float x = (v[j] - shift) * a.c, e = exp2_raw(x);
-    s.r += v[j] == m ? 0.0f : e;
-    best_n += v[j] == m;
-    s.E = __builtin_fmaf(e, fmaxf(x, -200.0f), s.E);
-    rank += v[j] > zt || (v[j] == zt && lane * N + j < token);
+  for (int e = 0; e < E; ++e) {
+    const float x = (v[e] - shift) * a.c, p = exp2_raw(x);
+    s.r += v[e] == m ? 0.0f : p;
+    best_n += v[e] == m;
+    s.E = __builtin_fmaf(p, fmaxf(x, -200.0f), s.E);
+    rank += v[e] > zt || (v[e] == zt && g.index(e) < tok);
   }
   s.r = lanes_sum<G>(s.r);
   s.E = lanes_sum<G>(s.E);
-  rank = lanes_isum<G>(rank);
+  if (a.tokens) rank = lanes_isum<G>(rank);
   best_n = lanes_isum<G>(best_n);
   if (m == -__builtin_inff()) best_n = 0;
   if (m == __builtin_inff()) s.r = __builtin_nanf("");
   s.r += static_cast<float>(best_n - 1);
   s.S = 1.0f + s.r;
-  if (live && lane == 0) put_row(a, row, s, token, zt, rank);
+  if (live && g.lane == 0) put_row(a, row, s, token, zt, rank);
   if (a.top_k == 0) return;
   const bool bad = !(s.S < __builtin_inff());
-  const float log_s = log1pf(s.r);
-  uint64_t key[N];
+  const float log_s = log1p_of(s.r);
+  // one round an alternative: the largest value, then the first class that has it
+  uint32_t key[E];
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    key[j] = v[j] > -__builtin_inff() && !bad ? key_of(v[j], lane * N + j) : 0;
+  for (int e = 0; e < E; ++e)
+    key[e] = v[e] > -__builtin_inff() && !bad ? order_of(v[e]) : 0;
   for (int k = 0; k < a.top_k; ++k) {
-    uint64_t best = key[0];
+    uint32_t best = key[0];
 #pragma unroll
-    for (int j = 1; j < N; ++j) best = key[j] > best ? key[j] : best;
-    best = lanes_key_max<G>(best);
+    for (int e = 1; e < E; ++e) best = key[e] > best ? key[e] : best;
+    uint64_t q = best;
+    int mine = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (key[j] == best) key[j] = 0;
-    if (live && lane == (k & (G - 1))) {
+    for (int e = E - 1; e >= 0; --e) mine = key[e] == best ? e : mine;
+    const int at = (mine / N * G + g.lane) * N + (mine & (N - 1));
+    q = lanes_key_max<G>(q << 32 | (0xffffffffu - static_cast<uint32_t>(at)));
+    best = static_cast<uint32_t>(q >> 32);
+    const bool ours = key_index(q) == at;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (ours && mine == e) key[e] = 0;
+    if (live && g.lane == (k & (G - 1))) {
       if (best != 0)
-        put_top(a, row, k, value_of(static_cast<uint32_t>(best >> 32)), key_index(best), m, log_s);
+        put_top(a, row, k, value_of(best), key_index(q), m, log_s);
       else
         put_no_top(a, row, k, bad);
     }
@@ -153,20 +295,23 @@ struct BlockLds {
   int n[NT / kWave];
 };
 
-// The block's sum from its threads', in every thread, and the total of `n`.
+// The block's sum from its threads', in every thread; with ENT also E and the total
+// of `n`.
 template <int NT, bool ENT>
 __device__ __forceinline__ Soft soft_block(BlockLds<NT> &l, Soft s, float c, int &n) {
   constexpr int W = NT / kWave;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   soft_lanes<kWave, ENT>(s, c);
-  n = lanes_isum<kWave>(n);
+  if (ENT) n = lanes_isum<kWave>(n);
   if (W == 1) return s;
   if (lane == 0) {
     l.m[wave] = s.m;
     l.R[wave] = s.R;
     l.S[wave] = s.S;
-    l.E[wave] = s.E;
-    l.n[wave] = n;
+    if (ENT) {
+      l.E[wave] = s.E;
+      l.n[wave] = n;
+    }
   }
   __syncthreads();
   const int i = lane & (W - 1);
@@ -174,8 +319,10 @@ __device__ __forceinline__ Soft soft_block(BlockLds<NT> &l, Soft s, float c, int
   o.m = l.m[i];
   o.R = l.R[i];
   o.S = l.S[i];
-  o.E = l.E[i];
-  n = lanes_isum<W>(l.n[i]);
+  if (ENT) {
+    o.E = l.E[i];
+    n = lanes_isum<W>(l.n[i]);
+  }
   soft_lanes<W, ENT>(o, c);
   return o;
 }
@@ -345,7 +492,7 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
   }
   if (a.top_k == 0) return;
   const bool bad = !(s.S < __builtin_inff()) || s.m == __builtin_inff();
-  const float log_s = log1pf(s.r);
+  const float log_s = log1p_of(s.r);
   int got = 0;
   if (!bad && s.S != 0.0f) {
     const uint64_t key =
@@ -403,7 +550,7 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
     put_row(a, row, s, token, zt, rank);
   }
   if (a.top_k == 0) return;
-  const float m = s.m, log_s = log1pf(s.r);
+  const float m = s.m, log_s = log1p_of(s.r);
   int got = 0;
   if (!bad && s.S != 0.0f) {
     const uint64_t *keys = a.part_key + row * a.parts * a.top_k;
@@ -446,7 +593,7 @@ __device__ __forceinline__ LogprobRow logprob_row(const LogprobArgs &a, int64_t 
   const float gh = a.d_entropy ? a.d_entropy[row] : 0.0f;
   r.token = token < a.classes ? static_cast<int>(token) : -1;
   const float h = gh != 0.0f ? spread(S) : 0.0f;
-  const float scale = a.inv_t / S;
+  const float scale = quotient(a.inv_t, S);
   r.a = -(g + top_sum + gh * h) * scale;
   r.b = -gh * kLn2 * scale;
   r.g_token = g * a.inv_t;
@@ -455,69 +602,110 @@ __device__ __forceinline__ LogprobRow logprob_row(const LogprobArgs &a, int64_t 
   return r;
 }
 
-template <class T, int G>
+// LDS words of a group's rows: kUnlisted, or what a listed class brings.
+constexpr int kUnlisted = 0x7fffffff;
+
+// A word for each class of the block's rows, laid out as the lanes hold them.
+template <class T, int G, int NV>
+struct GroupWords {
+  static constexpr int N = Row<T>::n, pitch = Group<T, G, NV>::pitch;
+  __attribute__((aligned(16))) int word[kGroupThreads * pitch];
+  // of this lane's classes, and of a class of this lane's row
+  __device__ __forceinline__ int *lane() { return word + threadIdx.x * pitch; }
+  __device__ __forceinline__ int &of(int id) {
+    const int row = threadIdx.x & ~(G - 1);
+    return word[(row + (id / N & (G - 1))) * pitch + id / (N * G) * N + (id & (N - 1))];
+  }
+};
+
+template <class T, int G, int NV>
 __global__ __launch_bounds__(kGroupThreads) void logprob_grad_group_kernel(LogprobArgs a) {
-  constexpr int N = Row<T>::n;
-  __shared__ int owner[kGroupThreads * N];    // the first entry that lists a class
-  __shared__ float extra[kGroupThreads * N];  // its term
-  const int lane = threadIdx.x & (G - 1);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kGroupThreads / G) + threadIdx.x / G;
+  constexpr int N = Row<T>::n, E = N * NV;
+  __shared__ GroupWords<T, G, NV> words;  // the first entry that lists a class, then its term
+  const Group<T, G, NV> g;
+  const int64_t row = g.row;
   const bool live = row < a.rows;
-  const T *z = static_cast<const T *>(a.logits) + (live ? row : 0) * a.row_stride;
-  float v[N];
-  load_vec<T>(z, lane * N, live ? a.classes : 0, v);
-  int *own = owner + (threadIdx.x - lane) * N;
-  float *ext = extra + (threadIdx.x - lane) * N;
+  float v[E];
+  g.load_rows(a.logits, a.row_stride, a.rows, a.classes, live, words.word, v);
   const int k = live && a.d_top ? a.top_k : 0;
-  float top_sum = 0.0f, any = 0.0f;
+  int *mine = words.lane();
+  float top_sum = 0.0f;
+  bool any = false;
   if (a.d_top) {
+    constexpr int kKept = G <= 4 ? 4 / G : 1;
+    int id[kKept];
+    float term[kKept];
+    auto entry = [&](int j, int &i, float &t) {
+      i = a.top_in[row * a.top_k + j];
+      t = a.d_top[row * a.top_k + j];
+      if (i >= a.classes) i = -1;
+    };
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      own[lane * N + j] = 0x7fffffff;
-      ext[lane * N + j] = 0.0f;
+    for (int e = 0; e < kKept; ++e) {
+      id[e] = -1;
+      if (g.lane + e * G < k) entry(g.lane + e * G, id[e], term[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) mine[e] = kUnlisted;
+    wave_fence();
+#pragma unroll
+    for (int e = 0; e < kKept; ++e)
+      if (id[e] >= 0) atomicMin(&words.of(id[e]), g.lane + e * G);
+    for (int j = g.lane + kKept * G; j < k; j += G) {
+      int i;
+      float t;
+      entry(j, i, t);
+      if (i >= 0) atomicMin(&words.of(i), j);
     }
     wave_fence();
-    for (int j = lane; j < k; j += G) {
-      const int id = a.top_in[row * a.top_k + j];
-      if (id >= 0 && id < a.classes) atomicMin(&own[id], j);
+    // Kept entries look before any term goes in; the others may meet a term, whose bits
+    // are no entry's number (a term too small to be normal counts as 0).
+    bool first[kKept];
+#pragma unroll
+    for (int e = 0; e < kKept; ++e)
+      first[e] = id[e] >= 0 && words.of(id[e]) == g.lane + e * G;
+    auto put = [&](int i, float t) {
+      const float d = t * a.inv_t;
+      words.of(i) = fabsf(d) < 1.2e-38f ? 0 : __float_as_int(d);
+      top_sum += t;
+      any |= t != 0.0f;
+    };
+    for (int j = g.lane + kKept * G; j < k; j += G) {
+      int i;
+      float t;
+      entry(j, i, t);
+      if (i >= 0 && words.of(i) == j) put(i, t);
     }
-    wave_fence();
-    for (int j = lane; j < k; j += G) {
-      const int id = a.top_in[row * a.top_k + j];
-      if (id >= 0 && id < a.classes && own[id] == j) {
-        const float g = a.d_top[row * a.top_k + j];
-        ext[id] = g * a.inv_t;
-        top_sum += g;
-        if (g != 0.0f) any = 1.0f;
-      }
-    }
+#pragma unroll
+    for (int e = 0; e < kKept; ++e)
+      if (first[e]) put(id[e], term[e]);
     wave_fence();
     top_sum = lanes_sum<G>(top_sum);
-    any = lanes_max<G>(any);
+    any = lanes_any<G>(any);
   }
   const float m = live ? a.stats_in[2 * row] : 0.0f;
-  float x[N], e[N], E = 0.0f;
+  float x[E], p[E], sum = 0.0f;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    x[j] = (v[j] - m) * a.c;
-    e[j] = exp2_raw(x[j]);
-    x[j] = fmaxf(x[j], -200.0f);
-    E = __builtin_fmaf(e[j], x[j], E);
+  for (int e = 0; e < E; ++e) {
+    x[e] = (v[e] - m) * a.c;
+    p[e] = exp2_raw(x[e]);
+    x[e] = fmaxf(x[e], -200.0f);
+    sum = __builtin_fmaf(p[e], x[e], sum);
   }
   // H - ln S from the row itself: the entropy's own rounding does not enter
-  E = lanes_sum<G>(E);
-  if (!live) return;
-  const LogprobRow r =
-      logprob_row(a, row, top_sum, any != 0.0f, [&](float S) { return -kLn2 * (E / S); });
-  float d[N];
+  sum = lanes_sum<G>(sum);
+  LogprobRow r{};
+  r.token = -1;
+  if (live)
+    r = logprob_row(a, row, top_sum, any, [&](float S) { return -kLn2 * quotient(sum, S); });
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    float t = e[j] * __builtin_fmaf(r.b, x[j], r.a);
-    if (a.d_top) t += ext[lane * N + j];
-    if (lane * N + j == r.token) t += r.g_token;
-    d[j] = r.skip ? 0.0f : t;
+  for (int e = 0; e < E; ++e) {
+    float t = p[e] * __builtin_fmaf(r.b, x[e], r.a);
+    if (a.d_top && mine[e] != kUnlisted) t += __int_as_float(mine[e]);
+    if (g.index(e) == r.token) t += r.g_token;
+    v[e] = r.skip ? 0.0f : t;
   }
-  store_vec<T>(static_cast<T *>(a.d_logits) + row * a.d_row_stride, lane * N, a.classes, d);
+  g.store_rows(a.d_logits, a.d_row_stride, a.rows, a.classes, words.word, v);
 }
 
 // Writes f(z) for the classes begin .. end of a row, all of a block's threads.
@@ -593,16 +781,17 @@ __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
     }
     __syncthreads();
     if (tid < kWave) {
-      float s = 0.0f, any = 0.0f;
+      float s = 0.0f;
+      bool any = false;
       for (int j = tid; j < k; j += kWave) {
         s += term[j];
-        if (term[j] != 0.0f) any = 1.0f;
+        any |= term[j] != 0.0f;
       }
       s = lanes_sum<kWave>(s);
-      any = lanes_max<kWave>(any);
+      any = lanes_any<kWave>(any);
       if (tid == 0) {
         sums[0] = s;
-        sums[1] = any;
+        sums[1] = any ? 1.0f : 0.0f;
       }
     }
     __syncthreads();
@@ -610,7 +799,7 @@ __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
     top_any = sums[1] != 0.0f;
   }
   const LogprobRow r = logprob_row(a, row, top_sum, top_any,
-                                   [&](float S) { return a.entropy_in[row] - logf(S); });
+                                   [&](float S) { return a.entropy_in[row] - log_of(S); });
   if (r.skip) {
     zero_part<T, NT>(out, begin, end);
     return;
