@@ -284,37 +284,42 @@ __global__ __launch_bounds__(kGroupThreads) void distill_group_kernel(DistillArg
 // ---- long rows ---------------------------------------------------------------------
 
 struct ListLds {
-  int id[kMaxTeacher];
+  __attribute__((aligned(16))) int id[kMaxTeacher];
   float z[kMaxTeacher], t[kMaxTeacher], q[kMaxTeacher];
   float wrong;
   DistillRow row;
   float scale;
 };
 
-// The listed classes: -1 for unused entries and for classes listed before (the
-// first entry counts). An entry beyond the classes makes the row NaN. NT >= k.
-template <int NT>
-__device__ __forceinline__ int read_list(const DistillArgs &a, ListLds &l, int64_t row) {
+// The thread's entry: its class, or -1 for an unused entry. An entry beyond the classes
+// makes the row NaN. NT >= k.
+__device__ __forceinline__ int list_entry(const DistillArgs &a, int64_t row, bool *wrong) {
+  const int tid = threadIdx.x;
+  if (tid >= a.k) return -1;
+  const int64_t i = load_index(a.ids, row * a.k + tid, a.wide_index);
+  if (i >= a.classes) *wrong = true;
+  return i >= 0 && i < a.classes ? static_cast<int>(i) : -1;
+}
+
+// Puts the entries into LDS; a class counts by its first entry (the others: -1). Returns
+// the thread's.
+__device__ __forceinline__ int put_list(const DistillArgs &a, ListLds &l, int64_t row, int id,
+                                        float z, bool wrong) {
   const int tid = threadIdx.x;
   if (tid == 0) l.wrong = 0.0f;
-  __syncthreads();
-  int id = -1;
-  if (tid < a.k) {
-    const int64_t i = load_index(a.ids, row * a.k + tid, a.wide_index);
-    if (i >= a.classes) l.wrong = __builtin_nanf("");  // every writer writes the same
-    id = i >= 0 && i < a.classes ? static_cast<int>(i) : -1;
+  if (tid < ((a.k + 3) & ~3)) {
     l.id[tid] = id;
-    l.t[tid] = a.teacher[row * a.k + tid];
+    if (tid < a.k) {
+      l.t[tid] = a.teacher[row * a.k + tid];
+      l.z[tid] = z;
+    }
   }
   __syncthreads();
-  if (id >= 0)
-    for (int j = 0; j < tid; ++j)
-      if (l.id[j] == id) {
-        id = -1;
-        break;
-      }
+  const bool again = tid < a.k && id >= 0 && listed_before(l.id, a.k, tid, id);
+  if (wrong) l.wrong = __builtin_nanf("");  // every writer writes the same
   __syncthreads();
-  if (tid < a.k) l.id[tid] = id;
+  if (again) l.id[tid] = id = -1;
+  __syncthreads();
   return id;
 }
 
@@ -348,12 +353,13 @@ __device__ __forceinline__ TeacherMass teacher_sums(const DistillArgs &a, ListLd
   return m;
 }
 
-// Writes the gradient of a part: all classes as unlisted ones, then the listed.
-// The caller has read the listed logits and synchronised since.
-template <class T, int NT>
+// Writes the gradient of a part: all classes as unlisted ones, then the listed; between
+// the two listed() returns the thread's class (-1: none) and its q. The thread's logit
+// zj has been read.
+template <class T, int NT, class Listed>
 __device__ __forceinline__ void distill_gradient(const DistillArgs &a, const T *z, T *out,
                                                  int begin, int end, const DistillRow &r,
-                                                 float scale, int id, float zj, float q) {
+                                                 float scale, float zj, Listed listed) {
   if (r.m_a == -__builtin_inff() && r.a_a == r.a_a) {  // every class is masked
     zero_part<T, NT>(out, begin, end);
     return;
@@ -364,6 +370,8 @@ __device__ __forceinline__ void distill_gradient(const DistillArgs &a, const T *
     map_part<T, NT>(z, out, begin, end, [&](float v) { return f * exp2_raw(e.x_huge(v)); });
   else
     map_part<T, NT>(z, out, begin, end, [&](float v) { return f * exp2_raw(e.x_plain(v)); });
+  float q;
+  const int id = listed(&q);
   __syncthreads();
   if (id >= begin && id < end)
     out[id] = Row<T>::down(scale * (r.a_a * exp2_raw((zj - r.m_a) * a.c) - q));
@@ -375,8 +383,6 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
                                                int part, const T *z, int begin, int end,
                                                const Soft &dense, int id, float zj, float w) {
   const int tid = threadIdx.x;
-  if (tid < a.k) l.z[tid] = zj;
-  __syncthreads();
   if (tid < kWave) {
     float top, log_z, rest_loss, loss = 0.0f;
     const TeacherMass mass = teacher_sums<TAIL>(a, l, &top, &log_z);
@@ -427,8 +433,10 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
   __syncthreads();
   if (!a.d_logits) return;
   T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
-  distill_gradient<T, NT>(a, z, out, begin, end, l.row, w * a.t, id, zj,
-                          tid < a.k ? l.q[tid] : 0.0f);
+  distill_gradient<T, NT>(a, z, out, begin, end, l.row, w * a.t, zj, [&](float *q) {
+    *q = tid < a.k ? l.q[tid] : 0.0f;
+    return id;
+  });
 }
 
 // A row of weight 0 is not read.
@@ -464,7 +472,9 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
   }
   if (TAIL)
     for (int i = tid; i * 32 < end - begin; i += NT) listed[i] = 0u;
-  const int id = read_list<NT>(a, list, row);
+  if (TAIL) __syncthreads();
+  bool wrong = false;
+  int id = list_entry(a, row, &wrong);
   float zj = 0.0f;
   if (id >= begin && id < end) {
     zj = Row<T>::up(z[id]);
@@ -501,6 +511,7 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
     if (id >= begin && id < end) a.list_z[row * a.k + tid] = zj;
     return;
   }
+  id = put_list(a, list, row, id, zj, wrong);
   distill_finish<T, NT, TAIL>(a, list, row, 0, z, begin, end, s, id, zj, w);
 }
 
@@ -520,7 +531,8 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
     distill_no_weight<T, NT>(a, row, part, begin, end);
     return;
   }
-  const int id = read_list<NT>(a, list, row);
+  bool wrong = false;
+  int id = list_entry(a, row, &wrong);
   const float zj = id >= 0 ? a.list_z[row * a.k + tid] : 0.0f;
   int n = 0;
   const Soft s = soft_join_parts(a.parts, a.c, n, [&](int p, int &) {
@@ -530,6 +542,7 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
     b.r = q.y;
     return b;
   });
+  id = put_list(a, list, row, id, zj, wrong);
   distill_finish<T, NT, TAIL>(a, list, row, part, z, begin, end, s, id, zj, w);
 }
 
@@ -549,17 +562,22 @@ __global__ __launch_bounds__(NT) void distill_grad_block_kernel(DistillArgs a) {
     zero_part<T, NT>(out, begin, end);
     return;
   }
-  const int id = read_list<NT>(a, list, row);
-  const float zj = id >= begin && id < end ? Row<T>::up(z[id]) : 0.0f;
+  bool wrong = false;
+  const int entry = list_entry(a, row, &wrong);
+  const float zj = entry >= begin && entry < end ? Row<T>::up(z[entry]) : 0.0f;
   const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
-  __syncthreads();
-  if (tid < kWave) {
-    float top, log_z;
-    (void)teacher_sums<TAIL>(a, list, &top, &log_z);
-  }
-  __syncthreads();
-  distill_gradient<T, NT>(a, z, out, begin, end, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, id, zj,
-                          tid < a.k ? list.q[tid] : 0.0f);
+  if (a.d_logits == a.logits) __syncthreads();
+  distill_gradient<T, NT>(
+      a, z, out, begin, end, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, zj, [&](float *q) {
+        const int id = put_list(a, list, row, entry, zj, wrong);
+        if (tid < kWave) {
+          float top, log_z;
+          (void)teacher_sums<TAIL>(a, list, &top, &log_z);
+        }
+        __syncthreads();
+        *q = tid < a.k ? list.q[tid] : 0.0f;
+        return id;
+      });
 }
 
 }  // namespace tmnn_hip

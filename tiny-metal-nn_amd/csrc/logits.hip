@@ -22,7 +22,8 @@ namespace {
 // Workspace of the calls that split rows: at most kMaxSplit parts at a time.
 constexpr int kMaxSplit = 4096;
 constexpr size_t kSumBytes = kMaxSplit * sizeof(float4);
-constexpr size_t kKeyBytes = static_cast<size_t>(kMaxSplit) * kMaxTop * sizeof(uint64_t);
+constexpr int64_t kSplitKeys = 1 << 20;  // threads of these parts
+constexpr size_t kKeyBytes = static_cast<size_t>(kSplitKeys) * sizeof(uint64_t);
 constexpr size_t kListBytes = static_cast<size_t>(kMaxSplit) * kMaxTeacher * sizeof(float);
 
 }  // namespace
@@ -192,7 +193,7 @@ Split split_of(int64_t rows, int64_t classes, int n, int (*threads)(int64_t), in
   Split s;
   const int64_t vecs = (classes + n - 1) / n;
   int64_t parts = 1;
-  if (rows < blocks) parts = std::min<int64_t>(blocks / rows, vecs / (4 * 256));
+  if (rows < blocks) parts = std::min<int64_t>(blocks / rows, vecs / (2 * 256));
   parts = std::max<int64_t>(parts, (classes + kMaxPartLen - 1) / kMaxPartLen);
   parts = std::min<int64_t>(std::max<int64_t>(parts, 1), kMaxParts);
   int64_t len = (classes + parts - 1) / parts;
@@ -211,7 +212,8 @@ constexpr int kGroupTop = 4;
 template <class F>
 int in_slices(int64_t rows, int64_t threads_per_row, int parts, F launch) {
   int64_t step = std::max<int64_t>(1, (1ll << 31) / threads_per_row - 1);
-  if (parts > 1) step = std::min<int64_t>(step, kMaxSplit / parts);
+  if (parts > 1)
+    step = std::min<int64_t>(step, std::min<int64_t>(kMaxSplit / parts, kSplitKeys / threads_per_row));
   for (int64_t at = 0; at < rows; at += step) {
     launch(at, static_cast<int32_t>(std::min(step, rows - at)));
     TMNN_HIP_TRY(hipGetLastError());
@@ -293,6 +295,7 @@ int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
   const Split sp = split_of(rows, a.classes, n, sum_threads, 2 * a.top_k, kSplitBlocks);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
+  a.part_threads = sp.threads;
   a.part_sum = static_cast<float4 *>(h->work.ptr);
   a.part_key = reinterpret_cast<uint64_t *>(static_cast<char *>(h->work.ptr) + kSumBytes);
   if (a.parts > 1) {

@@ -385,6 +385,7 @@ __device__ __forceinline__ float next_above(float z) {
 // ---- the k largest keys of a block ---------------------------------------------
 
 constexpr int kCandidates = 1024;
+constexpr int kSources = 1024;
 // The threads' keys in groups: 256, or one a thread (at least k either way).
 constexpr int key_groups(int threads) { return threads < 256 ? threads : 256; }
 
@@ -393,8 +394,8 @@ struct SelectLds {
   uint64_t key[NT];
   uint64_t cand[kCandidates];
   uint64_t tau;
-  int count, threads;
-  uint16_t thread[NT];
+  int count, sources;
+  int source[kSources];
 };
 
 // A key that at least k of the groups' keys reach (the largest of their
@@ -456,24 +457,25 @@ __device__ __forceinline__ uint64_t kth_key(const uint64_t *key, int k) {
 }
 
 // The k largest keys of the block's elements, in order, to put(j, key) for j up
-// to the returned count (fewer than k where the block has fewer). Every thread owns
-// `vectors` groups of elements; visit(thread, i, f) calls f(key) for those of a
-// thread's i-th. `mine` is a key that one of the thread's elements reaches (0: it
-// has none) and whose high word none of them exceeds.
+// to the returned count (fewer than k where the block has fewer). The elements belong
+// to sources of `vectors` groups each: visit(source, i, f) calls f(key) for a source's
+// i-th group, and each(f) calls f(source, key) for the thread's own sources with a key
+// that one of the source's elements reaches (0: it has none) and whose high word none
+// of them exceeds; `mine` is the largest of these.
 //
 // No element costs anything beyond the running maximum of the first pass: the k-th
 // largest of the groups' maxima bounds the answer from below, and the block looks
-// again only at the elements of the threads that reach it (about k threads, and about
-// k (1 + k / 512) elements that reach it, in no special order). Where more
-// than kCandidates elements do, the bound is made exact by counting.
-template <int NT, class Visit, class Put>
+// again only at the sources that reach it (about k of them, and about
+// k (1 + k / 512) elements that reach it, in no special order). Where more than
+// kCandidates elements do, the bound is made exact by counting.
+template <int NT, class Each, class Visit, class Put>
 __device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int k, int vectors,
-                                            Visit visit, Put put) {
+                                            Each each, Visit visit, Put put) {
   const int tid = threadIdx.x;
   s.key[tid] = mine;
   if (tid == 0) {
     s.count = 0;
-    s.threads = 0;
+    s.sources = 0;
   }
   __syncthreads();
   if (tid < kWave) {
@@ -488,16 +490,27 @@ __device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int
       if (at < kCandidates) s.cand[at] = q;
     }
   };
-  if (mine != 0 && (mine | 0xffffffffu) >= tau) s.thread[atomicAdd(&s.threads, 1)] = tid;
+  if ((mine | 0xffffffffu) >= tau)
+    each([&](int source, uint64_t key) {
+      if (key != 0 && (key | 0xffffffffu) >= tau) {
+        const int at = atomicAdd(&s.sources, 1);
+        if (at < kSources) s.source[at] = source;
+      }
+    });
   __syncthreads();
-  const int threads = s.threads;
-  for (int i = tid; i < threads * vectors; i += NT) visit(s.thread[i % threads], i / threads, gather);
-  __syncthreads();
+  const int sources = s.sources;
+  if (sources <= kSources) {
+    for (int i = tid; i < sources * vectors; i += NT)
+      visit(s.source[i % sources], i / sources, gather);
+    __syncthreads();
+  }
   int n = s.count;
-  if (n > kCandidates) {
+  if (n > kCandidates || sources > kSources) {
     auto all_mine = [&](auto f) {
-      if (mine != 0)
-        for (int i = 0; i < vectors; ++i) visit(tid, i, f);
+      each([&](int source, uint64_t key) {
+        if (key != 0)
+          for (int i = 0; i < vectors; ++i) visit(source, i, f);
+      });
     };
     uint64_t t = 0;
     for (int b = 63; b >= 0; --b) {
@@ -527,6 +540,18 @@ __device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int
     if (place < k) put(place, q);
   }
   return n < k ? n : k;
+}
+
+// Whether an earlier entry of a list in LDS, 16-byte aligned and filled up with -1 to a
+// multiple of four, has the same id as entry `j`.
+__device__ __forceinline__ bool listed_before(const int *ids, int k, int j, int id) {
+  bool before = false;
+  for (int i = 0; i < k; i += 4) {
+    const int4 q = *reinterpret_cast<const int4 *>(ids + i);
+    before |= (i < j && q.x == id) || (i + 1 < j && q.y == id) || (i + 2 < j && q.z == id) ||
+              (i + 3 < j && q.w == id);
+  }
+  return before;
 }
 
 }  // namespace tmnn_hip

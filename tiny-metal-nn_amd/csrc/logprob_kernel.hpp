@@ -22,6 +22,7 @@ struct LogprobArgs {
   int32_t wide_index;
   int32_t rows, classes, top_k;
   int32_t parts, part_len;  // blocks of a row and the classes of each
+  int32_t part_threads;     // threads of a block (a power of two)
   float c;                  // log2(e) / T
   float inv_t;
   float *logprob, *entropy;
@@ -29,7 +30,7 @@ struct LogprobArgs {
   float *stats;  // [rows][2]: m, S
   int32_t *top_ids;
   float *top_logprobs;
-  // sums of a row's parts, [rows][parts]: m, r, E, rank; [rows][parts][top_k] keys
+  // sums of a row's parts, [rows][parts]: m, r, E, rank; [rows][parts][part_threads] keys
   float4 *part_sum;
   uint64_t *part_key;
   // backward
@@ -418,7 +419,8 @@ __device__ __forceinline__ Soft soft_finish(BlockLds<NT> &l, const Soft &mine, c
 }
 
 // One part of a row: its sums, the count of its classes before the token, and
-// its best classes. `parts` == 1: the row's outputs; else to the workspace.
+// its best classes. `parts` == 1: the row's outputs; else the sums and the threads' keys
+// go to the workspace.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
   constexpr int N = Row<T>::n;
@@ -491,14 +493,18 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
       a.part_sum[blockIdx.x] = make_float4(s.m, s.r, s.E, __int_as_float(rank));
   }
   if (a.top_k == 0) return;
+  const uint64_t key = mine > -__builtin_inff()
+                           ? static_cast<uint64_t>(order_of(mine)) << 32 |
+                                 (0xffffffffu - static_cast<uint32_t>(first + N - 1))
+                           : 0;
+  if (!whole) {
+    a.part_key[static_cast<int64_t>(blockIdx.x) * NT + tid] = key;
+    return;
+  }
   const bool bad = !(s.S < __builtin_inff()) || s.m == __builtin_inff();
   const float log_s = log1p_of(s.r);
   int got = 0;
   if (!bad && s.S != 0.0f) {
-    const uint64_t key =
-        mine > -__builtin_inff()
-            ? static_cast<uint64_t>(order_of(mine)) << 32 | (0xffffffffu - static_cast<uint32_t>(first + N - 1))
-            : 0;
     const int vectors = (end - begin + NT * N - 1) / (NT * N);
     auto visit = [&](int thread, int it, auto f) {
       const int i = begin + (it * NT + thread) * N;
@@ -508,19 +514,12 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(LogprobArgs a) {
       for (int j = 0; j < N; ++j)
         if (v[j] > -__builtin_inff()) f(key_of(v[j], i + j));
     };
-    got = block_select<NT>(sel, key, a.top_k, vectors, visit, [&](int j, uint64_t q) {
-      if (whole)
-        put_top(a, row, j, value_of(static_cast<uint32_t>(q >> 32)), key_index(q), s.m, log_s);
-      else
-        a.part_key[static_cast<int64_t>(blockIdx.x) * a.top_k + j] = q;
-    });
+    got = block_select<NT>(
+        sel, key, a.top_k, vectors, [&](auto f) { f(tid, key); }, visit, [&](int j, uint64_t q) {
+          put_top(a, row, j, value_of(static_cast<uint32_t>(q >> 32)), key_index(q), s.m, log_s);
+        });
   }
-  for (int j = got + tid; j < a.top_k; j += NT) {
-    if (whole)
-      put_no_top(a, row, j, bad);
-    else
-      a.part_key[static_cast<int64_t>(blockIdx.x) * a.top_k + j] = 0;
-  }
+  for (int j = got + tid; j < a.top_k; j += NT) put_no_top(a, row, j, bad);
 }
 
 // Joins the parts of a row.
@@ -532,6 +531,19 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
   __shared__ SelectLds<kJoinThreads> sel;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
+  const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
+  const int64_t token = a.tokens ? load_index(a.tokens, row, a.wide_index) : -1;
+  const float zt = token >= 0 && token < a.classes ? Row<T>::up(z[token]) : 0.0f;
+  // the keys of the parts' threads: the first kKept of a thread in registers
+  constexpr int kKept = 8;
+  const int n = a.parts * a.part_threads;
+  const uint64_t *keys = a.part_key + row * n;
+  uint64_t kept[kKept], best = 0;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    const int at = i * kJoinThreads + tid;
+    kept[i] = a.top_k > 0 && at < n ? keys[at] : 0;
+  }
   int rank = 0;
   const Soft s = soft_join_parts(a.parts, a.c, rank, [&](int p, int &n) {
     const float4 q = a.part_sum[row * a.parts + p];
@@ -543,28 +555,41 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
     return b;
   });
   const bool bad = !(s.S < __builtin_inff()) || s.m == __builtin_inff();
-  if (tid == 0) {
-    const int64_t token = a.tokens ? load_index(a.tokens, row, a.wide_index) : -1;
-    const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
-    const float zt = token >= 0 && token < a.classes ? Row<T>::up(z[token]) : 0.0f;
-    put_row(a, row, s, token, zt, rank);
-  }
+  // (not the wave that searches)
+  if (tid == kJoinThreads - kWave) put_row(a, row, s, token, zt, rank);
   if (a.top_k == 0) return;
   const float m = s.m, log_s = log1p_of(s.r);
   int got = 0;
   if (!bad && s.S != 0.0f) {
-    const uint64_t *keys = a.part_key + row * a.parts * a.top_k;
-    const int n = a.parts * a.top_k;
-    uint64_t best = 0;
-    for (int i = tid; i < n; i += kJoinThreads) best = keys[i] > best ? keys[i] : best;
-    auto visit = [&](int thread, int it, auto f) {
-      const int i = it * kJoinThreads + thread;
-      if (i < n && keys[i] != 0) f(keys[i]);
+    // the sources are the parts' threads
+    constexpr int N = Row<T>::n;
+    const int stride = a.part_threads * N;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) best = kept[i] > best ? kept[i] : best;
+    for (int i = kKept * kJoinThreads + tid; i < n; i += kJoinThreads)
+      best = keys[i] > best ? keys[i] : best;
+    auto each = [&](auto f) {
+#pragma unroll
+      for (int i = 0; i < kKept; ++i)
+        if (kept[i] != 0) f(i * kJoinThreads + tid, kept[i]);
+      for (int i = kKept * kJoinThreads + tid; i < n; i += kJoinThreads) f(i, keys[i]);
     };
-    const int vectors = (n + kJoinThreads - 1) / kJoinThreads;
-    got = block_select<kJoinThreads>(sel, best, a.top_k, vectors, visit, [&](int j, uint64_t q) {
-      put_top(a, row, j, value_of(static_cast<uint32_t>(q >> 32)), key_index(q), m, log_s);
-    });
+    auto visit = [&](int source, int it, auto f) {
+      const int part = source / a.part_threads;
+      const int begin = part * a.part_len;
+      const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+      const int i = begin + it * stride + (source & (a.part_threads - 1)) * N;
+      float v[N];
+      load_vec<T>(z, i, end, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (v[j] > -__builtin_inff()) f(key_of(v[j], i + j));
+    };
+    const int vectors = (a.part_len + stride - 1) / stride;
+    got = block_select<kJoinThreads>(
+        sel, best, a.top_k, vectors, each, visit, [&](int j, uint64_t q) {
+          put_top(a, row, j, value_of(static_cast<uint32_t>(q >> 32)), key_index(q), m, log_s);
+        });
   }
   for (int j = got + tid; j < a.top_k; j += kJoinThreads) put_no_top(a, row, j, bad);
 }
@@ -751,7 +776,7 @@ __device__ __forceinline__ void zero_part(T *out, int begin, int end) {
 // and one for the token.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
-  __shared__ int list[kMaxTop];
+  __shared__ __attribute__((aligned(16))) int list[kMaxTop];
   __shared__ float term[kMaxTop];
   __shared__ float sums[2];
   const int tid = threadIdx.x;
@@ -767,16 +792,17 @@ __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
   int mine = -1;
   float g = 0.0f;
   if (k > 0) {
-    if (tid < k) {
-      const int id = a.top_in[row * a.top_k + tid];
-      list[tid] = id >= 0 && id < a.classes ? id : -1;
+    if (tid < ((k + 3) & ~3)) {
+      const int id = tid < k ? a.top_in[row * a.top_k + tid] : -1;
+      mine = id >= 0 && id < a.classes ? id : -1;
+      g = mine >= 0 ? a.d_top[row * a.top_k + tid] : 0.0f;
+      list[tid] = mine;
     }
     __syncthreads();
     if (tid < k) {
-      mine = list[tid];
-      for (int j = 0; j < tid; ++j)
-        if (list[j] == mine) mine = -1;  // a class counts by its first entry
-      g = mine >= 0 ? a.d_top[row * a.top_k + tid] : 0.0f;
+      // a class counts by its first entry
+      if (listed_before(list, k, tid, mine)) mine = -1;
+      if (mine < 0) g = 0.0f;
       term[tid] = g;
     }
     __syncthreads();
@@ -807,15 +833,14 @@ __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
   g *= a.inv_t;
   if (tid == k) {
     mine = r.token;
-    for (int j = 0; j < k; ++j)
-      if (list[j] == mine) mine = -1;  // its entry's thread writes it
+    if (listed_before(list, k, k, mine)) mine = -1;  // its entry's thread writes it
     g = r.g_token;
   } else if (mine >= 0 && mine == r.token) {
     g += r.g_token;
   }
   if (mine < begin || mine >= end) mine = -1;
   const float zm = mine >= 0 ? Row<T>::up(z[mine]) : 0.0f;
-  __syncthreads();
+  if (a.d_logits == a.logits) __syncthreads();
   const ExpAt e(r.m, a.c);
   // 2^x of the fma form carries `fix`, and its x the same correction
   const float rho = e.huge ? 0.0f : __builtin_fmaf(r.m, a.c, -e.R);
