@@ -357,31 +357,31 @@ __device__ __forceinline__ TeacherMass teacher_sums(const DistillArgs &a, ListLd
 // the two listed() returns the thread's class (-1: none) and its q. The thread's logit
 // zj has been read.
 template <class T, int NT, class Listed>
-__device__ __forceinline__ void distill_gradient(const DistillArgs &a, const T *z, T *out,
-                                                 int begin, int end, const DistillRow &r,
-                                                 float scale, float zj, Listed listed) {
+__device__ __forceinline__ void distill_gradient(const DistillArgs &a, const Part<T, NT> &p, T *out,
+                                                 const DistillRow &r, float scale, float zj,
+                                                 Listed listed) {
   if (r.m_a == -__builtin_inff() && r.a_a == r.a_a) {  // every class is masked
-    zero_part<T, NT>(out, begin, end);
+    p.zero(out);
     return;
   }
   const ExpAt e(r.m_d, a.c);
   const float f = scale * r.a_d * e.fix;
   if (e.huge)
-    map_part<T, NT>(z, out, begin, end, [&](float v) { return f * exp2_raw(e.x_huge(v)); });
+    p.map(out, [&](float v) { return f * exp2_raw(e.x_huge(v)); });
   else
-    map_part<T, NT>(z, out, begin, end, [&](float v) { return f * exp2_raw(e.x_plain(v)); });
+    p.map(out, [&](float v) { return f * exp2_raw(e.x_plain(v)); });
   float q;
   const int id = listed(&q);
   __syncthreads();
-  if (id >= begin && id < end)
+  if (id >= p.begin && id < p.end)
     out[id] = Row<T>::down(scale * (r.a_a * exp2_raw((zj - r.m_a) * a.c) - q));
 }
 
 // From the sums of a row: its loss, statistics and gradient (of one part).
 template <class T, int NT, bool TAIL>
 __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l, int64_t row,
-                                               int part, const T *z, int begin, int end,
-                                               const Soft &dense, int id, float zj, float w) {
+                                               int part, const Part<T, NT> &p, const Soft &dense,
+                                               int id, float zj, float w) {
   const int tid = threadIdx.x;
   if (tid < kWave) {
     float top, log_z, rest_loss, loss = 0.0f;
@@ -433,7 +433,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
   __syncthreads();
   if (!a.d_logits) return;
   T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
-  distill_gradient<T, NT>(a, z, out, begin, end, l.row, w * a.t, zj, [&](float *q) {
+  distill_gradient<T, NT>(a, p, out, l.row, w * a.t, zj, [&](float *q) {
     *q = tid < a.k ? l.q[tid] : 0.0f;
     return id;
   });
@@ -442,15 +442,14 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
 // A row of weight 0 is not read.
 template <class T, int NT>
 __device__ __forceinline__ void distill_no_weight(const DistillArgs &a, int64_t row, int part,
-                                                  int begin, int end) {
+                                                  const Part<T, NT> &p) {
   if (part == 0 && threadIdx.x == 0) {
     if (a.loss) a.loss[row] = 0.0f;
     if (a.stats)
       reinterpret_cast<float4 *>(a.stats)[row] =
           make_float4(0.0f, 0.0f, -__builtin_inff(), 0.0f);
   }
-  if (a.d_logits)
-    zero_part<T, NT>(static_cast<T *>(a.d_logits) + row * a.d_row_stride, begin, end);
+  if (a.d_logits) p.zero(static_cast<T *>(a.d_logits) + row * a.d_row_stride);
 }
 
 template <class T, int NT, bool TAIL>
@@ -463,29 +462,28 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
   const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
-  const int begin = part * a.part_len;
-  const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+  const Part<T, NT> p(z, part, a.part_len, a.classes);
   const float w = a.weights ? a.weights[row] : 1.0f;
   if (w == 0.0f) {
-    if (a.parts == 1) distill_no_weight<T, NT>(a, row, part, begin, end);
+    if (a.parts == 1) distill_no_weight<T, NT>(a, row, part, p);
     return;
   }
   if (TAIL)
-    for (int i = tid; i * 32 < end - begin; i += NT) listed[i] = 0u;
+    for (int i = tid; i * 32 < p.end - p.begin; i += NT) listed[i] = 0u;
   if (TAIL) __syncthreads();
   bool wrong = false;
   int id = list_entry(a, row, &wrong);
   float zj = 0.0f;
-  if (id >= begin && id < end) {
+  if (id >= p.begin && id < p.end) {
     zj = Row<T>::up(z[id]);
-    if (TAIL) atomicOr(&listed[(id - begin) >> 5], 1u << ((id - begin) & 31));
+    if (TAIL) atomicOr(&listed[(id - p.begin) >> 5], 1u << ((id - p.begin) & 31));
   }
   if (TAIL) __syncthreads();
   // a listed class counts apart from the rest
   auto hide = [&](int i, float *v) {
     if (!TAIL) return;
-    const int o = i - begin;
-    if (i >= end) return;
+    const int o = i - p.begin;
+    if (i >= p.end) return;
     const uint32_t bits = (listed[o >> 5] >> (o & 31)) & ((1u << N) - 1u);
     if (bits == 0) return;
 #pragma unroll
@@ -493,7 +491,7 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
       if (bits >> j & 1u) v[j] = -__builtin_inff();
   };
   Soft s;
-  scan_part<T, NT>(z, begin, end, [&](int at, auto &v) {
+  p.scan([&](int at, auto &v) {
     constexpr int W = sizeof(v) / sizeof(v[0]);
     float cm = -__builtin_inff();
 #pragma unroll
@@ -505,14 +503,14 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
     soft_add<W * N, false>(s, &v[0][0], cm, a.c);
   });
   int n = 0;
-  s = soft_finish<T, NT, false>(lds, s, z, begin, end, a.c, n, hide);
+  s = soft_finish<T, NT, false>(lds, s, p, a.c, n, hide);
   if (a.parts > 1) {
     if (tid == 0) a.part_sum[blockIdx.x] = make_float2(s.m, s.r);
-    if (id >= begin && id < end) a.list_z[row * a.k + tid] = zj;
+    if (id >= p.begin && id < p.end) a.list_z[row * a.k + tid] = zj;
     return;
   }
   id = put_list(a, list, row, id, zj, wrong);
-  distill_finish<T, NT, TAIL>(a, list, row, 0, z, begin, end, s, id, zj, w);
+  distill_finish<T, NT, TAIL>(a, list, row, 0, p, s, id, zj, w);
 }
 
 // Joins the sums of a row's parts (in their order), and finishes one part.
@@ -524,11 +522,10 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
   const int64_t row = blockIdx.x / blocks;
   const int part = blockIdx.x % blocks;
   const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
-  const int begin = part * a.part_len;
-  const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+  const Part<T, NT> p(z, part, a.part_len, a.classes);
   const float w = a.weights ? a.weights[row] : 1.0f;
   if (w == 0.0f) {
-    distill_no_weight<T, NT>(a, row, part, begin, end);
+    distill_no_weight<T, NT>(a, row, part, p);
     return;
   }
   bool wrong = false;
@@ -543,7 +540,7 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
     return b;
   });
   id = put_list(a, list, row, id, zj, wrong);
-  distill_finish<T, NT, TAIL>(a, list, row, part, z, begin, end, s, id, zj, w);
+  distill_finish<T, NT, TAIL>(a, list, row, part, p, s, id, zj, w);
 }
 
 // The gradient alone, from the statistics.
@@ -555,20 +552,19 @@ __global__ __launch_bounds__(NT) void distill_grad_block_kernel(DistillArgs a) {
   const int part = blockIdx.x % a.parts;
   const T *z = static_cast<const T *>(a.logits) + row * a.row_stride;
   T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
-  const int begin = part * a.part_len;
-  const int end = begin + a.part_len < a.classes ? begin + a.part_len : a.classes;
+  const Part<T, NT> p(z, part, a.part_len, a.classes);
   const float w = a.weights ? a.weights[row] : 1.0f;
   if (w == 0.0f) {
-    zero_part<T, NT>(out, begin, end);
+    p.zero(out);
     return;
   }
   bool wrong = false;
   const int entry = list_entry(a, row, &wrong);
-  const float zj = entry >= begin && entry < end ? Row<T>::up(z[entry]) : 0.0f;
+  const float zj = entry >= p.begin && entry < p.end ? Row<T>::up(z[entry]) : 0.0f;
   const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
   if (a.d_logits == a.logits) __syncthreads();
   distill_gradient<T, NT>(
-      a, z, out, begin, end, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, zj, [&](float *q) {
+      a, p, out, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, zj, [&](float *q) {
         const int id = put_list(a, list, row, entry, zj, wrong);
         if (tid < kWave) {
           float top, log_z;
