@@ -356,10 +356,10 @@ __device__ __forceinline__ TeacherMass teacher_sums(const DistillArgs &a, ListLd
 // Writes the gradient of a part: all classes as unlisted ones, then the listed; between
 // the two listed() returns the thread's class (-1: none) and its q. The thread's logit
 // zj has been read.
-template <class T, int NT, class Listed>
+template <class T, int NT, class Map, class Listed>
 __device__ __forceinline__ void distill_gradient(const DistillArgs &a, const Part<T, NT> &p, T *out,
                                                  const DistillRow &r, float scale, float zj,
-                                                 Listed listed) {
+                                                 Map map, Listed listed) {
   if (r.m_a == -__builtin_inff() && r.a_a == r.a_a) {  // every class is masked
     p.zero(out);
     return;
@@ -367,9 +367,9 @@ __device__ __forceinline__ void distill_gradient(const DistillArgs &a, const Par
   const ExpAt e(r.m_d, a.c);
   const float f = scale * r.a_d * e.fix;
   if (e.huge)
-    p.map(out, [&](float v) { return f * exp2_raw(e.x_huge(v)); });
+    map([&](float v) { return f * exp2_raw(e.x_huge(v)); });
   else
-    p.map(out, [&](float v) { return f * exp2_raw(e.x_plain(v)); });
+    map([&](float v) { return f * exp2_raw(e.x_plain(v)); });
   float q;
   const int id = listed(&q);
   __syncthreads();
@@ -378,10 +378,10 @@ __device__ __forceinline__ void distill_gradient(const DistillArgs &a, const Par
 }
 
 // From the sums of a row: its loss, statistics and gradient (of one part).
-template <class T, int NT, bool TAIL>
+template <bool TAIL, class T, int NT, class Map>
 __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l, int64_t row,
                                                int part, const Part<T, NT> &p, const Soft &dense,
-                                               int id, float zj, float w) {
+                                               int id, float zj, float w, Map map) {
   const int tid = threadIdx.x;
   if (tid < kWave) {
     float top, log_z, rest_loss, loss = 0.0f;
@@ -433,7 +433,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
   __syncthreads();
   if (!a.d_logits) return;
   T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
-  distill_gradient<T, NT>(a, p, out, l.row, w * a.t, zj, [&](float *q) {
+  distill_gradient<T, NT>(a, p, out, l.row, w * a.t, zj, [&](auto f) { map(out, f); }, [&](float *q) {
     *q = tid < a.k ? l.q[tid] : 0.0f;
     return id;
   });
@@ -452,7 +452,9 @@ __device__ __forceinline__ void distill_no_weight(const DistillArgs &a, int64_t 
   if (a.d_logits) p.zero(static_cast<T *>(a.d_logits) + row * a.d_row_stride);
 }
 
-template <class T, int NT, bool TAIL>
+// KEEP: the row's vectors stay in registers for the gradient, KEEP a thread (0: they are read
+// again).
+template <class T, int NT, bool TAIL, int KEEP>
 __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
   constexpr int N = Row<T>::n;
   extern __shared__ uint32_t listed[];  // TAIL: a bit for each class of the part
@@ -490,8 +492,10 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
     for (int j = 0; j < N; ++j)
       if (bits >> j & 1u) v[j] = -__builtin_inff();
   };
+  typename Part<T, NT>::template Kept<KEEP ? KEEP : 4> kept;
+  if (KEEP) p.load(kept);
   Soft s;
-  p.scan([&](int at, auto &v) {
+  auto take = [&](int at, auto &v) {
     constexpr int W = sizeof(v) / sizeof(v[0]);
     float cm = -__builtin_inff();
 #pragma unroll
@@ -501,7 +505,11 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
       for (int j = 0; j < N; ++j) cm = fmaxf(cm, v[u][j]);
     }
     soft_add<W * N, false>(s, &v[0][0], cm, a.c);
-  });
+  };
+  if (KEEP)
+    p.scan(kept, take);
+  else
+    p.scan(take);
   int n = 0;
   s = soft_finish<T, NT, false>(lds, s, p, a.c, n, hide);
   if (a.parts > 1) {
@@ -510,7 +518,12 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(DistillArgs a) {
     return;
   }
   id = put_list(a, list, row, id, zj, wrong);
-  distill_finish<T, NT, TAIL>(a, list, row, 0, p, s, id, zj, w);
+  distill_finish<TAIL>(a, list, row, 0, p, s, id, zj, w, [&](T *out, auto f) {
+    if (KEEP)
+      p.map(kept, out, f);
+    else
+      p.map(out, f);
+  });
 }
 
 // Joins the sums of a row's parts (in their order), and finishes one part.
@@ -540,7 +553,7 @@ __global__ __launch_bounds__(NT) void distill_join_kernel(DistillArgs a) {
     return b;
   });
   id = put_list(a, list, row, id, zj, wrong);
-  distill_finish<T, NT, TAIL>(a, list, row, part, p, s, id, zj, w);
+  distill_finish<TAIL>(a, list, row, part, p, s, id, zj, w, [&](T *out, auto f) { p.map(out, f); });
 }
 
 // The gradient alone, from the statistics.
@@ -564,7 +577,8 @@ __global__ __launch_bounds__(NT) void distill_grad_block_kernel(DistillArgs a) {
   const float4 s = reinterpret_cast<const float4 *>(a.stats)[row];
   if (a.d_logits == a.logits) __syncthreads();
   distill_gradient<T, NT>(
-      a, p, out, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, zj, [&](float *q) {
+      a, p, out, DistillRow{s.x, s.y, s.z, s.w}, w * a.t, zj,
+      [&](auto f) { p.map(out, f); }, [&](float *q) {
         const int id = put_list(a, list, row, entry, zj, wrong);
         if (tid < kWave) {
           float top, log_z;

@@ -177,11 +177,15 @@ int sum_threads(int64_t vecs) {
 int map_threads(int64_t vecs) {
   return vecs < 512 ? 64 : vecs < 1024 ? 128 : vecs < 2048 ? 256 : vecs < 4096 ? 512 : 1024;
 }
-// Sums and gradient in one block (16384 x 5003 bf16 114 / 111 / 137 / 193 / 306, 8192 x 20011 233 /
-// 223 / 198 / 212 / 266, 4096 x 131072 841 / 703 / 650 / 586 / 490).
+// Sums and gradient in one block. Up to 8 vectors a thread stay in registers in between, while
+// several blocks of up to 256 threads share a unit then (16384 x 8192 bf16, 1024 vectors, kept at
+// 128 threads 111, read again at 128 / 256 131 / 129; f32, 2048 vectors, kept at 256 187, read
+// again 238); longer rows are read again (8192 x 65536 bf16, 8192 vectors, kept at 1024 threads
+// 567, read again at 512 / 1024 484 / 455; 8192 x 20011 at 128 / 256 / 512 223 / 198 / 212).
 int both_threads(int64_t vecs) {
-  return vecs < 512 ? 64 : vecs < 1024 ? 128 : vecs < 4096 ? 256 : vecs < 8192 ? 512 : 1024;
+  return vecs <= 512 ? 64 : vecs <= 1024 ? 128 : vecs < 4096 ? 256 : vecs < 8192 ? 512 : 1024;
 }
+constexpr int kKeptVecs = 8;
 
 struct Split {
   int threads, parts, part_len;
@@ -392,6 +396,8 @@ int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStrea
                        TMNN_BY_THREADS(sp.threads, CALL)
 #undef CALL
                      });
+  const bool keep = a.parts == 1 && a.d_logits && sp.threads <= 256 &&
+                    a.classes <= static_cast<int64_t>(sp.threads) * n * kKeptVecs;
   a.part_sum = static_cast<float2 *>(h->work.ptr);
   a.list_z = reinterpret_cast<float *>(static_cast<char *>(h->work.ptr) + kSumBytes + kKeyBytes);
   if (a.parts > 1) {
@@ -402,14 +408,17 @@ int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStrea
                    [&](int64_t at, int32_t r) {
                      const DistillArgs s = distill_slice<T>(a, at, r);
                      const size_t bits = (static_cast<size_t>(sp.part_len) + 31) / 32 * 4;
-#define CALL(NT)                                                                                   \
-  if (tail)                                                                                        \
-    hipLaunchKernelGGL((distill_block_kernel<T, NT, true>), dim3(r * a.parts), dim3(NT), bits, st, \
-                       s);                                                                         \
-  else                                                                                             \
-    hipLaunchKernelGGL((distill_block_kernel<T, NT, false>), dim3(r * a.parts), dim3(NT), 0, st, s)
+#define LAUNCH(NT, TAIL, KEEP)                                                               \
+  hipLaunchKernelGGL((distill_block_kernel<T, NT, TAIL, KEEP>), dim3(r * a.parts), dim3(NT), \
+                     TAIL ? bits : 0, st, s)
+#define CALL(NT)                                                  \
+  if (tail && keep) LAUNCH(NT, true, (NT <= 256 ? kKeptVecs : 0)); \
+  else if (tail) LAUNCH(NT, true, 0);                              \
+  else if (keep) LAUNCH(NT, false, (NT <= 256 ? kKeptVecs : 0));   \
+  else LAUNCH(NT, false, 0)
                      TMNN_BY_THREADS(sp.threads, CALL)
 #undef CALL
+#undef LAUNCH
                      if (a.parts > 1) {
                        const dim3 grid(r * (a.d_logits ? a.parts : 1));
 #define CALL(NT)                                                                            \

@@ -412,6 +412,55 @@ struct Part {
       }
     }
   }
+  // The same with up to K vectors of the thread kept in between: load, then any number of
+  // scans and one map. The part has at most K NT vectors.
+  template <int K>
+  struct Kept {
+    typename Row<T>::V raw[K];
+  };
+  template <int K>
+  __device__ __forceinline__ void load(Kept<K> &k) const {
+    constexpr int N = Row<T>::n;
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      const int i = begin + (u * NT + static_cast<int>(threadIdx.x)) * N;
+      if (i + N <= end) {
+        k.raw[u] = load_raw(z + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) k.raw[u][j] = i + j < end ? z[i + j] : Row<T>::down(-__builtin_inff());
+      }
+    }
+  }
+  template <int K, class Take>
+  __device__ __forceinline__ void scan(const Kept<K> &k, Take take) const {
+    constexpr int N = Row<T>::n, U = kLogitVecs;
+    static_assert(K % U == 0, "");
+#pragma unroll
+    for (int g = 0; g < K; g += U) {
+      const int at = begin + g * NT * N;
+      if (at >= end) break;
+      float v[U][N];
+#pragma unroll
+      for (int u = 0; u < U; ++u) widen<T>(k.raw[g + u], v[u]);
+      take(at, v);
+    }
+  }
+  template <int K, class F>
+  __device__ __forceinline__ void map(const Kept<K> &k, T *out, F f) const {
+    constexpr int N = Row<T>::n;
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      const int i = begin + (u * NT + static_cast<int>(threadIdx.x)) * N;
+      if (i < end) {
+        float v[N];
+        widen<T>(k.raw[u], v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = f(v[j]);
+        store_vec<T>(out, i, end, v);
+      }
+    }
+  }
   __device__ __forceinline__ void zero(T *out) const {
     constexpr int N = Row<T>::n;
     const float v[N] = {};
