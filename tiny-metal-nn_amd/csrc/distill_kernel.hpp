@@ -89,11 +89,12 @@ __device__ __forceinline__ TeacherMass teacher_total(const DistillArgs &a, float
 
 // The row's statistics and the part of its loss that the listed classes do not
 // bring: dense = settled sums of all classes (kind 0) or of the unlisted ones
-// (kind 1); all = of all classes; mass = sum q, left = 1 - mass (kind 1).
+// (kind 1); all = of all classes; listed = the sum of the listed ones in the shift of
+// all.m (kind 1); mass = sum q, left = 1 - mass (kind 1).
 template <bool TAIL>
 __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const Soft &dense,
-                                                  const Soft &all, float mass, float left,
-                                                  float *rest_loss) {
+                                                  const Soft &all, float listed, float mass,
+                                                  float left, float *rest_loss) {
   DistillRow r;
   r.m_a = all.m;
   *rest_loss = 0.0f;
@@ -111,8 +112,14 @@ __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const So
   // (no rest: 0, or the NaN of the listed classes)
   r.a_d = rest ? exp2_raw((dense.m - all.m) * a.c) * r.a_a - quotient(qr, dense.S) : 0.0f * r.a_a;
   if (qr > 0.0f) {
-    const float log_pr = (dense.m - all.m) * a.inv_t + (log1p_of(dense.r) - log1p_of(all.r));
-    *rest_loss = qr * (log_of(qr) - log_pr);
+    // Where the rest is most of both, its two logarithms are small, and are taken from what
+    // is missing to 1: rounded logarithms of the sums would be off by half an ulp of ln
+    // of the class count, which the loss of a flat teacher is not large against.
+    const float over = quotient(listed, dense.S * exp2_raw((dense.m - all.m) * a.c));
+    const float log_pr = over < 1.0f ? -log1p_of(over)
+                                     : ((dense.m - all.m) * a.inv_t + log1p_of(dense.r)) - log1p_of(all.r);
+    const float log_qr = mass < 0.5f ? log1p_of(-mass) : logf(qr);
+    *rest_loss = qr * (log_qr - log_pr);
   }
   return r;
 }
@@ -199,7 +206,7 @@ __global__ __launch_bounds__(kGroupThreads) void distill_group_kernel(DistillArg
   const float mass = (TAIL ? total : none ? 0.0f : total * inv_z) + tm.poison;
 
   DistillRow r{};
-  float loss = 0.0f, rest_loss = 0.0f;
+  float loss = 0.0f, rest_loss = 0.0f, listed = 0.0f;
   Soft all;
   if (BACK) {
     if (live) {
@@ -245,11 +252,13 @@ __global__ __launch_bounds__(kGroupThreads) void distill_group_kernel(DistillArg
       const bool one = dense.m == all.m;  // the 1 that r leaves out is the rest's, or a listed class's
       all.r = 0.0f;
       soft_join(all, dense, a.c, one && dense.m != -inf);
-      all.r += lanes_sum<G>(p) + static_cast<float>(all.m == -inf ? -1 : one ? n : n - 1);
+      p = lanes_sum<G>(p);
+      listed = p + static_cast<float>(n);
+      all.r += p + static_cast<float>(all.m == -inf ? -1 : one ? n : n - 1);
       if (all.m == inf) all.r = __builtin_nanf("");
       all.S = 1.0f + all.r;
     }
-    r = distill_row<TAIL>(a, dense, all, mass, tm.left, &rest_loss);
+    r = distill_row<TAIL>(a, dense, all, listed, mass, tm.left, &rest_loss);
     if (all.m == -inf && all.S == 0.0f) r.m_a = -inf;
   }
   const bool zero = !live || (r.m_a == -inf && r.a_a == r.a_a);
@@ -386,6 +395,7 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
   if (tid < kWave) {
     float top, log_z, rest_loss, loss = 0.0f;
     const TeacherMass mass = teacher_sums<TAIL>(a, l, &top, &log_z);
+    float listed = 0.0f;
     Soft all = dense;
     if (TAIL) {
       for (int j = tid; j < a.k; j += kWave)
@@ -404,12 +414,14 @@ __device__ __forceinline__ void distill_finish(const DistillArgs &a, ListLds &l,
       float s = 0.0f;
       for (int j = tid; j < a.k; j += kWave)
         if (l.id[j] >= 0 && j != one) s += exp2_raw((l.z[j] - shift) * a.c);
-      all.r += lanes_sum<kWave>(s);
+      s = lanes_sum<kWave>(s);
+      listed = one >= 0 ? s + 1.0f : s;
+      all.r += s;
       if (all.m == -__builtin_inff()) all.r -= 1.0f;  // no class: S = 0 (or NaN)
       if (all.m == __builtin_inff()) all.r = __builtin_nanf("");
       all.S = 1.0f + all.r;
     }
-    const DistillRow r = distill_row<TAIL>(a, dense, all, mass.all, mass.left, &rest_loss);
+    const DistillRow r = distill_row<TAIL>(a, dense, all, listed, mass.all, mass.left, &rest_loss);
     const float log_s = log1p_of(all.r);
     for (int j = tid; j < a.k; j += kWave) {
       const float q = l.q[j];

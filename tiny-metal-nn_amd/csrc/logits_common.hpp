@@ -112,14 +112,12 @@ __device__ __forceinline__ float exp_of(float t) {
   return x > -150.0f ? exp2_raw(x) * __builtin_fmaf(rest, kLn2, 1.0f) : 0.0f;
 }
 
-// ln(1 + r), r >= -1, by what rounding 1 + r leaves out: ln u + (r - (u - 1)) / u. The
-// hardware's log2 is good to an ulp of its result.
+// ln(1 + r), r >= -1, by what rounding 1 + r leaves out: ln u + (r - (u - 1)) / u.
 __device__ __forceinline__ float log1p_of(float r) {
-  const float u = 1.0f + r;
+  const float u = 1.0f + r, l = logf(u);
   const float rest = (r - (u - 1.0f)) * __builtin_amdgcn_rcpf(u);
-  const float l = __builtin_amdgcn_logf(u);
   // u = 0, inf and NaN leave no rest
-  return u > 0.0f && u < __builtin_inff() ? __builtin_fmaf(l, kLn2, rest) : l;
+  return u > 0.0f && u < __builtin_inff() ? l + rest : l;
 }
 
 // ---- sums over G consecutive lanes (all lanes get the result) ----------------
