@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <memory>
 #include <mutex>
 #include <new>
@@ -521,30 +522,45 @@ class HostArrays {
     if (!slot || rows == 0 || width == 0) return;
     items_.push_back({const_cast<void *>(static_cast<const void *>(slot)),
                       const_cast<void **>(reinterpret_cast<const void *const *>(&slot)), dir, rows,
-                      width, pitch, bytes_});
+                      width, rows == 1 ? width : pitch, bytes_, {}});
     bytes_ += (static_cast<size_t>(rows) * width + 255) / 256 * 256;
   }
   template <class P>
   void add(P *&slot, Dir dir, int64_t rows, size_t width) {
     add(slot, dir, rows, width, width);
   }
+  // Rows that are not adjacent on the host are packed there (a copy of rows over a pitch takes
+  // the runtime a transfer a row).
   int enter(tmnn_logits *h) {
     TMNN_HIP_TRY(h->arena.ensure(std::max<size_t>(bytes_, 256)));
-    for (const Item &i : items_) {
+    for (Item &i : items_) {
       char *d = h->arena.as<char>() + i.at;
       *i.slot = d;
-      if (i.dir == kIn)
-        TMNN_HIP_TRY(hipMemcpy2DAsync(d, i.width, i.host, i.pitch, i.width, i.rows,
-                                      hipMemcpyHostToDevice, h->ctx->stream));
+      const size_t bytes = static_cast<size_t>(i.rows) * i.width;
+      if (i.pitch != i.width) i.packed.resize(bytes);
+      if (i.dir != kIn) continue;
+      const char *from = static_cast<const char *>(i.host);
+      for (int64_t r = 0; i.pitch != i.width && r < i.rows; ++r)
+        std::memcpy(i.packed.data() + r * i.width, from + r * i.pitch, i.width);
+      TMNN_HIP_TRY(hipMemcpyAsync(d, i.pitch != i.width ? i.packed.data() : from, bytes,
+                                  hipMemcpyHostToDevice, h->ctx->stream));
     }
     return TMNN_OK;
   }
+  // Enqueues the copies out; `place` puts them where they belong once they are there.
   int leave(tmnn_logits *h) {
-    for (const Item &i : items_)
+    for (Item &i : items_)
       if (i.dir == kOut)
-        TMNN_HIP_TRY(hipMemcpy2DAsync(i.host, i.pitch, h->arena.as<char>() + i.at, i.width, i.width,
-                                      i.rows, hipMemcpyDeviceToHost, h->ctx->stream));
+        TMNN_HIP_TRY(hipMemcpyAsync(i.pitch != i.width ? i.packed.data() : i.host,
+                                    h->arena.as<char>() + i.at,
+                                    static_cast<size_t>(i.rows) * i.width, hipMemcpyDeviceToHost,
+                                    h->ctx->stream));
     return TMNN_OK;
+  }
+  void place() const {
+    for (const Item &i : items_)
+      for (int64_t r = 0; i.dir == kOut && i.pitch != i.width && r < i.rows; ++r)
+        std::memcpy(static_cast<char *>(i.host) + r * i.pitch, i.packed.data() + r * i.width, i.width);
   }
 
  private:
@@ -554,6 +570,7 @@ class HostArrays {
     Dir dir;
     int64_t rows;
     size_t width, pitch, at;
+    std::vector<char> packed;
   };
   std::vector<Item> items_;
   size_t bytes_ = 0;
@@ -568,6 +585,7 @@ int on_host(tmnn_logits *h, HostArrays &arrays, Run run) {
   const hipError_t e = hipStreamSynchronize(h->ctx->stream);
   if (rc == TMNN_OK && e != hipSuccess)
     rc = fail(TMNN_ERR_GPU, std::string("hipStreamSynchronize: ") + hipGetErrorString(e));
+  if (rc == TMNN_OK) arrays.place();
   return rc;
 }
 
