@@ -16,6 +16,12 @@
 // and that of listed class j is w T (a_a 2^(c (z_j - m_a)) - q_j); (m_d, a_d, m_a,
 // a_a) are the row's statistics. m_a = -inf marks a row whose classes are all
 // masked: loss and gradient 0.
+//
+// Bound: reading the logits once and writing the gradient, and, for rows that do not stay in
+// registers, reading them again from the caches: 8192 x 65536 bf16, 32 values with the tail
+// 454 us (4.7 TB/s of the 2.1 GB that have to move; a copy of them takes 430); 16384 x 8192 bf16, in
+// registers, 111 us (4.8 TB/s). Short rows are bound by their instructions: 30011 x 1000 fp16
+// 42 us, 2^18 x 16 fp32 14 us.
 #pragma once
 
 #include "logprob_kernel.hpp"

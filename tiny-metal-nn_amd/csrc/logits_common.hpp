@@ -382,13 +382,16 @@ __device__ __forceinline__ float next_above(float z) {
 
 // ---- the k largest keys of a block ---------------------------------------------
 
-constexpr int kCandidates = 1024;
-constexpr int kSources = 1024;
+// Elements that may reach the bound before it is made exact: rows of equal logits bring
+// up to 8 (k + 1), k at most half the groups. Small blocks keep their LDS small (65536 x 1000 bf16,
+// 20 alternatives, 64 threads: 178 us with room for 1024, 12 waves on a unit).
+constexpr int candidates(int threads) { return (threads < 256 ? threads : 256) * 4 + 64; }
 // The threads' keys in groups: 256, or one a thread (at least k either way).
 constexpr int key_groups(int threads) { return threads < 256 ? threads : 256; }
 
-template <int NT>
+template <int NT, int SOURCES = NT>
 struct SelectLds {
+  static constexpr int kCandidates = candidates(NT), kSources = SOURCES;
   uint64_t key[NT];
   uint64_t cand[kCandidates];
   uint64_t tau;
@@ -464,11 +467,12 @@ __device__ __forceinline__ uint64_t kth_key(const uint64_t *key, int k) {
 // No element costs anything beyond the running maximum of the first pass: the k-th
 // largest of the groups' maxima bounds the answer from below, and the block looks
 // again only at the sources that reach it (about k of them, and about
-// k (1 + k / 512) elements that reach it, in no special order). Where more than
-// kCandidates elements do, the bound is made exact by counting.
-template <int NT, class Each, class Visit, class Put>
-__device__ __forceinline__ int block_select(SelectLds<NT> &s, uint64_t mine, int k, int vectors,
-                                            Each each, Visit visit, Put put) {
+// k (1 + k / 512) elements that reach it, in no special order). Where more elements do than
+// there is room for, the bound is made exact by counting.
+template <int NT, int SOURCES, class Each, class Visit, class Put>
+__device__ __forceinline__ int block_select(SelectLds<NT, SOURCES> &s, uint64_t mine, int k,
+                                            int vectors, Each each, Visit visit, Put put) {
+  constexpr int kCandidates = candidates(NT), kSources = SOURCES;
   const int tid = threadIdx.x;
   s.key[tid] = mine;
   if (tid == 0) {
