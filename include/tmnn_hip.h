@@ -762,7 +762,7 @@ int tmnn_token_logprobs_backward_device(tmnn_logits *h, const tmnn_token_logprob
  * row_weights (stats of a call without weights, or with weights that are not 0).
  * Negative teacher_ids mark unused entries; an id that is listed twice counts by its
  * first entry; an id >= classes or a NaN value makes its row NaN. Rows of weight 0
- * are not read: loss and gradient 0. A row without entries: loss and gradient 0.
+ * have loss and gradient 0, whatever they hold. A row without entries: loss and gradient 0.
  * d_logits has the type of the logits and may be the logits. */
 typedef struct tmnn_distill_args {
   uint32_t struct_size;       /* sizeof(tmnn_distill_args) */

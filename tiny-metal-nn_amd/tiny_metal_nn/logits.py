@@ -313,7 +313,7 @@ class LogitOps:
         the gradient of its sum. `kind` "logits": q = softmax(teacher / T) over the
         listed classes; "logprobs": q = exp(teacher), and the classes that are not
         listed count as one class of the remaining mass. Negative ids mark unused
-        entries. Rows of weight 0 give 0 and are not read. `stats` [rows, 4] is
+        entries. Rows of weight 0 give 0, whatever they hold. `stats` [rows, 4] is
         what distill_backward takes.
 
         `out`: arrays to write to, by these names; it gets those that it lacks, and is
