@@ -504,6 +504,37 @@ def test_streams_and_a_shared_handle(ops):
         check_forward(got[12 + i], want[i], k)
 
 
+@pytest.mark.parametrize("raw", [False, True])
+def test_new_arrays_belong_to_the_calls_stream(ops, raw):
+    """Memory of the current stream that is free to it may still be in use there: what a
+    call makes for another stream comes from that stream's memory."""
+    rng = np.random.default_rng(15)
+    n, v = 3, 5000
+    z = matrix(logits_of(rng, n, v), "f32")
+    want = ref.token_logprobs(host(z), None, 4, 1.0)
+    ids, val = teacher_of(rng, host(z), 4, "logits", 1.0)
+    did, dval, ones = dev(ids), dev(val), dev(np.ones(n, np.float32))
+    s = torch.cuda.Stream()
+    on = s.cuda_stream if raw else s
+    torch.cuda.synchronize()
+    a = ops.token_logprobs(z, None, top_k=4, stream=on)
+    b = ops.distill(z, did, dval, stream=on)
+    made = [*a.values(), *b.values(),
+            ops.token_logprobs_backward(z, None, a, d_entropy=ones, stream=on),
+            ops.distill_backward(z, did, dval, b["stats"], ones, stream=on)]
+    here = ops.token_logprobs(z, None)["stats"]
+    torch.cuda.synchronize()
+
+    def owner(x):
+        at = x.data_ptr()
+        return [q["stream"] for q in torch.cuda.memory_snapshot()
+                if q["address"] <= at < q["address"] + q["total_size"]]
+
+    assert all(owner(x) == [s.cuda_stream] for x in made)
+    assert owner(here) == [torch.cuda.current_stream().cuda_stream]
+    check_forward(a, want, 4)
+
+
 def test_graph_capture():
     """A captured step, replayed on new contents, with eager calls between."""
     from tiny_metal_nn import LogitOps

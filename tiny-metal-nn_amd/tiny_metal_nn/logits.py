@@ -4,13 +4,14 @@ alternatives, their gradient, and distillation from a teacher's top values.
 
 Arrays are numpy arrays (copied in and out; the results are there on return) or
 torch tensors of the operators' device (the call is only enqueued, on torch's
-current stream unless `stream` says otherwise). All arrays of a call are of one
-sort. Logits are float32, float16 or (tensors) bfloat16, [rows, classes] with unit
-stride within a row; class ids int32 or int64; everything else float32 / int32 and
-contiguous. No counterpart in the reference.
+current stream unless `stream` says otherwise; arrays that a call makes belong to its
+stream). All arrays of a call are of one sort. Logits are float32, float16 or (tensors)
+bfloat16, [rows, classes] with unit stride within a row; class ids int32 or int64;
+everything else float32 / int32 and contiguous. No counterpart in the reference.
 """
 from __future__ import annotations
 
+import copy
 import ctypes
 import struct
 import sys
@@ -128,6 +129,19 @@ class _DeviceArrays(_Arrays):
         self.index_codes = {getattr(torch, k): c for k, c in _lib.INDEX_DTYPES.items()}
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: torch.cuda.current_stream(d).cuda_stream)
+        self.side = None  # the stream that new arrays belong to, if not the current one
+
+    def on(self, stream) -> "_DeviceArrays":
+        """The same for a call on a stream of the caller's. Its new arrays are of that
+        stream's memory: memory that the current stream has freed may still be in use there."""
+        cuda = self.torch.cuda
+        if isinstance(stream, int):
+            if stream == -1:  # the context's own (TMNN_STREAM_CONTEXT): torch has none of its memory
+                return self
+            stream = cuda.ExternalStream(stream, self.device)
+        a = copy.copy(self)
+        a.side = stream
+        return a
 
     @staticmethod
     def ours(x) -> bool:
@@ -154,7 +168,10 @@ class _DeviceArrays(_Arrays):
         return (x.data_ptr(), *x.stride())
 
     def empty(self, shape: tuple, dtype):
-        return self.torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        if self.side is None:
+            return self.torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        with self.torch.cuda.stream(self.side):
+            return self.torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
 
 
 class LogitOps:
@@ -195,10 +212,12 @@ class LogitOps:
         except Exception:
             pass
 
-    def _arrays(self, logits) -> _Arrays:
+    def _arrays(self, logits, stream) -> _Arrays:
         if self._h is None:
             raise ClosedError("LogitOps is closed")
         if isinstance(logits, np.ndarray):
+            if stream is not None:
+                raise ValueError("stream goes with torch tensors")
             return self._host
         if self._device is None:
             torch = sys.modules.get("torch")
@@ -207,12 +226,10 @@ class LogitOps:
             self._device = _DeviceArrays(torch, self._ordinal)
         elif not hasattr(logits, "data_ptr"):
             raise TypeError(f"logits must be a numpy array or a torch tensor, got {type(logits).__name__}")
-        return self._device
+        return self._device if stream is None else self._device.on(stream)
 
     def _run(self, a: _Arrays, on_host, on_device, packed: bytes, stream) -> None:
         if a.device is None:
-            if stream is not None:
-                raise ValueError("stream goes with torch tensors")
             rc = on_host(self._h, packed)
         else:
             if stream is None:
@@ -236,7 +253,7 @@ class LogitOps:
         `out`: arrays to write to, by these names; it gets those that it lacks, and
         is returned. -inf masks a class; a row whose classes are all masked has log p
         -inf and entropy 0, a row with NaN or +inf gives NaN."""
-        a = self._arrays(logits)
+        a = self._arrays(logits, stream)
         at, stride, n, v, code = a.logits(logits, "logits")
         if not 0 <= top_k <= _lib.LOGITS_MAX_TOP:
             raise ValueError(f"top_k must be in [0, {_lib.LOGITS_MAX_TOP}], got {top_k}")
@@ -263,7 +280,7 @@ class LogitOps:
         """The gradient, in the logits' type, of sum(d_logprob * logprob + d_entropy *
         entropy) + sum(d_top_logprobs * top_logprobs). `forward`: what token_logprobs
         returned for these logits. `out` may be the logits."""
-        a = self._arrays(logits)
+        a = self._arrays(logits, stream)
         at, stride, n, v, code = a.logits(logits, "logits")
         if out is None:
             out = a.empty(logits.shape, logits.dtype)
@@ -318,7 +335,7 @@ class LogitOps:
 
         `out`: arrays to write to, by these names; it gets those that it lacks, and is
         returned. out["d_logits"] may be the logits."""
-        a = self._arrays(logits)
+        a = self._arrays(logits, stream)
         at, stride, n, v, code = a.logits(logits, "logits")
         if out is None:
             out = {}
@@ -342,7 +359,7 @@ class LogitOps:
                          temperature: float = 1.0, out=None, stream=None):
         """The gradient, in the logits' type, of sum(d_loss * loss) of an unweighted
         distill call, from its `stats`. `out` may be the logits."""
-        a = self._arrays(logits)
+        a = self._arrays(logits, stream)
         at, stride, n, v, code = a.logits(logits, "logits")
         kind_code, k, ids, index, values = self._teacher(a, n, teacher_ids, teacher, kind)
         if out is None:
