@@ -670,6 +670,25 @@ def test_refusals(ops):
         other.token_logprobs(z, tok)
 
 
+def test_gradients_in_place_need_the_logits_layout(ops):
+    """From one address with another row stride, a row's gradient would lie over the
+    logits of the next."""
+    buf = torch.zeros(4 * 20, device="cuda:0")
+    z, d = buf.view(4, 20)[:, :10], buf[:40].view(4, 10)
+    ids = torch.zeros(4, 2, dtype=torch.int64, device="cuda:0")
+    val, ones = torch.zeros(4, 2, device="cuda:0"), torch.ones(4, device="cuda:0")
+    fwd = ops.token_logprobs(z, None)
+    with pytest.raises(ValueError, match="row_stride"):
+        ops.token_logprobs_backward(z, None, fwd, d_entropy=ones, out=d)
+    with pytest.raises(ValueError, match="row_stride"):
+        ops.distill(z, ids, val, out={"d_logits": d})
+    with pytest.raises(ValueError, match="row_stride"):
+        ops.distill_backward(z, ids, val, torch.zeros(4, 4, device="cuda:0"), ones, out=d)
+    assert not buf.any()
+    # one row has no stride
+    assert ops.distill(z[:1], ids[:1], val[:1], out={"d_logits": d[:1]})["d_logits"] is not None
+
+
 def test_a_captured_stream_needs_its_own_handle():
     """A capture cannot wait for another stream's work: the call says so."""
     from tiny_metal_nn import LogitOps

@@ -69,6 +69,9 @@ int check_matrix(const A *a, const char *what) {
   const size_t size = dtype_size(a->dtype);
   if (!aligned(a->logits, size) || !aligned(a->d_logits, size))
     return bad("logits and d_logits must be aligned to their type");
+  // one row's gradient would lie over another row's logits, which it may not have read yet
+  if (a->d_logits == a->logits && a->rows > 1 && a->d_row_stride != a->row_stride)
+    return bad("d_logits in the place of the logits needs their row_stride");
   return TMNN_OK;
 }
 
