@@ -97,3 +97,20 @@ def test_oracle_distill_gradient_against_differences(kind, t):
     _, d, _, _ = ref.distill(z, ids, teacher, kind, t, w)
     diff = _differences(lambda x: ref.distill(x, ids, teacher, kind, t, w)[0].sum(), z)
     assert np.abs(d - diff).max() < 1e-8
+
+
+def test_host_outputs_must_be_writeable():
+    """A mapped read-only array would fault where the copy out writes to it."""
+    from tiny_metal_nn import logits
+    arrays = logits._HostArrays()
+    z = np.zeros((2, 3), np.float32)
+    fixed, free = np.zeros((2, 3), np.float32), np.zeros((2, 3), np.float32)
+    fixed.setflags(write=False)
+    assert arrays.output({"loss": free[0]}, "loss", (3,), np.float32) == free.ctypes.data
+    with pytest.raises(ValueError, match="loss must be writeable"):
+        arrays.output({"loss": fixed[0]}, "loss", (3,), np.float32)
+    assert arrays.like(free, "d_logits", z) == (free.ctypes.data, 3)
+    with pytest.raises(ValueError, match="d_logits must be writeable"):
+        arrays.like(fixed, "d_logits", z)
+    # what is only read need not be
+    assert arrays.logits(fixed, "logits")[0] == fixed.ctypes.data

@@ -71,9 +71,10 @@ class _Arrays:
         return at, row, rows, classes, code
 
     def like(self, x, name: str, logits) -> tuple[int, int]:
-        """Address and row stride of a second matrix like the logits."""
+        """Address and row stride of a matrix to write to, like the logits."""
         if not self.ours(x):
             raise TypeError(f"{name} must be {self.sort}, as the logits are, got {type(x).__name__}")
+        self.writeable(x, name)
         return self.logits(x, name, logits.shape, logits.dtype)[:2]
 
     def ids(self, x, name: str, shape: tuple) -> tuple[int, int]:
@@ -88,7 +89,12 @@ class _Arrays:
         x = out.get(key)
         if x is None:
             x = out[key] = self.empty(shape, dtype)
-        return self.array(x, key, shape, dtype)
+        at = self.array(x, key, shape, dtype)
+        self.writeable(x, key)
+        return at
+
+    def writeable(self, x, name: str) -> None:
+        pass
 
 
 class _HostArrays(_Arrays):
@@ -115,6 +121,10 @@ class _HostArrays(_Arrays):
         size = x.itemsize
         row, col = (s // size if s % size == 0 else -1 for s in x.strides)
         return x.ctypes.data, row, col
+
+    def writeable(self, x, name: str) -> None:
+        if not x.flags.writeable:
+            raise ValueError(f"{name} must be writeable")
 
     @staticmethod
     def empty(shape: tuple, dtype):
