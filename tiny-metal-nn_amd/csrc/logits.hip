@@ -195,11 +195,24 @@ struct Split {
   int threads, parts, part_len;
 };
 
-// Threads of a block, at least so many, and blocks of a row.
+// Threads of a block, at least so many, and blocks of a row, which a second kernel joins or not.
+// Few rows go to one block each, with four vectors a thread, where its time alone is less than
+// that of shorter parts and the kernel that joins them: up to 4096 vectors, and up to 16384 where
+// there would be fewer than four parts. us in parts / in one block, log-probabilities without
+// alternatives and distillation: 1 x 32768 bf16 (4096 vectors) 5.6 / 5.0 and 9.3 / 7.9, 1 x 65536
+// 5.7 / 7.0 and 9.4 / 10.7, 128 x 65536 8.3 / 8.2 and 13.3 / 13.0, 200 x 131072 17.3 / 14.3 and
+// 29.5 / 25.3. Rows that would not be split gain from the threads alone while their blocks
+// share a unit easily: 512 x 8192 bf16 5.6 / 4.4 and 9.7 / 9.1, but 512 x 32768 fp32 13.2 / 14.8.
 Split split_of(int64_t rows, int64_t classes, int n, int (*threads)(int64_t), int at_least,
-               int64_t blocks) {
+               int64_t blocks, bool joined) {
   Split s;
   const int64_t vecs = (classes + n - 1) / n;
+  const int64_t one = 2 * rows > blocks ? 2048 : 4 * rows > blocks ? 16384 : 4096;
+  if (joined && rows <= blocks && vecs <= one) {
+    s = {64, 1, static_cast<int>(classes)};
+    while (s.threads < 1024 && (s.threads * kLogitVecs < vecs || s.threads < at_least)) s.threads *= 2;
+    return s;
+  }
   int64_t parts = 1;
   if (rows < blocks) parts = std::min<int64_t>(blocks / rows, vecs / (2 * 256));
   parts = std::max<int64_t>(parts, (classes + kMaxPartLen - 1) / kMaxPartLen);
@@ -305,7 +318,7 @@ int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
 #undef CALL
     });
   }
-  const Split sp = split_of(rows, a.classes, n, sum_threads, 2 * a.top_k, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, sum_threads, 2 * a.top_k, kSplitBlocks, true);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   a.part_threads = sp.threads;
@@ -341,7 +354,8 @@ int run_logprobs_grad(LogprobArgs a, int64_t rows, hipStream_t st) {
 #undef CALL
     });
   }
-  const Split sp = split_of(rows, a.classes, n, map_threads, a.d_top ? a.top_k + 1 : 1, kSplitBlocks);
+  const Split sp = split_of(rows, a.classes, n, map_threads, a.d_top ? a.top_k + 1 : 1, kSplitBlocks,
+                            false);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1, [&](int64_t at, int32_t r) {
@@ -388,7 +402,7 @@ int run_distill(tmnn_logits *h, DistillArgs a, int64_t rows, bool back, hipStrea
     });
   }
   const Split sp = split_of(rows, a.classes, n, back ? map_threads : a.d_logits ? both_threads : sum_threads,
-                            a.k, kSplitBlocks);
+                            a.k, kSplitBlocks, !back);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
   if (back)
