@@ -11,11 +11,12 @@
 // whose sums and best classes a second kernel joins (few rows).
 //
 // Bound: the forward pass by reading the logits (4096 x 131072 bf16 with 20 alternatives
-// 200 us, 5.4 TB/s; without alternatives 184 us, the rest is the selection at each block's
+// 195 us, 5.5 TB/s; without alternatives 184 us, the rest is the selection at each block's
 // end; the vector units issue in 88% of the time, yet counting the ranks with scalar
-// instructions, two vector ones a class less, leaves it at 200 us), the gradient by reading
-// and writing them (8192 x 65536 bf16 380 us, 5.6 TB/s). Few rows are bound by the latency
-// of two dependent kernels (one row of 32768 bf16: 4.8 + 6.5 us).
+// instructions, two vector ones a class less, did not change it), the gradient by reading
+// and writing them (8192 x 65536 bf16 380 us, 5.6 TB/s). Few rows are bound by latency:
+// one block's loads, sums and selection (one row of 32768 bf16: 8.1 us; in parts and a join 4.8 +
+// 6.5), or two dependent kernels for rows of more than 4096 vectors.
 #pragma once
 
 #include "logits_common.hpp"
