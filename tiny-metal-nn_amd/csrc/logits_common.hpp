@@ -17,8 +17,13 @@
 namespace tmnn_hip {
 
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kNoShift = -1e37f;   // R of a sum without terms; every other R is larger
-constexpr float kPlainShift = 1e30f; // |m c| up to which z c - R cannot overflow
+// |m c| up to which the fma form is used: R is off by at most 4 there, so no term passes 2^4,
+// and logits of up to 93 have it at the lowest temperature (1e-6).
+constexpr float kPlainShift = 134217728.0f;  // 2^27
+// The lowest R, that of a sum without terms too. A thread whose classes all lie below (a finite
+// mask fill) adds 0 with it, as every class does that is so far below its row's maximum; where
+// the row's maximum is below itself, |m c| is above kPlainShift.
+constexpr float kNoShift = -kPlainShift;
 constexpr int kWave = 64;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -290,7 +295,8 @@ __device__ __forceinline__ void soft_lanes(Soft &s, float c) {
   s.R = R;
 }
 
-// m c is too large for the fma form, or not a number that can be a shift.
+// m c is too large for the fma form, or not a number that can be a shift. What the form made
+// of such a row (an R that is off by more than an exponent holds gives infinities) is not used.
 __device__ __forceinline__ bool soft_is_huge(float m, float c) {
   return !(fabsf(m * c) <= kPlainShift) && m != -__builtin_inff();
 }
