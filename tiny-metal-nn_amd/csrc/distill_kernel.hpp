@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kGroupThreads) void distill_group_kernel(DistillArg
       all.S = 1.0f + all.r;
     }
     r = distill_row<TAIL>(a, dense, all, listed, mass, tm.left, &rest_loss);
-    if (all.m == -inf && all.S == 0.0f) r.m_a = -inf;
+    if (all.m == -inf && all.S == 0.0f) r = DistillRow{0.0f, 0.0f, -inf, 0.0f};  // every class is masked
   }
   const bool zero = !live || (r.m_a == -inf && r.a_a == r.a_a);
   const float scale = w * a.t, log_s = log1p_of(all.r);
