@@ -342,7 +342,7 @@ int run_logprobs(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
 }
 
 template <class T>
-int run_logprobs_grad(LogprobArgs a, int64_t rows, hipStream_t st) {
+int run_logprobs_grad(tmnn_logits *h, LogprobArgs a, int64_t rows, hipStream_t st) {
   constexpr int n = Row<T>::n;
   if (const int g = group_lanes(a.classes)) {
     return in_slices(rows, g, 1, [&](int64_t at, int32_t r) {
@@ -358,13 +358,22 @@ int run_logprobs_grad(LogprobArgs a, int64_t rows, hipStream_t st) {
                             false);
   a.parts = sp.parts;
   a.part_len = sp.part_len;
-  return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, 1, [&](int64_t at, int32_t r) {
-    const LogprobArgs s = logprob_slice<T>(a, at, r);
+  a.part_sum = static_cast<float4 *>(h->work.ptr);
+  if (a.parts > 1) {
+    const int rc = take_workspace(h, st);
+    if (rc != TMNN_OK) return rc;
+  }
+  return in_slices(rows, static_cast<int64_t>(sp.threads) * a.parts, a.parts,
+                   [&](int64_t at, int32_t r) {
+                     const LogprobArgs s = logprob_slice<T>(a, at, r);
 #define CALL(NT) \
   hipLaunchKernelGGL((logprob_grad_block_kernel<T, NT>), dim3(r * a.parts), dim3(NT), 0, st, s)
-    TMNN_BY_THREADS(sp.threads, CALL)
+                     TMNN_BY_THREADS(sp.threads, CALL)
 #undef CALL
-  });
+                     if (a.parts > 1)
+                       hipLaunchKernelGGL((logprob_grad_best_kernel<T>), dim3(r), dim3(kBestThreads),
+                                          0, st, s);
+                   });
 }
 
 template <class T>
@@ -488,12 +497,12 @@ int logprobs_device(tmnn_logits *h, const tmnn_token_logprobs_args &u, bool back
   std::lock_guard<std::mutex> lock(h->mu);
   switch (u.dtype) {
     case TMNN_DTYPE_F32:
-      return back ? run_logprobs_grad<float>(a, u.rows, st) : run_logprobs<float>(h, a, u.rows, st);
+      return back ? run_logprobs_grad<float>(h, a, u.rows, st) : run_logprobs<float>(h, a, u.rows, st);
     case TMNN_DTYPE_F16:
-      return back ? run_logprobs_grad<_Float16>(a, u.rows, st)
+      return back ? run_logprobs_grad<_Float16>(h, a, u.rows, st)
                   : run_logprobs<_Float16>(h, a, u.rows, st);
     default:
-      return back ? run_logprobs_grad<__bf16>(a, u.rows, st) : run_logprobs<__bf16>(h, a, u.rows, st);
+      return back ? run_logprobs_grad<__bf16>(h, a, u.rows, st) : run_logprobs<__bf16>(h, a, u.rows, st);
   }
 }
 

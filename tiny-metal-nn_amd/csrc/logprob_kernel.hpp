@@ -708,32 +708,50 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(LogprobArgs 
 
 // A row's gradient: class v gets 2^x (a + b x) with x = c (z_v - m), plus its
 // listed terms.
+//
+// Where the best class outweighs all others (S = 1 + r, r < 1/8), its own terms cancel: with g
+// listed and w = sum of all that are, T d z = (g - w) / S + g r / S - g_H (H - ln S) / S, the
+// first difference 0 for a row with this one term. S holds r to 2^-24 only, 12% of it at
+// 1 - p = 2e-7; so r and H - ln S = -ln2 E / S come from a sum over the other classes again.
 struct LogprobRow {
-  float m, a, b;
+  float m, S, a, b;
   int token;       // -1: none, or without a term
   float g_token;   // times 1 / T
+  float all;       // w times 1 / T
+  float g_entropy;
+  float spread;    // g_H (H - ln S) / T
   bool skip;       // 0 everywhere
+  bool peaked;
+  // H - ln S (where the entropy has a gradient)
+  __device__ __forceinline__ void finish(const LogprobArgs &args, float g, float top_sum, float h) {
+    const float scale = quotient(args.inv_t, S);
+    a = -(g + top_sum + g_entropy * h) * scale;
+    b = -g_entropy * kLn2 * scale;
+    spread = g_entropy * h * args.inv_t;
+  }
+  // of the best class of a peaked row, with `g` (times 1 / T) listed; `rest`: r
+  __device__ __forceinline__ float best(float g, float rest) const {
+    return quotient(__builtin_fmaf(g, rest, (g - all) - spread), S);
+  }
 };
 
-// top_sum: the sum of the listed terms; top_any: one of them is not 0; spread(S):
-// H - ln S.
-template <class Spread>
+// top_sum: the sum of the listed terms; top_any: one of them is not 0. `*token_g`: the token's
+// term. finish() completes it.
 __device__ __forceinline__ LogprobRow logprob_row(const LogprobArgs &a, int64_t row, float top_sum,
-                                                  bool top_any, Spread spread) {
+                                                  bool top_any, float *token_g) {
   LogprobRow r;
   const int64_t token = a.tokens && a.d_logprob ? load_index(a.tokens, row, a.wide_index) : -1;
   r.m = a.stats_in[2 * row];
-  const float S = a.stats_in[2 * row + 1];
-  const float g = token >= 0 ? a.d_logprob[row] : 0.0f;
-  const float gh = a.d_entropy ? a.d_entropy[row] : 0.0f;
+  r.S = a.stats_in[2 * row + 1];
+  float g = token >= 0 ? a.d_logprob[row] : 0.0f;
+  r.g_entropy = a.d_entropy ? a.d_entropy[row] : 0.0f;
   r.token = token < a.classes ? static_cast<int>(token) : -1;
-  const float h = gh != 0.0f ? spread(S) : 0.0f;
-  const float scale = quotient(a.inv_t, S);
-  r.a = -(g + top_sum + gh * h) * scale;
-  r.b = -gh * kLn2 * scale;
+  r.skip = r.S == 0.0f || (g == 0.0f && r.g_entropy == 0.0f && !top_any);
+  r.peaked = r.S < kPeaked && !r.skip;
+  if (token >= a.classes && g != 0.0f) g = __builtin_nanf("");
   r.g_token = g * a.inv_t;
-  if (token >= a.classes && g != 0.0f) r.a = __builtin_nanf("");
-  r.skip = S == 0.0f || (g == 0.0f && gh == 0.0f && !top_any);
+  r.all = r.g_token + top_sum * a.inv_t;
+  *token_g = g;
   return r;
 }
 
@@ -831,8 +849,30 @@ __global__ __launch_bounds__(kGroupThreads) void logprob_grad_group_kernel(Logpr
   sum = lanes_sum<G>(sum);
   LogprobRow r{};
   r.token = -1;
-  if (live)
-    r = logprob_row(a, row, top_sum, any, [&](float S) { return -kLn2 * quotient(sum, S); });
+  if (live) {
+    float token_g;
+    r = logprob_row(a, row, top_sum, any, &token_g);
+    r.finish(a, token_g, top_sum, r.g_entropy != 0.0f ? -kLn2 * quotient(sum, r.S) : 0.0f);
+  }
+  // the best class of a peaked row, and what it gets (known before the others, in few registers)
+  const bool some = __any(r.peaked);
+  int best = -1;
+  float best_d = 0.0f;
+  if (some) {
+    float rest = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      rest += __builtin_amdgcn_fractf(p[e]);  // the best class has 1, all others less
+      best = x[e] == 0.0f ? e : best;
+    }
+    rest = lanes_sum<G>(rest);
+    if (!r.peaked) best = -1;
+    if (best >= 0) {
+      float listed = a.d_top && mine[best] != kUnlisted ? __int_as_float(mine[best]) : 0.0f;
+      if (g.index(best) == r.token) listed += r.g_token;
+      best_d = r.best(listed, rest);
+    }
+  }
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     float t = p[e] * __builtin_fmaf(r.b, x[e], r.a);
@@ -840,18 +880,78 @@ __global__ __launch_bounds__(kGroupThreads) void logprob_grad_group_kernel(Logpr
     if (g.index(e) == r.token) t += r.g_token;
     v[e] = r.skip ? 0.0f : t;
   }
+  if (some)
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e == best ? best_d : v[e];
   g.store_rows(a.d_logits, a.d_row_stride, a.rows, a.classes, words.word, v);
+}
+
+// What the long rows' gradient kernels have of a row's listed classes.
+struct ListedLds {
+  __attribute__((aligned(16))) int id[kMaxTop];
+  float term[kMaxTop];
+  float sum, any;
+};
+
+// The thread's listed class (-1: none, outside the classes or listed before) and its term, and
+// the row's totals. NT > top_k.
+struct Listed {
+  int id = -1;
+  float g = 0.0f, sum = 0.0f;
+  bool any = false;
+};
+__device__ __forceinline__ Listed listed_terms(const LogprobArgs &a, ListedLds &l, int64_t row) {
+  Listed o;
+  const int tid = threadIdx.x, k = a.d_top ? a.top_k : 0;
+  if (k == 0) return o;
+  if (tid < ((k + 3) & ~3)) {
+    const int id = tid < k ? a.top_in[row * a.top_k + tid] : -1;
+    o.id = id >= 0 && id < a.classes ? id : -1;
+    o.g = o.id >= 0 ? a.d_top[row * a.top_k + tid] : 0.0f;
+    l.id[tid] = o.id;
+  }
+  __syncthreads();
+  if (tid < k) {
+    // a class counts by its first entry
+    if (listed_before(l.id, k, tid, o.id)) o.id = -1;
+    if (o.id < 0) o.g = 0.0f;
+    l.term[tid] = o.g;
+  }
+  __syncthreads();
+  if (tid < kWave) {
+    float s = 0.0f;
+    bool any = false;
+    for (int j = tid; j < k; j += kWave) {
+      s += l.term[j];
+      any |= l.term[j] != 0.0f;
+    }
+    s = lanes_sum<kWave>(s);
+    any = lanes_any<kWave>(any);
+    if (tid == 0) {
+      l.sum = s;
+      l.any = any ? 1.0f : 0.0f;
+    }
+  }
+  __syncthreads();
+  o.sum = l.sum;
+  o.any = l.any != 0.0f;
+  return o;
 }
 
 // One part of a row. The listed classes and the token are written after all
 // others; their logits are read before the block writes anything, so that the
 // gradient may take the place of the logits. NT > top_k: a thread for each listed class
 // and one for the token.
+//
+// A peaked row's r and E are summed up while it is written, with an H - ln S from the statistics
+// that is right for all classes but the best, which is written once more at the end (by a
+// second kernel where several blocks write the row: 64 x 131072 fp32 11.6 -> 13.2 us, peaked rows
+// 15.5). 4096 x 32768 bf16, all rows peaked, 104 us (ordinary rows 98; summed up in a pass
+// before it 117), 16384 x 5003 79 (71).
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
-  __shared__ __attribute__((aligned(16))) int list[kMaxTop];
-  __shared__ float term[kMaxTop];
-  __shared__ float sums[2];
+  __shared__ ListedLds list;
+  __shared__ BlockLds<NT> lds;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
@@ -859,53 +959,20 @@ __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
   T *out = static_cast<T *>(a.d_logits) + row * a.d_row_stride;
   const Part<T, NT> p(z, part, a.part_len, a.classes);
   const int k = a.d_top ? a.top_k : 0;
-  float top_sum = 0.0f;
-  bool top_any = false;
-  int mine = -1;
-  float g = 0.0f;
-  if (k > 0) {
-    if (tid < ((k + 3) & ~3)) {
-      const int id = tid < k ? a.top_in[row * a.top_k + tid] : -1;
-      mine = id >= 0 && id < a.classes ? id : -1;
-      g = mine >= 0 ? a.d_top[row * a.top_k + tid] : 0.0f;
-      list[tid] = mine;
-    }
-    __syncthreads();
-    if (tid < k) {
-      // a class counts by its first entry
-      if (listed_before(list, k, tid, mine)) mine = -1;
-      if (mine < 0) g = 0.0f;
-      term[tid] = g;
-    }
-    __syncthreads();
-    if (tid < kWave) {
-      float s = 0.0f;
-      bool any = false;
-      for (int j = tid; j < k; j += kWave) {
-        s += term[j];
-        any |= term[j] != 0.0f;
-      }
-      s = lanes_sum<kWave>(s);
-      any = lanes_any<kWave>(any);
-      if (tid == 0) {
-        sums[0] = s;
-        sums[1] = any ? 1.0f : 0.0f;
-      }
-    }
-    __syncthreads();
-    top_sum = sums[0];
-    top_any = sums[1] != 0.0f;
-  }
-  const LogprobRow r = logprob_row(a, row, top_sum, top_any,
-                                   [&](float S) { return a.entropy_in[row] - log_of(S); });
+  const Listed listed = listed_terms(a, list, row);
+  int mine = listed.id;
+  float g = listed.g;
+  float token_g;
+  LogprobRow r = logprob_row(a, row, listed.sum, listed.any, &token_g);
   if (r.skip) {
     p.zero(out);
     return;
   }
+  r.finish(a, token_g, listed.sum, r.g_entropy != 0.0f ? a.entropy_in[row] - log_of(r.S) : 0.0f);
   g *= a.inv_t;
   if (tid == k) {
     mine = r.token;
-    if (listed_before(list, k, k, mine)) mine = -1;  // its entry's thread writes it
+    if (listed_before(list.id, k, k, mine)) mine = -1;  // its entry's thread writes it
     g = r.g_token;
   } else if (mine >= 0 && mine == r.token) {
     g += r.g_token;
@@ -914,25 +981,102 @@ __global__ __launch_bounds__(NT) void logprob_grad_block_kernel(LogprobArgs a) {
   const float zm = mine >= 0 ? Row<T>::up(z[mine]) : 0.0f;
   if (a.d_logits == a.logits) __syncthreads();
   const ExpAt e(r.m, a.c);
-  // 2^x of the fma form carries `fix`, and its x the same correction
-  const float rho = e.huge ? 0.0f : __builtin_fmaf(r.m, a.c, -e.R);
-  const float fa = __builtin_fmaf(-r.b, rho, r.a) * e.fix, fb = r.b * e.fix;
-  if (e.huge) {
-    p.map(out, [&](float v) {
-      const float x = e.x_huge(v);
-      return exp2_raw(x) * __builtin_fmaf(fb, fmaxf(x, -200.0f), fa);
-    });
+  if (r.peaked) {
+    float rest = 0.0f, sum = 0.0f;
+    int best = -1;
+    constexpr int N = Row<T>::n;
+#pragma unroll 1  // (one vector in flight: registers for a class's index each cost the others)
+    for (int i = p.begin + tid * N; i < p.end; i += NT * N) {
+      float v[N];
+      load_vec<T>(z, i, p.end, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float x = e.x(v[j]), t = exp2_raw(x), y = fmaxf(x, -200.0f);
+        const bool top = v[j] == r.m;
+        rest += top ? 0.0f : t;
+        sum = __builtin_fmaf(t, y, sum);
+        best = top ? i + j : best;
+        v[j] = t * __builtin_fmaf(r.b, y, r.a);
+      }
+      store_vec<T>(out, i, p.end, v);
+    }
+    rest = block_sum<NT>(lds, rest);
+    sum = block_sum<NT>(lds, sum);
+    if (a.parts > 1) {
+      // (a class and 1 more is a whole number that 32 bits hold; one thread has one)
+      const float at = block_sum<NT>(lds, static_cast<float>(best + 1));
+      if (tid == 0) a.part_sum[blockIdx.x] = make_float4(rest, sum, at, 0.0f);
+    } else {
+      // (read again rather than kept in registers through the row)
+      const float top_sum = k > 0 ? list.sum : 0.0f;
+      r = logprob_row(a, row, top_sum, true, &token_g);
+      r.finish(a, token_g, top_sum, -kLn2 * quotient(sum, r.S));
+      if (best >= 0) out[best] = Row<T>::down(r.best(0.0f, rest));
+      __syncthreads();
+      if (mine >= 0 && zm == r.m) {
+        out[mine] = Row<T>::down(r.best(g, rest));
+        mine = -1;
+      }
+    }
   } else {
-    p.map(out, [&](float v) {
-      const float x = e.x_plain(v);
-      return exp2_raw(x) * __builtin_fmaf(fb, fmaxf(x, -200.0f), fa);
-    });
+    // 2^x of the fma form carries `fix`, and its x the same correction
+    const float rho = e.huge ? 0.0f : __builtin_fmaf(r.m, a.c, -e.R);
+    const float fa = __builtin_fmaf(-r.b, rho, r.a) * e.fix, fb = r.b * e.fix;
+    if (e.huge) {
+      p.map(out, [&](float v) {
+        const float x = e.x_huge(v);
+        return exp2_raw(x) * __builtin_fmaf(fb, fmaxf(x, -200.0f), fa);
+      });
+    } else {
+      p.map(out, [&](float v) {
+        const float x = e.x_plain(v);
+        return exp2_raw(x) * __builtin_fmaf(fb, fmaxf(x, -200.0f), fa);
+      });
+    }
   }
   __syncthreads();
   if (mine >= 0) {
     const float x = e.x(zm);
     out[mine] = Row<T>::down(exp2_raw(x) * __builtin_fmaf(r.b, fmaxf(x, -200.0f), r.a) + g);
   }
+}
+
+// The best class of the peaked rows that several blocks have written (the others' blocks
+// end at once).
+constexpr int kBestThreads = 256;
+static_assert(kBestThreads > kMaxTop, "");
+
+template <class T>
+__global__ __launch_bounds__(kBestThreads) void logprob_grad_best_kernel(LogprobArgs a) {
+  __shared__ ListedLds list;
+  __shared__ float term;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  if (!(a.stats_in[2 * row + 1] < kPeaked)) return;
+  const Listed listed = listed_terms(a, list, row);
+  float token_g;
+  LogprobRow r = logprob_row(a, row, listed.sum, listed.any, &token_g);
+  if (r.skip) return;
+  // the parts' sums, in every lane: a fixed tree
+  float rest = 0.0f, sum = 0.0f, at = 0.0f;
+  for (int i = tid & (kWave - 1); i < a.parts; i += kWave) {
+    const float4 q = a.part_sum[row * a.parts + i];
+    rest += q.x;
+    sum += q.y;
+    at += q.z;
+  }
+  rest = lanes_sum<kWave>(rest);
+  sum = lanes_sum<kWave>(sum);
+  const int best = static_cast<int>(lanes_sum<kWave>(at)) - 1;
+  if (best < 0 || best >= a.classes) return;  // statistics of other logits
+  r.finish(a, token_g, listed.sum, -kLn2 * quotient(sum, r.S));
+  if (tid == 0) term = 0.0f;
+  __syncthreads();
+  if (listed.id == best) term = listed.g * a.inv_t;
+  __syncthreads();
+  if (tid == 0)
+    static_cast<T *>(a.d_logits)[row * a.d_row_stride + best] =
+        Row<T>::down(r.best(best == r.token ? term + r.g_token : term, rest));
 }
 
 }  // namespace tmnn_hip
