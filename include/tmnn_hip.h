@@ -679,8 +679,10 @@ int tmnn_debug_philox_uniform(tmnn_context *ctx, uint64_t seed,
  * several blocks); nothing is allocated by the *_device calls, which only
  * enqueue on `stream` (a hipStream_t of the context's device, NULL being the null
  * stream, or TMNN_STREAM_CONTEXT). Calls through one handle on several streams
- * are ordered where they share the workspace; a handle of its own lets a stream
- * run freely, and is needed for a stream that is being captured into a graph. The
+ * are ordered where they share the workspace, and a stream may be destroyed once it
+ * has none left to run; a handle of its own lets a stream
+ * run freely, and is needed for a stream that is being captured into a graph (a call that
+ * would have to wait for a captured stream is refused). The
  * host-pointer calls copy in and out, on the context's stream, and return when the
  * results are there. */
 #define TMNN_STREAM_CONTEXT ((void *)(intptr_t)-1) /* the context's own stream */
