@@ -266,9 +266,9 @@ int in_slices(int64_t rows, int64_t threads_per_row, int parts, F launch) {
   return TMNN_OK;
 }
 
-dim3 group_grid(int rows, int g) {
-  const int per = kGroupThreads / g;
-  return dim3((rows + per - 1) / per);
+dim3 group_grid(int64_t rows, int g) {  // (rows of one lane pass 2^31 - per)
+  const int64_t per = kGroupThreads / g;
+  return dim3(static_cast<uint32_t>((rows + per - 1) / per));
 }
 
 #define TMNN_BY_GROUP(g, CALL)                          \
