@@ -717,7 +717,7 @@ int tmnn_logits_destroy(tmnn_logits *h);
  * (null: 0). Entries of top_ids outside the classes are not used, and a class
  * that is listed twice counts by its first entry. Rows whose upstream gradients are
  * all 0 get 0. d_logits has the type of the logits and may be the logits (with
- * their row_stride); it may not overlap them otherwise. */
+ * their row_stride); rows of both may interleave, but not overlap (refused). */
 typedef struct tmnn_token_logprobs_args {
   uint32_t struct_size;       /* sizeof(tmnn_token_logprobs_args) */
   int32_t dtype;              /* TMNN_DTYPE_* of logits and d_logits */
@@ -767,7 +767,7 @@ int tmnn_token_logprobs_backward_device(tmnn_logits *h, const tmnn_token_logprob
  * first entry; an id >= classes or a NaN value makes its row NaN. Rows of weight 0
  * have loss and gradient 0, whatever they hold. A row without entries: loss and gradient 0.
  * d_logits has the type of the logits and may be the logits (with their row_stride);
- * it may not overlap them otherwise. */
+ * rows of both may interleave, but not overlap (refused). */
 typedef struct tmnn_distill_args {
   uint32_t struct_size;       /* sizeof(tmnn_distill_args) */
   int32_t dtype;              /* TMNN_DTYPE_* of logits and d_logits */

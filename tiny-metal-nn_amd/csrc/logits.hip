@@ -47,8 +47,34 @@ size_t dtype_size(int32_t dtype) { return dtype == TMNN_DTYPE_F32 ? 4 : 2; }
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Whether a row of d_logits lies over a part of the logits other than its own place (at one address,
+// with one row stride). Rows of both may interleave.
 template <class A>
-int check_matrix(const A *a, const char *what) {
+bool overlaps(const A *a) {
+  typedef __int128 wide;  // strides are the caller's
+  const wide size = static_cast<wide>(dtype_size(a->dtype)), n = a->rows, width = a->classes * size;
+  const wide s = a->row_stride * size, ds = a->d_row_stride * size;
+  const wide z = reinterpret_cast<uintptr_t>(a->logits), d = reinterpret_cast<uintptr_t>(a->d_logits);
+  if (z == d) return n > 1 && s != ds;
+  if (d >= z + (n - 1) * s + width || z >= d + (n - 1) * ds + width) return false;
+  // the first row of logits that ends after `at`, whether there is one that begins before its end
+  auto meets = [&](wide at) {
+    const wide i = at < z + width ? 0 : (at - z - width) / s + 1;
+    return i < n && z + i * s < at + width;
+  };
+  if (s == ds) {
+    // rows are shifted by whole strides against each other, or lie alike in all: against the
+    // rows beside it, the first row of d_logits that is not before the logits says it for all
+    const wide j = d >= z ? 0 : std::min<wide>(n - 1, (z - d) / ds);
+    return meets(d + j * ds) || (j + 1 < n && meets(d + (j + 1) * ds));
+  }
+  for (wide j = 0; j < n; ++j)
+    if (meets(d + j * ds)) return true;
+  return false;
+}
+
+template <class A>
+int check_matrix(const A *a, const char *what, bool written) {
   auto bad = [&](const char *m) {
     return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
   };
@@ -73,16 +99,19 @@ int check_matrix(const A *a, const char *what) {
   // one row's gradient would lie over another row's logits, which it may not have read yet
   if (a->d_logits == a->logits && a->rows > 1 && a->d_row_stride != a->row_stride)
     return bad("d_logits in the place of the logits needs their row_stride");
+  if (written && a->d_logits && overlaps(a))
+    return bad("d_logits overlaps the logits (their own place, with their row_stride, is allowed)");
   return TMNN_OK;
 }
 
-int check_logprobs(const tmnn_token_logprobs_args *a, bool back) {
+int check_logprobs(const tmnn_token_logprobs_args *a, bool back, bool host) {
   const char *what = back ? "token_logprobs_backward" : "token_logprobs";
   auto bad = [&](const char *m) {
     return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
   };
   if (!a) return bad("args is null");
-  const int rc = check_matrix(a, what);
+  // (host arrays are written once everything has been read)
+  const int rc = check_matrix(a, what, back && !host);
   if (rc != TMNN_OK) return rc;
   if (a->top_k < 0 || a->top_k > TMNN_LOGITS_MAX_TOP) return bad("top_k must be in [0, 128]");
   if (a->rows == 0) return TMNN_OK;
@@ -115,7 +144,7 @@ int check_distill(const tmnn_distill_args *a, bool back, bool host) {
     return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
   };
   if (!a) return bad("args is null");
-  const int rc = check_matrix(a, what);
+  const int rc = check_matrix(a, what, !host);
   if (rc != TMNN_OK) return rc;
   if (a->teacher_kind != TMNN_TEACHER_LOGITS && a->teacher_kind != TMNN_TEACHER_LOGPROBS)
     return bad("invalid teacher_kind");
@@ -689,7 +718,7 @@ int entry(tmnn_logits *h, F f) {
 int token_logprobs(tmnn_logits *h, const tmnn_token_logprobs_args *args, bool back, bool host,
                    void *stream) {
   return entry(h, [&] {
-    const int rc = check_logprobs(args, back);
+    const int rc = check_logprobs(args, back, host);
     if (rc != TMNN_OK || args->rows == 0) return rc;
     TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
     return host ? logprobs_host(h, *args, back)
