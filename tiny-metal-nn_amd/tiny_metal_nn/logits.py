@@ -8,6 +8,11 @@ current stream unless `stream` says otherwise; arrays that a call makes belong t
 stream). All arrays of a call are of one sort. Logits are float32, float16 or (tensors)
 bfloat16, [rows, classes] with unit stride within a row; class ids int32 or int64;
 everything else float32 / int32 and contiguous. No counterpart in the reference.
+
+The calls are no part of torch's autograd: results have no history, whether or not the
+logits require gradients, and a loss's gradient is the *_backward calls' (in a
+torch.autograd.Function, or passed to logits.backward()). Tensors that a call writes to are
+marked as changed in place, so that autograd refuses a backward pass that saved their old values.
 """
 from __future__ import annotations
 
@@ -24,6 +29,8 @@ from .trainer import ClosedError, DTypeError, _Context
 # tmnn_token_logprobs_args, tmnn_distill_args
 _PACK_LOGPROBS = struct.Struct("=Iiii4q12Qfi")
 _PACK_DISTILL = struct.Struct("=Iiii4q7Qif")
+_FORWARD = ("logprob", "entropy", "rank", "stats")
+_FORWARD_TOP = _FORWARD + ("top_ids", "top_logprobs")
 _SIZE_LOGPROBS, _SIZE_DISTILL = _PACK_LOGPROBS.size, _PACK_DISTILL.size
 
 
@@ -54,11 +61,12 @@ class _Arrays:
         if code is None or (dtype is not None and x.dtype != dtype):
             want = "float32, float16 or bfloat16" if dtype is None else f"{self.name_of(dtype)} as the logits"
             raise DTypeError(f"{name} must be {want}, got {self.name_of(x.dtype)}")
-        if len(x.shape) != 2:
+        size = x.shape
+        if len(size) != 2:
             raise ValueError(f"{name} must be 2D (rows, classes)")
-        if shape is not None and x.shape != shape:
-            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
-        rows, classes = x.shape
+        if shape is not None and size != shape:
+            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(size)}")
+        rows, classes = size
         at, row, col = self.layout(x, name)
         if classes < 1:
             raise ValueError(f"{name} must have at least one class")
@@ -95,6 +103,9 @@ class _Arrays:
 
     def writeable(self, x, name: str) -> None:
         pass
+
+    def wrote(self, arrays: list) -> None:
+        """After a call: what it has written to."""
 
 
 class _HostArrays(_Arrays):
@@ -140,6 +151,7 @@ class _DeviceArrays(_Arrays):
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: torch.cuda.current_stream(d).cuda_stream)
         self.side = None  # the stream that new arrays belong to, if not the current one
+        self.wrote = torch.autograd.graph.increment_version
 
     def on(self, stream) -> "_DeviceArrays":
         """The same for a call on a stream of the caller's. Its new arrays are of that
@@ -171,6 +183,19 @@ class _DeviceArrays(_Arrays):
         self.refuse(x, name, shape, self.name_of(dtype))
         self.place(x, name)
         raise ValueError(f"{name} must be contiguous")
+
+    def output(self, out: dict, key: str, shape: tuple, dtype) -> int:
+        x = out.get(key)
+        if x is None:
+            x = out[key] = self.empty(shape, dtype)
+            return x.data_ptr()
+        try:  # (as in `array`, without its call)
+            if (x.dtype is dtype and x.shape == shape and x.get_device() == self.device
+                    and x.is_contiguous()):
+                return x.data_ptr()
+        except AttributeError:
+            pass
+        return self.array(x, key, shape, dtype)
 
     def layout(self, x, name: str) -> tuple[int, int, int]:
         if x.get_device() != self.device:
@@ -282,6 +307,7 @@ class LogitOps:
                       a.output(out, "logprob", rows, f32), a.output(out, "entropy", rows, f32),
                       a.output(out, "rank", rows, i32), a.output(out, "stats", (n, 2), f32),
                       ids, best, 0, 0, 0, 0, temperature, 0), stream)
+        a.wrote([out[name] for name in (_FORWARD_TOP if top_k else _FORWARD)])
         return out
 
     def token_logprobs_backward(self, logits, tokens, forward: dict, *, d_logprob=None,
@@ -318,6 +344,7 @@ class LogitOps:
                       _SIZE_LOGPROBS, code, index, k, n, v, stride, d_stride, at, tok, 0, entropy, 0,
                       a.array(forward["stats"], "stats", (n, 2), f32), ids, 0, g_token, g_entropy,
                       g_top, d_at, temperature, 0), stream)
+        a.wrote([out])
         return out
 
     # ---- distillation --------------------------------------------------------------
@@ -363,6 +390,7 @@ class LogitOps:
                       0 if row_weights is None else a.array(row_weights, "row_weights", (n,), f32),
                       a.output(out, "loss", (n,), f32), a.output(out, "stats", (n, 4), f32), d_at, k,
                       temperature), stream)
+        a.wrote([out["loss"], out["stats"], out["d_logits"]] if gradient else [out["loss"], out["stats"]])
         return out
 
     def distill_backward(self, logits, teacher_ids, teacher, stats, d_loss, *, kind: str = "logits",
@@ -380,4 +408,5 @@ class LogitOps:
                       _SIZE_DISTILL, code, index, kind_code, n, v, stride, d_stride, at, ids, values,
                       a.array(d_loss, "d_loss", (n,), a.f32), 0, a.array(stats, "stats", (n, 4), a.f32),
                       d_at, k, temperature), stream)
+        a.wrote([out])
         return out
