@@ -277,10 +277,17 @@ Split split_of(int64_t rows, int64_t classes, int n, int (*threads)(int64_t), in
 // fp32, 20 alternatives, part and join kernel: 11.4 + 7.5 us, with 1024 blocks 9.9 + 9.4).
 constexpr int64_t kSplitBlocks = 512;
 // Alternatives up to which rows stay in registers: each costs a round over the row there, all of
-// them one selection in a block of 64 threads. us in registers / in blocks: 131072 x 250 bf16 with
-// 3 and 20 alternatives 46 / - and 136 / 308, 65536 x 510 50 / 70 and 144 / 90, 65536 x 1000 92 / 78
-// and 289 / 90.
-int group_top(int g) { return g <= 16 ? kMaxTop : g == 32 ? 4 : 2; }
+// them one selection in a block of 64 threads and more. us in registers / in blocks, by the lanes
+// of a row:
+//   64  65536 x 600 bf16, fp32 with 1 66 / 64, 69 / 63, with 2 77 / 68, 77 / 64; 65536 x 1000 with 2
+//       78 / 69, 81 / 70
+//   32  65536 x 510 bf16 with 4 53 / 70 and with 20 144 / 79
+//   16  131072 x 250 bf16 with 3 44 / 119, 20 137 / 138, 32 201 / 469, 64 373 / 917, 128 719 / 955; fp32
+//       with 20 137 / 125, 32 202 / 129, 64 375 / 907
+//   8   131072 x 128 bf16 with 20 69 / 257, 64 188 / 292, 128 359 / 435
+// (a block selects among the maxima of its threads that have classes, and a row of 250 has few:
+// it bounds 32 and more of them badly).
+int group_top(int g) { return g <= 16 ? kMaxTop : g == 32 ? 4 : 0; }
 
 // Rows of one launch: at most 2^31 threads, and the workspace of its parts.
 template <class F>
