@@ -19,7 +19,8 @@
 //
 // Bound: reading the logits once and writing the gradient, and, for rows that do not stay in
 // registers, reading them again from the caches: 8192 x 65536 bf16, 32 values with the tail
-// 454 us (4.7 TB/s of the 2.1 GB that have to move; a copy of them takes 430); 16384 x 8192 bf16, in
+// 454 us (4.7 TB/s of the 2.1 GB that have to move; a pass that reads and writes each once takes
+// 345 at the card's best); 16384 x 8192 bf16, in
 // registers, 111 us (4.8 TB/s). Short rows are bound by their instructions: 30011 x 1000 fp16
 // 42 us, 2^18 x 16 fp32 14 us.
 #pragma once
@@ -303,7 +304,6 @@ struct ListLds {
   float z[kMaxTeacher], t[kMaxTeacher], q[kMaxTeacher];
   float wrong;
   DistillRow row;
-  float scale;
 };
 
 // The thread's entry: its class, or -1 for an unused entry. An entry beyond the classes

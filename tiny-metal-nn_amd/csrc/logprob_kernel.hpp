@@ -6,7 +6,7 @@
 //   d z_v = 1/T [ p_v (A + B log p_v) + g_token [v = token] + sum_j g_j [v = top_j] ],
 //   A = -(g_token + sum_j g_j + g_H H),  B = -g_H
 //
-// Short rows (one vector a lane on up to 64 lanes) stay in registers, several
+// Short rows (up to 16 classes a lane on up to 64 lanes) stay in registers, several
 // rows to a wave. Longer rows are read once by a block, or by several blocks
 // whose sums and best classes a second kernel joins (few rows).
 //
