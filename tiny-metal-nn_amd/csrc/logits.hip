@@ -249,8 +249,9 @@ struct Split {
 // alternatives and distillation: 1 x 32768 bf16 (4096 vectors) 5.6 / 5.0 and 9.3 / 7.9, 1 x 65536
 // 5.7 / 7.0 and 9.4 / 10.7, 128 x 65536 8.3 / 8.2 and 13.3 / 13.0, 200 x 131072 17.3 / 14.3 and
 // 29.5 / 25.3. The gradient of log-probabilities, whose parts leave a peaked row's best class to a
-// second kernel, 1 x 32768 bf16 4.6 / 4.4, 200 x 131072 25.6 / 22.9, and less host work in one. Rows that would not be split gain from the threads alone while their blocks
-// share a unit easily: 512 x 8192 bf16 5.6 / 4.4 and 9.7 / 9.1, but 512 x 32768 fp32 13.2 / 14.8.
+// second kernel, 1 x 32768 bf16 4.6 / 4.4, 200 x 131072 25.6 / 22.9, and less host work in one.
+// Rows that would not be split gain from the threads alone while their blocks share a unit easily:
+// 512 x 8192 bf16 5.6 / 4.4 and 9.7 / 9.1, but 512 x 32768 fp32 13.2 / 14.8.
 Split split_of(int64_t rows, int64_t classes, int n, int (*threads)(int64_t), int at_least,
                int64_t blocks, bool joined) {
   Split s;
