@@ -793,6 +793,116 @@ int tmnn_distill_device(tmnn_logits *h, const tmnn_distill_args *args, void *str
 int tmnn_distill_backward(tmnn_logits *h, const tmnn_distill_args *args);
 int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, void *stream);
 
+/* ---- class head ------------------------------------------------------------------ */
+/* Operators over features [rows][dims] and a table [classes][dims], whose class
+ * logits are z = features . table: a training loss that never keeps the logits, and the
+ * logits themselves from 8-bit operands. They take a tmnn_logits, as the operators above.
+ *
+ * Rows start at feature_stride, table_stride, ... elements (>= dims) from each other, at
+ * any alignment of an element. Nothing that a call writes to may overlap what it reads or
+ * writes otherwise (rows of two matrices of one stride may lie between each other). The
+ * *_device calls allocate nothing: they take device memory of the caller's as
+ * `workspace`, 256-byte aligned, of at least the bytes that the *_workspace calls give
+ * for the same args (pointers in them are not followed, but alignment and which are null count), and
+ * which belongs to the call until its stream has run it. Calls with workspaces of
+ * their own are independent, captured or not. */
+#define TMNN_HEAD_MAX_ROWS (1 << 24)
+#define TMNN_HEAD_MAX_DIMS (1 << 16)
+
+/* Softmax cross entropy of each row with label l, p = softmax(z / temperature):
+ *   loss[row]  = -row_weights[row] ln p_l
+ *   stats[row][4]  the largest logit m, sum exp((z - m) / temperature), 1 - p_l, 0
+ *   d_features, d_table  the gradients of sum_row loss[row], null where not wanted
+ * A negative label marks a row without one: loss and gradients 0. So do rows of weight 0,
+ * whatever they hold (their stats are computed). A label >= classes makes its loss and gradients NaN, as
+ * logits that are not finite do. The backward call takes the stats of a call with the same features, table,
+ * labels and temperature, and the loss's gradient as row_weights; it writes the gradients. All
+ * sums in fp32; gradients are rounded once at the end. Products of gradients take operands
+ * of 11 bits (16-bit inputs) or 22 bits (fp32), relative to the largest of a tensor below 2^-24 of it. */
+typedef struct tmnn_class_loss_args {
+  uint32_t struct_size;       /* sizeof(tmnn_class_loss_args) */
+  int32_t dtype;              /* TMNN_DTYPE_* of features, table and their gradients */
+  int32_t index_dtype;        /* TMNN_INDEX_* of labels */
+  float temperature;          /* > 0 */
+  int64_t rows;               /* 0..TMNN_HEAD_MAX_ROWS */
+  int64_t classes;            /* 1..TMNN_LOGITS_MAX_CLASSES */
+  int64_t dims;               /* 1..TMNN_HEAD_MAX_DIMS */
+  int64_t feature_stride;
+  int64_t table_stride;
+  int64_t d_feature_stride;
+  int64_t d_table_stride;
+  const void *features;
+  const void *table;
+  const void *labels;         /* [rows] */
+  const float *row_weights;   /* [rows], nullable: 1 (backward: the loss's gradient, not null) */
+  float *loss;                /* [rows], nullable */
+  float *stats;               /* [rows][4], 16-byte aligned, nullable (backward: read) */
+  void *d_features;           /* [rows][dims], nullable */
+  void *d_table;              /* [classes][dims], nullable; all zeros where no row counts */
+  void *workspace;
+  int64_t workspace_bytes;
+} tmnn_class_loss_args;
+
+int tmnn_class_loss_workspace(const tmnn_class_loss_args *args, int32_t backward, int64_t *bytes);
+int tmnn_class_loss(tmnn_logits *h, const tmnn_class_loss_args *args);
+int tmnn_class_loss_device(tmnn_logits *h, const tmnn_class_loss_args *args, void *stream);
+int tmnn_class_loss_backward(tmnn_logits *h, const tmnn_class_loss_args *args);
+int tmnn_class_loss_backward_device(tmnn_logits *h, const tmnn_class_loss_args *args, void *stream);
+
+/* Scales of 8-bit values: fp32 numbers, or powers of two as their fp32 exponent
+ * bytes (E8M0: 127 is 1, 255 NaN). */
+#define TMNN_SCALE_F32 0
+#define TMNN_SCALE_E8M0 1
+
+/* logits[row][class] = sum_k x w, where x = features[row][k] feature_scales[row][k / 128] and
+ * w = table[class][k] table_scales[class / 128][k / 128]; values are e4m3 (OCP; no
+ * infinities), sums fp32, rounded once to the logits' type. A NaN among values or scales makes
+ * the logits that it enters NaN. */
+typedef struct tmnn_class_logits_f8_args {
+  uint32_t struct_size;       /* sizeof(tmnn_class_logits_f8_args) */
+  int32_t dtype;              /* TMNN_DTYPE_* of logits */
+  int32_t scale_dtype;        /* TMNN_SCALE_* of both scales */
+  int32_t reserved;           /* 0 */
+  int64_t rows;
+  int64_t classes;
+  int64_t dims;
+  int64_t feature_stride;     /* bytes; rows at multiples of 16 bytes are read in place */
+  int64_t table_stride;
+  int64_t logit_stride;       /* elements */
+  const void *features;       /* [rows][dims] */
+  const void *feature_scales; /* [rows][ceil(dims / 128)], contiguous */
+  const void *table;          /* [classes][dims] */
+  const void *table_scales;   /* [ceil(classes / 128)][ceil(dims / 128)], contiguous */
+  void *logits;               /* [rows][classes] */
+  void *workspace;
+  int64_t workspace_bytes;
+} tmnn_class_logits_f8_args;
+
+int tmnn_class_logits_f8_workspace(const tmnn_class_logits_f8_args *args, int64_t *bytes);
+int tmnn_class_logits_f8(tmnn_logits *h, const tmnn_class_logits_f8_args *args);
+int tmnn_class_logits_f8_device(tmnn_logits *h, const tmnn_class_logits_f8_args *args, void *stream);
+
+/* Values in e4m3 with a scale for each block of block_rows x 128 (1: of features, 128: of a
+ * table): scale = max |input| / 448 of the block, or the power of two at or above that (E8M0), at
+ * least 2^-126; 1 where the block is all 0. values = input / scale, rounded to the nearest (ties to
+ * even). What is not finite becomes NaN and does not count for the scale. */
+typedef struct tmnn_quantize_f8_args {
+  uint32_t struct_size;       /* sizeof(tmnn_quantize_f8_args) */
+  int32_t dtype;              /* TMNN_DTYPE_* of input */
+  int32_t scale_dtype;        /* TMNN_SCALE_* */
+  int32_t block_rows;         /* 1 or 128 */
+  int64_t rows;
+  int64_t dims;
+  int64_t stride;             /* elements */
+  int64_t value_stride;       /* bytes */
+  const void *input;          /* [rows][dims] */
+  void *values;               /* [rows][dims] */
+  void *scales;               /* [ceil(rows / block_rows)][ceil(dims / 128)], contiguous */
+} tmnn_quantize_f8_args;
+
+int tmnn_quantize_f8(tmnn_logits *h, const tmnn_quantize_f8_args *args);
+int tmnn_quantize_f8_device(tmnn_logits *h, const tmnn_quantize_f8_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,7 +21,7 @@ OUT = HERE / "libtmnn_hip.so"
 BUILD_DIR = HERE / "_build"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
-SOURCES = ["tmnn_hip.hip", "sort.hip", "logits.hip"]
+SOURCES = ["tmnn_hip.hip", "sort.hip", "logits.hip", "class_head.hip"]
 
 COMMON = [
     "--offload-arch=gfx950",

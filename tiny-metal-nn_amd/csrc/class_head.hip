@@ -1,0 +1,795 @@
+// class_head.hip -- host side of the class head (include/tmnn_hip.h): argument
+// checks, the choice of tiles and parts, the workspace, and the host-pointer forms.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <memory>
+#include <string>
+
+#include "class_loss_kernel.hpp"
+#include "f8_kernel.hpp"
+#include "logits_host.hpp"
+#include "tmnn_hip.h"
+
+using namespace tmnn_hip;
+
+namespace {
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t parts_of(int64_t n, int64_t of) { return (n + of - 1) / of; }
+
+// ---- tiles --------------------------------------------------------------------------
+
+enum Shape { kLarge, kMiddle, kSmall };
+// waves, blocks of a wave, stages
+template <class E, bool XT, bool YT>
+using Large = TileShape<E, 2, 4, 8, 4, 2, XT, YT>;
+template <class E, bool XT, bool YT>
+using Middle = TileShape<E, 2, 2, 4, 4, 2, XT, YT>;
+template <class E, bool XT, bool YT>
+using Small = TileShape<E, 4, 1, 2, 2, 4, XT, YT>;
+
+struct Tiles {
+  Shape shape;
+  int32_t bc, br, r, c, parts, part_steps;
+};
+
+constexpr int kUnits = 256;  // compute units
+
+// The shape whose tiles take the least time together, and parts of k where there are too few
+// of them to keep every unit busy.
+Tiles choose(int64_t rows, int64_t cols, int64_t steps, bool large, bool small, bool split) {
+  Tiles best{};
+  double least = 1e300;
+  for (const Shape s : {kLarge, kMiddle, kSmall}) {
+    if ((s == kSmall && !small) || (s == kLarge && !large)) continue;
+    Tiles t{};
+    t.shape = s;
+    t.bc = s == kLarge ? 256 : 128;
+    t.br = s == kLarge ? 256 : s == kMiddle ? 128 : 32;
+    t.r = static_cast<int32_t>(parts_of(rows, t.br));
+    t.c = static_cast<int32_t>(parts_of(cols, t.bc));
+    t.parts = 1;
+    const int64_t tiles = static_cast<int64_t>(t.r) * t.c;
+    if (split) {
+      const int64_t want = (s == kLarge ? 1 : 2) * kUnits;
+      int64_t p = std::max<int64_t>(1, std::min<int64_t>(want / tiles, steps / 8));
+      t.parts = static_cast<int32_t>(std::min<int64_t>(p, 64));
+    }
+    t.part_steps = static_cast<int32_t>(parts_of(steps, t.parts));
+    t.parts = static_cast<int32_t>(parts_of(steps, t.part_steps));
+    const double rate = s == kLarge ? 1.0 : s == kMiddle ? 0.75 : 0.3;
+    const double time = static_cast<double>(parts_of(tiles * t.parts, kUnits)) * t.bc * t.br *
+                        (t.part_steps + 4) / rate;
+    if (time < least) {
+      least = time;
+      best = t;
+    }
+  }
+  return best;
+}
+
+
+template <class S, class Steps, class Epi, class StepArgs>
+struct TileLaunch {
+  static int run(const TileArgs &a, const StepArgs &sa, const Epi &epi, int device, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << (device & 63);
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+      TMNN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(tile_kernel<S, Steps, Epi, StepArgs>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds));
+      done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    const int64_t blocks = static_cast<int64_t>(a.tiles_r) * a.tiles_c * a.parts;
+    hipLaunchKernelGGL((tile_kernel<S, Steps, Epi, StepArgs>), dim3(static_cast<uint32_t>(blocks)),
+                       dim3(S::kThreads), S::kLds, st, a, sa, epi);
+    TMNN_HIP_TRY(hipGetLastError());
+    return TMNN_OK;
+  }
+};
+
+TileArgs tile_args(const Operand &x, const Operand &y, int64_t rows, int64_t cols, const Tiles &t,
+                   int64_t steps, int pairs) {
+  TileArgs a{};
+  a.x = x;
+  a.y = y;
+  a.rows = static_cast<int32_t>(rows);
+  a.cols = static_cast<int32_t>(cols);
+  a.tiles_r = t.r;
+  a.tiles_c = t.c;
+  a.parts = t.parts;
+  a.steps = static_cast<int32_t>(steps);
+  a.pairs = pairs;
+  a.part_steps = t.part_steps;
+  return a;
+}
+
+struct NoArgs {
+  int32_t unused;
+};
+
+template <class S, class Epi>
+int run_plain(const TileArgs &a, const Epi &epi, int device, hipStream_t st) {
+  return TileLaunch<S, PlainSteps<S>, Epi, NoArgs>::run(a, NoArgs{}, epi, device, st);
+}
+
+// Both operands' k contiguous.
+template <class E, class Epi>
+int run_rows(const TileArgs &a, Shape s, const Epi &epi, int device, hipStream_t st) {
+  switch (s) {
+    case kLarge: return run_plain<Large<E, false, false>>(a, epi, device, st);
+    case kMiddle: return run_plain<Middle<E, false, false>>(a, epi, device, st);
+    default: return run_plain<Small<E, false, false>>(a, epi, device, st);
+  }
+}
+
+// ---- arguments ------------------------------------------------------------------------
+
+struct Extent {  // rows of `width` bytes, `stride` bytes apart
+  const void *p;
+  int64_t rows, width, stride;
+  const char *name;
+};
+
+bool meet(const Extent &a, const Extent &b) {
+  typedef __int128 wide;
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const wide pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+  const wide ea = pa + static_cast<wide>(a.rows - 1) * a.stride + a.width;
+  const wide eb = pb + static_cast<wide>(b.rows - 1) * b.stride + b.width;
+  if (pa >= eb || pb >= ea) return false;
+  if (a.rows > 1 && b.rows > 1 && a.stride == b.stride) {  // rows between each other's
+    wide off = (pb - pa) % a.stride;
+    if (off < 0) off += a.stride;
+    if (off >= a.width && off + b.width <= a.stride) return false;
+  }
+  return true;
+}
+
+// Each of `out` against `in` and the others of `out`.
+int apart(const char *what, std::initializer_list<Extent> out, std::initializer_list<Extent> in) {
+  for (const Extent &o : out) {
+    for (const Extent &i : in)
+      if (meet(o, i))
+        return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + o.name + " overlaps " + i.name);
+    for (const Extent &p : out)
+      if (&p < &o && meet(o, p))
+        return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + o.name + " overlaps " + p.name);
+  }
+  return TMNN_OK;
+}
+
+int check_sizes(const char *what, int64_t rows, int64_t classes, int64_t dims) {
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (rows < 0 || rows > TMNN_HEAD_MAX_ROWS) return bad("rows must be in [0, 2^24]");
+  if (classes < 1 || classes > TMNN_LOGITS_MAX_CLASSES) return bad("classes must be in [1, 2^24]");
+  if (dims < 1 || dims > TMNN_HEAD_MAX_DIMS) return bad("dims must be in [1, 2^16]");
+  if (rows * classes > int64_t{1} << 40) return bad("rows x classes must be at most 2^40");  // (tiles are counted in 32 bits)
+  return TMNN_OK;
+}
+
+constexpr int64_t kMostStride = int64_t{1} << 40;  // elements: addresses stay 64-bit numbers
+
+int check_loss(const tmnn_class_loss_args *a, bool back) {
+  const char *what = back ? "class_loss_backward" : "class_loss";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (!a) return bad("args is null");
+  if (a->struct_size != sizeof(*a)) return bad("struct_size mismatch");
+  if (a->dtype < TMNN_DTYPE_F32 || a->dtype > TMNN_DTYPE_BF16) return bad("invalid dtype");
+  if (a->index_dtype != TMNN_INDEX_I32 && a->index_dtype != TMNN_INDEX_I64) return bad("invalid index_dtype");
+  const int rc = check_sizes(what, a->rows, a->classes, a->dims);
+  if (rc != TMNN_OK) return rc;
+  // c = log2(e) / T stays an ordinary number
+  if (!(a->temperature >= 1e-6f && a->temperature <= 1e6f)) return bad("temperature must be in [1e-6, 1e6]");
+  if (a->feature_stride < a->dims || a->feature_stride > kMostStride || a->table_stride < a->dims ||
+      a->table_stride > kMostStride)
+    return bad("strides must be at least dims");
+  if (a->d_features && (a->d_feature_stride < a->dims || a->d_feature_stride > kMostStride))
+    return bad("d_feature_stride must be at least dims");
+  if (a->d_table && (a->d_table_stride < a->dims || a->d_table_stride > kMostStride))
+    return bad("d_table_stride must be at least dims");
+  return TMNN_OK;
+}
+
+int check_loss_arrays(const tmnn_class_loss_args *a, bool back, bool host) {
+  const char *what = back ? "class_loss_backward" : "class_loss";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  const int64_t size = static_cast<int64_t>(dtype_size(a->dtype));
+  if (back && !a->d_features && !a->d_table) return bad("nothing to compute");
+  if (!back && !a->loss && !a->stats && !a->d_features && !a->d_table) return bad("nothing to compute");
+  if (!a->table) return bad("table is null");
+  if (a->rows > 0) {
+    if (!a->features) return bad("features is null");
+    if (!a->labels) return bad("labels is null");
+    if (back && !a->stats) return bad("stats is null");
+    if (back && !a->row_weights) return bad("row_weights (the loss's gradient) is null");
+  }
+  for (const void *p : {a->features, a->table, static_cast<const void *>(a->d_features),
+                        static_cast<const void *>(a->d_table)})
+    if (!aligned(p, size)) return bad("features, table and gradients must be aligned to their type");
+  if (!aligned(a->labels, a->index_dtype == TMNN_INDEX_I64 ? 8 : 4))
+    return bad("labels must be aligned to their type");
+  if (!aligned(a->row_weights, 4) || !aligned(a->loss, 4)) return bad("arrays of 32-bit values must be 4-byte aligned");
+  if (!host && !aligned(a->stats, 16)) return bad("stats must be 16-byte aligned");
+  if (host && !aligned(a->stats, 4)) return bad("arrays of 32-bit values must be 4-byte aligned");
+  const int64_t n = a->rows, w = a->dims * size;
+  const Extent x{a->features, n, w, a->feature_stride * size, "features"};
+  const Extent y{a->table, a->classes, w, a->table_stride * size, "the table"};
+  const int64_t index = a->index_dtype == TMNN_INDEX_I64 ? 8 : 4;
+  const Extent l{a->labels, 1, n * index, 0, "labels"}, rw{a->row_weights, 1, n * 4, 0, "row_weights"};
+  const Extent s{a->stats, 1, n * 16, 0, "stats"}, lo{back ? nullptr : a->loss, 1, n * 4, 0, "loss"};
+  const Extent dx{a->d_features, n, w, a->d_feature_stride * size, "d_features"};
+  const Extent dy{a->d_table, a->classes, w, a->d_table_stride * size, "d_table"};
+  const Extent ws{host ? nullptr : a->workspace, 1, a->workspace_bytes, 0, "the workspace"};
+  if (back) return apart(what, {dx, dy, ws}, {x, y, l, rw, s});
+  return apart(what, {lo, s, dx, dy, ws}, {x, y, l, rw});
+}
+
+// ---- class loss ---------------------------------------------------------------------------
+
+// Bytes of the piece's d up to which more classes go into one piece: larger pieces mean fewer
+// launches and fewer passes over the sums of d_features.
+constexpr int64_t kPieceBytes = int64_t{256} << 20;
+
+// What a call lays out, in which tiles it goes, and where in the workspace things are.
+struct LossPlan {
+  bool grad, sums, f32, scaled;      // scaled: operands in fp16 terms
+  bool lay_x, lay_y, weighted;       // copies that are made
+  int planes, pairs;
+  int64_t ld;                        // elements of a laid-out row
+  int64_t steps;                     // of k = dims
+  int64_t piece, ld_d;               // classes of a piece; elements of a row of d
+  Tiles t_sums, t_d, t_x, t_y;       // logits for sums, for d; d_features, d_table
+  int64_t slab_ld;
+  bool slabs_x, slabs_y;
+  int64_t at_exps, at_most, at_x, at_w, at_y, at_sums, at_own, at_stats, at_d, at_slab_x, at_slab_y, bytes;
+};
+
+LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
+  LossPlan p{};
+  const int64_t n = a.rows, v = a.classes, size = static_cast<int64_t>(dtype_size(a.dtype));
+  p.grad = a.d_features || a.d_table;
+  p.sums = !back;
+  p.f32 = a.dtype == TMNN_DTYPE_F32;
+  p.planes = p.f32 ? 2 : 1;
+  p.pairs = p.f32 ? 3 : 1;
+  p.ld = up(a.dims, 64);
+  p.steps = p.ld / 64;
+  // operands that lie well are read in place
+  auto lies_well = [&](const void *ptr, int64_t stride, int64_t rows) {
+    return size == 2 && aligned(ptr, 16) && (stride % 8 == 0 || rows <= 1) && a.dims % 8 == 0 &&
+           stride * size < (1 << 23);
+  };
+  const bool x_well = lies_well(a.features, a.feature_stride, n), y_well = lies_well(a.table, a.table_stride, v);
+  p.scaled = p.f32 || p.grad;
+  const bool convert = p.f32 || (p.grad && a.dtype == TMNN_DTYPE_BF16);
+  p.lay_x = convert || !x_well;
+  p.lay_y = convert || !y_well;
+  p.weighted = a.d_table != nullptr;
+  int64_t at = 0;
+  auto room = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  p.at_exps = room(sizeof(Exponents));
+  p.at_most = room(3 * kScaleParts * 4);
+  const int64_t x_bytes = n * p.ld * 2 * p.planes;
+  if (p.lay_x) p.at_x = room(x_bytes);
+  if (p.weighted) p.at_w = room(x_bytes);
+  if (p.lay_y) p.at_y = room(v * p.ld * 2 * p.planes);
+  if (p.sums) {
+    p.t_sums = choose(n, v, p.steps * p.pairs, true, true, false);
+    p.at_sums = room(n * p.t_sums.c * 8);
+    p.at_own = room(n * 4);
+    if (p.grad && !a.stats) p.at_stats = room(n * 16);
+  }
+  if (p.grad) {
+    int64_t piece = kPieceBytes / (std::max<int64_t>(n, 1) * 2 * p.planes) / 256 * 256;
+    piece = std::max<int64_t>(piece, 256);
+    if (piece >= v)
+      piece = v;
+    else
+      piece = up(parts_of(v, parts_of(v, piece)), 256);
+    p.piece = piece;
+    p.ld_d = up(piece, 64);
+    p.t_d = choose(n, piece, p.steps * p.pairs, true, true, false);
+    p.at_d = room(n * p.ld_d * 2 * p.planes);
+    p.slab_ld = up(a.dims, 4);
+    if (a.d_features) {
+      p.t_x = choose(n, a.dims, p.ld_d / 64 * p.pairs, true, false, true);
+      p.slabs_x = p.t_x.parts > 1 || piece < v;
+      if (p.slabs_x) p.at_slab_x = room(n * p.slab_ld * 4 * p.t_x.parts);
+    }
+    if (a.d_table) {
+      p.t_y = choose(piece, a.dims, up(n, 64) / 64 * p.pairs, true, false, true);
+      p.slabs_y = p.t_y.parts > 1;
+      if (p.slabs_y) p.at_slab_y = room(piece * p.slab_ld * 4 * p.t_y.parts);
+    }
+  }
+  p.bytes = std::max<int64_t>(at, 256);
+  return p;
+}
+
+// The same tiles for fewer columns: a last piece may be shorter.
+Tiles of_piece(Tiles t, int64_t cols) {
+  t.c = static_cast<int32_t>(parts_of(cols, t.bc));
+  return t;
+}
+
+template <class T>
+int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, bool back, hipStream_t st) {
+  const int device = h->ctx->device;
+  const int64_t n = a.rows, v = a.classes, size = sizeof(T);
+  char *ws = static_cast<char *>(a.workspace);
+  RowInfo row{a.labels, a.row_weights, a.index_dtype == TMNN_INDEX_I64, static_cast<int32_t>(v)};
+  const float c = static_cast<float>(1.4426950408889634 / a.temperature);
+  const float inv_t = static_cast<float>(1.0 / a.temperature);
+  const Exponents *exps = nullptr;
+
+  if (p.lay_x || p.lay_y || p.weighted) {
+    LayArgs l{};
+    const bool keep = !p.f32 && a.dtype == TMNN_DTYPE_F16;  // fp16 products take fp16 operands as they are
+    const int planes = p.planes;
+    auto blocks = [&](int64_t rows) {
+      int lanes = 1;
+      while (lanes < 256 && lanes < p.ld / 8) lanes *= 2;
+      return static_cast<int32_t>(std::min<int64_t>(parts_of(std::max<int64_t>(rows, 1), 256 / lanes), 2048));
+    };
+    const int32_t dims = static_cast<int32_t>(a.dims), ld = static_cast<int32_t>(p.ld);
+    l.part[0] = {a.features, a.feature_stride, static_cast<int32_t>(n), dims, p.lay_x ? ws + p.at_x : nullptr,
+                 p.weighted ? ws + p.at_w : nullptr, ld, !keep || p.weighted, !keep, planes,
+                 p.lay_x || p.weighted ? blocks(n) : 0};
+    l.part[1] = {a.table, a.table_stride, static_cast<int32_t>(v), dims, p.lay_y ? ws + p.at_y : nullptr, nullptr,
+                 ld, !keep, !keep, planes, p.lay_y ? blocks(v) : 0};
+    l.row = row;
+    l.most = reinterpret_cast<uint32_t *>(ws + p.at_most);
+    l.most_w = reinterpret_cast<int32_t *>(ws + p.at_most) + 2 * kScaleParts;
+    l.exps = reinterpret_cast<Exponents *>(ws + p.at_exps);
+    if (p.scaled) exps = l.exps;
+    const dim3 grid(l.part[0].blocks + l.part[1].blocks);
+    if (p.scaled) {
+      hipLaunchKernelGGL((class_scale_kernel<T>), dim3(3 * kScaleParts), dim3(256), 0, st, l);
+      hipLaunchKernelGGL((class_lay_kernel<T, true>), grid, dim3(256), 0, st, l);
+    } else {
+      hipLaunchKernelGGL((class_lay_kernel<T, false>), grid, dim3(256), 0, st, l);
+    }
+    TMNN_HIP_TRY(hipGetLastError());
+  }
+
+  // operands: rows of dims values
+  const int64_t row_bytes = up(a.dims, 8) * 2;
+  auto laid = [&](int64_t at, int64_t rows) {
+    return Operand{ws + at, p.ld * 2, rows * p.ld * 2, static_cast<int32_t>(rows), static_cast<int32_t>(p.ld * 2)};
+  };
+  auto in_place = [&](const void *ptr, int64_t stride, int64_t rows) {
+    return Operand{static_cast<const char *>(ptr), stride * size, 0, static_cast<int32_t>(rows),
+                   static_cast<int32_t>(row_bytes)};
+  };
+  const Operand x = p.lay_x ? laid(p.at_x, n) : in_place(a.features, a.feature_stride, n);
+  const Operand y = p.lay_y ? laid(p.at_y, v) : in_place(a.table, a.table_stride, v);
+  float4 *stats = reinterpret_cast<float4 *>(a.stats ? reinterpret_cast<char *>(a.stats) : ws + p.at_stats);
+
+  if (p.sums) {
+    SumsEpilogue e{exps, row, c, reinterpret_cast<float2 *>(ws + p.at_sums),
+                   reinterpret_cast<float *>(ws + p.at_own)};
+    const TileArgs t = tile_args(x, y, n, v, p.t_sums, p.steps, p.pairs);
+    int rc;
+    if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16))
+      rc = p.scaled ? run_rows<F16>(t, p.t_sums.shape, e, device, st) : run_rows<BF16>(t, p.t_sums.shape, e, device, st);
+    else
+      rc = run_rows<F16>(t, p.t_sums.shape, e, device, st);
+    if (rc != TMNN_OK) return rc;
+    JoinArgs j{row, e.sums, e.own, static_cast<int32_t>(n), p.t_sums.c, 1, c, inv_t, a.loss,
+               a.stats || p.grad ? stats : nullptr};
+    while (j.lanes < 64 && j.lanes * 4 < j.tiles) j.lanes *= 2;
+    hipLaunchKernelGGL(class_join_kernel, dim3(static_cast<uint32_t>(parts_of(n, 256 / j.lanes))), dim3(256), 0, st, j);
+    TMNN_HIP_TRY(hipGetLastError());
+  }
+  if (!p.grad) return TMNN_OK;
+
+  const Operand w = laid(p.at_w, n);
+  auto *d = reinterpret_cast<_Float16 *>(ws + p.at_d);
+  const int64_t d_plane = n * p.ld_d;
+  const Operand dop{ws + p.at_d, p.ld_d * 2, d_plane * 2, static_cast<int32_t>(n), static_cast<int32_t>(p.ld_d * 2)};
+  const GradScale by_row{exps, row, inv_t, 1}, by_all{exps, row, inv_t, 0};
+  auto reduce = [&](const GradScale &s, void *out, int64_t ld, int64_t at, int parts, int64_t rows) {
+    ReduceArgs r{s, out, ld, reinterpret_cast<const float *>(ws + at), static_cast<int32_t>(p.slab_ld), parts,
+                 static_cast<int32_t>(rows), static_cast<int32_t>(a.dims)};
+    const int64_t blocks = std::min<int64_t>(parts_of(rows * p.slab_ld / 4, 256), 8 * kUnits);
+    hipLaunchKernelGGL((class_reduce_kernel<T>), dim3(static_cast<uint32_t>(std::max<int64_t>(blocks, 1))), dim3(256),
+                       0, st, r);
+  };
+  for (int64_t first = 0; first < v; first += p.piece) {
+    const int64_t count = std::min(p.piece, v - first);
+    Operand yp = y;
+    yp.base += first * y.ld;
+    yp.rows = static_cast<int32_t>(count);
+    GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.ld_d), p.planes, d_plane, d};
+    // (columns up to d's row length, so that those past the piece become 0)
+    TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.ld_d), p.steps, p.pairs);
+    int rc = run_rows<F16>(t, p.t_d.shape, g, device, st);
+    if (rc != TMNN_OK) return rc;
+    if (a.d_features) {
+      GradOut<T> o{by_row, static_cast<T *>(a.d_features), a.d_feature_stride,
+                   p.slabs_x ? reinterpret_cast<float *>(ws + p.at_slab_x) : nullptr, static_cast<int32_t>(p.slab_ld),
+                   first > 0};
+      t = tile_args(dop, yp, n, a.dims, p.t_x, p.ld_d / 64, p.pairs);
+      rc = p.t_x.shape == kLarge ? run_plain<Large<F16, false, true>>(t, o, device, st)
+                                 : run_plain<Middle<F16, false, true>>(t, o, device, st);
+      if (rc != TMNN_OK) return rc;
+    }
+    if (a.d_table) {
+      T *out = static_cast<T *>(a.d_table) + first * a.d_table_stride;
+      GradOut<T> o{by_all, out, a.d_table_stride, p.slabs_y ? reinterpret_cast<float *>(ws + p.at_slab_y) : nullptr,
+                   static_cast<int32_t>(p.slab_ld), 0};
+      Tiles ty = p.t_y;
+      ty.r = static_cast<int32_t>(parts_of(count, ty.br));
+      t = tile_args(dop, w, count, a.dims, ty, parts_of(n, 64), p.pairs);
+      rc = ty.shape == kLarge ? run_plain<Large<F16, true, true>>(t, o, device, st)
+                              : run_plain<Middle<F16, true, true>>(t, o, device, st);
+      if (rc != TMNN_OK) return rc;
+      if (p.slabs_y) reduce(by_all, out, a.d_table_stride, p.at_slab_y, ty.parts, count);
+    }
+  }
+  if (a.d_features && p.slabs_x) reduce(by_row, a.d_features, a.d_feature_stride, p.at_slab_x, p.t_x.parts, n);
+  TMNN_HIP_TRY(hipGetLastError());
+  return TMNN_OK;
+}
+
+// Without rows the table's gradient is 0.
+__global__ __launch_bounds__(256) void class_zero_kernel(char *out, int64_t stride, int64_t rows, int64_t width) {
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < rows * width;
+       at += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = at / width;
+    reinterpret_cast<int16_t *>(out + r * stride)[at - r * width] = 0;
+  }
+}
+
+int loss_device(tmnn_logits *h, const tmnn_class_loss_args &a, bool back, hipStream_t st) {
+  if (a.rows == 0) {
+    if (!a.d_table) return TMNN_OK;
+    const int64_t size = static_cast<int64_t>(dtype_size(a.dtype));
+    hipLaunchKernelGGL(class_zero_kernel, dim3(1024), dim3(256), 0, st, static_cast<char *>(a.d_table),
+                       a.d_table_stride * size, a.classes, a.dims * size / 2);
+    TMNN_HIP_TRY(hipGetLastError());
+    return TMNN_OK;
+  }
+  const LossPlan p = plan_loss(a, back);
+  const char *what = back ? "class_loss_backward" : "class_loss";
+  if (!a.workspace || !aligned(a.workspace, 256) || a.workspace_bytes < p.bytes)
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": the workspace must be 256-byte aligned and hold " +
+                                               std::to_string(p.bytes) + " bytes");
+  switch (a.dtype) {
+    case TMNN_DTYPE_F32: return run_loss<float>(h, a, p, back, st);
+    case TMNN_DTYPE_F16: return run_loss<_Float16>(h, a, p, back, st);
+    default: return run_loss<__bf16>(h, a, p, back, st);
+  }
+}
+
+int loss_host(tmnn_logits *h, tmnn_class_loss_args u, bool back) {
+  const size_t size = dtype_size(u.dtype), index = u.index_dtype == TMNN_INDEX_I64 ? 8 : 4, w = u.dims * size;
+  HostArrays m;
+  m.add(u.features, HostArrays::kIn, u.rows, w, u.feature_stride * size);
+  m.add(u.table, HostArrays::kIn, u.classes, w, u.table_stride * size);
+  m.add(u.labels, HostArrays::kIn, u.rows, index);
+  m.add(u.row_weights, HostArrays::kIn, u.rows, 4);
+  m.add(u.stats, back ? HostArrays::kIn : HostArrays::kOut, u.rows, 16);
+  if (back)
+    u.loss = nullptr;
+  else
+    m.add(u.loss, HostArrays::kOut, u.rows, 4);
+  m.add(u.d_features, HostArrays::kOut, u.rows, w, u.d_feature_stride * size);
+  m.add(u.d_table, HostArrays::kOut, u.classes, w, u.d_table_stride * size);
+  u.feature_stride = u.table_stride = u.d_feature_stride = u.d_table_stride = u.dims;
+  // (planned for the places that the arrays will have: aligned)
+  tmnn_class_loss_args on_device = u;
+  on_device.features = on_device.table = nullptr;
+  u.workspace_bytes = u.rows > 0 ? plan_loss(on_device, back).bytes : 256;
+  m.room(u.workspace, u.workspace_bytes);
+  return on_host(h, m, [&] { return loss_device(h, u, back, h->ctx->stream); });
+}
+
+int class_loss(tmnn_logits *h, const tmnn_class_loss_args *args, bool back, bool host, void *stream) {
+  return entry(h, [&] {
+    int rc = check_loss(args, back);
+    if (rc == TMNN_OK) rc = check_loss_arrays(args, back, host);
+    if (rc != TMNN_OK || (args->rows == 0 && !args->d_table)) return rc;
+    TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
+    return host ? loss_host(h, *args, back) : loss_device(h, *args, back, stream_of(h, stream));
+  });
+}
+
+// ---- logits from 8-bit operands ------------------------------------------------------------
+
+int check_logits(const tmnn_class_logits_f8_args *a) {
+  const char *what = "class_logits_f8";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (!a) return bad("args is null");
+  if (a->struct_size != sizeof(*a)) return bad("struct_size mismatch");
+  if (a->dtype < TMNN_DTYPE_F32 || a->dtype > TMNN_DTYPE_BF16) return bad("invalid dtype");
+  if (a->scale_dtype != TMNN_SCALE_F32 && a->scale_dtype != TMNN_SCALE_E8M0) return bad("invalid scale_dtype");
+  const int rc = check_sizes(what, a->rows, a->classes, a->dims);
+  if (rc != TMNN_OK) return rc;
+  if (a->feature_stride < a->dims || a->feature_stride > kMostStride || a->table_stride < a->dims ||
+      a->table_stride > kMostStride)
+    return bad("strides must be at least dims");
+  if (a->logit_stride < a->classes || a->logit_stride > kMostStride) return bad("logit_stride must be at least classes");
+  return TMNN_OK;
+}
+
+int check_logits_arrays(const tmnn_class_logits_f8_args *a, bool host) {
+  const char *what = "class_logits_f8";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (a->rows == 0) return TMNN_OK;
+  if (!a->features || !a->feature_scales || !a->table || !a->table_scales || !a->logits)
+    return bad("features, table, their scales and logits must not be null");
+  const int64_t size = static_cast<int64_t>(dtype_size(a->dtype)), n = a->rows, v = a->classes;
+  if (!aligned(a->logits, size)) return bad("logits must be aligned to their type");
+  const int64_t s = a->scale_dtype == TMNN_SCALE_F32 ? 4 : 1;
+  if (!aligned(a->feature_scales, s) || !aligned(a->table_scales, s)) return bad("scales must be aligned to their type");
+  const int64_t blocks = parts_of(a->dims, kScaleBlock);
+  return apart(what,
+               {{a->logits, n, v * size, a->logit_stride * size, "logits"},
+                {host ? nullptr : a->workspace, 1, a->workspace_bytes, 0, "the workspace"}},
+               {{a->features, n, a->dims, a->feature_stride, "features"},
+                {a->table, v, a->dims, a->table_stride, "the table"},
+                {a->feature_scales, 1, n * blocks * s, 0, "feature_scales"},
+                {a->table_scales, 1, parts_of(v, kScaleBlock) * blocks * s, 0, "table_scales"}});
+}
+
+struct LogitsPlan {
+  bool lay_x, lay_y;
+  int64_t ld, steps;
+  Tiles t;
+  int64_t slab_ld, at_x, at_y, at_slabs, bytes;
+};
+
+LogitsPlan plan_logits(const tmnn_class_logits_f8_args &a) {
+  LogitsPlan p{};
+  auto lies_well = [&](const void *ptr, int64_t stride, int64_t rows) {
+    return aligned(ptr, 16) && (stride % 16 == 0 || rows <= 1) && stride < (1 << 23);
+  };
+  p.lay_x = !lies_well(a.features, a.feature_stride, a.rows);
+  p.lay_y = !lies_well(a.table, a.table_stride, a.classes);
+  p.ld = up(a.dims, 16);
+  p.steps = parts_of(a.dims, kScaleBlock);
+  p.t = choose(a.rows, a.classes, p.steps, a.dtype != TMNN_DTYPE_F32, true, true);
+  p.slab_ld = up(a.classes, 4);
+  int64_t at = 0;
+  auto room = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  if (p.lay_x) p.at_x = room(a.rows * p.ld);
+  if (p.lay_y) p.at_y = room(a.classes * p.ld);
+  if (p.t.parts > 1) p.at_slabs = room(a.rows * p.slab_ld * 4 * p.t.parts);
+  p.bytes = std::max<int64_t>(at, 256);
+  return p;
+}
+
+template <class S, bool WIDE, class T>
+int run_f8(const TileArgs &t, const F8Scales &s, const LogitsOut<T> &o, bool power, int device, hipStream_t st) {
+  return power ? TileLaunch<S, F8Steps<S, true, WIDE>, LogitsOut<T>, F8Scales>::run(t, s, o, device, st)
+               : TileLaunch<S, F8Steps<S, false, WIDE>, LogitsOut<T>, F8Scales>::run(t, s, o, device, st);
+}
+
+template <class T>
+int run_logits(tmnn_logits *h, const tmnn_class_logits_f8_args &a, const LogitsPlan &p, hipStream_t st) {
+  const int device = h->ctx->device;
+  const int64_t n = a.rows, v = a.classes;
+  char *ws = static_cast<char *>(a.workspace);
+  if (p.lay_x || p.lay_y) {
+    F8LayArgs l{};
+    l.in[0] = static_cast<const uint8_t *>(a.features);
+    l.in[1] = static_cast<const uint8_t *>(a.table);
+    l.stride[0] = a.feature_stride;
+    l.stride[1] = a.table_stride;
+    l.rows[0] = static_cast<int32_t>(n);
+    l.rows[1] = static_cast<int32_t>(v);
+    l.dims = static_cast<int32_t>(a.dims);
+    l.ld = static_cast<int32_t>(p.ld);
+    l.out[0] = p.lay_x ? reinterpret_cast<uint8_t *>(ws + p.at_x) : nullptr;
+    l.out[1] = p.lay_y ? reinterpret_cast<uint8_t *>(ws + p.at_y) : nullptr;
+    hipLaunchKernelGGL(f8_lay_kernel, dim3(8 * kUnits), dim3(256), 0, st, l);
+    TMNN_HIP_TRY(hipGetLastError());
+  }
+  auto operand = [&](const void *ptr, int64_t stride, bool lay, int64_t at, int64_t rows) {
+    return Operand{lay ? ws + at : static_cast<const char *>(ptr), lay ? p.ld : stride, 0, static_cast<int32_t>(rows),
+                   static_cast<int32_t>(p.ld)};
+  };
+  const TileArgs t = tile_args(operand(a.features, a.feature_stride, p.lay_x, p.at_x, n),
+                               operand(a.table, a.table_stride, p.lay_y, p.at_y, v), n, v, p.t, p.steps, 1);
+  const F8Scales s{a.feature_scales, a.table_scales, static_cast<int32_t>(p.steps),
+                   static_cast<int32_t>(parts_of(v, kScaleBlock)),
+                   static_cast<int32_t>(a.dims - (p.steps - 1) * kScaleBlock)};
+  float *slabs = p.t.parts > 1 ? reinterpret_cast<float *>(ws + p.at_slabs) : nullptr;
+  const LogitsOut<T> o{static_cast<T *>(a.logits), a.logit_stride, slabs, static_cast<int32_t>(p.slab_ld)};
+  const bool power = a.scale_dtype == TMNN_SCALE_E8M0;
+  constexpr bool wide = sizeof(T) == 4;
+  int rc;
+  switch (p.t.shape) {
+    case kLarge:
+      if constexpr (!wide) {  // (fp32 logits are never planned so: 256 x 256 widened takes too many registers)
+        rc = run_f8<Large<F8, false, false>, false>(t, s, o, power, device, st);
+        break;
+      }
+    case kMiddle: rc = run_f8<Middle<F8, false, false>, wide>(t, s, o, power, device, st); break;
+    default: rc = run_f8<Small<F8, false, false>, true>(t, s, o, power, device, st); break;
+  }
+  if (rc != TMNN_OK || !slabs) return rc;
+  SumSlabsArgs j{slabs, a.logits, a.logit_stride, static_cast<int32_t>(p.slab_ld), p.t.parts, static_cast<int32_t>(n),
+                 static_cast<int32_t>(v)};
+  const int64_t blocks = std::min<int64_t>(parts_of(n * v, 256), 8 * kUnits);
+  hipLaunchKernelGGL((f8_join_kernel<T>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st, j);
+  TMNN_HIP_TRY(hipGetLastError());
+  return TMNN_OK;
+}
+
+int logits_device(tmnn_logits *h, const tmnn_class_logits_f8_args &a, hipStream_t st) {
+  const LogitsPlan p = plan_logits(a);
+  if (!a.workspace || !aligned(a.workspace, 256) || a.workspace_bytes < p.bytes)
+    return fail(TMNN_ERR_INVALID_ARGUMENT, "class_logits_f8: the workspace must be 256-byte aligned and hold " +
+                                               std::to_string(p.bytes) + " bytes");
+  switch (a.dtype) {
+    case TMNN_DTYPE_F32: return run_logits<float>(h, a, p, st);
+    case TMNN_DTYPE_F16: return run_logits<_Float16>(h, a, p, st);
+    default: return run_logits<__bf16>(h, a, p, st);
+  }
+}
+
+int logits_host(tmnn_logits *h, tmnn_class_logits_f8_args u) {
+  const size_t size = dtype_size(u.dtype), s = u.scale_dtype == TMNN_SCALE_F32 ? 4 : 1;
+  const int64_t blocks = parts_of(u.dims, kScaleBlock);
+  HostArrays m;
+  m.add(u.features, HostArrays::kIn, u.rows, u.dims, u.feature_stride);
+  m.add(u.table, HostArrays::kIn, u.classes, u.dims, u.table_stride);
+  m.add(u.feature_scales, HostArrays::kIn, u.rows, blocks * s);
+  m.add(u.table_scales, HostArrays::kIn, parts_of(u.classes, kScaleBlock), blocks * s);
+  m.add(u.logits, HostArrays::kOut, u.rows, u.classes * size, u.logit_stride * size);
+  u.feature_stride = u.table_stride = u.dims;
+  u.logit_stride = u.classes;
+  tmnn_class_logits_f8_args on_device = u;
+  on_device.features = on_device.table = nullptr;
+  u.workspace_bytes = plan_logits(on_device).bytes;
+  m.room(u.workspace, u.workspace_bytes);
+  return on_host(h, m, [&] { return logits_device(h, u, h->ctx->stream); });
+}
+
+int class_logits(tmnn_logits *h, const tmnn_class_logits_f8_args *args, bool host, void *stream) {
+  return entry(h, [&] {
+    int rc = check_logits(args);
+    if (rc == TMNN_OK) rc = check_logits_arrays(args, host);
+    if (rc != TMNN_OK || args->rows == 0) return rc;
+    TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
+    return host ? logits_host(h, *args) : logits_device(h, *args, stream_of(h, stream));
+  });
+}
+
+// ---- quantisation -----------------------------------------------------------------------------
+
+int check_quantize(const tmnn_quantize_f8_args *a) {
+  const char *what = "quantize_f8";
+  auto bad = [&](const char *m) {
+    return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
+  };
+  if (!a) return bad("args is null");
+  if (a->struct_size != sizeof(*a)) return bad("struct_size mismatch");
+  if (a->dtype < TMNN_DTYPE_F32 || a->dtype > TMNN_DTYPE_BF16) return bad("invalid dtype");
+  if (a->scale_dtype != TMNN_SCALE_F32 && a->scale_dtype != TMNN_SCALE_E8M0) return bad("invalid scale_dtype");
+  if (a->block_rows != 1 && a->block_rows != kScaleBlock) return bad("block_rows must be 1 or 128");
+  const int rc = check_sizes(what, a->rows, 1, a->dims);
+  if (rc != TMNN_OK) return rc;
+  if (a->stride < a->dims || a->stride > kMostStride || a->value_stride < a->dims || a->value_stride > kMostStride)
+    return bad("strides must be at least dims");
+  if (a->rows == 0) return TMNN_OK;
+  if (!a->input || !a->values || !a->scales) return bad("input, values and scales must not be null");
+  const int64_t size = static_cast<int64_t>(dtype_size(a->dtype)), s = a->scale_dtype == TMNN_SCALE_F32 ? 4 : 1;
+  if (!aligned(a->input, size) || !aligned(a->scales, s)) return bad("input and scales must be aligned to their type");
+  const int64_t blocks = parts_of(a->rows, a->block_rows) * parts_of(a->dims, kScaleBlock);
+  return apart(what,
+               {{a->values, a->rows, a->dims, a->value_stride, "values"}, {a->scales, 1, blocks * s, 0, "scales"}},
+               {{a->input, a->rows, a->dims * size, a->stride * size, "input"}});
+}
+
+template <class T, bool POWER>
+int run_quantize(const tmnn_quantize_f8_args &u, hipStream_t st) {
+  QuantizeArgs a{u.input, u.stride, static_cast<int32_t>(u.rows), static_cast<int32_t>(u.dims),
+                 static_cast<int32_t>(parts_of(u.dims, kScaleBlock)), static_cast<uint8_t *>(u.values), u.value_stride,
+                 u.scales};
+  if (u.block_rows == 1) {
+    const int64_t blocks = parts_of(u.rows * a.blocks, 16);
+    hipLaunchKernelGGL((f8_rows_kernel<T, POWER>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st, a);
+  } else {
+    const int64_t blocks = parts_of(u.rows, kScaleBlock) * a.blocks;
+    hipLaunchKernelGGL((f8_table_kernel<T, POWER>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st, a);
+  }
+  TMNN_HIP_TRY(hipGetLastError());
+  return TMNN_OK;
+}
+
+int quantize_device(const tmnn_quantize_f8_args &u, hipStream_t st) {
+  const bool power = u.scale_dtype == TMNN_SCALE_E8M0;
+  switch (u.dtype) {
+    case TMNN_DTYPE_F32: return power ? run_quantize<float, true>(u, st) : run_quantize<float, false>(u, st);
+    case TMNN_DTYPE_F16: return power ? run_quantize<_Float16, true>(u, st) : run_quantize<_Float16, false>(u, st);
+    default: return power ? run_quantize<__bf16, true>(u, st) : run_quantize<__bf16, false>(u, st);
+  }
+}
+
+int quantize_host(tmnn_logits *h, tmnn_quantize_f8_args u) {
+  const size_t size = dtype_size(u.dtype), s = u.scale_dtype == TMNN_SCALE_F32 ? 4 : 1;
+  HostArrays m;
+  m.add(u.input, HostArrays::kIn, u.rows, u.dims * size, u.stride * size);
+  m.add(u.values, HostArrays::kOut, u.rows, u.dims, u.value_stride);
+  m.add(u.scales, HostArrays::kOut, parts_of(u.rows, u.block_rows), parts_of(u.dims, kScaleBlock) * s);
+  u.stride = u.value_stride = u.dims;
+  return on_host(h, m, [&] { return quantize_device(u, h->ctx->stream); });
+}
+
+int quantize(tmnn_logits *h, const tmnn_quantize_f8_args *args, bool host, void *stream) {
+  return entry(h, [&] {
+    const int rc = check_quantize(args);
+    if (rc != TMNN_OK || args->rows == 0) return rc;
+    TMNN_HIP_TRY(hipSetDevice(h->ctx->device));
+    return host ? quantize_host(h, *args) : quantize_device(*args, stream_of(h, stream));
+  });
+}
+
+}  // namespace
+
+extern "C" {
+
+int tmnn_class_loss_workspace(const tmnn_class_loss_args *args, int32_t backward, int64_t *bytes) {
+  if (!bytes) return fail(TMNN_ERR_INVALID_ARGUMENT, "bytes is null");
+  *bytes = 0;
+  const int rc = check_loss(args, backward != 0);
+  if (rc != TMNN_OK) return rc;
+  *bytes = args->rows == 0 ? 256 : plan_loss(*args, backward != 0).bytes;
+  return TMNN_OK;
+}
+int tmnn_class_loss(tmnn_logits *h, const tmnn_class_loss_args *args) {
+  return class_loss(h, args, false, true, nullptr);
+}
+int tmnn_class_loss_device(tmnn_logits *h, const tmnn_class_loss_args *args, void *stream) {
+  return class_loss(h, args, false, false, stream);
+}
+int tmnn_class_loss_backward(tmnn_logits *h, const tmnn_class_loss_args *args) {
+  return class_loss(h, args, true, true, nullptr);
+}
+int tmnn_class_loss_backward_device(tmnn_logits *h, const tmnn_class_loss_args *args, void *stream) {
+  return class_loss(h, args, true, false, stream);
+}
+int tmnn_class_logits_f8_workspace(const tmnn_class_logits_f8_args *args, int64_t *bytes) {
+  if (!bytes) return fail(TMNN_ERR_INVALID_ARGUMENT, "bytes is null");
+  *bytes = 0;
+  const int rc = check_logits(args);
+  if (rc != TMNN_OK) return rc;
+  *bytes = args->rows == 0 ? 256 : plan_logits(*args).bytes;
+  return TMNN_OK;
+}
+int tmnn_class_logits_f8(tmnn_logits *h, const tmnn_class_logits_f8_args *args) {
+  return class_logits(h, args, true, nullptr);
+}
+int tmnn_class_logits_f8_device(tmnn_logits *h, const tmnn_class_logits_f8_args *args, void *stream) {
+  return class_logits(h, args, false, stream);
+}
+int tmnn_quantize_f8(tmnn_logits *h, const tmnn_quantize_f8_args *args) { return quantize(h, args, true, nullptr); }
+int tmnn_quantize_f8_device(tmnn_logits *h, const tmnn_quantize_f8_args *args, void *stream) {
+  return quantize(h, args, false, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,495 @@
+// class_loss_kernel.hpp -- softmax cross entropy of features against a table of
+// classes, without keeping the logits, and its gradients.
+//
+// Of a row h with label l, logits z_v = h . W_v, c = log2(e) / T, m = max z:
+//   R = sum_{v != l} 2^(c (z_v - m)),  e = 2^(c (z_l - m)),  S = R + e
+//   loss = w ln(S / e): ln(1 + R) where the label is the best class (exact for small losses)
+//   d_v = w / T (p_v - [v = l]),  p_v = 2^(c (z_v - m)) / S,  d_l = -w / T R / S
+// The label's term is kept out of the sums, so that neither a small loss nor 1 - p of a
+// confident row is a difference of two numbers near 1.
+//
+// The logits are a tile product (tile_product.hpp) whose epilogue sums a tile up to (max, sum) per
+// row; a second kernel joins the tiles of a row. The backward pass computes the logits again, for a
+// piece of the classes at a time, writes d of the piece in 16 bits, and multiplies it with the table
+// (d_features) and with the features (d_table).
+//
+// Numbers in 16 bits. Products take fp16 operands wherever a gradient is formed, also of
+// bf16 inputs: a bf16 matrix times the power of two that brings its largest magnitude to 2^14 is
+// exact in fp16 for elements down to 2^-32 of the largest, and d keeps 11 bits instead of 8 (with
+// d in bf16 its rounding would add as much error as that of the results). fp32 inputs become two
+// fp16 terms, 22 bits, and three products: 3e-7 of a result's size, at a fifth of the time that fp32
+// matrix instructions would take. d is held as 2^14 m d T / w, m in [1, 2) being w's mantissa: its
+// exponent goes to the other factor or to the result, exactly, so rows of any weight keep their bits.
+#pragma once
+
+#include "tile_product.hpp"
+
+namespace tmnn_hip {
+
+constexpr int kScaleParts = 256;   // blocks that look for one operand's largest magnitude
+constexpr int kDTerm = 14;         // d is held times 2^14
+
+// Powers of two that the operands of the logits and the weighted features were multiplied with, and
+// the largest weight's. Where nothing was (a null pointer), all are 0.
+struct Exponents {
+  int32_t x, y, w, weighted;
+};
+
+struct RowInfo {  // of the rows of a call
+  const void *labels;
+  const float *weights;  // nullable: 1
+  int32_t wide;          // labels of 64 bits
+  int32_t classes;
+  __device__ __forceinline__ int32_t label(int64_t r) const {  // -1: none; `classes`: out of range
+    if (wide) {
+      const int64_t l = static_cast<const int64_t *>(labels)[r];
+      return l < 0 ? -1 : l < classes ? static_cast<int32_t>(l) : classes;
+    }
+    const int32_t l = static_cast<const int32_t *>(labels)[r];
+    return l < 0 ? -1 : l < classes ? l : classes;
+  }
+  __device__ __forceinline__ float weight(int64_t r) const { return weights ? weights[r] : 1.f; }
+};
+
+// w = m 2^e with |m| in [1, 2); what is not finite keeps e = 0.
+__device__ __forceinline__ int weight_exponent(float w) {
+  return w == 0.f || !__builtin_isfinite(w) ? 0 : __builtin_amdgcn_frexp_expf(w) - 1;
+}
+
+__device__ __forceinline__ float exponent_factor(int e) {  // 2^e, held to normal numbers
+  return ldexpf(1.f, e < -126 ? -126 : e > 126 ? 126 : e);
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v) {
+  return static_cast<float>(v);
+}
+
+// ---- operands laid out --------------------------------------------------------------------
+
+struct LayPart {
+  const void *in;
+  int64_t stride;      // elements
+  int32_t rows, dims;
+  char *out;           // [plane][rows][ld], nullable
+  char *weighted;      // the same, rows times their weight's exponent (0 where there is none); nullable
+  int32_t ld;          // elements, a multiple of 64: columns from dims on are 0
+  int32_t seen;        // its largest magnitude is looked for
+  int32_t scaled;      // `out` is scaled by it (`weighted` always is)
+  int32_t planes;      // 1, or 2 (high, low)
+  int32_t blocks;
+};
+
+struct LayArgs {
+  LayPart part[2];     // features, table
+  RowInfo row;
+  uint32_t *most;      // [2][kScaleParts] largest finite magnitudes, as bits
+  int32_t *most_w;     // [kScaleParts] largest weight exponents
+  Exponents *exps;
+};
+
+// The largest finite magnitude of each operand, one per block, and of the weights.
+template <class T>
+__global__ __launch_bounds__(256) void class_scale_kernel(LayArgs a) {
+  __shared__ uint32_t top[256];
+  const int which = blockIdx.x / kScaleParts, block = blockIdx.x % kScaleParts;
+  uint32_t most = 0;
+  if (which < 2) {
+    const LayPart &p = a.part[which];
+    if (!p.seen) return;
+    // a wave a row at a time, 8 elements a lane
+    for (int64_t r = block * 4 + threadIdx.x / 64; r < p.rows; r += 4 * kScaleParts) {
+      const T *row = static_cast<const T *>(p.in) + r * p.stride;
+      for (int c = (threadIdx.x % 64) * 8; c < p.dims; c += 64 * 8) {
+        if (c + 8 <= p.dims) {
+          typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+          const V v = *reinterpret_cast<const V *>(row + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(v[i])) & 0x7fffffffu;
+            most = b < 0x7f800000u && b > most ? b : most;
+          }
+        } else {
+          for (int i = c; i < p.dims; ++i) {
+            const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(row[i])) & 0x7fffffffu;
+            most = b < 0x7f800000u && b > most ? b : most;
+          }
+        }
+      }
+    }
+  } else {
+    // (exponents shifted by 1000, 0 being none)
+    for (int64_t r = block * 256 + threadIdx.x; r < a.part[0].rows; r += 256 * kScaleParts) {
+      const float w = a.row.weight(r);
+      if (a.row.label(r) >= 0 && w != 0.f) most = max(most, static_cast<uint32_t>(weight_exponent(w) + 1000));
+    }
+  }
+  top[threadIdx.x] = most;
+  __syncthreads();
+  for (int s = 128; s > 0; s /= 2) {
+    if (threadIdx.x < s) top[threadIdx.x] = max(top[threadIdx.x], top[threadIdx.x + s]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    if (which < 2)
+      a.most[which * kScaleParts + block] = top[0];
+    else
+      a.most_w[block] = static_cast<int32_t>(top[0]) - 1000;
+  }
+}
+
+__device__ __forceinline__ int block_max_256(int v, int *room) {
+#pragma unroll
+  for (int s = 32; s > 0; s /= 2) v = max(v, __shfl_xor(v, s));
+  if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
+  __syncthreads();
+  v = max(max(room[0], room[1]), max(room[2], room[3]));
+  __syncthreads();
+  return v;
+}
+
+// The exponent that brings a magnitude (its bits) to [2^14, 2^15).
+__device__ __forceinline__ int scale_exponent(int bits) {
+  if (bits == 0) return 0;
+  const int e = 14 - (__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, bits)) - 1);
+  return e > 126 ? 126 : e;
+}
+
+// Lays both operands out: scaled, in fp16 terms (or copied as they are), rows at
+// multiples of 128 bytes.
+template <class T, bool SCALED>
+__global__ __launch_bounds__(256) void class_lay_kernel(LayArgs a) {
+  __shared__ int room[4];
+  const int which = blockIdx.x < static_cast<uint32_t>(a.part[0].blocks) ? 0 : 1;
+  const LayPart &p = a.part[which];
+  const int block = which ? blockIdx.x - a.part[0].blocks : blockIdx.x;
+  int e = 0, seen = 0, top_w = 0;
+  if constexpr (SCALED) {
+    int exps[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (a.part[k].seen)
+        exps[k] = scale_exponent(block_max_256(static_cast<int>(a.most[k * kScaleParts + threadIdx.x]), room));
+    top_w = block_max_256(a.most_w[threadIdx.x], room);
+    seen = exps[which];
+    e = p.scaled ? seen : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+      *a.exps = {a.part[0].scaled ? exps[0] : 0, a.part[1].scaled ? exps[1] : 0, top_w, exps[0]};
+  }
+  const int chunks = p.ld / 8;
+  int lanes = 1;
+  while (lanes < 256 && lanes < chunks) lanes *= 2;
+  const int per = 256 / lanes;
+  typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  const int64_t plane = static_cast<int64_t>(p.rows) * p.ld;
+  for (int64_t r = static_cast<int64_t>(block) * per + threadIdx.x / lanes; r < p.rows;
+       r += static_cast<int64_t>(p.blocks) * per) {
+    const T *row = static_cast<const T *>(p.in) + r * p.stride;
+    float factor = 0.f;
+    bool used = false;
+    if (SCALED && p.weighted) {
+      const float w = a.row.weight(r);
+      used = a.row.label(r) >= 0 && w != 0.f;
+      factor = used ? ldexpf(1.f, max(weight_exponent(w) - top_w, -149)) : 0.f;
+    }
+    for (int c = threadIdx.x % lanes; c < chunks; c += lanes) {
+      V v = {};
+      if (c * 8 + 8 <= p.dims) {
+        v = *reinterpret_cast<const V *>(row + c * 8);
+      } else {
+        for (int i = 0; i < 8; ++i)
+          if (c * 8 + i < p.dims) v[i] = row[c * 8 + i];
+      }
+      const int64_t at = r * p.ld + c * 8;
+      if constexpr (!SCALED) {
+        *reinterpret_cast<V *>(reinterpret_cast<T *>(p.out) + at) = v;
+      } else {
+        f16x8 high, low;
+        float f[8];
+        if (p.out) {
+          const float s = exponent_factor(e);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = to_f32(v[i]) * s;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            high[i] = static_cast<_Float16>(f[i]);
+            low[i] = static_cast<_Float16>(f[i] - static_cast<float>(high[i]));
+          }
+          *reinterpret_cast<f16x8 *>(reinterpret_cast<_Float16 *>(p.out) + at) = high;
+          if (p.planes == 2) *reinterpret_cast<f16x8 *>(reinterpret_cast<_Float16 *>(p.out) + plane + at) = low;
+        }
+        if (p.weighted) {
+          const float s = exponent_factor(seen);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float g = used ? to_f32(v[i]) * s * factor : 0.f;  // (a row without weight may hold anything)
+            high[i] = static_cast<_Float16>(g);
+            low[i] = static_cast<_Float16>(g - static_cast<float>(high[i]));
+          }
+          *reinterpret_cast<f16x8 *>(reinterpret_cast<_Float16 *>(p.weighted) + at) = high;
+          if (p.planes == 2)
+            *reinterpret_cast<f16x8 *>(reinterpret_cast<_Float16 *>(p.weighted) + plane + at) = low;
+        }
+      }
+    }
+  }
+}
+
+// ---- the logits' epilogues -----------------------------------------------------------------
+
+__device__ __forceinline__ float logit_scale(const Exponents *e) { return e ? exponent_factor(-(e->x + e->y)) : 1.f; }
+
+// A tile's rows as (max, sum) over the classes other than the label's, and the label's logit.
+struct SumsEpilogue {
+  const Exponents *exps;  // nullable: operands as they are
+  RowInfo row;
+  float c;
+  float2 *sums;           // [rows][tiles_c]
+  float *own;             // [rows] the label's logit
+
+  template <class S>
+  __device__ __forceinline__ void finish(const TileArgs &a, const TilePlace &p, f32x4t (&acc)[S::FC][S::FR],
+                                         int c0, int r0, int wc, int wr, int lane) const {
+    float2 *part = reinterpret_cast<float2 *>(tile_lds);  // [WC][BR]
+    const float inv = logit_scale(exps);
+    const int g4 = 4 * (lane / 16);
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) {
+      const int r = r0 + j * 16 + lane % 16;
+      const int label = r < a.rows ? row.label(r) : -1;
+      float m = -3.4e38f, s = 0.f;
+#pragma unroll
+      for (int i = 0; i < S::FC; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = c0 + i * 16 + g4 + e;
+          float z = acc[i][j][e] * inv;
+          if (col == label) own[r] = z;
+          z = col == label || col >= a.cols ? -__builtin_inff() : z;
+          acc[i][j][e] = z;
+          m = fmaxf(m, z);
+        }
+#pragma unroll
+      for (int i = 0; i < S::FC; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - m) * c);
+#pragma unroll
+      for (int x = 16; x < 64; x *= 2) {
+        const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);
+        const float top = fmaxf(m, mo);
+        s = s * __builtin_amdgcn_exp2f((m - top) * c) + so * __builtin_amdgcn_exp2f((mo - top) * c);
+        m = top;
+      }
+      if (lane < 16) part[wc * S::BR + wr * S::FR * 16 + j * 16 + lane] = float2{m, s};
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < S::BR; t += S::kThreads) {
+      const int r = p.r * S::BR + t;
+      if (r >= a.rows) continue;
+      float2 v = part[t];
+#pragma unroll
+      for (int w = 1; w < S::WC; ++w) {
+        const float2 o = part[w * S::BR + t];
+        const float top = fmaxf(v.x, o.x);
+        v.y = v.y * __builtin_amdgcn_exp2f((v.x - top) * c) + o.y * __builtin_amdgcn_exp2f((o.x - top) * c);
+        v.x = top;
+      }
+      sums[static_cast<int64_t>(r) * a.tiles_c + p.c] = v;
+    }
+  }
+};
+
+struct JoinArgs {
+  RowInfo row;
+  const float2 *sums;
+  const float *own;
+  int32_t rows, tiles, lanes;  // lanes of a row, a power of two
+  float c, inv_t;
+  float *loss;                 // nullable
+  float4 *stats;               // (m, S, R / S, 0)
+};
+
+__global__ __launch_bounds__(256) void class_join_kernel(JoinArgs a) {
+  const int lane = threadIdx.x % a.lanes;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / a.lanes) + threadIdx.x / a.lanes;
+  const bool here = r < a.rows;
+  const int label = here ? a.row.label(r) : -1;
+  float m = -3.4e38f, s = 0.f;
+  if (here)
+    for (int t = lane; t < a.tiles; t += a.lanes) {
+      const float2 v = a.sums[r * a.tiles + t];
+      const float top = fmaxf(m, v.x);
+      s = s * __builtin_amdgcn_exp2f((m - top) * a.c) + v.y * __builtin_amdgcn_exp2f((v.x - top) * a.c);
+      m = top;
+    }
+  for (int x = 1; x < a.lanes; x *= 2) {
+    const float mo = __shfl_xor(m, x), so = __shfl_xor(s, x);
+    const float top = fmaxf(m, mo);
+    s = s * __builtin_amdgcn_exp2f((m - top) * a.c) + so * __builtin_amdgcn_exp2f((mo - top) * a.c);
+    m = top;
+  }
+  if (!here || lane != 0) return;
+  float loss = 0.f, big = m, total = s, missing = 1.f;
+  if (label >= 0) {
+    const float z = label < a.row.classes ? a.own[r] : __builtin_nanf("");
+    big = fmaxf(m, z);
+    s *= __builtin_amdgcn_exp2f((m - big) * a.c);
+    total = s + __builtin_amdgcn_exp2f((z - big) * a.c);
+    missing = s / total;
+    loss = z >= m ? log1pf(s) : logf(total) + (m - z) * a.inv_t;
+    const float w = a.row.weight(r);
+    loss = w == 0.f ? 0.f : loss * w;
+  }
+  if (a.loss) a.loss[r] = loss;
+  if (a.stats) a.stats[r] = float4{big, total, missing, 0.f};
+}
+
+// The piece's d in fp16 terms, times 2^14, the weight's mantissa and T / w.
+struct GradEpilogue {
+  const Exponents *exps;
+  RowInfo row;
+  float c;
+  const float4 *stats;
+  int32_t first;       // class of the piece's first column
+  int32_t ld, planes;
+  int64_t plane;       // elements
+  _Float16 *d;         // [plane][rows][ld]
+
+  template <class S>
+  __device__ __forceinline__ void finish(const TileArgs &a, const TilePlace &, f32x4t (&acc)[S::FC][S::FR],
+                                         int c0, int r0, int, int, int lane) const {
+    const float inv = logit_scale(exps);
+    const int g4 = 4 * (lane / 16);
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) {
+      const int r = r0 + j * 16 + lane % 16;
+      if (r >= a.rows) continue;
+      const float w = row.weight(r);
+      const int label = row.label(r) - first;
+      const bool used = row.label(r) >= 0 && w != 0.f;
+      const float4 st = stats[r];
+      float f = __builtin_isfinite(w) ? __builtin_amdgcn_frexp_mantf(w) * (2.f * (1 << kDTerm)) : w;
+      if (row.label(r) == row.classes) f = __builtin_nanf("");
+      const float share = f / st.y, mine = -f * st.z;
+#pragma unroll
+      for (int i = 0; i < S::FC; ++i) {
+        const int col = c0 + i * 16 + g4;
+        if (col >= ld) continue;
+        f16x4 high, low;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = __builtin_amdgcn_exp2f((acc[i][j][e] * inv - st.x) * c) * share;
+          v = col + e == label ? mine : v;
+          v = used && col + e < a.cols ? v : 0.f;
+          high[e] = static_cast<_Float16>(v);
+          low[e] = static_cast<_Float16>(v - static_cast<float>(high[e]));
+        }
+        const int64_t at = static_cast<int64_t>(r) * ld + col;
+        *reinterpret_cast<f16x4 *>(d + at) = high;
+        if (planes == 2) *reinterpret_cast<f16x4 *>(d + plane + at) = low;
+      }
+    }
+  }
+};
+
+// ---- the gradients' epilogues ----------------------------------------------------------------
+
+// What a sum of products is multiplied with: 2^e / T, e of the row (d_features) or of all (d_table).
+struct GradScale {
+  const Exponents *exps;  // nullable
+  RowInfo row;
+  float inv_t;
+  int32_t by_row;
+  __device__ __forceinline__ float operator()(float v, int r, const Exponents &e, bool &none) const {
+    int k = -kDTerm;
+    none = false;
+    if (by_row) {
+      const float w = row.weight(r);
+      none = row.label(r) < 0 || w == 0.f;
+      k += weight_exponent(w) - e.y;
+    } else {
+      k += e.w - e.weighted;
+    }
+    return none ? 0.f : ldexpf(v * inv_t, k);
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void store_four(T *p, const float (&v)[4], int n) {
+  typedef T V __attribute__((ext_vector_type(4)));
+  typedef V VU __attribute__((aligned(sizeof(T))));
+  if (n >= 4) {
+    V o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = static_cast<T>(v[i]);
+    *reinterpret_cast<VU *>(p) = o;
+  } else {
+    for (int i = 0; i < n; ++i) p[i] = static_cast<T>(v[i]);
+  }
+}
+
+// The finished gradient, or, where it comes in parts, sums in fp32 that class_reduce_kernel ends.
+template <class T>
+struct GradOut {
+  GradScale scale;
+  T *out;          // [rows][cols]
+  int64_t ld;
+  float *slabs;    // [part][rows][slab_ld], nullable
+  int32_t slab_ld;
+  int32_t add;     // to what the slabs hold (pieces after the first)
+
+  template <class S>
+  __device__ __forceinline__ void finish(const TileArgs &a, const TilePlace &p, f32x4t (&acc)[S::FC][S::FR],
+                                         int c0, int r0, int, int, int lane) const {
+    const int g4 = 4 * (lane / 16);
+    Exponents e = {};
+    if (!slabs && scale.exps) e = *scale.exps;
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) {
+      const int r = r0 + j * 16 + lane % 16;
+      if (r >= a.rows) continue;
+#pragma unroll
+      for (int i = 0; i < S::FC; ++i) {
+        const int col = c0 + i * 16 + g4;
+        if (col >= a.cols) continue;
+        if (slabs) {
+          f32x4t *s = reinterpret_cast<f32x4t *>(slabs + (static_cast<int64_t>(p.part) * a.rows + r) * slab_ld + col);
+          *s = add ? *s + acc[i][j] : acc[i][j];
+        } else {
+          float v[4];
+          bool none;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = scale(acc[i][j][k], r, e, none);
+          store_four<T>(out + r * ld + col, v, a.cols - col);
+        }
+      }
+    }
+  }
+};
+
+struct ReduceArgs {
+  GradScale scale;
+  void *out;
+  int64_t ld;
+  const float *slabs;
+  int32_t slab_ld, parts, rows, cols;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void class_reduce_kernel(ReduceArgs a) {
+  const int64_t per = a.slab_ld / 4, n = per * a.rows;
+  const Exponents e = a.scale.exps ? *a.scale.exps : Exponents{};
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < n;
+       at += static_cast<int64_t>(gridDim.x) * 256) {
+    const int r = static_cast<int>(at / per), c = static_cast<int>(at - r * per) * 4;
+    const f32x4t *s = reinterpret_cast<const f32x4t *>(a.slabs + static_cast<int64_t>(r) * a.slab_ld + c);
+    f32x4t sum = *s;
+    for (int p = 1; p < a.parts; ++p) sum += s[p * n];
+    float v[4];
+    bool none;
+    for (int k = 0; k < 4; ++k) v[k] = a.scale(sum[k], r, e, none);
+    if (c < a.cols) store_four<T>(static_cast<T *>(a.out) + r * a.ld + c, v, a.cols - c);
+  }
+}
+
+}  // namespace tmnn_hip

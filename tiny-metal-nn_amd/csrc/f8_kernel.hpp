@@ -1,0 +1,396 @@
+// f8_kernel.hpp -- logits from features and a table of classes in e4m3 with a
+// scale for each 128 values of a row (features) and each 128 x 128 (table), and the
+// quantisation that makes both.
+//
+//   z[n][v] = sum_b sx[n][b] sw[v / 128][b] sum_{k in block b} x[n][k] w[v][k]
+//
+// A step of the tile product is 128 bytes of k, one block of scales. There are two ways to
+// multiply it, by the logits' type:
+//   16-bit logits: one 16 x 16 x 128 instruction on the 8-bit values themselves, at twice the rate of
+//     16-bit ones. It does not sum up in fp32 inside: measured against 64 bits it is off by up to 2^-11.3 of
+//     the largest of its products (1.3e-5 of a logit's size for normal values, 5e-5 for e4m3 bits drawn
+//     evenly), which is far below the rounding of a logit to 16 bits. Powers of two as scales go into
+//     the instruction; fp32 ones multiply its result, four fma an instruction.
+//   fp32 logits, and calls of few rows, which wait for memory anyway: values widened to fp16 (exact) and four
+//     16 x 16 x 32 instructions, whose products are exact and whose sums are fp32.
+#pragma once
+
+#include "tile_product.hpp"
+
+namespace tmnn_hip {
+
+constexpr int kScaleBlock = 128;
+constexpr float kF8Largest = 448.f;
+
+struct F8Scales {
+  const void *x;       // [rows][blocks]
+  const void *y;       // [col blocks][blocks]
+  int32_t blocks;      // of k
+  int32_t y_blocks;
+  int32_t tail;        // bytes of the last step that exist, a multiple of 16 or not
+};
+
+// e4m3 to fp16, exactly.
+__device__ __forceinline__ f16x8 widen(int32_t a, int32_t b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false),
+              q = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true),
+              r = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false),
+              s = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
+  return f16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+
+__device__ __forceinline__ float power_of(uint32_t byte) {  // of an e8m0 scale
+  byte &= 255;
+  return byte == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, byte ? byte << 23 : 1u << 22);
+}
+
+// POWER: e8m0 scales, else fp32. WIDE: values widened to fp16.
+template <class S, bool POWER, bool WIDE>
+struct F8Steps {
+  uint32_t at, last_at;        // of this lane's row's first scale, in bytes from the buffer's base
+  int32_t blocks, tail;
+  i32x4t rsrc;
+  const char *ybase;           // of this wave's classes
+  const char *place;           // the wave's scales in LDS, of stage 0
+  uint32_t x_low;              // misalignment of the e8m0 scales' base
+  float sy = 0.f;                    // of the step
+  uint32_t by = 0;
+
+  __device__ __forceinline__ F8Steps(const F8Scales &s, const TileArgs &a, int c0, int r0, int wave, int lane) {
+    blocks = s.blocks;
+    tail = s.tail;
+    constexpr int size = POWER ? 1 : 4;
+    const uintptr_t base = reinterpret_cast<uintptr_t>(s.x);
+    x_low = POWER ? static_cast<uint32_t>(base & 3) : 0;
+    // from the tile's first row on
+    const int row = lane < S::FR * 16 && r0 + lane < a.rows ? lane : -1;
+    const uintptr_t first = base - x_low;
+    const int64_t skip = static_cast<int64_t>(r0) * blocks * size;
+    const uintptr_t b = first + (POWER ? (skip + x_low) / 4 * 4 : skip);
+    x_low = POWER ? static_cast<uint32_t>((skip + x_low) & 3) : 0;
+    rsrc[0] = static_cast<int32_t>(b);
+    rsrc[1] = static_cast<int32_t>((b >> 32) & 0xffff);
+    rsrc[2] = 0x7fffffff;
+    rsrc[3] = 0x00020000;
+    at = row < 0 ? kOutside : row * blocks * size + x_low;
+    const int cb = min(c0 / kScaleBlock, s.y_blocks - 1);
+    ybase = static_cast<const char *>(s.y) + static_cast<int64_t>(cb) * blocks * size;
+    place = tile_lds + (S::BC + S::BR) * kStepBytes + wave * 256;
+  }
+  // The rows' scales of step k, on their way into LDS with the step's stage.
+  __device__ __forceinline__ void load(int k, bool exists, uint32_t to) const {
+    const uint32_t off = !exists || at == kOutside ? kOutside : POWER ? ((at + k) & ~3u) : at + k * 4;
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dword %1, %2, 0 offen lds"
+        :
+        : "s"(to), "v"(off), "s"(rsrc)
+        : "memory", "m0");
+  }
+  __device__ __forceinline__ void before(int k) {
+    if constexpr (POWER)
+      by = *reinterpret_cast<const __attribute__((address_space(4))) uint32_t *>(
+               reinterpret_cast<uintptr_t>(ybase + k) & ~static_cast<uintptr_t>(3)) >>
+           (8 * (reinterpret_cast<uintptr_t>(ybase + k) & 3));
+    else
+      sy = *reinterpret_cast<const __attribute__((address_space(4))) float *>(
+          reinterpret_cast<uintptr_t>(ybase + k * 4));
+  }
+  // Bytes of k that do not exist count as 0 (what lies there may be anything).
+  __device__ __forceinline__ void mask(i32x8t &v, int lane) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int have = tail - (h * 64 + lane / 16 * 16 + d * 4);
+        v[h * 4 + d] &= have >= 4 ? -1 : have <= 0 ? 0 : (1 << (8 * have)) - 1;
+      }
+  }
+  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, const char *x, int k, int wc,
+                                       int wr, int lane) {
+    i32x8t fx[S::FR];
+    f16x8 wx[WIDE ? S::FR : 1][4];
+    float sx[S::FR];
+    uint32_t bx[S::FR];
+    const bool cut = k == blocks - 1 && tail < kStepBytes;
+    const char *scales = place + (y - tile_lds);
+    auto whole = [&](const char *tile, int row) {
+      const i32x4t lo = read_row<i32x4t>(tile, row, 0, lane), hi = read_row<i32x4t>(tile, row, 4, lane);
+      i32x8t v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (cut) mask(v, lane);
+      return v;
+    };
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) {
+      fx[j] = whole(x, (wr * S::FR + j) * 16 + lane % 16);
+      if constexpr (WIDE)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) wx[j][q] = widen(fx[j][2 * q], fx[j][2 * q + 1]);
+      const uint32_t word = *reinterpret_cast<const uint32_t *>(scales + (j * 16 + lane % 16) * 4);
+      if constexpr (POWER)
+        bx[j] = word >> (8 * ((x_low + (j * 16 + lane % 16) * blocks + k) & 3));
+      if constexpr (POWER && WIDE)
+        sx[j] = power_of(bx[j]) * power_of(by);
+      else
+        sx[j] = __builtin_bit_cast(float, word) * sy;
+    }
+#pragma unroll
+    for (int i = 0; i < S::FC; ++i) {
+      const i32x8t fy = whole(y, (wc * S::FC + i) * 16 + lane % 16);
+      f16x8 wy[4];
+      if constexpr (WIDE)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) wy[q] = widen(fy[2 * q], fy[2 * q + 1]);
+#pragma unroll
+      for (int j = 0; j < S::FR; ++j) {
+        if constexpr (POWER && !WIDE) {
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fy, fx[j], acc[i][j], 0, 0, 0, by, 0, bx[j]);
+        } else {
+          f32x4t part{0.f, 0.f, 0.f, 0.f};
+          if constexpr (WIDE) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part = Fragment<F16>::mul(wy[q], wx[j][q], part);
+          } else {
+            part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fy, fx[j], part, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[e], sx[j], acc[i][j][e]);
+        }
+      }
+    }
+  }
+};
+
+template <class T>
+struct LogitsOut {
+  T *out;
+  int64_t ld;
+  float *slabs;     // [part][rows][slab_ld] where k is in parts
+  int32_t slab_ld;
+
+  template <class S>
+  __device__ __forceinline__ void finish(const TileArgs &a, const TilePlace &p, f32x4t (&acc)[S::FC][S::FR],
+                                         int c0, int r0, int, int, int lane) const {
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) {
+      const int r = r0 + j * 16 + lane % 16;
+      if (r >= a.rows) continue;
+#pragma unroll
+      for (int i = 0; i < S::FC; ++i) {
+        const int col = c0 + i * 16 + 4 * (lane / 16);
+        if (col >= a.cols) continue;
+        if (slabs) {
+          *reinterpret_cast<f32x4t *>(slabs + (static_cast<int64_t>(p.part) * a.rows + r) * slab_ld + col) = acc[i][j];
+          continue;
+        }
+        typedef T V __attribute__((ext_vector_type(4)));
+        typedef V VU __attribute__((aligned(sizeof(T))));
+        T *to = out + r * ld + col;
+        if (col + 4 <= a.cols) {
+          V v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(acc[i][j][e]);
+          *reinterpret_cast<VU *>(to) = v;
+        } else {
+          for (int e = 0; e < a.cols - col; ++e) to[e] = static_cast<T>(acc[i][j][e]);
+        }
+      }
+    }
+  }
+};
+
+struct SumSlabsArgs {
+  const float *slabs;
+  void *out;
+  int64_t ld;
+  int32_t slab_ld, parts, rows, cols;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void f8_join_kernel(SumSlabsArgs a) {
+  const int64_t n = static_cast<int64_t>(a.rows) * a.cols;
+  const int64_t part = static_cast<int64_t>(a.rows) * a.slab_ld;
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < n;
+       at += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t r = at / a.cols, c = at - r * a.cols;
+    const float *s = a.slabs + r * a.slab_ld + c;
+    float v = s[0];
+    for (int p = 1; p < a.parts; ++p) v += s[p * part];
+    static_cast<T *>(a.out)[r * a.ld + c] = static_cast<T>(v);
+  }
+}
+
+// Values whose rows do not start at multiples of 16 bytes, laid out so that they do.
+struct F8LayArgs {
+  const uint8_t *in[2];
+  int64_t stride[2];
+  int32_t rows[2], dims, ld;
+  uint8_t *out[2];
+};
+
+__global__ __launch_bounds__(256) void f8_lay_kernel(F8LayArgs a) {
+  const int64_t chunks = a.ld / 4;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    if (!a.out[w]) continue;
+    for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < chunks * a.rows[w];
+         at += static_cast<int64_t>(gridDim.x) * 256) {
+      const int64_t r = at / chunks, c = (at - r * chunks) * 4;
+      const uint8_t *from = a.in[w] + r * a.stride[w] + c;
+      uint32_t v = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < a.dims) v |= static_cast<uint32_t>(from[i]) << (8 * i);
+      *reinterpret_cast<uint32_t *>(a.out[w] + r * a.ld + c) = v;
+    }
+  }
+}
+
+// ---- quantisation ---------------------------------------------------------------------------
+
+// A block of scales is 128 values of one row, or 128 rows of them. 16 lanes hold 128 values of a
+// row, 8 each. What is not finite becomes NaN and takes no part in the scale; a block
+// without anything but zeros has scale 1.
+struct QuantizeArgs {
+  const void *in;
+  int64_t stride;
+  int32_t rows, dims, blocks;  // blocks of a row
+  uint8_t *out;
+  int64_t ld;
+  void *scales;                // [rows or rows / 128][blocks]
+};
+
+// The scale of a block, as a number, and how it is stored.
+template <bool POWER>
+__device__ __forceinline__ float f8_scale(float most) {
+  if (most == 0.f) return 1.f;
+  const float s = fmaxf(most / kF8Largest, 1.17549435e-38f);
+  if constexpr (!POWER) return s;
+  const uint32_t b = __builtin_bit_cast(uint32_t, s);
+  return __builtin_bit_cast(float, (b + 0x7fffffu) & 0x7f800000u);  // the power of two at or above it
+}
+
+// x / s rounded to the nearest e4m3 (ties to even) of the exact quotient: the fp32 quotient is
+// made odd where it is not exact, so that it never lies on a border that the exact one is beside.
+template <bool POWER>
+__device__ __forceinline__ float f8_quotient(float x, float s, float inv) {
+  if constexpr (POWER) return x * inv;  // (inv is exact)
+  float y = x * inv;
+  y = __builtin_fmaf(__builtin_fmaf(-y, s, x), inv, y);
+  const float left = __builtin_fmaf(-y, s, x);
+  const uint32_t b = __builtin_bit_cast(uint32_t, y);
+  if (left != 0.f && y != 0.f && !(b & 1)) {
+    const bool away = (__builtin_bit_cast(uint32_t, left) ^ b) >> 31 == 0;  // |x / s| > |y|
+    y = __builtin_bit_cast(float, away ? b + 1 : b - 1);
+  }
+  return y;
+}
+
+template <class T>
+__device__ __forceinline__ void f8_load8(const T *row, int c, int dims, float (&v)[8]) {
+  typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (c + 8 <= dims) {
+    const V x = *reinterpret_cast<const V *>(row + c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < dims ? static_cast<float>(row[c + i]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ float f8_most(const float (&v)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(v[i]);
+    m = a < __builtin_inff() && a > m ? a : m;
+  }
+  return m;
+}
+
+template <bool POWER>
+__device__ __forceinline__ void f8_store8(uint8_t *row, int c, int dims, const float (&v)[8], float s, float inv) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    y[i] = fabsf(v[i]) < __builtin_inff() ? f8_quotient<POWER>(v[i], s, inv) : __builtin_nanf("");
+  int32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    w[h] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w[h], true);
+  }
+  if (c + 8 <= dims) {
+    typedef int32_t V __attribute__((ext_vector_type(2), aligned(1)));
+    *reinterpret_cast<V *>(row + c) = V{w[0], w[1]};
+  } else {
+    for (int i = 0; i < 8; ++i)
+      if (c + i < dims) row[c + i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+template <bool POWER>
+__device__ __forceinline__ void f8_put_scale(void *scales, int64_t at, float s) {
+  if constexpr (POWER)
+    static_cast<uint8_t *>(scales)[at] = static_cast<uint8_t>(__builtin_bit_cast(uint32_t, s) >> 23);
+  else
+    static_cast<float *>(scales)[at] = s;
+}
+
+template <class T, bool POWER>
+__global__ __launch_bounds__(256) void f8_rows_kernel(QuantizeArgs a) {
+  const int64_t n = static_cast<int64_t>(a.rows) * a.blocks;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+  const int lane = threadIdx.x % 16;
+  if (at >= n) return;  // (16 lanes together)
+  const int64_t r = at / a.blocks;
+  const int b = static_cast<int>(at - r * a.blocks), c = b * kScaleBlock + lane * 8;
+  float v[8];
+  f8_load8(static_cast<const T *>(a.in) + r * a.stride, c, a.dims, v);
+  float m = f8_most(v);
+#pragma unroll
+  for (int x = 1; x < 16; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 16));
+  const float s = f8_scale<POWER>(m);
+  f8_store8<POWER>(a.out + r * a.ld, c, a.dims, v, s, 1.f / s);
+  if (lane == 0) f8_put_scale<POWER>(a.scales, at, s);
+}
+
+template <class T, bool POWER>
+__global__ __launch_bounds__(256) void f8_table_kernel(QuantizeArgs a) {
+  __shared__ float room[4];
+  const int64_t at = blockIdx.x;
+  const int rb = static_cast<int>(at / a.blocks), b = static_cast<int>(at - static_cast<int64_t>(rb) * a.blocks);
+  const int c = b * kScaleBlock + (threadIdx.x % 16) * 8;
+  const int64_t first = static_cast<int64_t>(rb) * kScaleBlock + threadIdx.x / 16;
+  float v[8][8];
+  float m = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int64_t r = first + k * 16;
+    if (r < a.rows) {
+      f8_load8(static_cast<const T *>(a.in) + r * a.stride, c, a.dims, v[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m = fmaxf(m, f8_most(v[k]));
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
+  if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(room[0], room[1]), fmaxf(room[2], room[3]));
+  const float s = f8_scale<POWER>(m), inv = 1.f / s;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int64_t r = first + k * 16;
+    if (r < a.rows) f8_store8<POWER>(a.out + r * a.ld, c, a.dims, v[k], s, inv);
+  }
+  if (threadIdx.x == 0) f8_put_scale<POWER>(a.scales, at, s);
+}
+
+}  // namespace tmnn_hip

@@ -232,6 +232,9 @@ DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
 INDEX_DTYPES = {"int32": 0, "int64": 1}
 TEACHER_KINDS = {"logits": 0, "logprobs": 1}
 LOGITS_MAX_CLASSES, LOGITS_MAX_TOP, LOGITS_MAX_TEACHER = 1 << 24, 128, 256
+# TMNN_SCALE_* and the limits of the class head
+SCALE_DTYPES = {"float32": 0, "float8_e8m0fnu": 1}
+HEAD_MAX_ROWS, HEAD_MAX_DIMS = 1 << 24, 1 << 16
 
 
 class TokenLogprobsArgs(ctypes.Structure):
@@ -251,6 +254,31 @@ class DistillArgs(ctypes.Structure):
         (k, ctypes.c_void_p) for k in (
             "logits", "teacher_ids", "teacher", "row_weights", "loss", "stats", "d_logits")] + [
         ("teacher_k", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
+class ClassLossArgs(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(k, ctypes.c_int32) for k in ("dtype", "index_dtype")] + [
+        ("temperature", ctypes.c_float)] + [(k, ctypes.c_int64) for k in (
+            "rows", "classes", "dims", "feature_stride", "table_stride", "d_feature_stride", "d_table_stride")] + [
+        (k, ctypes.c_void_p) for k in (
+            "features", "table", "labels", "row_weights", "loss", "stats", "d_features", "d_table", "workspace")] + [
+        ("workspace_bytes", ctypes.c_int64)]
+
+
+class ClassLogitsF8Args(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(k, ctypes.c_int32) for k in (
+        "dtype", "scale_dtype", "reserved")] + [(k, ctypes.c_int64) for k in (
+            "rows", "classes", "dims", "feature_stride", "table_stride", "logit_stride")] + [
+        (k, ctypes.c_void_p) for k in (
+            "features", "feature_scales", "table", "table_scales", "logits", "workspace")] + [
+        ("workspace_bytes", ctypes.c_int64)]
+
+
+class QuantizeF8Args(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(k, ctypes.c_int32) for k in (
+        "dtype", "scale_dtype", "block_rows")] + [(k, ctypes.c_int64) for k in (
+            "rows", "dims", "stride", "value_stride")] + [
+        (k, ctypes.c_void_p) for k in ("input", "values", "scales")]
 
 
 _V = ctypes.c_void_p
@@ -334,6 +362,16 @@ SIGNATURES = {
     "tmnn_distill_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
     "tmnn_distill_backward": (ctypes.c_int, [_V, ctypes.c_char_p]),
     "tmnn_distill_backward_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_class_loss_workspace": (ctypes.c_int, [ctypes.c_char_p, _I32, ctypes.POINTER(ctypes.c_int64)]),
+    "tmnn_class_loss": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_class_loss_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_class_loss_backward": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_class_loss_backward_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_class_logits_f8_workspace": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
+    "tmnn_class_logits_f8": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_class_logits_f8_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
+    "tmnn_quantize_f8": (ctypes.c_int, [_V, ctypes.c_char_p]),
+    "tmnn_quantize_f8_device": (ctypes.c_int, [_V, ctypes.c_char_p, _V]),
     "tmnn_debug_philox_uniform": (ctypes.c_int, [_V, ctypes.c_uint64, _U32, _U32, _F, _F, _V]),
 }
 

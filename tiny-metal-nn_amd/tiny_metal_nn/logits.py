@@ -24,6 +24,7 @@ import sys
 import numpy as np
 
 from . import _lib
+from .class_head import _HeadCalls
 from .trainer import ClosedError, DTypeError, _Context
 
 # tmnn_token_logprobs_args, tmnn_distill_args
@@ -104,6 +105,17 @@ class _Arrays:
     def writeable(self, x, name: str) -> None:
         pass
 
+    def dtype_name(self, dtype) -> str:
+        """A type's name, given as a type of the library's or by name."""
+        return dtype if isinstance(dtype, str) else self.name_of(dtype)
+
+    def float_type(self, dtype):
+        name = self.dtype_name(dtype)
+        for t in self.float_codes:
+            if self.name_of(t) == name:
+                return t
+        raise DTypeError(f"dtype must be float32, float16 or bfloat16, got {name}")
+
     def wrote(self, arrays: list) -> None:
         """After a call: what it has written to."""
 
@@ -115,6 +127,14 @@ class _HostArrays(_Arrays):
         super().__init__(np, "a numpy array")
         self.float_codes = {np.dtype(k): c for k, c in _lib.DTYPES.items() if k != "bfloat16"}
         self.index_codes = {np.dtype(k): c for k, c in _lib.INDEX_DTYPES.items()}
+        # numpy has no 8-bit floating point: its bytes
+        self.f8 = self.e8m0 = np.uint8
+        self.f8_codes = {np.dtype(np.uint8): 0}
+        self.scale_codes = {np.dtype(np.float32): 0, np.dtype(np.uint8): 1}
+        self.scale_names = "float32 or uint8"
+
+    def dtype_name(self, dtype) -> str:
+        return dtype if isinstance(dtype, str) else np.dtype(dtype).name
 
     @staticmethod
     def ours(x) -> bool:
@@ -148,6 +168,10 @@ class _DeviceArrays(_Arrays):
         self.torch, self.device = torch, device
         self.float_codes = {getattr(torch, k): c for k, c in _lib.DTYPES.items()}
         self.index_codes = {getattr(torch, k): c for k, c in _lib.INDEX_DTYPES.items()}
+        self.f8, self.e8m0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+        self.f8_codes = {self.f8: 0}
+        self.scale_codes = {getattr(torch, k): c for k, c in _lib.SCALE_DTYPES.items()}
+        self.scale_names = " or ".join(_lib.SCALE_DTYPES)
         self.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda d: torch.cuda.current_stream(d).cuda_stream)
         self.side = None  # the stream that new arrays belong to, if not the current one
@@ -209,8 +233,9 @@ class _DeviceArrays(_Arrays):
             return self.torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
 
 
-class LogitOps:
-    """Operators over rows of class logits on one device.
+class LogitOps(_HeadCalls):
+    """Operators over rows of class logits, and over features and a table of classes
+    (class_head.py), on one device.
 
     Holds the workspace of its calls: calls through one object are ordered where
     they share it, also across streams. Use one object per thread, and one of its
