@@ -23,24 +23,24 @@ int64_t parts_of(int64_t n, int64_t of) { return (n + of - 1) / of; }
 // ---- tiles --------------------------------------------------------------------------
 
 enum Shape { kLarge, kMiddle, kSmall };
-// waves, blocks of a wave, stages
+// waves, blocks of a wave, bytes of a step, stages
 template <class E, bool XT, bool YT>
-using Large = TileShape<E, 2, 4, 8, 4, 2, XT, YT>;
+using Large = TileShape<E, 2, 4, 8, 4, 128, 2, XT, YT>;
 template <class E, bool XT, bool YT>
-using Middle = TileShape<E, 2, 2, 4, 4, 2, XT, YT>;
+using Middle = TileShape<E, 2, 2, 4, 4, 128, 2, XT, YT>;
 template <class E, bool XT, bool YT>
-using Small = TileShape<E, 4, 1, 2, 2, 4, XT, YT>;
+using Small = TileShape<E, 4, 1, 2, 2, 128, 4, XT, YT>;
 
 struct Tiles {
   Shape shape;
-  int32_t bc, br, r, c, parts, part_steps;
+  int32_t bc, br, r, c, parts, steps, part_steps;  // steps: of one pair of planes
 };
 
 constexpr int kUnits = 256;  // compute units
 
 // The shape whose tiles take the least time together, and parts of k where there are too few
 // of them to keep every unit busy.
-Tiles choose(int64_t rows, int64_t cols, int64_t steps, bool large, bool small, bool split) {
+Tiles choose(int64_t rows, int64_t cols, int64_t k_bytes, int pairs, bool f8, bool large, bool small, bool split) {
   Tiles best{};
   double least = 1e300;
   for (const Shape s : {kLarge, kMiddle, kSmall}) {
@@ -51,18 +51,21 @@ Tiles choose(int64_t rows, int64_t cols, int64_t steps, bool large, bool small, 
     t.br = s == kLarge ? 256 : s == kMiddle ? 128 : 32;
     t.r = static_cast<int32_t>(parts_of(rows, t.br));
     t.c = static_cast<int32_t>(parts_of(cols, t.bc));
+    const int64_t kb = 128;
+    t.steps = static_cast<int32_t>(parts_of(k_bytes, kb));
+    const int64_t steps = static_cast<int64_t>(t.steps) * pairs;
     t.parts = 1;
     const int64_t tiles = static_cast<int64_t>(t.r) * t.c;
     if (split) {
       const int64_t want = (s == kLarge ? 1 : 2) * kUnits;
-      int64_t p = std::max<int64_t>(1, std::min<int64_t>(want / tiles, steps / 8));
+      int64_t p = std::max<int64_t>(1, std::min<int64_t>(want / tiles, steps * kb / 1024));
       t.parts = static_cast<int32_t>(std::min<int64_t>(p, 64));
     }
     t.part_steps = static_cast<int32_t>(parts_of(steps, t.parts));
     t.parts = static_cast<int32_t>(parts_of(steps, t.part_steps));
     const double rate = s == kLarge ? 1.0 : s == kMiddle ? 0.75 : 0.3;
     const double time = static_cast<double>(parts_of(tiles * t.parts, kUnits)) * t.bc * t.br *
-                        (t.part_steps + 4) / rate;
+                        (t.part_steps * kb + 512) / rate;
     if (time < least) {
       least = time;
       best = t;
@@ -70,7 +73,6 @@ Tiles choose(int64_t rows, int64_t cols, int64_t steps, bool large, bool small, 
   }
   return best;
 }
-
 
 template <class S, class Steps, class Epi, class StepArgs>
 struct TileLaunch {
@@ -91,7 +93,7 @@ struct TileLaunch {
 };
 
 TileArgs tile_args(const Operand &x, const Operand &y, int64_t rows, int64_t cols, const Tiles &t,
-                   int64_t steps, int pairs) {
+                   int pairs) {
   TileArgs a{};
   a.x = x;
   a.y = y;
@@ -100,7 +102,7 @@ TileArgs tile_args(const Operand &x, const Operand &y, int64_t rows, int64_t col
   a.tiles_r = t.r;
   a.tiles_c = t.c;
   a.parts = t.parts;
-  a.steps = static_cast<int32_t>(steps);
+  a.steps = t.steps;
   a.pairs = pairs;
   a.part_steps = t.part_steps;
   return a;
@@ -245,7 +247,6 @@ struct LossPlan {
   bool lay_x, lay_y, weighted;       // copies that are made
   int planes, pairs;
   int64_t ld;                        // elements of a laid-out row
-  int64_t steps;                     // of k = dims
   int64_t piece, ld_d;               // classes of a piece; elements of a row of d
   Tiles t_sums, t_d, t_x, t_y;       // logits for sums, for d; d_features, d_table
   int64_t slab_ld;
@@ -262,7 +263,6 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   p.planes = p.f32 ? 2 : 1;
   p.pairs = p.f32 ? 3 : 1;
   p.ld = up(a.dims, 64);
-  p.steps = p.ld / 64;
   // operands that lie well are read in place
   auto lies_well = [&](const void *ptr, int64_t stride, int64_t rows) {
     return size == 2 && aligned(ptr, 16) && (stride % 8 == 0 || rows <= 1) && a.dims % 8 == 0 &&
@@ -287,7 +287,7 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   if (p.weighted) p.at_w = room(x_bytes);
   if (p.lay_y) p.at_y = room(v * p.ld * 2 * p.planes);
   if (p.sums) {
-    p.t_sums = choose(n, v, p.steps * p.pairs, true, true, false);
+    p.t_sums = choose(n, v, p.ld * 2, p.pairs, false, true, true, false);
     p.at_sums = room(n * p.t_sums.c * 8);
     p.at_own = room(n * 4);
     if (p.grad && !a.stats) p.at_stats = room(n * 16);
@@ -301,16 +301,16 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
       piece = up(parts_of(v, parts_of(v, piece)), 256);
     p.piece = piece;
     p.ld_d = up(piece, 64);
-    p.t_d = choose(n, piece, p.steps * p.pairs, true, true, false);
+    p.t_d = choose(n, piece, p.ld * 2, p.pairs, false, true, true, false);
     p.at_d = room(n * p.ld_d * 2 * p.planes);
     p.slab_ld = up(a.dims, 4);
     if (a.d_features) {
-      p.t_x = choose(n, a.dims, p.ld_d / 64 * p.pairs, true, false, true);
+      p.t_x = choose(n, a.dims, p.ld_d * 2, p.pairs, false, true, false, true);
       p.slabs_x = p.t_x.parts > 1 || piece < v;
       if (p.slabs_x) p.at_slab_x = room(n * p.slab_ld * 4 * p.t_x.parts);
     }
     if (a.d_table) {
-      p.t_y = choose(piece, a.dims, up(n, 64) / 64 * p.pairs, true, false, true);
+      p.t_y = choose(piece, a.dims, n * 2, p.pairs, false, true, false, true);
       p.slabs_y = p.t_y.parts > 1;
       if (p.slabs_y) p.at_slab_y = room(piece * p.slab_ld * 4 * p.t_y.parts);
     }
@@ -344,20 +344,25 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
       while (lanes < 256 && lanes < p.ld / 8) lanes *= 2;
       return static_cast<int32_t>(std::min<int64_t>(parts_of(std::max<int64_t>(rows, 1), 256 / lanes), 2048));
     };
+    // (16 rows of a wave's vectors a block: four loads each on their way, four times)
+    auto scale_parts = [&](int64_t rows) {
+      return static_cast<int32_t>(std::min<int64_t>(parts_of(rows * parts_of(a.dims, 8), 16 * 256), kScaleParts));
+    };
     const int32_t dims = static_cast<int32_t>(a.dims), ld = static_cast<int32_t>(p.ld);
     l.part[0] = {a.features, a.feature_stride, static_cast<int32_t>(n), dims, p.lay_x ? ws + p.at_x : nullptr,
-                 p.weighted ? ws + p.at_w : nullptr, ld, !keep || p.weighted, !keep, planes,
-                 p.lay_x || p.weighted ? blocks(n) : 0};
+                 p.weighted ? ws + p.at_w : nullptr, ld, !keep, planes,
+                 p.lay_x || p.weighted ? blocks(n) : 0, !keep || p.weighted ? scale_parts(n) : 0};
     l.part[1] = {a.table, a.table_stride, static_cast<int32_t>(v), dims, p.lay_y ? ws + p.at_y : nullptr, nullptr,
-                 ld, !keep, !keep, planes, p.lay_y ? blocks(v) : 0};
+                 ld, !keep, planes, p.lay_y ? blocks(v) : 0, !keep ? scale_parts(v) : 0};
     l.row = row;
     l.most = reinterpret_cast<uint32_t *>(ws + p.at_most);
     l.most_w = reinterpret_cast<int32_t *>(ws + p.at_most) + 2 * kScaleParts;
+    l.parts_w = static_cast<int32_t>(std::min<int64_t>(parts_of(n, 256), kScaleParts));
     l.exps = reinterpret_cast<Exponents *>(ws + p.at_exps);
     if (p.scaled) exps = l.exps;
     const dim3 grid(l.part[0].blocks + l.part[1].blocks);
     if (p.scaled) {
-      hipLaunchKernelGGL((class_scale_kernel<T>), dim3(3 * kScaleParts), dim3(256), 0, st, l);
+      hipLaunchKernelGGL((class_scale_kernel<T>), dim3(l.part[0].parts + l.part[1].parts + l.parts_w), dim3(256), 0, st, l);
       hipLaunchKernelGGL((class_lay_kernel<T, true>), grid, dim3(256), 0, st, l);
     } else {
       hipLaunchKernelGGL((class_lay_kernel<T, false>), grid, dim3(256), 0, st, l);
@@ -381,7 +386,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
   if (p.sums) {
     SumsEpilogue e{exps, row, c, reinterpret_cast<float2 *>(ws + p.at_sums),
                    reinterpret_cast<float *>(ws + p.at_own)};
-    const TileArgs t = tile_args(x, y, n, v, p.t_sums, p.steps, p.pairs);
+    const TileArgs t = tile_args(x, y, n, v, p.t_sums, p.pairs);
     int rc;
     if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16))
       rc = p.scaled ? run_rows<F16>(t, p.t_sums.shape, e, device, st) : run_rows<BF16>(t, p.t_sums.shape, e, device, st);
@@ -415,14 +420,14 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
     yp.rows = static_cast<int32_t>(count);
     GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.ld_d), p.planes, d_plane, d};
     // (columns up to d's row length, so that those past the piece become 0)
-    TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.ld_d), p.steps, p.pairs);
+    TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.ld_d), p.pairs);
     int rc = run_rows<F16>(t, p.t_d.shape, g, device, st);
     if (rc != TMNN_OK) return rc;
     if (a.d_features) {
       GradOut<T> o{by_row, static_cast<T *>(a.d_features), a.d_feature_stride,
                    p.slabs_x ? reinterpret_cast<float *>(ws + p.at_slab_x) : nullptr, static_cast<int32_t>(p.slab_ld),
                    first > 0};
-      t = tile_args(dop, yp, n, a.dims, p.t_x, p.ld_d / 64, p.pairs);
+      t = tile_args(dop, yp, n, a.dims, p.t_x, p.pairs);
       rc = p.t_x.shape == kLarge ? run_plain<Large<F16, false, true>>(t, o, device, st)
                                  : run_plain<Middle<F16, false, true>>(t, o, device, st);
       if (rc != TMNN_OK) return rc;
@@ -433,7 +438,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
                    static_cast<int32_t>(p.slab_ld), 0};
       Tiles ty = p.t_y;
       ty.r = static_cast<int32_t>(parts_of(count, ty.br));
-      t = tile_args(dop, w, count, a.dims, ty, parts_of(n, 64), p.pairs);
+      t = tile_args(dop, w, count, a.dims, ty, p.pairs);
       rc = ty.shape == kLarge ? run_plain<Large<F16, true, true>>(t, o, device, st)
                               : run_plain<Middle<F16, true, true>>(t, o, device, st);
       if (rc != TMNN_OK) return rc;
@@ -566,7 +571,7 @@ LogitsPlan plan_logits(const tmnn_class_logits_f8_args &a) {
   p.lay_y = !lies_well(a.table, a.table_stride, a.classes);
   p.ld = up(a.dims, 16);
   p.steps = parts_of(a.dims, kScaleBlock);
-  p.t = choose(a.rows, a.classes, p.steps, a.dtype != TMNN_DTYPE_F32, true, true);
+  p.t = choose(a.rows, a.classes, a.dims, 1, true, a.dtype != TMNN_DTYPE_F32, true, true);
   p.slab_ld = up(a.classes, 4);
   int64_t at = 0;
   auto room = [&](int64_t bytes) {
@@ -612,7 +617,7 @@ int run_logits(tmnn_logits *h, const tmnn_class_logits_f8_args &a, const LogitsP
                    static_cast<int32_t>(p.ld)};
   };
   const TileArgs t = tile_args(operand(a.features, a.feature_stride, p.lay_x, p.at_x, n),
-                               operand(a.table, a.table_stride, p.lay_y, p.at_y, v), n, v, p.t, p.steps, 1);
+                               operand(a.table, a.table_stride, p.lay_y, p.at_y, v), n, v, p.t, 1);
   const F8Scales s{a.feature_scales, a.table_scales, static_cast<int32_t>(p.steps),
                    static_cast<int32_t>(parts_of(v, kScaleBlock)),
                    static_cast<int32_t>(a.dims - (p.steps - 1) * kScaleBlock)};

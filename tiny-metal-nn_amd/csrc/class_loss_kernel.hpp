@@ -26,7 +26,7 @@
 
 namespace tmnn_hip {
 
-constexpr int kScaleParts = 256;   // blocks that look for one operand's largest magnitude
+constexpr int kScaleParts = 1024;  // most blocks that look for one operand's largest magnitude
 constexpr int kDTerm = 14;         // d is held times 2^14
 
 // Powers of two that the operands of the logits and the weighted features were multiplied with, and
@@ -74,67 +74,87 @@ struct LayPart {
   char *out;           // [plane][rows][ld], nullable
   char *weighted;      // the same, rows times their weight's exponent (0 where there is none); nullable
   int32_t ld;          // elements, a multiple of 64: columns from dims on are 0
-  int32_t seen;        // its largest magnitude is looked for
-  int32_t scaled;      // `out` is scaled by it (`weighted` always is)
+  int32_t scaled;      // `out` is scaled by its largest magnitude (`weighted` always is)
   int32_t planes;      // 1, or 2 (high, low)
-  int32_t blocks;
+  int32_t blocks;      // that lay it out
+  int32_t parts;       // blocks that look for its largest magnitude, up to kScaleParts
 };
 
 struct LayArgs {
   LayPart part[2];     // features, table
   RowInfo row;
   uint32_t *most;      // [2][kScaleParts] largest finite magnitudes, as bits
-  int32_t *most_w;     // [kScaleParts] largest weight exponents
+  int32_t *most_w;     // [parts_w] largest weight exponents
+  int32_t parts_w;
   Exponents *exps;
 };
+
+// Threads that take a row of 8-element vectors together, so that short rows go several to a block.
+__device__ __forceinline__ int row_lanes(int chunks) {
+  int lanes = 1;
+  while (lanes < 256 && lanes < chunks) lanes *= 2;
+  return lanes;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t magnitude(T v) {  // its bits, 0 for what is not finite
+  const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(v)) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0;
+}
 
 // The largest finite magnitude of each operand, one per block, and of the weights.
 template <class T>
 __global__ __launch_bounds__(256) void class_scale_kernel(LayArgs a) {
-  __shared__ uint32_t top[256];
-  const int which = blockIdx.x / kScaleParts, block = blockIdx.x % kScaleParts;
+  __shared__ uint32_t top[4];
+  const int parts_x = a.part[0].parts, parts_y = a.part[1].parts;
+  const int which = static_cast<int>(blockIdx.x) < parts_x ? 0 : static_cast<int>(blockIdx.x) < parts_x + parts_y ? 1 : 2;
+  const int block = blockIdx.x - (which > 0 ? parts_x : 0) - (which > 1 ? parts_y : 0);
   uint32_t most = 0;
   if (which < 2) {
     const LayPart &p = a.part[which];
-    if (!p.seen) return;
-    // a wave a row at a time, 8 elements a lane
-    for (int64_t r = block * 4 + threadIdx.x / 64; r < p.rows; r += 4 * kScaleParts) {
-      const T *row = static_cast<const T *>(p.in) + r * p.stride;
-      for (int c = (threadIdx.x % 64) * 8; c < p.dims; c += 64 * 8) {
-        if (c + 8 <= p.dims) {
-          typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-          const V v = *reinterpret_cast<const V *>(row + c);
+    typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    const int chunks = (p.dims + 7) / 8, lanes = row_lanes(chunks), per = 256 / lanes;
+    const int64_t step = static_cast<int64_t>(p.parts) * per;
+    for (int c = threadIdx.x % lanes; c < chunks; c += lanes) {
+      const T *at = static_cast<const T *>(p.in) + c * 8;
+      int64_t r = static_cast<int64_t>(block) * per + threadIdx.x / lanes;
+      if (c * 8 + 8 <= p.dims) {
+        for (; r + 3 * step < p.rows; r += 4 * step) {  // four loads on their way
+          V v[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(v[i])) & 0x7fffffffu;
-            most = b < 0x7f800000u && b > most ? b : most;
-          }
-        } else {
-          for (int i = c; i < p.dims; ++i) {
-            const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(row[i])) & 0x7fffffffu;
-            most = b < 0x7f800000u && b > most ? b : most;
-          }
+          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const V *>(at + (r + u * step) * p.stride);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[u][i]));
         }
+        for (; r < p.rows; r += step) {
+          const V v = *reinterpret_cast<const V *>(at + r * p.stride);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[i]));
+        }
+      } else {
+        for (; r < p.rows; r += step)
+          for (int i = 0; i < p.dims - c * 8; ++i) most = max(most, magnitude(at[r * p.stride + i]));
       }
     }
   } else {
     // (exponents shifted by 1000, 0 being none)
-    for (int64_t r = block * 256 + threadIdx.x; r < a.part[0].rows; r += 256 * kScaleParts) {
+    for (int64_t r = static_cast<int64_t>(block) * 256 + threadIdx.x; r < a.part[0].rows; r += 256ll * a.parts_w) {
       const float w = a.row.weight(r);
       if (a.row.label(r) >= 0 && w != 0.f) most = max(most, static_cast<uint32_t>(weight_exponent(w) + 1000));
     }
   }
-  top[threadIdx.x] = most;
+#pragma unroll
+  for (int s = 32; s > 0; s /= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), s)));
+  if (threadIdx.x % 64 == 0) top[threadIdx.x / 64] = most;
   __syncthreads();
-  for (int s = 128; s > 0; s /= 2) {
-    if (threadIdx.x < s) top[threadIdx.x] = max(top[threadIdx.x], top[threadIdx.x + s]);
-    __syncthreads();
-  }
   if (threadIdx.x == 0) {
+    most = max(max(top[0], top[1]), max(top[2], top[3]));
     if (which < 2)
-      a.most[which * kScaleParts + block] = top[0];
+      a.most[which * kScaleParts + block] = most;
     else
-      a.most_w[block] = static_cast<int32_t>(top[0]) - 1000;
+      a.most_w[block] = static_cast<int32_t>(most) - 1000;
   }
 }
 
@@ -146,6 +166,11 @@ __device__ __forceinline__ int block_max_256(int v, int *room) {
   v = max(max(room[0], room[1]), max(room[2], room[3]));
   __syncthreads();
   return v;
+}
+
+__device__ __forceinline__ int largest(const int *v, int n, int least) {
+  for (int i = threadIdx.x; i < n; i += 256) least = max(least, v[i]);
+  return least;
 }
 
 // The exponent that brings a magnitude (its bits) to [2^14, 2^15).
@@ -168,18 +193,17 @@ __global__ __launch_bounds__(256) void class_lay_kernel(LayArgs a) {
     int exps[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-      if (a.part[k].seen)
-        exps[k] = scale_exponent(block_max_256(static_cast<int>(a.most[k * kScaleParts + threadIdx.x]), room));
-    top_w = block_max_256(a.most_w[threadIdx.x], room);
+      if (a.part[k].parts > 0)
+        exps[k] = scale_exponent(block_max_256(largest(reinterpret_cast<const int *>(a.most) + k * kScaleParts,
+                                                       a.part[k].parts, 0), room));
+    top_w = block_max_256(largest(a.most_w, a.parts_w, -1000), room);
     seen = exps[which];
     e = p.scaled ? seen : 0;
     if (blockIdx.x == 0 && threadIdx.x == 0)
       *a.exps = {a.part[0].scaled ? exps[0] : 0, a.part[1].scaled ? exps[1] : 0, top_w, exps[0]};
   }
   const int chunks = p.ld / 8;
-  int lanes = 1;
-  while (lanes < 256 && lanes < chunks) lanes *= 2;
-  const int per = 256 / lanes;
+  const int lanes = row_lanes(chunks), per = 256 / lanes;
   typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   const int64_t plane = static_cast<int64_t>(p.rows) * p.ld;
   for (int64_t r = static_cast<int64_t>(block) * per + threadIdx.x / lanes; r < p.rows;

@@ -48,6 +48,8 @@ __device__ __forceinline__ float power_of(uint32_t byte) {  // of an e8m0 scale
 // POWER: e8m0 scales, else fp32. WIDE: values widened to fp16.
 template <class S, bool POWER, bool WIDE>
 struct F8Steps {
+  static constexpr bool kAhead = false;
+  static_assert(S::KB == 128, "a step is a block of scales");
   uint32_t at, last_at;        // of this lane's row's first scale, in bytes from the buffer's base
   int32_t blocks, tail;
   i32x4t rsrc;
@@ -76,7 +78,7 @@ struct F8Steps {
     at = row < 0 ? kOutside : row * blocks * size + x_low;
     const int cb = min(c0 / kScaleBlock, s.y_blocks - 1);
     ybase = static_cast<const char *>(s.y) + static_cast<int64_t>(cb) * blocks * size;
-    place = tile_lds + (S::BC + S::BR) * kStepBytes + wave * 256;
+    place = tile_lds + (S::BC + S::BR) * S::KB + wave * 256;
   }
   // The rows' scales of step k, on their way into LDS with the step's stage.
   __device__ __forceinline__ void load(int k, bool exists, uint32_t to) const {
@@ -108,16 +110,17 @@ struct F8Steps {
         v[h * 4 + d] &= have >= 4 ? -1 : have <= 0 ? 0 : (1 << (8 * have)) - 1;
       }
   }
-  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, const char *x, int k, int wc,
-                                       int wr, int lane) {
+  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, int k, int wc, int wr,
+                                       int lane) {
+    const char *x = y + S::BC * S::KB;
     i32x8t fx[S::FR];
     f16x8 wx[WIDE ? S::FR : 1][4];
     float sx[S::FR];
     uint32_t bx[S::FR];
-    const bool cut = k == blocks - 1 && tail < kStepBytes;
+    const bool cut = k == blocks - 1 && tail < S::KB;
     const char *scales = place + (y - tile_lds);
     auto whole = [&](const char *tile, int row) {
-      const i32x4t lo = read_row<i32x4t>(tile, row, 0, lane), hi = read_row<i32x4t>(tile, row, 4, lane);
+      const i32x4t lo = read_row<S::KB, i32x4t>(tile, row, 0, lane), hi = read_row<S::KB, i32x4t>(tile, row, 4, lane);
       i32x8t v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       if (cut) mask(v, lane);
       return v;

@@ -2,13 +2,15 @@
 // matrix cores, one tile of the output a block, with what happens to a finished tile
 // left to an epilogue. 16-bit floating point or e4m3, sums in fp32.
 //
-// The tile's steps of k (128 bytes of each row: 64 16-bit elements, 128 8-bit ones) pass through
-// LDS in a ring of stages, loaded straight from memory without registers in between. One
-// barrier a step: when it is passed, the step's stage has arrived and the stage before
-// it is free for the next load. An operand whose k is contiguous lies in LDS as
-// rows of 128 bytes; one whose k goes from row to row (a transposed operand) as 64 rows of the
+// The tile's steps of k (64 or 128 bytes of each row) pass through LDS in a ring of stages, loaded
+// straight from memory without registers in between. One barrier a step: when it is passed, a
+// stage has arrived and another is free for the next load. An operand whose k is contiguous lies in
+// LDS as rows of a step's bytes; one whose k goes from row to row (a transposed operand) as rows of the
 // tile's width, read with the transposing LDS loads, so that no transposed copy of
-// it is ever made. Both lie swizzled, so that neither reading wave meets a bank twice.
+// it is ever made. Both lie swizzled: by the counters no two lanes of a read meet in a bank.
+//
+// Tiles of 256 x 256 go in steps of 64 bytes through five stages of 32 KB, all of a unit's LDS:
+// four of them on their way cover the latency of a loaded memory.
 //
 // Layout of a result: lane l of a 16 x 16 block holds row r = l % 16, columns
 // c = 4 (l / 16) .. + 3: y is the matrix instruction's first operand.
@@ -27,8 +29,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4t __attribute__((ext_vector_type(4)));
 typedef int32_t i32x4t __attribute__((ext_vector_type(4)));
 typedef int32_t i32x8t __attribute__((ext_vector_type(8)));
-
-constexpr int kStepBytes = 128;  // of k, in a row of a stage
 
 // One operand. Rows of it are the output's rows (x) or columns (y), or, of a transposed
 // one, the values of k. Everything of it that a tile reads starts at multiples of 16 bytes.
@@ -81,21 +81,22 @@ struct F8 {
   static constexpr int bytes = 1;
 };
 
-// WC x WR waves of FC x FR blocks of 16 x 16; NS stages; XT, YT: transposed operands.
-template <class E_, int WC_, int WR_, int FC_, int FR_, int NS_, bool XT_, bool YT_>
+// WC x WR waves of FC x FR blocks of 16 x 16; NS stages of KB bytes of k; XT, YT: transposed operands.
+template <class E_, int WC_, int WR_, int FC_, int FR_, int KB_, int NS_, bool XT_, bool YT_>
 struct TileShape {
   typedef E_ E;
+  static constexpr int KB = KB_, KN = KB_ / E::bytes;  // of a step: bytes, elements
   static constexpr int WC = WC_, WR = WR_, FC = FC_, FR = FR_, NS = NS_;
   static constexpr bool XT = XT_, YT = YT_;
   static constexpr int kWaves = WC * WR, kThreads = kWaves * 64;
   static constexpr int BC = WC * FC * 16, BR = WR * FR * 16;
   // (8-bit operands: and 64 words a wave, the scales of its rows)
-  static constexpr int kStage = (BC + BR) * kStepBytes + (E::bytes == 1 ? kWaves * 256 : 0);
+  static constexpr int kStage = (BC + BR) * KB + (E::bytes == 1 ? kWaves * 256 : 0);
   static constexpr int kLds = NS * kStage;
-  static constexpr int QY = BC / 8 / kWaves, QX = BR / 8 / kWaves;  // loads of a thread in a stage
-  static_assert(BC / 8 % kWaves == 0 && BR / 8 % kWaves == 0, "every wave loads as much");
+  static constexpr int QY = BC * KB / 1024 / kWaves, QX = BR * KB / 1024 / kWaves;  // loads of a thread in a stage
+  static_assert(BC * KB / 1024 % kWaves == 0 && BR * KB / 1024 % kWaves == 0, "every wave loads as much");
   static constexpr int kLoads = QX + QY + (E::bytes == 1 ? 1 : 0);
-  static_assert(NS >= 2 && (NS - 2) * kLoads < 64 && kLds <= 160 * 1024, "");
+  static_assert(NS >= 2 && (NS - 1) * kLoads < 64 && kLds <= 160 * 1024, "");
   static_assert(!(XT || YT) || E::bytes == 2, "the transposing loads take 16-bit elements");
 };
 
@@ -106,9 +107,12 @@ __device__ __forceinline__ uint32_t lds_address(const char *p) {
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char *)p));
 }
 
-// Which 16 bytes of a row of 128 lie at a place in LDS: rows r and r + 1 fill the 64 banks, the
-// pairs of rows beside them have their chunks elsewhere.
-__device__ __forceinline__ int swizzle_row(int row) { return (row >> 1) & 7; }
+// Which 16 bytes of a row lie at a place in LDS: two rows of 128 bytes, or four of 64, fill the 64
+// banks, and the ones beside them have their chunks elsewhere.
+template <int KB>
+__device__ __forceinline__ int swizzle_row(int row) {
+  return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
 // The same for a transposed operand, in pairs of chunks: a transposing read takes 32 bytes of
 // rows k .. k + 3 and k + 8 .. k + 11 at a time.
 __device__ __forceinline__ int swizzle_k(int k, int chunks) {
@@ -117,73 +121,72 @@ __device__ __forceinline__ int swizzle_k(int k, int chunks) {
 
 constexpr uint32_t kOutside = 0x80000000u;  // an offset past the end of every buffer: loads give 0
 
-// One thread's loads of one operand's part of a stage: B rows (columns) of the tile.
+// One thread's loads of one operand's part of a stage: B rows (columns) of the tile. What changes from
+// step to step is in scalar registers: the base and how much of k is left.
 template <class S, int B, bool T, int Q>
 struct TileLoad {
-  uint32_t at[Q];  // byte offsets from the step's base
-  uint32_t chunk;  // of k, in a row (contiguous k): bytes from the step's first
-  const char *base;
-  int64_t advance, plane;
-  int64_t left;    // bytes of k (contiguous), or rows of k, that exist
+  static constexpr int kChunks = T ? B / 8 : S::KB / 16, kRows = 64 / kChunks;  // of a row; rows of a load
+  uint32_t at[Q];   // byte offsets from the step's base
+  int32_t place;    // of the thread in k: bytes (contiguous k) or rows of its first load
+  i32x4t rsrc;
+  int64_t advance;
+  int32_t left;     // of k, bytes or rows, from the step on
 
   __device__ __forceinline__ void begin(const Operand &o, int first, int wave, int lane) {
-    plane = o.plane;
-    if constexpr (!T) {
-      const int row = wave * 8 + lane / 8;
-      chunk = 16 * ((lane % 8) ^ swizzle_row(row));
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int r = q * S::kWaves * 8 + row;
-        at[q] = first + r < o.rows ? static_cast<uint32_t>(r * o.ld) + chunk : kOutside;
-      }
-      base = o.base + first * o.ld;
-      advance = kStepBytes;
-      left = o.bytes;
-    } else {
-      constexpr int chunks = B / 8, rows = 64 / chunks;  // of a row; rows that one load takes
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int k = (q * S::kWaves + wave) * rows + lane / chunks;
-        const int c = 16 * ((lane % chunks) ^ swizzle_k(k, chunks));
-        at[q] = first * 2 + c < o.bytes ? static_cast<uint32_t>(k * o.ld) + c : kOutside;
-      }
-      chunk = 0;
-      base = o.base + first * 2;
-      advance = 64 * o.ld;
-      left = o.rows;
-    }
-  }
-
-  // Loads step `st` of plane `pl` into LDS at `to` (the wave's first place of the operand's part).
-  __device__ __forceinline__ void step(int pl, int st, bool exists, uint32_t to, int64_t ld) const {
-    const char *b = base + pl * plane + st * advance;
-    i32x4t rsrc;
-    rsrc[0] = static_cast<int32_t>(reinterpret_cast<uintptr_t>(b));
-    rsrc[1] = static_cast<int32_t>((reinterpret_cast<uintptr_t>(b) >> 32) & 0xffff);
-    rsrc[3] = 0x00020000;
-    uint32_t most = 0;
-    if constexpr (!T) {
-      const int64_t l = exists ? left - static_cast<int64_t>(st) * kStepBytes : 0;
-      most = static_cast<uint32_t>(l < 0 ? 0 : l < kStepBytes ? l : kStepBytes);
-      rsrc[2] = 0x7fffffff;
-    } else {
-      const int64_t l = exists ? (left - static_cast<int64_t>(st) * 64) * ld : 0;
-      rsrc[2] = static_cast<int32_t>(l < 0 ? 0 : l < 0x7fffffff ? l : 0x7fffffff);
-    }
+    const int row = wave * kRows + lane / kChunks;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const uint32_t off = T || chunk < most ? at[q] : kOutside;
-      // (nothing here is an output: the data goes to LDS, and the main loop waits for it)
-      asm volatile(
-          "s_mov_b32 m0, %0\n\t"
-          "s_nop 0\n\t"
-          "buffer_load_dwordx4 %1, %2, 0 offen lds"
-          :
-          : "s"(to + q * S::kWaves * 1024), "v"(off), "s"(rsrc)
-          : "memory", "m0");
+      const int r = q * S::kWaves * kRows + row;
+      if constexpr (T) {
+        const int c = 16 * ((lane % kChunks) ^ swizzle_k(r, kChunks));
+        at[q] = first * 2 + c < o.bytes ? static_cast<uint32_t>(r * o.ld) + c : kOutside;
+      } else {
+        place = 16 * ((lane % kChunks) ^ swizzle_row<S::KB>(row));
+        at[q] = first + r < o.rows ? static_cast<uint32_t>(r * o.ld) + place : kOutside;
+      }
     }
+    if constexpr (T) place = row;
+    advance = T ? S::KN * o.ld : S::KB;
+    rsrc[2] = 0x7fffffff;
+    rsrc[3] = 0x00020000;
+  }
+  // To step `st` of a plane.
+  __device__ __forceinline__ void seek(const Operand &o, int first, int pl, int st) {
+    const char *b = o.base + (T ? first * 2 : first * o.ld) + pl * o.plane + st * advance;
+    rsrc[0] = static_cast<int32_t>(reinterpret_cast<uintptr_t>(b));
+    rsrc[1] = static_cast<int32_t>((reinterpret_cast<uintptr_t>(b) >> 32) & 0xffff);
+    left = (T ? o.rows : o.bytes) - st * (T ? S::KN : S::KB);
+  }
+  __device__ __forceinline__ void next() {
+    const uint64_t b = (static_cast<uint64_t>(static_cast<uint32_t>(rsrc[1])) << 32 | static_cast<uint32_t>(rsrc[0])) + advance;
+    rsrc[0] = static_cast<int32_t>(b);
+    rsrc[1] = static_cast<int32_t>(b >> 32);
+    left -= T ? S::KN : S::KB;
+  }
+  // Load q of the step to LDS, from `to` on (the wave's first place of the operand).
+  __device__ __forceinline__ void load(int q, uint32_t to) const {
+    const uint32_t off = place + (T ? q * S::kWaves * kRows : 0) < left ? at[q] : kOutside;
+    // (nothing here is an output: the data goes to LDS, and the main loop waits for it)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(to + q * S::kWaves * 1024), "v"(off), "s"(rsrc)
+        : "memory", "m0");
   }
 };
+
+// All of a wave's own loads from LDS, and of its loads into it all but the last `n`, are done; then
+// all waves'. (The builtin, unlike inline assembly, is seen by the compiler, which
+// then needs no wait of its own before the fragments are used.)
+template <int n>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((n & 15) | 7 << 4 | 0 << 8 | (n >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // What a lane holds of 16 rows x 32 values of k.
 template <class E>
@@ -222,45 +225,62 @@ __device__ __forceinline__ V read_transposed(const char *tile, int width, int co
   return u.v;
 }
 
-template <class V>
+template <int KB, class V>
 __device__ __forceinline__ V read_row(const char *tile, int row, int chunk, int lane) {
-  return *reinterpret_cast<const V *>(tile + row * kStepBytes + ((chunk + lane / 16) ^ swizzle_row(row)) * 16);
+  return *reinterpret_cast<const V *>(tile + row * KB + ((chunk + lane / 16) ^ swizzle_row<KB>(row)) * 16);
 }
 
-// What a step multiplies: 16-bit operands.
+// What a step multiplies: 16-bit operands. In steps of 64 bytes the next step's fragments are on their
+// way from LDS while this one's are multiplied.
 template <class S>
 struct PlainSteps {
+  static constexpr bool kAhead = S::FC * S::FR >= 16;  // (small tiles wait for memory)
+  typedef Fragment<typename S::E> M;
+  typedef typename M::V V;
+  struct Held {
+    V y[S::FC], x[S::FR];
+  };
   template <class A>
   __device__ __forceinline__ PlainSteps(const A &, const TileArgs &, int, int, int, int) {}
   __device__ __forceinline__ void load(int, bool, uint32_t) const {}
   __device__ __forceinline__ void before(int) {}
-  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, const char *x, int, int wc,
-                                       int wr, int lane) {
-    typedef Fragment<typename S::E> M;
-    typedef typename M::V V;
+  __device__ __forceinline__ void read_x(Held &f, const char *y, int ks, int j, int wr, int lane) const {
+    const char *x = y + S::BC * S::KB;
+    const int at = (wr * S::FR + j) * 16;
+    if constexpr (S::XT)
+      f.x[j] = read_transposed<V>(x, S::BR, at, ks, lane);
+    else
+      f.x[j] = read_row<S::KB, V>(x, at + lane % 16, ks * 4, lane);
+  }
+  __device__ __forceinline__ void read_y(Held &f, const char *y, int ks, int i, int wc, int lane) const {
+    const int at = (wc * S::FC + i) * 16;
+    if constexpr (S::YT)
+      f.y[i] = read_transposed<V>(y, S::BC, at, ks, lane);
+    else
+      f.y[i] = read_row<S::KB, V>(y, at + lane % 16, ks * 4, lane);
+  }
+  // Part g of `of` of a fragment set, and of the products.
+  __device__ __forceinline__ void read(Held &f, const char *y, int ks, int g, int of, int wc, int wr, int lane) const {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      V fy[S::FC], fx[S::FR];
+    for (int j = 0; j < S::FR; ++j)
+      if (j * of / S::FR == g) read_x(f, y, ks, j, wr, lane);
 #pragma unroll
-      for (int j = 0; j < S::FR; ++j) {
-        const int at = (wr * S::FR + j) * 16;
-        if constexpr (S::XT)
-          fx[j] = read_transposed<V>(x, S::BR, at, ks, lane);
-        else
-          fx[j] = read_row<V>(x, at + lane % 16, ks * 4, lane);
-      }
+    for (int i = 0; i < S::FC; ++i)
+      if (i * of / S::FC == g) read_y(f, y, ks, i, wc, lane);
+  }
+  __device__ __forceinline__ void multiply(f32x4t (&acc)[S::FC][S::FR], const Held &f, int g, int of) const {
 #pragma unroll
-      for (int i = 0; i < S::FC; ++i) {
-        const int at = (wc * S::FC + i) * 16;
-        if constexpr (S::YT)
-          fy[i] = read_transposed<V>(y, S::BC, at, ks, lane);
-        else
-          fy[i] = read_row<V>(y, at + lane % 16, ks * 4, lane);
-      }
+    for (int i = 0; i < S::FC; ++i)
+      if (i * of / S::FC == g)
 #pragma unroll
-      for (int i = 0; i < S::FC; ++i)
+        for (int j = 0; j < S::FR; ++j) acc[i][j] = M::mul(f.y[i], f.x[j], acc[i][j]);
+  }
+  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, int, int wc, int wr, int lane) {
 #pragma unroll
-        for (int j = 0; j < S::FR; ++j) acc[i][j] = M::mul(fy[i], fx[j], acc[i][j]);
+    for (int ks = 0; ks < S::KB / 64; ++ks) {
+      Held f;
+      read(f, y, ks, 0, 1, wc, wr, lane);
+      multiply(acc, f, 0, 1);
     }
   }
 };
@@ -276,10 +296,6 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
   const TilePlace p = tile_place(a);
   const int first_c = p.c * S::BC, first_r = p.r * S::BR;
 
-  TileLoad<S, S::BC, S::YT, S::QY> ly;
-  TileLoad<S, S::BR, S::XT, S::QX> lx;
-  ly.begin(a.y, first_c, wave, lane);
-  lx.begin(a.x, first_r, wave, lane);
   const uint32_t lds_first = __builtin_amdgcn_readfirstlane(lds_address(tile_lds));
   const uint32_t lds = lds_first + wave * 1024;
   Steps steps(sa, a, first_c + wc * S::FC * 16, first_r + wr * S::FR * 16, wave, lane);
@@ -287,18 +303,39 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
   const int total = a.steps * a.pairs;
   const int from = p.part * a.part_steps, to = min(total, from + a.part_steps);
   int next = from, pair = from / a.steps, st = from - pair * a.steps;
-  auto load = [&](int stage) {
-    const bool exists = next < to;
+  TileLoad<S, S::BC, S::YT, S::QY> ly;
+  TileLoad<S, S::BR, S::XT, S::QX> lx;
+  ly.begin(a.y, first_c, wave, lane);
+  lx.begin(a.x, first_r, wave, lane);
+  auto seek = [&] {
+    ly.seek(a.y, first_c, pair == 1, st);
+    lx.seek(a.x, first_r, pair == 2, st);
+  };
+  seek();
+  // Loads the next step into a stage (zeros, without touching memory, after the last one), with
+  // `between` after each load.
+  auto load = [&](int stage, auto between) {
     const uint32_t at = lds + stage * S::kStage;
-    ly.step(pair == 1, st, exists, at, a.y.ld);
-    lx.step(pair == 2, st, exists, at + S::BC * kStepBytes, a.x.ld);
-    steps.load(next, exists, lds_first + stage * S::kStage + (S::BC + S::BR) * kStepBytes + wave * 256);
+    if (next >= to) ly.left = lx.left = 0;
+    steps.load(next, next < to, lds_first + stage * S::kStage + (S::BC + S::BR) * S::KB + wave * 256);
+#pragma unroll
+    for (int q = 0; q < S::QY + S::QX; ++q) {
+      if (q < S::QY)
+        ly.load(q, at);
+      else
+        lx.load(q - S::QY, at + S::BC * S::KB);
+      between(q);
+    }
     ++next;
-    if (++st == a.steps) {
+    ly.next();
+    lx.next();
+    if (++st == a.steps && next < to) {
       st = 0;
       ++pair;
+      seek();
     }
   };
+  auto nothing = [](int) {};
 
   f32x4t acc[S::FC][S::FR];
 #pragma unroll
@@ -306,21 +343,68 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
 #pragma unroll
     for (int j = 0; j < S::FR; ++j) acc[i][j] = f32x4t{0.f, 0.f, 0.f, 0.f};
 
+  int now = 0;
+  auto next_stage = [](int s) { return s + 1 == S::NS ? 0 : s + 1; };
+  if constexpr (Steps::kAhead) {
+    // All stages on their way. Fragments are read 64 bytes of k ahead of their products; when the barrier
+    // in a step's last half is passed, all waves hold that half in registers, so its stage is
+    // free, and the next step has arrived.
+    constexpr int halves = S::KB / 64;
+    typename Steps::Held f[2];
 #pragma unroll
-  for (int s = 0; s < S::NS - 1; ++s) load(s);
-  int now = 0, free = S::NS - 1;
-  for (int k = from; k < to; ++k) {
-    // this step's stage has arrived (later ones may be on their way), and this wave's
-    // reads of the stage before it are done
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::NS - 2) * S::kLoads) : "memory");
-    steps.before(k);
-    load(free);
-    const char *y = tile_lds + now * S::kStage;
-    steps.step(acc, y, y + S::BC * kStepBytes, k, wc, wr, lane);
-    free = now;
-    now = now + 1 == S::NS ? 0 : now + 1;
+    for (int s = 0; s < S::NS; ++s) load(s, nothing);
+    wait_and_meet<(S::NS - 1) * S::kLoads>();
+    steps.read(f[0], tile_lds, 0, 0, 1, wc, wr, lane);
+    auto first = [&](typename Steps::Held &held, typename Steps::Held &coming) {
+      const char *y = tile_lds + now * S::kStage;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        steps.read(coming, y, 1, g, 4, wc, wr, lane);
+        steps.multiply(acc, held, g, 4);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto last = [&](typename Steps::Held &held, typename Steps::Held &coming) {
+      wait_and_meet<(S::NS - 2) * S::kLoads>();
+      const int free = now;
+      now = next_stage(now);
+      const char *y = tile_lds + now * S::kStage;
+      // Loads, reads and products take turns: a wave that issues its loads in a row waits for the
+      // memory pipeline with the matrix cores idle.
+      load(free, [&](int q) {
+        steps.read(coming, y, 0, q, S::kLoads, wc, wr, lane);
+        steps.multiply(acc, held, q, S::kLoads);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    if constexpr (halves == 2) {
+      for (int k = from; k < to; ++k) {
+        first(f[0], f[1]);
+        last(f[1], f[0]);
+      }
+    } else {
+      for (int k = from; k < to; k += 2) {
+        last(f[0], f[1]);
+        if (k + 1 < to) last(f[1], f[0]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < S::NS - 1; ++s) load(s, nothing);
+    int free = S::NS - 1;
+    for (int k = from; k < to; ++k) {
+      // this step's stage has arrived (later ones may be on their way), and this wave's
+      // reads of the stage before it are done
+      wait_and_meet<(S::NS - 2) * S::kLoads>();
+      steps.before(k);
+      load(free, nothing);
+      const char *y = tile_lds + now * S::kStage;
+      steps.step(acc, y, k, wc, wr, lane);
+      free = now;
+      now = next_stage(now);
+    }
   }
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  wait_and_meet<0>();
   epi.template finish<S>(a, p, acc, first_c + wc * S::FC * 16, first_r + wr * S::FR * 16, wc, wr, lane);
 }
 
