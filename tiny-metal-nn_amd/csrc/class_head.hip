@@ -11,6 +11,7 @@
 #include "class_loss_kernel.hpp"
 #include "f8_kernel.hpp"
 #include "logits_host.hpp"
+#include "narrow_kernel.hpp"
 #include "tmnn_hip.h"
 
 using namespace tmnn_hip;
@@ -251,8 +252,22 @@ struct LossPlan {
   Tiles t_sums, t_d, t_x, t_y;       // logits for sums, for d; d_features, d_table
   int64_t slab_ld;
   bool slabs_x, slabs_y;
+  // features of up to 128 dims: parts of the walks
+  bool narrow, wide_r, wide_t;
+  int32_t blocks_r, tiles_r, parts_r, blocks_t, tiles_t, parts_t;
+  int64_t at_part_sum, at_part_own, at_part_out;
   int64_t at_exps, at_most, at_x, at_w, at_y, at_sums, at_own, at_stats, at_d, at_slab_x, at_slab_y, bytes;
 };
+
+// Dims up to which the walks of narrow_kernel.hpp take a call.
+constexpr int64_t kNarrow = 128;
+
+// Parts of a walk's tiles, where the items of one side alone make too few blocks: four blocks a unit, and
+// four tiles a part at least.
+int32_t walk_parts(int64_t blocks, int64_t tiles) {
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>(4 * kUnits / blocks, tiles / 4));
+  return static_cast<int32_t>(parts_of(tiles, parts_of(tiles, parts)));
+}
 
 LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   LossPlan p{};
@@ -262,7 +277,8 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   p.f32 = a.dtype == TMNN_DTYPE_F32;
   p.planes = p.f32 ? 2 : 1;
   p.pairs = p.f32 ? 3 : 1;
-  p.ld = up(a.dims, 64);
+  p.narrow = a.dims <= kNarrow;
+  p.ld = !p.narrow ? up(a.dims, 64) : a.dims <= 32 ? 32 : a.dims <= 64 ? 64 : 128;
   // operands that lie well are read in place
   auto lies_well = [&](const void *ptr, int64_t stride, int64_t rows) {
     return size == 2 && aligned(ptr, 16) && (stride % 8 == 0 || rows <= 1) && a.dims % 8 == 0 &&
@@ -270,7 +286,8 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   };
   const bool x_well = lies_well(a.features, a.feature_stride, n), y_well = lies_well(a.table, a.table_stride, v);
   p.scaled = p.f32 || p.grad;
-  const bool convert = p.f32 || (p.grad && a.dtype == TMNN_DTYPE_BF16);
+  const bool convert = p.narrow || p.f32 || (p.grad && a.dtype == TMNN_DTYPE_BF16);
+  if (p.narrow) p.scaled = true;
   p.lay_x = convert || !x_well;
   p.lay_y = convert || !y_well;
   p.weighted = a.d_table != nullptr;
@@ -286,6 +303,32 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   if (p.lay_x) p.at_x = room(x_bytes);
   if (p.weighted) p.at_w = room(x_bytes);
   if (p.lay_y) p.at_y = room(v * p.ld * 2 * p.planes);
+  if (p.narrow) {
+    // 32 items a wave where that still makes four blocks a unit
+    auto wide = [](int64_t items) { return items >= 4 * kUnits * kWalkWaves * 32; };
+    auto blocks = [](int64_t items, bool w) { return static_cast<int32_t>(parts_of(items, kWalkWaves * (w ? 32 : 16))); };
+    p.wide_r = wide(n);
+    p.blocks_r = blocks(n, p.wide_r);
+    p.tiles_r = static_cast<int32_t>(parts_of(v, kWalkItems));
+    p.parts_r = walk_parts(p.blocks_r, p.tiles_r);
+    if (p.sums && p.grad && !a.stats) p.at_stats = room(n * 16);
+    if (p.parts_r > 1) {
+      p.at_part_sum = room(n * p.parts_r * 8);
+      p.at_part_own = room(n * 4);
+      if (a.d_features) p.at_part_out = room(n * p.parts_r * p.ld * 4);
+    }
+    if (a.d_table) {
+      p.wide_t = wide(v);
+      p.blocks_t = blocks(v, p.wide_t);
+      p.tiles_t = static_cast<int32_t>(parts_of(n, kWalkItems));
+      p.parts_t = walk_parts(p.blocks_t, p.tiles_t);
+      p.slab_ld = up(a.dims, 4);
+      p.slabs_y = p.parts_t > 1;
+      if (p.slabs_y) p.at_slab_y = room(v * p.slab_ld * 4 * p.parts_t);
+    }
+    p.bytes = std::max<int64_t>(at, 256);
+    return p;
+  }
   if (p.sums) {
     p.t_sums = choose(n, v, p.ld * 2, p.pairs, false, true, true, false);
     p.at_sums = room(n * p.t_sums.c * 8);
@@ -326,6 +369,108 @@ Tiles of_piece(Tiles t, int64_t cols) {
 }
 
 template <class T>
+int run_reduce(const GradScale &s, void *out, int64_t ld, const float *slabs, int64_t slab_ld, int32_t parts, int64_t rows,
+               int64_t cols, hipStream_t st) {
+  ReduceArgs r{s, out, ld, slabs, static_cast<int32_t>(slab_ld), parts, static_cast<int32_t>(rows),
+               static_cast<int32_t>(cols)};
+  const int64_t blocks = std::min<int64_t>(parts_of(rows * slab_ld / 4, 256), 8 * kUnits);
+  hipLaunchKernelGGL((class_reduce_kernel<T>), dim3(static_cast<uint32_t>(std::max<int64_t>(blocks, 1))), dim3(256), 0, st,
+                     r);
+  TMNN_HIP_TRY(hipGetLastError());
+  return TMNN_OK;
+}
+
+typedef std::integral_constant<int, 1> One;
+typedef std::integral_constant<int, 2> Two;
+
+template <int DP, int PL, int RJ, class Op>
+int run_walk(const WalkArgs &a, int32_t parts, const Op &op, int device, hipStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    TMNN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(walk_kernel<DP, PL, RJ, Op>),
+                                     hipFuncAttributeMaxDynamicSharedMemorySize, WalkTile<DP, PL>::kLds));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL((walk_kernel<DP, PL, RJ, Op>), dim3(static_cast<uint32_t>(static_cast<int64_t>(a.blocks) * parts)),
+                     dim3(kWalkThreads), (WalkTile<DP, PL>::kLds), st, a, op);
+  TMNN_HIP_TRY(hipGetLastError());
+  return TMNN_OK;
+}
+
+// Features of up to 128 dims, both sides laid out.
+template <class T, int DP>
+int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, const RowInfo &row, float c, float inv_t,
+               const Exponents *exps, hipStream_t st) {
+  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
+  const int device = h->ctx->device;
+  char *ws = static_cast<char *>(a.workspace);
+  const int32_t n = static_cast<int32_t>(a.rows), v = static_cast<int32_t>(a.classes), dims = static_cast<int32_t>(a.dims);
+  const int64_t x_plane = a.rows * DP * 2, y_plane = a.classes * DP * 2;
+  float4 *stats = reinterpret_cast<float4 *>(a.stats ? reinterpret_cast<char *>(a.stats) : ws + p.at_stats);
+  if (p.sums || a.d_features) {
+    RowsShared g{};
+    g.exps = exps;
+    g.row = row;
+    g.c = c;
+    g.inv_t = inv_t;
+    g.loss = p.sums ? a.loss : nullptr;
+    g.stats = p.sums && (a.stats || a.d_table) ? stats : nullptr;
+    if (p.parts_r > 1) {
+      g.part_sum = reinterpret_cast<float2 *>(ws + p.at_part_sum);
+      g.own = reinterpret_cast<float *>(ws + p.at_part_own);
+      g.part_out = reinterpret_cast<float *>(ws + p.at_part_out);
+    }
+    const T *table = static_cast<const T *>(a.table);
+    T *out = static_cast<T *>(a.d_features);
+    const WalkArgs w{ws + p.at_x, ws + p.at_y, x_plane, y_plane, n, v, p.blocks_r,
+                     static_cast<int32_t>(parts_of(p.tiles_r, p.parts_r))};
+    auto walk = [&](auto rj, auto op) {
+      static_cast<RowsShared &>(op) = g;
+      op.table = table;
+      op.table_ld = a.table_stride;
+      op.out = out;
+      op.out_ld = a.d_feature_stride;
+      op.dims = dims;
+      return run_walk<DP, PL, decltype(rj)::value>(w, p.parts_r, op, device, st);
+    };
+    const One one;
+    const Two two;
+    const int rc = p.wide_r ? (out ? walk(two, RowsWalk<T, true, 2>{}) : walk(two, RowsWalk<T, false, 2>{}))
+                            : (out ? walk(one, RowsWalk<T, true, 1>{}) : walk(one, RowsWalk<T, false, 1>{}));
+    if (rc != TMNN_OK) return rc;
+    if (p.parts_r > 1) {
+      hipLaunchKernelGGL((walk_join_kernel<T, DP>), dim3(static_cast<uint32_t>(parts_of(n, 256 / (DP / 4)))), dim3(256), 0,
+                         st, g, n, p.parts_r, table, a.table_stride, out, a.d_feature_stride, dims);
+      TMNN_HIP_TRY(hipGetLastError());
+    }
+  }
+  if (!a.d_table) return TMNN_OK;
+  float *slabs = p.slabs_y ? reinterpret_cast<float *>(ws + p.at_slab_y) : nullptr;
+  const GradScale scale{exps, row, inv_t, 0};
+  const WalkArgs w{ws + p.at_y, ws + p.at_w, y_plane, x_plane, v, n, p.blocks_t,
+                   static_cast<int32_t>(parts_of(p.tiles_t, p.parts_t))};
+  auto walk = [&](auto rj) {
+    constexpr int RJ = decltype(rj)::value;
+    TableWalk<T, RJ> t{};
+    t.exps = exps;
+    t.row = row;
+    t.c = c;
+    t.stats = stats;
+    t.scale = scale;
+    t.out = static_cast<T *>(a.d_table);
+    t.out_ld = a.d_table_stride;
+    t.dims = dims;
+    t.slabs = slabs;
+    t.slab_ld = static_cast<int32_t>(p.slab_ld);
+    return run_walk<DP, PL, RJ>(w, p.parts_t, t, device, st);
+  };
+  const int rc = p.wide_t ? walk(Two{}) : walk(One{});
+  if (rc != TMNN_OK || !slabs) return rc;
+  return run_reduce<T>(scale, a.d_table, a.d_table_stride, slabs, p.slab_ld, p.parts_t, v, dims, st);
+}
+
+template <class T>
 int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, bool back, hipStream_t st) {
   const int device = h->ctx->device;
   const int64_t n = a.rows, v = a.classes, size = sizeof(T);
@@ -357,6 +502,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
     l.row = row;
     l.most = reinterpret_cast<uint32_t *>(ws + p.at_most);
     l.most_w = reinterpret_cast<int32_t *>(ws + p.at_most) + 2 * kScaleParts;
+    l.by_weight = !p.narrow;
     l.parts_w = static_cast<int32_t>(std::min<int64_t>(parts_of(n, 256), kScaleParts));
     l.exps = reinterpret_cast<Exponents *>(ws + p.at_exps);
     if (p.scaled) exps = l.exps;
@@ -370,6 +516,13 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
     TMNN_HIP_TRY(hipGetLastError());
   }
 
+  if (p.narrow) {
+    switch (p.ld) {
+      case 32: return run_narrow<T, 32>(h, a, p, row, c, inv_t, exps, st);
+      case 64: return run_narrow<T, 64>(h, a, p, row, c, inv_t, exps, st);
+      default: return run_narrow<T, 128>(h, a, p, row, c, inv_t, exps, st);
+    }
+  }
   // operands: rows of dims values
   const int64_t row_bytes = up(a.dims, 8) * 2;
   auto laid = [&](int64_t at, int64_t rows) {
@@ -406,13 +559,6 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
   const int64_t d_plane = n * p.ld_d;
   const Operand dop{ws + p.at_d, p.ld_d * 2, d_plane * 2, static_cast<int32_t>(n), static_cast<int32_t>(p.ld_d * 2)};
   const GradScale by_row{exps, row, inv_t, 1}, by_all{exps, row, inv_t, 0};
-  auto reduce = [&](const GradScale &s, void *out, int64_t ld, int64_t at, int parts, int64_t rows) {
-    ReduceArgs r{s, out, ld, reinterpret_cast<const float *>(ws + at), static_cast<int32_t>(p.slab_ld), parts,
-                 static_cast<int32_t>(rows), static_cast<int32_t>(a.dims)};
-    const int64_t blocks = std::min<int64_t>(parts_of(rows * p.slab_ld / 4, 256), 8 * kUnits);
-    hipLaunchKernelGGL((class_reduce_kernel<T>), dim3(static_cast<uint32_t>(std::max<int64_t>(blocks, 1))), dim3(256),
-                       0, st, r);
-  };
   for (int64_t first = 0; first < v; first += p.piece) {
     const int64_t count = std::min(p.piece, v - first);
     Operand yp = y;
@@ -442,11 +588,15 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
       rc = ty.shape == kLarge ? run_plain<Large<F16, true, true>>(t, o, device, st)
                               : run_plain<Middle<F16, true, true>>(t, o, device, st);
       if (rc != TMNN_OK) return rc;
-      if (p.slabs_y) reduce(by_all, out, a.d_table_stride, p.at_slab_y, ty.parts, count);
+      if (p.slabs_y) {
+        rc = run_reduce<T>(by_all, out, a.d_table_stride, o.slabs, p.slab_ld, ty.parts, count, a.dims, st);
+        if (rc != TMNN_OK) return rc;
+      }
     }
   }
-  if (a.d_features && p.slabs_x) reduce(by_row, a.d_features, a.d_feature_stride, p.at_slab_x, p.t_x.parts, n);
-  TMNN_HIP_TRY(hipGetLastError());
+  if (a.d_features && p.slabs_x)
+    return run_reduce<T>(by_row, a.d_features, a.d_feature_stride, reinterpret_cast<float *>(ws + p.at_slab_x), p.slab_ld,
+                         p.t_x.parts, n, a.dims, st);
   return TMNN_OK;
 }
 

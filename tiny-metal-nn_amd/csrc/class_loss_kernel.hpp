@@ -72,7 +72,8 @@ struct LayPart {
   int64_t stride;      // elements
   int32_t rows, dims;
   char *out;           // [plane][rows][ld], nullable
-  char *weighted;      // the same, rows times their weight's exponent (0 where there is none); nullable
+  char *weighted;      // the same, rows times 2^exponent of their weights or as they are, and 0 where they do
+                       // not count; nullable
   int32_t ld;          // elements, a multiple of 64: columns from dims on are 0
   int32_t scaled;      // `out` is scaled by its largest magnitude (`weighted` always is)
   int32_t planes;      // 1, or 2 (high, low)
@@ -86,6 +87,7 @@ struct LayArgs {
   uint32_t *most;      // [2][kScaleParts] largest finite magnitudes, as bits
   int32_t *most_w;     // [parts_w] largest weight exponents
   int32_t parts_w;
+  int32_t by_weight;   // `weighted` is multiplied
   Exponents *exps;
 };
 
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(256) void class_lay_kernel(LayArgs a) {
     seen = exps[which];
     e = p.scaled ? seen : 0;
     if (blockIdx.x == 0 && threadIdx.x == 0)
-      *a.exps = {a.part[0].scaled ? exps[0] : 0, a.part[1].scaled ? exps[1] : 0, top_w, exps[0]};
+      *a.exps = {a.part[0].scaled ? exps[0] : 0, a.part[1].scaled ? exps[1] : 0, top_w, exps[0] * (a.by_weight | a.part[0].scaled)};
   }
   const int chunks = p.ld / 8;
   const int lanes = row_lanes(chunks), per = 256 / lanes;
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(256) void class_lay_kernel(LayArgs a) {
     if (SCALED && p.weighted) {
       const float w = a.row.weight(r);
       used = a.row.label(r) >= 0 && w != 0.f;
-      factor = used ? ldexpf(1.f, max(weight_exponent(w) - top_w, -149)) : 0.f;
+      factor = used ? a.by_weight == 0 ? 1.f : ldexpf(1.f, max(weight_exponent(w) - top_w, -149)) : 0.f;
     }
     for (int c = threadIdx.x % lanes; c < chunks; c += lanes) {
       V v = {};
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(256) void class_lay_kernel(LayArgs a) {
           if (p.planes == 2) *reinterpret_cast<f16x8 *>(reinterpret_cast<_Float16 *>(p.out) + plane + at) = low;
         }
         if (p.weighted) {
-          const float s = exponent_factor(seen);
+          const float s = exponent_factor(a.by_weight ? seen : e);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float g = used ? to_f32(v[i]) * s * factor : 0.f;  // (a row without weight may hold anything)
