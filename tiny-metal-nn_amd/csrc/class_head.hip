@@ -763,8 +763,9 @@ int run_logits(tmnn_logits *h, const tmnn_class_logits_f8_args &a, const LogitsP
     TMNN_HIP_TRY(hipGetLastError());
   }
   auto operand = [&](const void *ptr, int64_t stride, bool lay, int64_t at, int64_t rows) {
-    return Operand{lay ? ws + at : static_cast<const char *>(ptr), lay ? p.ld : stride, 0, static_cast<int32_t>(rows),
-                   static_cast<int32_t>(p.ld)};
+    // (a row's end counts in whole 16 bytes, also that of a single row)
+    return Operand{lay ? ws + at : static_cast<const char *>(ptr), lay ? p.ld : std::max(stride, p.ld), 0,
+                   static_cast<int32_t>(rows), static_cast<int32_t>(p.ld)};
   };
   const TileArgs t = tile_args(operand(a.features, a.feature_stride, p.lay_x, p.at_x, n),
                                operand(a.table, a.table_stride, p.lay_y, p.at_y, v), n, v, p.t, 1);

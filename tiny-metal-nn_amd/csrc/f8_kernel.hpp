@@ -48,7 +48,7 @@ __device__ __forceinline__ float power_of(uint32_t byte) {  // of an e8m0 scale
 // POWER: e8m0 scales, else fp32. WIDE: values widened to fp16.
 template <class S, bool POWER, bool WIDE>
 struct F8Steps {
-  static constexpr bool kAhead = false;
+  static constexpr bool kAhead = false, kStream = S::FC >= 4;
   static_assert(S::KB == 128, "a step is a block of scales");
   uint32_t at, last_at;        // of this lane's row's first scale, in bytes from the buffer's base
   int32_t blocks, tail;
@@ -89,8 +89,9 @@ struct F8Steps {
         "buffer_load_dword %1, %2, 0 offen lds"
         :
         : "s"(to), "v"(off), "s"(rsrc)
-        : "memory", "m0");
+        : "memory");
   }
+  // The classes' scale of step k.
   __device__ __forceinline__ void before(int k) {
     if constexpr (POWER)
       by = *reinterpret_cast<const __attribute__((address_space(4))) uint32_t *>(
@@ -100,68 +101,71 @@ struct F8Steps {
       sy = *reinterpret_cast<const __attribute__((address_space(4))) float *>(
           reinterpret_cast<uintptr_t>(ybase + k * 4));
   }
-  // Bytes of k that do not exist count as 0 (what lies there may be anything).
-  __device__ __forceinline__ void mask(i32x8t &v, int lane) const {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int have = tail - (h * 64 + lane / 16 * 16 + d * 4);
-        v[h * 4 + d] &= have >= 4 ? -1 : have <= 0 ? 0 : (1 << (8 * have)) - 1;
-      }
+  // Bytes of k past the end count as 0, whatever lies there: those that share 16 bytes with the end are
+  // cleared where they arrived, before the last step is read.
+  __device__ __forceinline__ void arrived(int stage, int k) const {
+    if (k != blocks - 1 || tail % 16 == 0) return;
+    for (int r = threadIdx.x; r < S::BC + S::BR; r += S::kThreads) {
+      const int row = r < S::BC ? r : r - S::BC;  // (both operands' rows lie alike)
+      char *p = tile_lds + stage * S::kStage + r * S::KB + ((tail / 16) ^ swizzle_row<S::KB>(row)) * 16;
+      for (int b = tail % 16; b < 16; ++b) p[b] = 0;
+    }
+    __syncthreads();
   }
-  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, int k, int wc, int wr,
-                                       int lane) {
-    const char *x = y + S::BC * S::KB;
-    i32x8t fx[S::FR];
-    f16x8 wx[WIDE ? S::FR : 1][4];
-    float sx[S::FR];
-    uint32_t bx[S::FR];
-    const bool cut = k == blocks - 1 && tail < S::KB;
-    const char *scales = place + (y - tile_lds);
-    auto whole = [&](const char *tile, int row) {
-      const i32x4t lo = read_row<S::KB, i32x4t>(tile, row, 0, lane), hi = read_row<S::KB, i32x4t>(tile, row, 4, lane);
-      i32x8t v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if (cut) mask(v, lane);
-      return v;
-    };
+  // What a step's products need of the rows: values and scales.
+  struct Rows {
+    i32x8t v[S::FR];
+    uint32_t scale[S::FR];
+  };
+  __device__ __forceinline__ i32x8t whole(const char *tile, int row, int lane) const {
+    const i32x4t lo = read_row<S::KB, i32x4t>(tile, row, 0, lane), hi = read_row<S::KB, i32x4t>(tile, row, 4, lane);
+    return i32x8t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+  __device__ __forceinline__ void read(Rows &f, const char *y, int k, int j, int wr, int lane) const {
+    f.v[j] = whole(y + S::BC * S::KB, (wr * S::FR + j) * 16 + lane % 16, lane);
+    const uint32_t word = *reinterpret_cast<const uint32_t *>(place + (y - tile_lds) + (j * 16 + lane % 16) * 4);
+    f.scale[j] = POWER ? word >> (8 * ((x_low + (j * 16 + lane % 16) * blocks + k) & 3)) : word;
+  }
+  __device__ __forceinline__ i32x8t classes(const char *y, int i, int wc, int lane) const {
+    return whole(y, (wc * S::FC + i) * 16 + lane % 16, lane);
+  }
+  // Before the rows of a step are used: their scales times the classes'.
+  __device__ __forceinline__ void ready(Rows &f) const {
 #pragma unroll
     for (int j = 0; j < S::FR; ++j) {
-      fx[j] = whole(x, (wr * S::FR + j) * 16 + lane % 16);
-      if constexpr (WIDE)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) wx[j][q] = widen(fx[j][2 * q], fx[j][2 * q + 1]);
-      const uint32_t word = *reinterpret_cast<const uint32_t *>(scales + (j * 16 + lane % 16) * 4);
-      if constexpr (POWER)
-        bx[j] = word >> (8 * ((x_low + (j * 16 + lane % 16) * blocks + k) & 3));
-      if constexpr (POWER && WIDE)
-        sx[j] = power_of(bx[j]) * power_of(by);
-      else
-        sx[j] = __builtin_bit_cast(float, word) * sy;
+      if constexpr (!POWER)
+        f.scale[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, f.scale[j]) * sy);
+      else if constexpr (WIDE)
+        f.scale[j] = __builtin_bit_cast(uint32_t, power_of(f.scale[j]) * power_of(by));
     }
+  }
+  __device__ __forceinline__ void multiply(f32x4t (&acc)[S::FC][S::FR], const Rows &x, const i32x8t &y, int i, int j) const {
+    if constexpr (POWER && !WIDE) {
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x.v[j], acc[i][j], 0, 0, 0, by, 0, x.scale[j]);
+    } else {
+      f32x4t part{0.f, 0.f, 0.f, 0.f};
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          part = Fragment<F16>::mul(widen(y[2 * h], y[2 * h + 1]), widen(x.v[j][2 * h], x.v[j][2 * h + 1]), part);
+      } else {
+        part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x.v[j], part, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[i][j][e] = __builtin_fmaf(part[e], __builtin_bit_cast(float, x.scale[j]), acc[i][j][e]);
+    }
+  }
+  __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, int k, int wc, int wr, int lane) {
+    Rows x;
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) read(x, y, k, j, wr, lane);
+    ready(x);
 #pragma unroll
     for (int i = 0; i < S::FC; ++i) {
-      const i32x8t fy = whole(y, (wc * S::FC + i) * 16 + lane % 16);
-      f16x8 wy[4];
-      if constexpr (WIDE)
+      const i32x8t c = classes(y, i, wc, lane);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) wy[q] = widen(fy[2 * q], fy[2 * q + 1]);
-#pragma unroll
-      for (int j = 0; j < S::FR; ++j) {
-        if constexpr (POWER && !WIDE) {
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fy, fx[j], acc[i][j], 0, 0, 0, by, 0, bx[j]);
-        } else {
-          f32x4t part{0.f, 0.f, 0.f, 0.f};
-          if constexpr (WIDE) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) part = Fragment<F16>::mul(wy[q], wx[j][q], part);
-          } else {
-            part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fy, fx[j], part, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[e], sx[j], acc[i][j][e]);
-        }
-      }
+      for (int j = 0; j < S::FR; ++j) multiply(acc, x, c, i, j);
     }
   }
 };

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kWalkThreads, RJ == 1 ? (DP <= 64 ? 4 : 3) : DP <= 
           "buffer_load_dwordx4 %1, %2, 0 offen lds"
           :
           : "s"(first + stage * W::kBytes + (q * kWalkWaves + wave) * 1024), "v"(o), "s"(rsrc)
-          : "memory", "m0");
+          : "memory");
     }
   };
 

@@ -126,7 +126,10 @@ constexpr uint32_t kOutside = 0x80000000u;  // an offset past the end of every b
 template <class S, int B, bool T, int Q>
 struct TileLoad {
   static constexpr int kChunks = T ? B / 8 : S::KB / 16, kRows = 64 / kChunks;  // of a row; rows of a load
-  uint32_t at[Q];   // byte offsets from the step's base
+  static constexpr int kEach = S::kWaves * kRows;  // rows from one load of a thread to its next
+  static_assert(kEach % 16 == 0, "its places are swizzled alike");
+  uint32_t at;      // byte offset of its first load from the step's base
+  uint32_t each;    // bytes from one load to the next
   int32_t place;    // of the thread in k: bytes (contiguous k) or rows of its first load
   i32x4t rsrc;
   int64_t advance;
@@ -134,20 +137,19 @@ struct TileLoad {
 
   __device__ __forceinline__ void begin(const Operand &o, int first, int wave, int lane) {
     const int row = wave * kRows + lane / kChunks;
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int r = q * S::kWaves * kRows + row;
-      if constexpr (T) {
-        const int c = 16 * ((lane % kChunks) ^ swizzle_k(r, kChunks));
-        at[q] = first * 2 + c < o.bytes ? static_cast<uint32_t>(r * o.ld) + c : kOutside;
-      } else {
-        place = 16 * ((lane % kChunks) ^ swizzle_row<S::KB>(row));
-        at[q] = first + r < o.rows ? static_cast<uint32_t>(r * o.ld) + place : kOutside;
-      }
+    if constexpr (T) {
+      const int c = 16 * ((lane % kChunks) ^ swizzle_k(row, kChunks));
+      place = row;
+      at = first * 2 + c < o.bytes ? static_cast<uint32_t>(row * o.ld) + c : kOutside;
+      rsrc[2] = 0x7fffffff;
+    } else {
+      place = 16 * ((lane % kChunks) ^ swizzle_row<S::KB>(row));
+      at = static_cast<uint32_t>(row * o.ld) + place;
+      // (rows past the last one lie past the buffer's end)
+      rsrc[2] = static_cast<int32_t>(min(o.rows - first, B) * o.ld);
     }
-    if constexpr (T) place = row;
+    each = static_cast<uint32_t>(kEach * o.ld);
     advance = T ? S::KN * o.ld : S::KB;
-    rsrc[2] = 0x7fffffff;
     rsrc[3] = 0x00020000;
   }
   // To step `st` of a plane.
@@ -165,7 +167,7 @@ struct TileLoad {
   }
   // Load q of the step to LDS, from `to` on (the wave's first place of the operand).
   __device__ __forceinline__ void load(int q, uint32_t to) const {
-    const uint32_t off = place + (T ? q * S::kWaves * kRows : 0) < left ? at[q] : kOutside;
+    const uint32_t off = place + (T ? q * kEach : 0) < left ? at + q * each : kOutside;
     // (nothing here is an output: the data goes to LDS, and the main loop waits for it)
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
@@ -173,7 +175,7 @@ struct TileLoad {
         "buffer_load_dwordx4 %1, %2, 0 offen lds"
         :
         : "s"(to + q * S::kWaves * 1024), "v"(off), "s"(rsrc)
-        : "memory", "m0");
+        : "memory");
   }
 };
 
@@ -235,6 +237,7 @@ __device__ __forceinline__ V read_row(const char *tile, int row, int chunk, int 
 template <class S>
 struct PlainSteps {
   static constexpr bool kAhead = S::FC * S::FR >= 16;  // (small tiles wait for memory)
+  static constexpr bool kStream = false;
   typedef Fragment<typename S::E> M;
   typedef typename M::V V;
   struct Held {
@@ -244,6 +247,7 @@ struct PlainSteps {
   __device__ __forceinline__ PlainSteps(const A &, const TileArgs &, int, int, int, int) {}
   __device__ __forceinline__ void load(int, bool, uint32_t) const {}
   __device__ __forceinline__ void before(int) {}
+  __device__ __forceinline__ void arrived(int, int) const {}
   __device__ __forceinline__ void read_x(Held &f, const char *y, int ks, int j, int wr, int lane) const {
     const char *x = y + S::BC * S::KB;
     const int at = (wr * S::FR + j) * 16;
@@ -388,6 +392,45 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
         if (k + 1 < to) last(f[1], f[0]);
       }
     }
+  } else if constexpr (Steps::kStream) {
+    // The classes' fragments go one by one, one ahead; the barrier is before the last one's products, when
+    // all of the step is in registers.
+    // Each of the rows' is read anew behind its last product.
+    typename Steps::Rows x;
+    i32x8t c[2];
+#pragma unroll
+    for (int s = 0; s < S::NS; ++s) load(s, nothing);
+    steps.before(from);
+    wait_and_meet<(S::NS - 1) * S::kLoads>();
+    steps.arrived(0, from);
+#pragma unroll
+    for (int j = 0; j < S::FR; ++j) steps.read(x, tile_lds, from, j, wr, lane);
+    c[0] = steps.classes(tile_lds, 0, wc, lane);
+    for (int k = from; k < to; ++k) {
+      const char *y = tile_lds + now * S::kStage;
+      steps.ready(x);
+#pragma unroll
+      for (int i = 0; i < S::FC - 1; ++i) {
+        c[(i + 1) % 2] = steps.classes(y, i + 1, wc, lane);
+#pragma unroll
+        for (int j = 0; j < S::FR; ++j) steps.multiply(acc, x, c[i % 2], i, j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_and_meet<(S::NS - 2) * S::kLoads>();
+      load(now, nothing);
+      now = next_stage(now);
+      steps.arrived(now, k + 1);
+      y = tile_lds + now * S::kStage;
+      static_assert(S::FC % 2 == 0, "");
+      c[0] = steps.classes(y, 0, wc, lane);
+#pragma unroll
+      for (int j = 0; j < S::FR; ++j) {
+        steps.multiply(acc, x, c[1], S::FC - 1, j);
+        steps.read(x, y, k + 1, j, wr, lane);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      steps.before(min(k + 1, to - 1));
+    }
   } else {
 #pragma unroll
     for (int s = 0; s < S::NS - 1; ++s) load(s, nothing);
@@ -397,6 +440,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
       // reads of the stage before it are done
       wait_and_meet<(S::NS - 2) * S::kLoads>();
       steps.before(k);
+      steps.arrived(now, k);
       load(free, nothing);
       const char *y = tile_lds + now * S::kStage;
       steps.step(acc, y, k, wc, wr, lane);
