@@ -802,7 +802,7 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
  * any alignment of an element. Nothing that a call writes to may overlap what it reads or
  * writes otherwise (rows of two matrices of one stride may lie between each other). The
  * *_device calls allocate nothing: they take device memory of the caller's as
- * `workspace`, 256-byte aligned, of at least the bytes that the *_workspace calls give
+ * `workspace`, 256-byte aligned, of at least the bytes that the *_workspace calls give (0: none is needed)
  * for the same args (pointers in them are not followed, but alignment and which are null count), and
  * which belongs to the call until its stream has run it. Calls with workspaces of
  * their own are independent, captured or not. */

@@ -23,14 +23,18 @@ int64_t parts_of(int64_t n, int64_t of) { return (n + of - 1) / of; }
 
 // ---- tiles --------------------------------------------------------------------------
 
-enum Shape { kLarge, kMiddle, kSmall };
+enum Shape { kLarge, kWide, kMiddle, kFlat, kSmall };
 // waves, blocks of a wave, bytes of a step, stages
 template <class E, bool XT, bool YT>
-using Large = TileShape<E, 2, 4, 8, 4, 128, 2, XT, YT>;
+using Large = TileShape<E, 2, 4, 8, 4, 128, 2, XT, YT>;  // 256 classes x 256 rows
 template <class E, bool XT, bool YT>
-using Middle = TileShape<E, 2, 2, 4, 4, 128, 2, XT, YT>;
+using Wide = TileShape<E, 4, 2, 4, 4, 128, 3, XT, YT>;  // 256 x 128
 template <class E, bool XT, bool YT>
-using Small = TileShape<E, 4, 1, 2, 2, 128, 4, XT, YT>;
+using Middle = TileShape<E, 2, 2, 4, 4, 128, 2, XT, YT>;  // 128 x 128
+template <class E, bool XT, bool YT>
+using Flat = TileShape<E, 4, 1, 2, 4, 128, 3, XT, YT>;  // 128 x 64
+template <class E, bool XT, bool YT>
+using Small = TileShape<E, 4, 1, 2, 2, 128, 4, XT, YT>;  // 128 x 32
 
 struct Tiles {
   Shape shape;
@@ -39,37 +43,51 @@ struct Tiles {
 
 constexpr int kUnits = 256;  // compute units
 
-// The shape whose tiles take the least time together, and parts of k where there are too few
-// of them to keep every unit busy.
+// What a tile's step of 128 bytes of k takes, in us, with one block on a unit and with two, and what a tile
+// takes besides. All shapes are bound by the way from the L2 into LDS, 9 to 12 TB/s over the chip, so
+// the larger the tile the less a product takes, and the smaller the less is left over at the edges. Measured
+// (us): 515 x 1000 x 50021 fp16, logits and sums, Large 84 (588 tiles, 3 rounds), Wide 98 (980, 4), Middle 102
+// (1955, 4), Flat 116 (3519, 7), Small 176 (6647, 13); 64 x 1024 x 32768 Wide 20, Middle 22, Flat 15, Small 15;
+// 1 x 4096 x 131072 Wide 190, Middle 183, Flat 179, Small 176. 8-bit, 64 x 2048 x 65536 to fp32 Wide 45, Middle 44, Flat
+// 32, Small 52; 777 x 1000 x 10007 to fp16 Large 30, Wide 35, Middle 29, Flat 41, Small 64; 256 x 2048 x 32768 to bf16
+// Wide 36, Middle 37, Flat 64, Small 108.
+struct StepTime {
+  double one, two, besides;
+};
+constexpr StepTime kTimes[] = {{1.75, 0, 10}, {1.5, 0, 6}, {1.0, 1.6, 3}, {0.75, 1.04, 2}, {0.6, 0.85, 1.5}};
+constexpr StepTime kTimes8[] = {{2.1, 0, 11}, {1.9, 0, 6}, {1.3, 1.7, 3}, {1.5, 1.9, 2}, {1.2, 1.6, 1.5}};
+constexpr StepTime kTimes8Wide[] = {{0, 0, 0}, {2.5, 0, 6}, {1.9, 2.6, 3}, {1.5, 1.9, 2}, {1.2, 1.6, 1.5}};  // widened
+
+// The shape, and parts of k where the epilogue allows them (sums in fp32 that a second kernel ends), that
+// take the least time by these.
 Tiles choose(int64_t rows, int64_t cols, int64_t k_bytes, int pairs, bool f8, bool large, bool small, bool split) {
   Tiles best{};
   double least = 1e300;
-  for (const Shape s : {kLarge, kMiddle, kSmall}) {
-    if ((s == kSmall && !small) || (s == kLarge && !large)) continue;
+  for (const Shape s : {kLarge, kWide, kMiddle, kFlat, kSmall}) {
+    if ((s >= kFlat && !small) || (s == kLarge && !large)) continue;
     Tiles t{};
     t.shape = s;
-    t.bc = s == kLarge ? 256 : 128;
-    t.br = s == kLarge ? 256 : s == kMiddle ? 128 : 32;
+    t.bc = s <= kWide ? 256 : 128;
+    t.br = s == kLarge ? 256 : s <= kMiddle ? 128 : s == kFlat ? 64 : 32;
     t.r = static_cast<int32_t>(parts_of(rows, t.br));
     t.c = static_cast<int32_t>(parts_of(cols, t.bc));
-    const int64_t kb = 128;
-    t.steps = static_cast<int32_t>(parts_of(k_bytes, kb));
-    const int64_t steps = static_cast<int64_t>(t.steps) * pairs;
-    t.parts = 1;
-    const int64_t tiles = static_cast<int64_t>(t.r) * t.c;
-    if (split) {
-      const int64_t want = (s == kLarge ? 1 : 2) * kUnits;
-      int64_t p = std::max<int64_t>(1, std::min<int64_t>(want / tiles, steps * kb / 1024));
-      t.parts = static_cast<int32_t>(std::min<int64_t>(p, 64));
-    }
-    t.part_steps = static_cast<int32_t>(parts_of(steps, t.parts));
-    t.parts = static_cast<int32_t>(parts_of(steps, t.part_steps));
-    const double rate = s == kLarge ? 1.0 : s == kMiddle ? 0.75 : 0.3;
-    const double time = static_cast<double>(parts_of(tiles * t.parts, kUnits)) * t.bc * t.br *
-                        (t.part_steps * kb + 512) / rate;
-    if (time < least) {
-      least = time;
-      best = t;
+    t.steps = static_cast<int32_t>(parts_of(k_bytes, 128));
+    const int64_t steps = static_cast<int64_t>(t.steps) * pairs, tiles = static_cast<int64_t>(t.r) * t.c;
+    const StepTime &m = (!f8 ? kTimes : large ? kTimes8 : kTimes8Wide)[s];
+    for (int64_t parts = 1; parts <= 64 && parts <= steps; ++parts) {
+      if (parts > 1 && (!split || tiles * parts > 4 * kUnits || steps / parts < 4)) break;
+      const int64_t part_steps = parts_of(steps, parts), blocks = tiles * parts;
+      const bool two = m.two > 0 && blocks > kUnits;
+      double time = static_cast<double>(parts_of(blocks, two ? 2 * kUnits : kUnits)) *
+                    (static_cast<double>(part_steps) * (two ? m.two : m.one) + m.besides);
+      if (parts > 1)  // parts are written and read again, by one more kernel
+        time += 3 + static_cast<double>(parts) * static_cast<double>(rows) * static_cast<double>(cols) * 8 / 5e6;
+      if (time < least) {
+        least = time;
+        t.part_steps = static_cast<int32_t>(part_steps);
+        t.parts = static_cast<int32_t>(parts_of(steps, part_steps));
+        best = t;
+      }
     }
   }
   return best;
@@ -78,6 +96,7 @@ Tiles choose(int64_t rows, int64_t cols, int64_t k_bytes, int pairs, bool f8, bo
 template <class S, class Steps, class Epi, class StepArgs>
 struct TileLaunch {
   static int run(const TileArgs &a, const StepArgs &sa, const Epi &epi, int device, hipStream_t st) {
+    // more LDS than a kernel gets unasked, asked for once a device
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = 1ull << (device & 63);
     if (!(done.load(std::memory_order_relaxed) & bit)) {
@@ -123,8 +142,20 @@ template <class E, class Epi>
 int run_rows(const TileArgs &a, Shape s, const Epi &epi, int device, hipStream_t st) {
   switch (s) {
     case kLarge: return run_plain<Large<E, false, false>>(a, epi, device, st);
+    case kWide: return run_plain<Wide<E, false, false>>(a, epi, device, st);
     case kMiddle: return run_plain<Middle<E, false, false>>(a, epi, device, st);
+    case kFlat: return run_plain<Flat<E, false, false>>(a, epi, device, st);
     default: return run_plain<Small<E, false, false>>(a, epi, device, st);
+  }
+}
+
+// The gradients' products: d and the table, or both transposed.
+template <bool XT, class Epi>
+int run_grad(const TileArgs &a, Shape s, const Epi &epi, int device, hipStream_t st) {
+  switch (s) {
+    case kLarge: return run_plain<Large<F16, XT, true>>(a, epi, device, st);
+    case kWide: return run_plain<Wide<F16, XT, true>>(a, epi, device, st);
+    default: return run_plain<Middle<F16, XT, true>>(a, epi, device, st);
   }
 }
 
@@ -247,8 +278,8 @@ struct LossPlan {
   bool grad, sums, f32, scaled;      // scaled: operands in fp16 terms
   bool lay_x, lay_y, weighted;       // copies that are made
   int planes, pairs;
-  int64_t ld;                        // elements of a laid-out row
-  int64_t piece, ld_d;               // classes of a piece; elements of a row of d
+  int64_t k, ld;                     // elements of a laid-out row, and from row to row
+  int64_t piece, k_d, ld_d;          // classes of a piece; elements of a row of d, and from row to row
   Tiles t_sums, t_d, t_x, t_y;       // logits for sums, for d; d_features, d_table
   int64_t slab_ld;
   bool slabs_x, slabs_y;
@@ -278,7 +309,8 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   p.planes = p.f32 ? 2 : 1;
   p.pairs = p.f32 ? 3 : 1;
   p.narrow = a.dims <= kNarrow;
-  p.ld = !p.narrow ? up(a.dims, 64) : a.dims <= 32 ? 32 : a.dims <= 64 ? 64 : 128;
+  p.k = up(a.dims, 64);
+  p.ld = !p.narrow ? p.k : a.dims <= 32 ? 32 : a.dims <= 64 ? 64 : 128;
   // operands that lie well are read in place
   auto lies_well = [&](const void *ptr, int64_t stride, int64_t rows) {
     return size == 2 && aligned(ptr, 16) && (stride % 8 == 0 || rows <= 1) && a.dims % 8 == 0 &&
@@ -330,7 +362,7 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
     return p;
   }
   if (p.sums) {
-    p.t_sums = choose(n, v, p.ld * 2, p.pairs, false, true, true, false);
+    p.t_sums = choose(n, v, p.k * 2, p.pairs, false, true, true, false);
     p.at_sums = room(n * p.t_sums.c * 8);
     p.at_own = room(n * 4);
     if (p.grad && !a.stats) p.at_stats = room(n * 16);
@@ -343,12 +375,15 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
     else
       piece = up(parts_of(v, parts_of(v, piece)), 256);
     p.piece = piece;
-    p.ld_d = up(piece, 64);
-    p.t_d = choose(n, piece, p.ld * 2, p.pairs, false, true, true, false);
+    p.k_d = up(piece, 64);
+    // (an odd number of 128-byte lines from row to row: tiles that read rows of d side by side meet in fewer
+    // channels of the caches: 2048 x 768 x 32768 fp32's d_features 285 -> 264 us, 4096 x 2048 x 131072 bf16's 440 -> 430)
+    p.ld_d = p.k_d / 64 % 2 ? p.k_d : p.k_d + 64;
+    p.t_d = choose(n, piece, p.k * 2, p.pairs, false, true, true, false);
     p.at_d = room(n * p.ld_d * 2 * p.planes);
     p.slab_ld = up(a.dims, 4);
     if (a.d_features) {
-      p.t_x = choose(n, a.dims, p.ld_d * 2, p.pairs, false, true, false, true);
+      p.t_x = choose(n, a.dims, p.k_d * 2, p.pairs, false, true, false, true);
       p.slabs_x = p.t_x.parts > 1 || piece < v;
       if (p.slabs_x) p.at_slab_x = room(n * p.slab_ld * 4 * p.t_x.parts);
     }
@@ -526,7 +561,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
   // operands: rows of dims values
   const int64_t row_bytes = up(a.dims, 8) * 2;
   auto laid = [&](int64_t at, int64_t rows) {
-    return Operand{ws + at, p.ld * 2, rows * p.ld * 2, static_cast<int32_t>(rows), static_cast<int32_t>(p.ld * 2)};
+    return Operand{ws + at, p.ld * 2, rows * p.ld * 2, static_cast<int32_t>(rows), static_cast<int32_t>(p.k * 2)};
   };
   auto in_place = [&](const void *ptr, int64_t stride, int64_t rows) {
     return Operand{static_cast<const char *>(ptr), stride * size, 0, static_cast<int32_t>(rows),
@@ -557,16 +592,16 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
   const Operand w = laid(p.at_w, n);
   auto *d = reinterpret_cast<_Float16 *>(ws + p.at_d);
   const int64_t d_plane = n * p.ld_d;
-  const Operand dop{ws + p.at_d, p.ld_d * 2, d_plane * 2, static_cast<int32_t>(n), static_cast<int32_t>(p.ld_d * 2)};
+  const Operand dop{ws + p.at_d, p.ld_d * 2, d_plane * 2, static_cast<int32_t>(n), static_cast<int32_t>(p.k_d * 2)};
   const GradScale by_row{exps, row, inv_t, 1}, by_all{exps, row, inv_t, 0};
   for (int64_t first = 0; first < v; first += p.piece) {
     const int64_t count = std::min(p.piece, v - first);
     Operand yp = y;
     yp.base += first * y.ld;
     yp.rows = static_cast<int32_t>(count);
-    GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.ld_d), p.planes, d_plane, d};
-    // (columns up to d's row length, so that those past the piece become 0)
-    TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.ld_d), p.pairs);
+    GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.k_d), p.ld_d, p.planes, d_plane, d};
+    // (columns up to d's padded width, so that those past the piece become 0)
+    TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.k_d), p.pairs);
     int rc = run_rows<F16>(t, p.t_d.shape, g, device, st);
     if (rc != TMNN_OK) return rc;
     if (a.d_features) {
@@ -574,8 +609,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
                    p.slabs_x ? reinterpret_cast<float *>(ws + p.at_slab_x) : nullptr, static_cast<int32_t>(p.slab_ld),
                    first > 0};
       t = tile_args(dop, yp, n, a.dims, p.t_x, p.pairs);
-      rc = p.t_x.shape == kLarge ? run_plain<Large<F16, false, true>>(t, o, device, st)
-                                 : run_plain<Middle<F16, false, true>>(t, o, device, st);
+      rc = run_grad<false>(t, p.t_x.shape, o, device, st);
       if (rc != TMNN_OK) return rc;
     }
     if (a.d_table) {
@@ -585,8 +619,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
       Tiles ty = p.t_y;
       ty.r = static_cast<int32_t>(parts_of(count, ty.br));
       t = tile_args(dop, w, count, a.dims, ty, p.pairs);
-      rc = ty.shape == kLarge ? run_plain<Large<F16, true, true>>(t, o, device, st)
-                              : run_plain<Middle<F16, true, true>>(t, o, device, st);
+      rc = run_grad<true>(t, ty.shape, o, device, st);
       if (rc != TMNN_OK) return rc;
       if (p.slabs_y) {
         rc = run_reduce<T>(by_all, out, a.d_table_stride, o.slabs, p.slab_ld, ty.parts, count, a.dims, st);
@@ -732,7 +765,7 @@ LogitsPlan plan_logits(const tmnn_class_logits_f8_args &a) {
   if (p.lay_x) p.at_x = room(a.rows * p.ld);
   if (p.lay_y) p.at_y = room(a.classes * p.ld);
   if (p.t.parts > 1) p.at_slabs = room(a.rows * p.slab_ld * 4 * p.t.parts);
-  p.bytes = std::max<int64_t>(at, 256);
+  p.bytes = at;  // (0: most calls need none)
   return p;
 }
 
@@ -783,7 +816,9 @@ int run_logits(tmnn_logits *h, const tmnn_class_logits_f8_args &a, const LogitsP
         rc = run_f8<Large<F8, false, false>, false>(t, s, o, power, device, st);
         break;
       }
+    case kWide: rc = run_f8<Wide<F8, false, false>, wide>(t, s, o, power, device, st); break;
     case kMiddle: rc = run_f8<Middle<F8, false, false>, wide>(t, s, o, power, device, st); break;
+    case kFlat: rc = run_f8<Flat<F8, false, false>, true>(t, s, o, power, device, st); break;
     default: rc = run_f8<Small<F8, false, false>, true>(t, s, o, power, device, st); break;
   }
   if (rc != TMNN_OK || !slabs) return rc;
@@ -797,7 +832,7 @@ int run_logits(tmnn_logits *h, const tmnn_class_logits_f8_args &a, const LogitsP
 
 int logits_device(tmnn_logits *h, const tmnn_class_logits_f8_args &a, hipStream_t st) {
   const LogitsPlan p = plan_logits(a);
-  if (!a.workspace || !aligned(a.workspace, 256) || a.workspace_bytes < p.bytes)
+  if (p.bytes > 0 && (!a.workspace || !aligned(a.workspace, 256) || a.workspace_bytes < p.bytes))
     return fail(TMNN_ERR_INVALID_ARGUMENT, "class_logits_f8: the workspace must be 256-byte aligned and hold " +
                                                std::to_string(p.bytes) + " bytes");
   switch (a.dtype) {
@@ -821,7 +856,7 @@ int logits_host(tmnn_logits *h, tmnn_class_logits_f8_args u) {
   tmnn_class_logits_f8_args on_device = u;
   on_device.features = on_device.table = nullptr;
   u.workspace_bytes = plan_logits(on_device).bytes;
-  m.room(u.workspace, u.workspace_bytes);
+  if (u.workspace_bytes > 0) m.room(u.workspace, u.workspace_bytes);
   return on_host(h, m, [&] { return logits_device(h, u, h->ctx->stream); });
 }
 
@@ -914,7 +949,7 @@ int tmnn_class_loss_workspace(const tmnn_class_loss_args *args, int32_t backward
   *bytes = 0;
   const int rc = check_loss(args, backward != 0);
   if (rc != TMNN_OK) return rc;
-  *bytes = args->rows == 0 ? 256 : plan_loss(*args, backward != 0).bytes;
+  *bytes = args->rows == 0 ? 0 : plan_loss(*args, backward != 0).bytes;
   return TMNN_OK;
 }
 int tmnn_class_loss(tmnn_logits *h, const tmnn_class_loss_args *args) {
@@ -934,7 +969,7 @@ int tmnn_class_logits_f8_workspace(const tmnn_class_logits_f8_args *args, int64_
   *bytes = 0;
   const int rc = check_logits(args);
   if (rc != TMNN_OK) return rc;
-  *bytes = args->rows == 0 ? 256 : plan_logits(*args).bytes;
+  *bytes = args->rows == 0 ? 0 : plan_logits(*args).bytes;
   return TMNN_OK;
 }
 int tmnn_class_logits_f8(tmnn_logits *h, const tmnn_class_logits_f8_args *args) {

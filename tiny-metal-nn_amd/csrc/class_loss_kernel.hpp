@@ -342,10 +342,17 @@ __global__ __launch_bounds__(256) void class_join_kernel(JoinArgs a) {
   const int label = here ? a.row.label(r) : -1;
   float m = -3.4e38f, s = 0.f;
   if (here)
-    for (int t = lane; t < a.tiles; t += a.lanes) {
-      const float2 v = a.sums[r * a.tiles + t];
-      const float top = fmaxf(m, v.x);
-      s = s * __builtin_amdgcn_exp2f((m - top) * a.c) + v.y * __builtin_amdgcn_exp2f((v.x - top) * a.c);
+    for (int t = lane; t < a.tiles; t += 8 * a.lanes) {  // (eight loads on their way)
+      float2 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = t + u * a.lanes < a.tiles ? a.sums[r * a.tiles + t + u * a.lanes] : float2{-3.4e38f, 0.f};
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) top = fmaxf(top, v[u].x);
+      s *= __builtin_amdgcn_exp2f((m - top) * a.c);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u].y * __builtin_amdgcn_exp2f((v[u].x - top) * a.c);
       m = top;
     }
   for (int x = 1; x < a.lanes; x *= 2) {
@@ -377,7 +384,9 @@ struct GradEpilogue {
   float c;
   const float4 *stats;
   int32_t first;       // class of the piece's first column
-  int32_t ld, planes;
+  int32_t width;       // columns to write: those past the piece are 0
+  int64_t ld;
+  int32_t planes;
   int64_t plane;       // elements
   _Float16 *d;         // [plane][rows][ld]
 
@@ -400,7 +409,7 @@ struct GradEpilogue {
 #pragma unroll
       for (int i = 0; i < S::FC; ++i) {
         const int col = c0 + i * 16 + g4;
-        if (col >= ld) continue;
+        if (col >= width) continue;
         f16x4 high, low;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

@@ -61,12 +61,15 @@ class _HeadCalls:
             self._run(a, on_host, on_device, head + _NO_WORKSPACE, stream)
             return
         if workspace is None:
-            if isinstance(stream, int) and stream == -1:
-                raise ValueError("the context's own stream needs a workspace of the caller's")
             need = ctypes.c_int64()
             rc = size_of(head + _NO_WORKSPACE, ctypes.byref(need))
             if rc:
                 _lib.check(rc)
+            if need.value == 0:
+                self._run(a, on_host, on_device, head + _NO_WORKSPACE, stream)
+                return
+            if isinstance(stream, int) and stream == -1:
+                raise ValueError("the context's own stream needs a workspace of the caller's")
             workspace = a.empty((need.value,), a.torch.uint8)
         elif not a.ours(workspace) or a.name_of(workspace.dtype) != "uint8" or not workspace.is_contiguous():
             raise TypeError("workspace must be a contiguous uint8 tensor")
