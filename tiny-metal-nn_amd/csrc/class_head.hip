@@ -277,7 +277,8 @@ constexpr int64_t kPieceBytes = int64_t{256} << 20;
 struct LossPlan {
   bool grad, sums, f32, scaled;      // scaled: operands in fp16 terms
   bool lay_x, lay_y, weighted;       // copies that are made
-  int planes, pairs;
+  int planes, pairs;                 // terms of the operands, products of them
+  int planes_d, pairs_d;             // of d, and of the gradients' products
   int64_t k, ld;                     // elements of a laid-out row, and from row to row
   int64_t piece, k_d, ld_d;          // classes of a piece; elements of a row of d, and from row to row
   Tiles t_sums, t_d, t_x, t_y;       // logits for sums, for d; d_features, d_table
@@ -289,6 +290,10 @@ struct LossPlan {
   int64_t at_part_sum, at_part_own, at_part_out;
   int64_t at_exps, at_most, at_x, at_w, at_y, at_sums, at_own, at_stats, at_d, at_slab_x, at_slab_y, bytes;
 };
+
+// Rows up to which d of fp16 inputs goes in two terms (512 x 1000 x 50000, one term and two: d_features 66 and ~130
+// us, d_table 112 and ~180; few rows wait for memory).
+constexpr int64_t kFewRows = 128;
 
 // Dims up to which the walks of narrow_kernel.hpp take a call.
 constexpr int64_t kNarrow = 128;
@@ -308,6 +313,10 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   p.f32 = a.dtype == TMNN_DTYPE_F32;
   p.planes = p.f32 ? 2 : 1;
   p.pairs = p.f32 ? 3 : 1;
+  // fp16 gradients hold as many bits as d in one term: over many rows its rounding adds as much error as theirs
+  // (1.4 times it together), over few a row's largest d alone can add twice as much
+  p.planes_d = p.f32 || (a.dtype == TMNN_DTYPE_F16 && n <= kFewRows) ? 2 : 1;
+  p.pairs_d = p.f32 ? 3 : p.planes_d;
   p.narrow = a.dims <= kNarrow;
   p.k = up(a.dims, 64);
   p.ld = !p.narrow ? p.k : a.dims <= 32 ? 32 : a.dims <= 64 ? 64 : 128;
@@ -368,7 +377,7 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
     if (p.grad && !a.stats) p.at_stats = room(n * 16);
   }
   if (p.grad) {
-    int64_t piece = kPieceBytes / (std::max<int64_t>(n, 1) * 2 * p.planes) / 256 * 256;
+    int64_t piece = kPieceBytes / (std::max<int64_t>(n, 1) * 2 * p.planes_d) / 256 * 256;
     piece = std::max<int64_t>(piece, 256);
     if (piece >= v)
       piece = v;
@@ -380,15 +389,15 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
     // channels of the caches: 2048 x 768 x 32768 fp32's d_features 285 -> 264 us, 4096 x 2048 x 131072 bf16's 440 -> 430)
     p.ld_d = p.k_d / 64 % 2 ? p.k_d : p.k_d + 64;
     p.t_d = choose(n, piece, p.k * 2, p.pairs, false, true, true, false);
-    p.at_d = room(n * p.ld_d * 2 * p.planes);
+    p.at_d = room(n * p.ld_d * 2 * p.planes_d);
     p.slab_ld = up(a.dims, 4);
     if (a.d_features) {
-      p.t_x = choose(n, a.dims, p.k_d * 2, p.pairs, false, true, false, true);
+      p.t_x = choose(n, a.dims, p.k_d * 2, p.pairs_d, false, true, false, true);
       p.slabs_x = p.t_x.parts > 1 || piece < v;
       if (p.slabs_x) p.at_slab_x = room(n * p.slab_ld * 4 * p.t_x.parts);
     }
     if (a.d_table) {
-      p.t_y = choose(piece, a.dims, n * 2, p.pairs, false, true, false, true);
+      p.t_y = choose(piece, a.dims, n * 2, p.pairs_d, false, true, false, true);
       p.slabs_y = p.t_y.parts > 1;
       if (p.slabs_y) p.at_slab_y = room(piece * p.slab_ld * 4 * p.t_y.parts);
     }
@@ -418,16 +427,16 @@ int run_reduce(const GradScale &s, void *out, int64_t ld, const float *slabs, in
 typedef std::integral_constant<int, 1> One;
 typedef std::integral_constant<int, 2> Two;
 
-template <int DP, int PL, int RJ, class Op>
+template <int DP, int PL, int PD, int RJ, class Op>
 int run_walk(const WalkArgs &a, int32_t parts, const Op &op, int device, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
   const uint64_t bit = 1ull << (device & 63);
   if (!(done.load(std::memory_order_relaxed) & bit)) {
-    TMNN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(walk_kernel<DP, PL, RJ, Op>),
+    TMNN_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void *>(walk_kernel<DP, PL, PD, RJ, Op>),
                                      hipFuncAttributeMaxDynamicSharedMemorySize, WalkTile<DP, PL>::kLds));
     done.fetch_or(bit, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL((walk_kernel<DP, PL, RJ, Op>), dim3(static_cast<uint32_t>(static_cast<int64_t>(a.blocks) * parts)),
+  hipLaunchKernelGGL((walk_kernel<DP, PL, PD, RJ, Op>), dim3(static_cast<uint32_t>(static_cast<int64_t>(a.blocks) * parts)),
                      dim3(kWalkThreads), (WalkTile<DP, PL>::kLds), st, a, op);
   TMNN_HIP_TRY(hipGetLastError());
   return TMNN_OK;
@@ -437,7 +446,7 @@ int run_walk(const WalkArgs &a, int32_t parts, const Op &op, int device, hipStre
 template <class T, int DP>
 int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, const RowInfo &row, float c, float inv_t,
                const Exponents *exps, hipStream_t st) {
-  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
+  constexpr int PL = sizeof(T) == 4 ? 2 : 1, PD = __is_same(T, __bf16) ? 1 : 2;
   const int device = h->ctx->device;
   char *ws = static_cast<char *>(a.workspace);
   const int32_t n = static_cast<int32_t>(a.rows), v = static_cast<int32_t>(a.classes), dims = static_cast<int32_t>(a.dims);
@@ -467,7 +476,7 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
       op.out = out;
       op.out_ld = a.d_feature_stride;
       op.dims = dims;
-      return run_walk<DP, PL, decltype(rj)::value>(w, p.parts_r, op, device, st);
+      return run_walk<DP, PL, PD, decltype(rj)::value>(w, p.parts_r, op, device, st);
     };
     const One one;
     const Two two;
@@ -498,7 +507,7 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
     t.dims = dims;
     t.slabs = slabs;
     t.slab_ld = static_cast<int32_t>(p.slab_ld);
-    return run_walk<DP, PL, RJ>(w, p.parts_t, t, device, st);
+    return run_walk<DP, PL, PD, RJ>(w, p.parts_t, t, device, st);
   };
   const int rc = p.wide_t ? walk(Two{}) : walk(One{});
   if (rc != TMNN_OK || !slabs) return rc;
@@ -599,7 +608,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
     Operand yp = y;
     yp.base += first * y.ld;
     yp.rows = static_cast<int32_t>(count);
-    GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.k_d), p.ld_d, p.planes, d_plane, d};
+    GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.k_d), p.ld_d, p.planes_d, d_plane, d};
     // (columns up to d's padded width, so that those past the piece become 0)
     TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.k_d), p.pairs);
     int rc = run_rows<F16>(t, p.t_d.shape, g, device, st);
@@ -608,7 +617,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
       GradOut<T> o{by_row, static_cast<T *>(a.d_features), a.d_feature_stride,
                    p.slabs_x ? reinterpret_cast<float *>(ws + p.at_slab_x) : nullptr, static_cast<int32_t>(p.slab_ld),
                    first > 0};
-      t = tile_args(dop, yp, n, a.dims, p.t_x, p.pairs);
+      t = tile_args(dop, yp, n, a.dims, p.t_x, p.pairs_d);
       rc = run_grad<false>(t, p.t_x.shape, o, device, st);
       if (rc != TMNN_OK) return rc;
     }
@@ -618,7 +627,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
                    static_cast<int32_t>(p.slab_ld), 0};
       Tiles ty = p.t_y;
       ty.r = static_cast<int32_t>(parts_of(count, ty.br));
-      t = tile_args(dop, w, count, a.dims, ty, p.pairs);
+      t = tile_args(dop, w, count, a.dims, ty, p.pairs_d);
       rc = run_grad<true>(t, ty.shape, o, device, st);
       if (rc != TMNN_OK) return rc;
       if (p.slabs_y) {

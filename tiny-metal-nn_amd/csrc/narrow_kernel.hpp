@@ -99,9 +99,10 @@ __device__ __forceinline__ void ahead() {
   }
 }
 
+// PL, PD: terms of the operands and of d (d of fp16 gradients, which hold as many bits as one term, goes in two).
 // RJ: 16 items x of a wave, or 32. 32 halve the reads from LDS; with 16 a call has twice the blocks, of
 // half the registers, so that some multiply while others take exponentials.
-template <int DP, int PL, int RJ, class Op>
+template <int DP, int PL, int PD, int RJ, class Op>
 __global__ __launch_bounds__(kWalkThreads, RJ == 1 ? (DP <= 64 ? 4 : 3) : DP <= 64 ? 3 : 2) void walk_kernel(WalkArgs a, Op op) {
   typedef WalkTile<DP, PL> W;
   constexpr int KS = DP / 32, FD = DP / 16;
@@ -202,11 +203,11 @@ __global__ __launch_bounds__(kWalkThreads, RJ == 1 ? (DP <= 64 ? 4 : 3) : DP <= 
     ahead<KS * 4, PL, (PL == 2 ? 3 : 1) * RJ>();
     op.template transform<decltype(edge)::value>(z, out, info, tile * kWalkItems, a.ny, lane);
     if constexpr (Op::kGradient) {
-      f16x8 dx[2][RJ][PL];
+      f16x8 dx[2][RJ][PD];
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int j = 0; j < RJ; ++j) to_terms<PL>(z[2 * kk][j], z[2 * kk + 1][j], dx[kk][j]);
+        for (int j = 0; j < RJ; ++j) to_terms<PD>(z[2 * kk][j], z[2 * kk + 1][j], dx[kk][j]);
       __builtin_amdgcn_sched_barrier(0);
       auto read_t = [&](f16x8 (&ft)[PL], int s) {
         const int kk = s / FD, f = s % FD, t = lane % 16;
@@ -234,12 +235,12 @@ __global__ __launch_bounds__(kWalkThreads, RJ == 1 ? (DP <= 64 ? 4 : 3) : DP <= 
         const int kk = s / FD, f = s % FD;
         if (s + 1 < 2 * FD) read_t(ft[(s + 1) % 2], s + 1);
 #pragma unroll
-        for (int t = 0; t < (PL == 2 ? 3 : 1); ++t)
+        for (int t = 0; t < PL + PD - 1; ++t)  // high and high, y low, d low
 #pragma unroll
           for (int j = 0; j < RJ; ++j)
-            out[f][j] = Fragment<F16>::mul(ft[s % 2][t == 1], dx[kk][j][t == 2], out[f][j]);
+            out[f][j] = Fragment<F16>::mul(ft[s % 2][PL == 2 && t == 1], dx[kk][j][t > 0 && t == PL + PD - 2], out[f][j]);
       }
-      ahead<2 * FD, 2 * PL, (PL == 2 ? 3 : 1) * RJ>();
+      ahead<2 * FD, 2 * PL, (PL + PD - 1) * RJ>();
     }
     stage ^= 1;
   };

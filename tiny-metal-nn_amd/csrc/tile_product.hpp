@@ -45,7 +45,7 @@ struct TileArgs {
   int32_t rows, cols;          // of the output
   int32_t tiles_r, tiles_c, parts;
   int32_t steps;               // of k, in one pair of planes
-  int32_t pairs;               // 1: one plane each; 3: high x high, high x low, low x high
+  int32_t pairs;               // 1: one plane each; 2: and x low; 3: x high, y low first, x low then
   int32_t part_steps;          // steps of one part, counted over all pairs
 };
 
@@ -312,8 +312,8 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
   ly.begin(a.y, first_c, wave, lane);
   lx.begin(a.x, first_r, wave, lane);
   auto seek = [&] {
-    ly.seek(a.y, first_c, pair == 1, st);
-    lx.seek(a.x, first_r, pair == 2, st);
+    ly.seek(a.y, first_c, a.pairs == 3 && pair == 1, st);
+    lx.seek(a.x, first_r, pair > 0 && pair == a.pairs - 1, st);
   };
   seek();
   // Loads the next step into a stage (zeros, without touching memory, after the last one), with
