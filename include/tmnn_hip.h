@@ -806,6 +806,7 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
  * for the same args (pointers in them are not followed, but alignment and which are null count), and
  * which belongs to the call until its stream has run it. Calls with workspaces of
  * their own are independent, captured or not. */
+/* Largest `rows` and `dims`; rows x classes is at most 2^38. */
 #define TMNN_HEAD_MAX_ROWS (1 << 24)
 #define TMNN_HEAD_MAX_DIMS (1 << 16)
 

@@ -202,7 +202,8 @@ int check_sizes(const char *what, int64_t rows, int64_t classes, int64_t dims) {
   if (rows < 0 || rows > TMNN_HEAD_MAX_ROWS) return bad("rows must be in [0, 2^24]");
   if (classes < 1 || classes > TMNN_LOGITS_MAX_CLASSES) return bad("classes must be in [1, 2^24]");
   if (dims < 1 || dims > TMNN_HEAD_MAX_DIMS) return bad("dims must be in [1, 2^16]");
-  if (rows * classes > int64_t{1} << 40) return bad("rows x classes must be at most 2^40");  // (tiles are counted in 32 bits)
+  // (the threads of a launch are counted in 32 bits)
+  if (rows * classes > int64_t{1} << 38) return bad("rows x classes must be at most 2^38");
   return TMNN_OK;
 }
 
@@ -237,8 +238,8 @@ int check_loss_arrays(const tmnn_class_loss_args *a, bool back, bool host) {
     return fail(TMNN_ERR_INVALID_ARGUMENT, std::string(what) + ": " + m);
   };
   const int64_t size = static_cast<int64_t>(dtype_size(a->dtype));
-  if (back && !a->d_features && !a->d_table) return bad("nothing to compute");
-  if (!back && !a->loss && !a->stats && !a->d_features && !a->d_table) return bad("nothing to compute");
+  if (a->rows > 0 && !a->d_features && !a->d_table && (back || (!a->loss && !a->stats)))
+    return bad("nothing to compute");
   if (!a->table) return bad("table is null");
   if (a->rows > 0) {
     if (!a->features) return bad("features is null");
@@ -484,8 +485,7 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
                             : (out ? walk(one, RowsWalk<T, true, 1>{}) : walk(one, RowsWalk<T, false, 1>{}));
     if (rc != TMNN_OK) return rc;
     if (p.parts_r > 1) {
-      hipLaunchKernelGGL((walk_join_kernel<T, DP>), dim3(static_cast<uint32_t>(parts_of(n, 256 / (DP / 4)))), dim3(256), 0,
-                         st, g, n, p.parts_r, table, a.table_stride, out, a.d_feature_stride, dims);
+      hipLaunchKernelGGL((walk_join_kernel<T, DP>), dim3(static_cast<uint32_t>(n)), dim3(256), 0, st, g, n, p.parts_r, table, a.table_stride, out, a.d_feature_stride, dims);
       TMNN_HIP_TRY(hipGetLastError());
     }
   }
@@ -540,7 +540,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
     const int32_t dims = static_cast<int32_t>(a.dims), ld = static_cast<int32_t>(p.ld);
     l.part[0] = {a.features, a.feature_stride, static_cast<int32_t>(n), dims, p.lay_x ? ws + p.at_x : nullptr,
                  p.weighted ? ws + p.at_w : nullptr, ld, !keep, planes,
-                 p.lay_x || p.weighted ? blocks(n) : 0, !keep || p.weighted ? scale_parts(n) : 0};
+                 p.lay_x || p.weighted ? blocks(n) : 0, !keep || (p.weighted && !p.narrow) ? scale_parts(n) : 0};
     l.part[1] = {a.table, a.table_stride, static_cast<int32_t>(v), dims, p.lay_y ? ws + p.at_y : nullptr, nullptr,
                  ld, !keep, planes, p.lay_y ? blocks(v) : 0, !keep ? scale_parts(v) : 0};
     l.row = row;
@@ -911,7 +911,7 @@ int run_quantize(const tmnn_quantize_f8_args &u, hipStream_t st) {
                  static_cast<int32_t>(parts_of(u.dims, kScaleBlock)), static_cast<uint8_t *>(u.values), u.value_stride,
                  u.scales};
   if (u.block_rows == 1) {
-    const int64_t blocks = parts_of(u.rows * a.blocks, 16);
+    const int64_t blocks = std::min<int64_t>(parts_of(u.rows * a.blocks, 16), 1 << 20);
     hipLaunchKernelGGL((f8_rows_kernel<T, POWER>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st, a);
   } else {
     const int64_t blocks = parts_of(u.rows, kScaleBlock) * a.blocks;
@@ -954,12 +954,13 @@ int quantize(tmnn_logits *h, const tmnn_quantize_f8_args *args, bool host, void 
 extern "C" {
 
 int tmnn_class_loss_workspace(const tmnn_class_loss_args *args, int32_t backward, int64_t *bytes) {
-  if (!bytes) return fail(TMNN_ERR_INVALID_ARGUMENT, "bytes is null");
-  *bytes = 0;
-  const int rc = check_loss(args, backward != 0);
-  if (rc != TMNN_OK) return rc;
-  *bytes = args->rows == 0 ? 0 : plan_loss(*args, backward != 0).bytes;
-  return TMNN_OK;
+  return guarded([&] {
+    if (!bytes) return fail(TMNN_ERR_INVALID_ARGUMENT, "bytes is null");
+    *bytes = 0;
+    const int rc = check_loss(args, backward != 0);
+    if (rc == TMNN_OK && args->rows > 0) *bytes = plan_loss(*args, backward != 0).bytes;
+    return rc;
+  });
 }
 int tmnn_class_loss(tmnn_logits *h, const tmnn_class_loss_args *args) {
   return class_loss(h, args, false, true, nullptr);
@@ -974,12 +975,13 @@ int tmnn_class_loss_backward_device(tmnn_logits *h, const tmnn_class_loss_args *
   return class_loss(h, args, true, false, stream);
 }
 int tmnn_class_logits_f8_workspace(const tmnn_class_logits_f8_args *args, int64_t *bytes) {
-  if (!bytes) return fail(TMNN_ERR_INVALID_ARGUMENT, "bytes is null");
-  *bytes = 0;
-  const int rc = check_logits(args);
-  if (rc != TMNN_OK) return rc;
-  *bytes = args->rows == 0 ? 0 : plan_logits(*args).bytes;
-  return TMNN_OK;
+  return guarded([&] {
+    if (!bytes) return fail(TMNN_ERR_INVALID_ARGUMENT, "bytes is null");
+    *bytes = 0;
+    const int rc = check_logits(args);
+    if (rc == TMNN_OK && args->rows > 0) *bytes = plan_logits(*args).bytes;
+    return rc;
+  });
 }
 int tmnn_class_logits_f8(tmnn_logits *h, const tmnn_class_logits_f8_args *args) {
   return class_logits(h, args, true, nullptr);

@@ -350,19 +350,20 @@ __device__ __forceinline__ void f8_put_scale(void *scales, int64_t at, float s) 
 template <class T, bool POWER>
 __global__ __launch_bounds__(256) void f8_rows_kernel(QuantizeArgs a) {
   const int64_t n = static_cast<int64_t>(a.rows) * a.blocks;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
   const int lane = threadIdx.x % 16;
-  if (at >= n) return;  // (16 lanes together)
-  const int64_t r = at / a.blocks;
-  const int b = static_cast<int>(at - r * a.blocks), c = b * kScaleBlock + lane * 8;
-  float v[8];
-  f8_load8(static_cast<const T *>(a.in) + r * a.stride, c, a.dims, v);
-  float m = f8_most(v);
+  // (16 lanes together)
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16; at < n; at += 16ll * gridDim.x) {
+    const int64_t r = at / a.blocks;
+    const int b = static_cast<int>(at - r * a.blocks), c = b * kScaleBlock + lane * 8;
+    float v[8];
+    f8_load8(static_cast<const T *>(a.in) + r * a.stride, c, a.dims, v);
+    float m = f8_most(v);
 #pragma unroll
-  for (int x = 1; x < 16; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 16));
-  const float s = f8_scale<POWER>(m);
-  f8_store8<POWER>(a.out + r * a.ld, c, a.dims, v, s, 1.f / s);
-  if (lane == 0) f8_put_scale<POWER>(a.scales, at, s);
+    for (int x = 1; x < 16; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 16));
+    const float s = f8_scale<POWER>(m);
+    f8_store8<POWER>(a.out + r * a.ld, c, a.dims, v, s, 1.f / s);
+    if (lane == 0) f8_put_scale<POWER>(a.scales, at, s);
+  }
 }
 
 template <class T, bool POWER>

@@ -119,8 +119,7 @@ int on_host(tmnn_logits *h, HostArrays &arrays, Run run) {
 
 // No exception leaves a C entry point.
 template <class F>
-int entry(tmnn_logits *h, F f) {
-  if (!h) return fail(TMNN_ERR_INVALID_ARGUMENT, "logits handle is null");
+int guarded(F f) {
   try {
     return f();
   } catch (const std::bad_alloc &) {
@@ -128,6 +127,10 @@ int entry(tmnn_logits *h, F f) {
   } catch (const std::exception &e) {
     return fail(TMNN_ERR_RUNTIME, e.what());
   }
+}
+template <class F>
+int entry(tmnn_logits *h, F f) {
+  return guarded([&] { return h ? f() : fail(TMNN_ERR_INVALID_ARGUMENT, "logits handle is null"); });
 }
 
 }  // namespace tmnn_hip

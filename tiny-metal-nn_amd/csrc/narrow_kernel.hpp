@@ -356,7 +356,7 @@ struct RowsWalk : RowsShared {
   __device__ __forceinline__ void transform(f32x4t (&z)[4][RJ], f32x4t (&o)[FD][RJ], const char *, int first, int ny,
                                             int lane) {
     // (m and z of the products as they are, scaled; probabilities times 2^14)
-    const float k = held.inv * c;
+    const float k = fminf(held.inv * c, 3e38f);
 #pragma unroll
     for (int j = 0; j < RJ; ++j) {
       float top = held.m[j];
@@ -441,41 +441,56 @@ struct RowsWalk : RowsShared {
   }
 };
 
-// Joins the parts of rows: DP / 4 threads a row.
+// Joins the parts of a row, a block a row: its threads take parts side by side (one after another, 340 parts of
+// three rows took 47 us), four dims a thread.
 template <class T, int DP>
 __global__ __launch_bounds__(256) void walk_join_kernel(RowsShared g, int32_t rows, int32_t parts, const T *table,
                                                        int64_t table_ld, T *out, int64_t out_ld, int32_t dims) {
-  constexpr int lanes = DP / 4;
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
-  const int at = threadIdx.x % lanes;
-  if (r >= rows) return;  // (a row's threads together)
-  // the maximum first, each thread over a share of the parts
+  constexpr int lanes = DP / 4, slices = 256 / lanes;
+  __shared__ float room[8];
+  __shared__ f32x4t shares[slices][lanes];
+  const int64_t r = blockIdx.x;
+  const int at = threadIdx.x % lanes, slice = threadIdx.x / lanes;
   float m = kLowest;
-  for (int p = at; p < parts; p += lanes) m = fmaxf(m, g.part_sum[static_cast<int64_t>(p) * rows + r].x);
+  for (int p = threadIdx.x; p < parts; p += 256) m = fmaxf(m, g.part_sum[p * static_cast<int64_t>(rows) + r].x);
 #pragma unroll
-  for (int x = 1; x < lanes; x *= 2) m = fmaxf(m, __shfl_xor(m, x, lanes));
+  for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
+  if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(room[0], room[1]), fmaxf(room[2], room[3]));
   float s = 0.f;
-  const float z = g.own[r];
-  f32x4t sum{0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p) {
-    const float2 v = g.part_sum[static_cast<int64_t>(p) * rows + r];
-    const float f = __builtin_amdgcn_exp2f((v.x - m) * g.c);
-    s += v.y * f;
-    if (out) {
-      const f32x4t o = *reinterpret_cast<const f32x4t *>(g.part_out + (static_cast<int64_t>(p) * rows + r) * DP + at * 4);
-      sum += o * f;
-    }
+  for (int p = threadIdx.x; p < parts; p += 256) {
+    const float2 v = g.part_sum[p * static_cast<int64_t>(rows) + r];
+    s += v.y * __builtin_amdgcn_exp2f((v.x - m) * g.c);
   }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) s += __shfl_xor(s, x);
+  if (threadIdx.x % 64 == 0) room[4 + threadIdx.x / 64] = s;
+  if (out) {
+    f32x4t sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = slice; p < parts; p += slices) {
+      const int64_t row = p * static_cast<int64_t>(rows) + r;
+      const float f = __builtin_amdgcn_exp2f((g.part_sum[row].x - m) * g.c);
+      sum += *reinterpret_cast<const f32x4t *>(g.part_out + row * DP + at * 4) * f;
+    }
+    shares[slice][at] = sum;
+  }
+  __syncthreads();
+  if (slice != 0) return;
+  s = (room[4] + room[5]) + (room[6] + room[7]);
   const int label = g.row.label(r);
   const float w = g.row.weight(r);
-  const RowEnd e = end_row(m, s, z, label, g.row.classes, w, g.c, g.inv_t);
+  const RowEnd e = end_row(m, s, g.own[r], label, g.row.classes, w, g.c, g.inv_t);
   if (at == 0) {
     if (g.loss) g.loss[r] = e.loss;
     if (g.stats) g.stats[r] = float4{e.big, e.total, e.missing, 0.f};
   }
-  if (out)
-    put_features<T>(g, e, w, label, static_cast<int>(r), at * 4, sum,
-                    ldexpf(1.f, -kDTerm - (g.exps ? g.exps->y : 0)), table, table_ld, out, out_ld, dims);
+  if (!out) return;
+  f32x4t sum = shares[0][at];
+  for (int k = 1; k < slices; ++k) sum += shares[k][at];
+  put_features<T>(g, e, w, label, static_cast<int>(r), at * 4, sum, ldexpf(1.f, -kDTerm - (g.exps ? g.exps->y : 0)),
+                  table, table_ld, out, out_ld, dims);
 }
 
 // The walk over the rows: classes are the items x. d is held times 2^14 T w / 2^top, top being the
@@ -500,7 +515,7 @@ struct TableWalk {
   __device__ __forceinline__ void begin(int r0, int, int) {
     c0 = r0;
     raw = 1.f / logit_scale(exps);
-    inv = logit_scale(exps) * c;
+    inv = fminf(logit_scale(exps) * c, 3e38f);
     top = exps ? exps->w : 0;
   }
   // Of each row of a tile: m, what its probabilities are multiplied with (0: the row does not count), the
