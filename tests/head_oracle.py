@@ -20,12 +20,14 @@ def class_loss(features, table, labels, weights=None, t=1.0):
     row = torch.arange(n, device=h.device)
     at = labels.clamp(0, v - 1)
     up = torch.where(used, weights, 0.0)
-    loss = torch.where(used, -logp[row, at], 0.0) * up
     p = logp.exp()
     d = p * (up / t).unsqueeze(1)
     # 1 - p of the label from the other classes
     others = torch.logsumexp(logp.scatter(1, at.unsqueeze(1), float("-inf")), 1).exp()
     d[row, at] = -others * up / t
+    # -ln p, small ones from 1 - p too
+    loss = torch.where(others < 0.5, -torch.log1p(-others), -logp[row, at])
+    loss = torch.where(used, loss, 0.0) * up
     return {"loss": loss, "m": z.amax(1) * t, "missing": others, "d_features": d @ w, "d_table": d.t() @ h,
             "z": (h.abs() @ w.abs().t()).amax(1) if n else loss, "x": d.abs() @ w.abs(), "y": d.abs().t() @ h.abs(),
             "d": d}

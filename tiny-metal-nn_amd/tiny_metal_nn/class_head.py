@@ -24,6 +24,7 @@ _SIZE_LOSS, _SIZE_LOGITS = _PACK_LOSS.size + _PACK_WORKSPACE.size, _PACK_LOGITS.
 _NO_WORKSPACE = _PACK_WORKSPACE.pack(0, 0)
 _GRADIENTS = {"both": (True, True), "features": (True, False), "table": (False, True), "none": (False, False)}
 _BLOCK = 128
+_FLOATS = "float32, float16 or bfloat16"
 
 
 def _matrix(a, x, name: str, codes: dict, want: str, dims: int | None = None) -> tuple[int, int, int, int, int]:
@@ -77,18 +78,17 @@ class _HeadCalls:
             a.place(workspace, "workspace")
         self._run(a, on_host, on_device, head + _PACK_WORKSPACE.pack(workspace.data_ptr(), workspace.numel()), stream)
 
-    def _loss_call(self, a, features, table, labels, temperature, weights, gradient, out, loss, stats, back):
-        """(packed args without the workspace, arrays written)."""
+    def _loss_call(self, a, x, table, labels, temperature, weights, gradient, out, loss, stats, back):
+        """(packed args without the workspace, arrays written), for the features and their `x` of _matrix."""
         wanted = _GRADIENTS.get(gradient)
         if wanted is None or (back and gradient == "none"):
             names = "'both', 'features' or 'table'" + ("" if back else " or 'none'")
             raise ValueError(f"gradient must be {names}, got {gradient!r}")
-        want = "float32, float16 or bfloat16"
-        x, x_row, n, d, code = _matrix(a, features, "features", a.float_codes, want)
+        features, (x, x_row, n, d, code) = x
         if a.ours(table) and table.dtype != features.dtype:
             raise DTypeError(f"table must be {a.name_of(features.dtype)} as the features, "
                              f"got {a.name_of(table.dtype)}")
-        y, y_row, v, _, _ = _matrix(a, table, "table", a.float_codes, want, d)
+        y, y_row, v, _, _ = _matrix(a, table, "table", a.float_codes, _FLOATS, d)
         at_labels, index = a.ids(labels, "labels", (n,))
         wrote = [] if back else [out["loss"], out["stats"]]
         grads = [(0, d), (0, d)]
@@ -118,11 +118,12 @@ class _HeadCalls:
         a = self._arrays(features, stream)
         if out is None:
             out = {}
-        rows = (features.shape[0],) if len(features.shape) else (0,)
+        x = _matrix(a, features, "features", a.float_codes, _FLOATS)
+        rows = (x[2],)
         loss = a.output(out, "loss", rows, a.f32)
         stats = a.output(out, "stats", rows + (4,), a.f32)
         weights = 0 if row_weights is None else a.array(row_weights, "row_weights", rows, a.f32)
-        head, wrote = self._loss_call(a, features, table, labels, temperature, weights, gradient, out, loss, stats,
+        head, wrote = self._loss_call(a, (features, x), table, labels, temperature, weights, gradient, out, loss, stats,
                                       False)
         lib = self._lib
         self._enqueue(a, lambda args, n: lib.tmnn_class_loss_workspace(args, 0, n), lib.tmnn_class_loss,
@@ -138,10 +139,11 @@ class _HeadCalls:
         a = self._arrays(features, stream)
         if out is None:
             out = {}
-        rows = (features.shape[0],) if len(features.shape) else (0,)
+        x = _matrix(a, features, "features", a.float_codes, _FLOATS)
+        rows = (x[2],)
         at_stats = a.array(stats, "stats", rows + (4,), a.f32)
         weights = a.array(d_loss, "d_loss", rows, a.f32)
-        head, wrote = self._loss_call(a, features, table, labels, temperature, weights, gradient, out, 0, at_stats,
+        head, wrote = self._loss_call(a, (features, x), table, labels, temperature, weights, gradient, out, 0, at_stats,
                                       True)
         lib = self._lib
         self._enqueue(a, lambda args, n: lib.tmnn_class_loss_workspace(args, 1, n), lib.tmnn_class_loss_backward,
@@ -191,7 +193,7 @@ class _HeadCalls:
         start at multiples of 16 bytes. `out`: arrays to write to, by these names; it gets
         those that it lacks, and is returned."""
         a = self._arrays(x, stream)
-        at, row, n, d, code = _matrix(a, x, "x", a.float_codes, "float32, float16 or bfloat16")
+        at, row, n, d, code = _matrix(a, x, "x", a.float_codes, _FLOATS)
         if block_rows not in (1, _BLOCK):
             raise ValueError(f"block_rows must be 1 or {_BLOCK}, got {block_rows}")
         scale = _lib.SCALE_DTYPES.get(a.dtype_name(scale_dtype))
