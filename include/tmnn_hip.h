@@ -818,8 +818,9 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
  * whatever they hold (their stats are computed). A label >= classes makes its loss and gradients NaN, as
  * logits that are not finite do. The backward call takes the stats of a call with the same features, table,
  * labels and temperature, and the loss's gradient as row_weights; it writes the gradients. All
- * sums in fp32; gradients are rounded once at the end. Products of gradients take operands
- * of 11 bits (16-bit inputs) or 22 bits (fp32), relative to the largest of a tensor below 2^-24 of it. */
+ * sums in fp32; gradients are rounded once at the end. Products of gradients take the inputs as they are
+ * (16 bits; bf16 below 2^-32 of a tensor's largest loses bits) or with 22 bits (fp32, of values from 2^-16 of a
+ * tensor's largest on), and d loss / d z with 11 bits (bf16, and fp16 of many rows) or 22. */
 typedef struct tmnn_class_loss_args {
   uint32_t struct_size;       /* sizeof(tmnn_class_loss_args) */
   int32_t dtype;              /* TMNN_DTYPE_* of features, table and their gradients */
@@ -857,7 +858,8 @@ int tmnn_class_loss_backward_device(tmnn_logits *h, const tmnn_class_loss_args *
 
 /* logits[row][class] = sum_k x w, where x = features[row][k] feature_scales[row][k / 128] and
  * w = table[class][k] table_scales[class / 128][k / 128]; values are e4m3 (OCP; no
- * infinities), sums fp32, rounded once to the logits' type. A NaN among values or scales makes
+ * infinities), sums fp32, rounded once to the logits' type. On the way to 16-bit logits the matrix
+ * instructions may cut each product to 2^-13 of the largest of the eight that they add. A NaN among values or scales makes
  * the logits that it enters NaN. */
 typedef struct tmnn_class_logits_f8_args {
   uint32_t struct_size;       /* sizeof(tmnn_class_logits_f8_args) */

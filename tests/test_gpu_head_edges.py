@@ -416,3 +416,17 @@ def test_outputs_are_marked_as_changed(ops):
     before = {name: t._version for name, t in q.items()}
     ops.quantize_f8(w, block_rows=128, out=q)
     assert all(t._version > before[name] for name, t in q.items())
+
+
+# many rows of few classes: the table's gradient comes in hundreds of parts; few rows of wide features in a
+# few; many classes of many rows go 32 a wave
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n, d, v", [(60001, 16, 5), (30000, 40, 70), (9, 136, 3), (2000, 200, 3), (600, 8, 131200)])
+def test_parts_of_few_sums(ops, n, d, v, dtype):
+    h, w, labels, weights = inputs(n, d, v, 5)
+    h, w = matrix(h, dtype), matrix(w, dtype)
+    got = ops.class_loss(h, w, labels, row_weights=weights)
+    check_all(got, ref.class_loss(h, w, labels, weights), h, w, weights, dtype, 1.0)
+    again = ops.class_loss(h, w, labels, row_weights=weights)
+    for name in NAMES:  # sums are added in one order
+        assert torch.equal(got[name], again[name])

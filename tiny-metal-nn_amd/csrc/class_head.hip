@@ -24,17 +24,17 @@ int64_t parts_of(int64_t n, int64_t of) { return (n + of - 1) / of; }
 // ---- tiles --------------------------------------------------------------------------
 
 enum Shape { kLarge, kWide, kMiddle, kFlat, kSmall };
-// waves, blocks of a wave, bytes of a step, stages
+// waves, blocks of a wave, stages
 template <class E, bool XT, bool YT>
-using Large = TileShape<E, 2, 4, 8, 4, 128, 2, XT, YT>;  // 256 classes x 256 rows
+using Large = TileShape<E, 2, 4, 8, 4, 2, XT, YT>;  // 256 classes x 256 rows
 template <class E, bool XT, bool YT>
-using Wide = TileShape<E, 4, 2, 4, 4, 128, 3, XT, YT>;  // 256 x 128
+using Wide = TileShape<E, 4, 2, 4, 4, 3, XT, YT>;  // 256 x 128
 template <class E, bool XT, bool YT>
-using Middle = TileShape<E, 2, 2, 4, 4, 128, 2, XT, YT>;  // 128 x 128
+using Middle = TileShape<E, 2, 2, 4, 4, 2, XT, YT>;  // 128 x 128
 template <class E, bool XT, bool YT>
-using Flat = TileShape<E, 4, 1, 2, 4, 128, 3, XT, YT>;  // 128 x 64
+using Flat = TileShape<E, 4, 1, 2, 4, 3, XT, YT>;  // 128 x 64
 template <class E, bool XT, bool YT>
-using Small = TileShape<E, 4, 1, 2, 2, 128, 4, XT, YT>;  // 128 x 32
+using Small = TileShape<E, 4, 1, 2, 2, 4, XT, YT>;  // 128 x 32
 
 struct Tiles {
   Shape shape;
@@ -271,7 +271,8 @@ int check_loss_arrays(const tmnn_class_loss_args *a, bool back, bool host) {
 // ---- class loss ---------------------------------------------------------------------------
 
 // Bytes of the piece's d up to which more classes go into one piece: larger pieces mean fewer
-// launches and fewer passes over the sums of d_features.
+// launches and fewer passes over the sums of d_features (4096 x 2048 x 131072 bf16: 8.16 ms with 64 MiB, 7.86 with
+// 256, 7.82 with 1 GiB).
 constexpr int64_t kPieceBytes = int64_t{256} << 20;
 
 // What a call lays out, in which tiles it goes, and where in the workspace things are.
@@ -286,17 +287,19 @@ struct LossPlan {
   int64_t slab_ld;
   bool slabs_x, slabs_y;
   // features of up to 128 dims: parts of the walks
-  bool narrow, wide_r, wide_t;
+  bool narrow, wide_t;
   int32_t blocks_r, tiles_r, parts_r, blocks_t, tiles_t, parts_t;
   int64_t at_part_sum, at_part_own, at_part_out;
   int64_t at_exps, at_most, at_x, at_w, at_y, at_sums, at_own, at_stats, at_d, at_slab_x, at_slab_y, bytes;
 };
 
-// Rows up to which d of fp16 inputs goes in two terms (512 x 1000 x 50000, one term and two: d_features 66 and ~130
-// us, d_table 112 and ~180; few rows wait for memory).
+// Rows up to which d of fp16 inputs goes in two terms. (rows x 1000 x 50000, a call with one term and with two, us:
+// 64 rows 166 and 190, 128 rows 182 and 219, 256 rows 225 and 299, 512 rows 358 and 476: few rows wait for memory.)
 constexpr int64_t kFewRows = 128;
 
-// Dims up to which the walks of narrow_kernel.hpp take a call.
+// Dims up to which the walks of narrow_kernel.hpp take a call. (By them and by products of tiles, with both gradients:
+// 65536 x 128 x 1000 bf16 172 and 275 us, 4096 x 128 x 131072 bf16 755 and 1838, fp32 1522 and 3148, 64 x 128 x
+// 131072 bf16 77 and 128. Beyond 128 dims a wave's accumulators do not fit.)
 constexpr int64_t kNarrow = 128;
 
 // Parts of a walk's tiles, where the items of one side alone make too few blocks: four blocks a unit, and
@@ -346,11 +349,10 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
   if (p.weighted) p.at_w = room(x_bytes);
   if (p.lay_y) p.at_y = room(v * p.ld * 2 * p.planes);
   if (p.narrow) {
-    // 32 items a wave where that still makes four blocks a unit
-    auto wide = [](int64_t items) { return items >= 4 * kUnits * kWalkWaves * 32; };
-    auto blocks = [](int64_t items, bool w) { return static_cast<int32_t>(parts_of(items, kWalkWaves * (w ? 32 : 16))); };
-    p.wide_r = wide(n);
-    p.blocks_r = blocks(n, p.wide_r);
+    auto blocks = [](int64_t items, bool wide) {
+      return static_cast<int32_t>(parts_of(items, kWalkWaves * (wide ? 32 : 16)));
+    };
+    p.blocks_r = blocks(n, false);
     p.tiles_r = static_cast<int32_t>(parts_of(v, kWalkItems));
     p.parts_r = walk_parts(p.blocks_r, p.tiles_r);
     if (p.sums && p.grad && !a.stats) p.at_stats = room(n * 16);
@@ -360,7 +362,11 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
       if (a.d_features) p.at_part_out = room(n * p.parts_r * p.ld * 4);
     }
     if (a.d_table) {
-      p.wide_t = wide(v);
+      // 32 classes a wave where that still makes four blocks a unit, and the walk is long enough (16 a wave and 32,
+      // us: 4096 x 128 x 131072 bf16 415 and 352, fp32 838 and 730, 512 x 64 x 262144 fp16 91 and 83, 64 x 128 x
+      // 1000000 bf16 169 and 182). Rows go 16 a wave: 262144 x 128 x 1000 fp16 261 and 280, 1048576 x 64 x 150
+      // bf16 219 and 240.
+      p.wide_t = v >= 4 * kUnits * kWalkWaves * 32 && n >= 512;
       p.blocks_t = blocks(v, p.wide_t);
       p.tiles_t = static_cast<int32_t>(parts_of(n, kWalkItems));
       p.parts_t = walk_parts(p.blocks_t, p.tiles_t);
@@ -417,16 +423,15 @@ template <class T>
 int run_reduce(const GradScale &s, void *out, int64_t ld, const float *slabs, int64_t slab_ld, int32_t parts, int64_t rows,
                int64_t cols, hipStream_t st) {
   ReduceArgs r{s, out, ld, slabs, static_cast<int32_t>(slab_ld), parts, static_cast<int32_t>(rows),
-               static_cast<int32_t>(cols)};
-  const int64_t blocks = std::min<int64_t>(parts_of(rows * slab_ld / 4, 256), 8 * kUnits);
+               static_cast<int32_t>(cols), 1};
+  // (four parts a thread at least, and threads enough for two blocks a unit)
+  while (r.lanes < 16 && r.lanes * 4 < parts && parts_of(rows * slab_ld / 4, 256 / r.lanes) < 2 * kUnits) r.lanes *= 2;
+  const int64_t blocks = std::min<int64_t>(parts_of(rows * slab_ld / 4, 256 / r.lanes), 8 * kUnits);
   hipLaunchKernelGGL((class_reduce_kernel<T>), dim3(static_cast<uint32_t>(std::max<int64_t>(blocks, 1))), dim3(256), 0, st,
                      r);
   TMNN_HIP_TRY(hipGetLastError());
   return TMNN_OK;
 }
-
-typedef std::integral_constant<int, 1> One;
-typedef std::integral_constant<int, 2> Two;
 
 template <int DP, int PL, int PD, int RJ, class Op>
 int run_walk(const WalkArgs &a, int32_t parts, const Op &op, int device, hipStream_t st) {
@@ -470,19 +475,16 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
     T *out = static_cast<T *>(a.d_features);
     const WalkArgs w{ws + p.at_x, ws + p.at_y, x_plane, y_plane, n, v, p.blocks_r,
                      static_cast<int32_t>(parts_of(p.tiles_r, p.parts_r))};
-    auto walk = [&](auto rj, auto op) {
+    auto walk = [&](auto op) {
       static_cast<RowsShared &>(op) = g;
       op.table = table;
       op.table_ld = a.table_stride;
       op.out = out;
       op.out_ld = a.d_feature_stride;
       op.dims = dims;
-      return run_walk<DP, PL, PD, decltype(rj)::value>(w, p.parts_r, op, device, st);
+      return run_walk<DP, PL, PD, 1>(w, p.parts_r, op, device, st);
     };
-    const One one;
-    const Two two;
-    const int rc = p.wide_r ? (out ? walk(two, RowsWalk<T, true, 2>{}) : walk(two, RowsWalk<T, false, 2>{}))
-                            : (out ? walk(one, RowsWalk<T, true, 1>{}) : walk(one, RowsWalk<T, false, 1>{}));
+    const int rc = out ? walk(RowsWalk<T, true>{}) : walk(RowsWalk<T, false>{});
     if (rc != TMNN_OK) return rc;
     if (p.parts_r > 1) {
       hipLaunchKernelGGL((walk_join_kernel<T, DP>), dim3(static_cast<uint32_t>(n)), dim3(256), 0, st, g, n, p.parts_r, table, a.table_stride, out, a.d_feature_stride, dims);
@@ -509,7 +511,7 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
     t.slab_ld = static_cast<int32_t>(p.slab_ld);
     return run_walk<DP, PL, PD, RJ>(w, p.parts_t, t, device, st);
   };
-  const int rc = p.wide_t ? walk(Two{}) : walk(One{});
+  const int rc = p.wide_t ? walk(std::integral_constant<int, 2>{}) : walk(std::integral_constant<int, 1>{});
   if (rc != TMNN_OK || !slabs) return rc;
   return run_reduce<T>(scale, a.d_table, a.d_table_stride, slabs, p.slab_ld, p.parts_t, v, dims, st);
 }

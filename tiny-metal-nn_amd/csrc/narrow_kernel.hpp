@@ -2,7 +2,7 @@
 // d_features in one walk over the table, d_table in one walk over the rows, with
 // neither logits nor d ever in memory.
 //
-// A wave holds 16 or 32 items (rows, or classes for d_table) in registers and walks over the other
+// A wave holds 16 items (rows, or classes for d_table; of many classes 32) in registers and walks over the other
 // side's items in tiles of 64 that the block shares in LDS:
 //   z = x y^T          16 x 16 x 32 products; a lane gets 4 neighbouring items y of one item x
 //   d = f(z)           the softmax's terms or its gradient, in fp16 (two terms for fp32 inputs)
@@ -12,6 +12,9 @@
 // For wide features this would hold dims / 16 accumulators of the second product a 16 x 16 block; up to
 // 128 dims they fit beside the rest. The walk over the table keeps a running maximum, as an online
 // softmax does, and the label's class out of its sums.
+//
+// Products and exponentials take turns on a unit. 4096 x 128 x 131072 bf16, 275 GFLOP a walk: 327 us for loss and
+// d_features (0.84 PFLOP/s), 352 for d_table; 262144 x 64 x 1000 bf16, 67 GFLOP a walk: 125 and 144 us (0.5).
 #pragma once
 
 #include <type_traits>
@@ -327,8 +330,9 @@ __device__ __forceinline__ void put_features(const RowsShared &g, const RowEnd &
   if (dim < dims) store_four<T>(out + r * out_ld + dim, v, dims - dim);
 }
 
-template <class T, bool GRADIENT, int RJ>
+template <class T, bool GRADIENT>
 struct RowsWalk : RowsShared {
+  static constexpr int RJ = 1;  // 16 rows of a wave
   static constexpr bool kGradient = GRADIENT, kInfo = false;
   const T *table;
   int64_t table_ld;

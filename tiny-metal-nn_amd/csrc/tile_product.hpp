@@ -2,15 +2,17 @@
 // matrix cores, one tile of the output a block, with what happens to a finished tile
 // left to an epilogue. 16-bit floating point or e4m3, sums in fp32.
 //
-// The tile's steps of k (64 or 128 bytes of each row) pass through LDS in a ring of stages, loaded
+// The tile's steps of k (128 bytes of each row) pass through LDS in a ring of stages, loaded
 // straight from memory without registers in between. One barrier a step: when it is passed, a
 // stage has arrived and another is free for the next load. An operand whose k is contiguous lies in
 // LDS as rows of a step's bytes; one whose k goes from row to row (a transposed operand) as rows of the
 // tile's width, read with the transposing LDS loads, so that no transposed copy of
 // it is ever made. Both lie swizzled: by the counters no two lanes of a read meet in a bank.
 //
-// Tiles of 256 x 256 go in steps of 64 bytes through five stages of 32 KB, all of a unit's LDS:
-// four of them on their way cover the latency of a loaded memory.
+// What bounds it is the way of the operands from the L2 into LDS, 9 to 12 TB/s over the chip: a tile of 256 x 256
+// takes 64 KB for 8.4 MFLOP of 16-bit products. With two stages of that a unit is full; half steps of 64 bytes
+// in five stages were slower (half a cache line a row, a barrier for half the products). 16-bit products reach 1.2
+// to 1.3 PFLOP/s, 8-bit ones with scales 1.7 to 2.2.
 //
 // Layout of a result: lane l of a 16 x 16 block holds row r = l % 16, columns
 // c = 4 (l / 16) .. + 3: y is the matrix instruction's first operand.
@@ -81,11 +83,11 @@ struct F8 {
   static constexpr int bytes = 1;
 };
 
-// WC x WR waves of FC x FR blocks of 16 x 16; NS stages of KB bytes of k; XT, YT: transposed operands.
-template <class E_, int WC_, int WR_, int FC_, int FR_, int KB_, int NS_, bool XT_, bool YT_>
+// WC x WR waves of FC x FR blocks of 16 x 16; NS stages; XT, YT: transposed operands.
+template <class E_, int WC_, int WR_, int FC_, int FR_, int NS_, bool XT_, bool YT_>
 struct TileShape {
   typedef E_ E;
-  static constexpr int KB = KB_, KN = KB_ / E::bytes;  // of a step: bytes, elements
+  static constexpr int KB = 128, KN = KB / E::bytes;  // of a step: bytes, elements
   static constexpr int WC = WC_, WR = WR_, FC = FC_, FR = FR_, NS = NS_;
   static constexpr bool XT = XT_, YT = YT_;
   static constexpr int kWaves = WC * WR, kThreads = kWaves * 64;
@@ -107,12 +109,9 @@ __device__ __forceinline__ uint32_t lds_address(const char *p) {
       reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char *)p));
 }
 
-// Which 16 bytes of a row lie at a place in LDS: two rows of 128 bytes, or four of 64, fill the 64
-// banks, and the ones beside them have their chunks elsewhere.
-template <int KB>
-__device__ __forceinline__ int swizzle_row(int row) {
-  return KB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
-}
+// Which 16 bytes of a row lie at a place in LDS: two rows of 128 bytes fill the 64 banks, and the ones
+// beside them have their chunks elsewhere.
+__device__ __forceinline__ int swizzle_row(int row) { return (row >> 1) & 7; }
 // The same for a transposed operand, in pairs of chunks: a transposing read takes 32 bytes of
 // rows k .. k + 3 and k + 8 .. k + 11 at a time.
 __device__ __forceinline__ int swizzle_k(int k, int chunks) {
@@ -143,7 +142,7 @@ struct TileLoad {
       at = first * 2 + c < o.bytes ? static_cast<uint32_t>(row * o.ld) + c : kOutside;
       rsrc[2] = 0x7fffffff;
     } else {
-      place = 16 * ((lane % kChunks) ^ swizzle_row<S::KB>(row));
+      place = 16 * ((lane % kChunks) ^ swizzle_row(row));
       at = static_cast<uint32_t>(row * o.ld) + place;
       // (rows past the last one lie past the buffer's end)
       rsrc[2] = static_cast<int32_t>(min(o.rows - first, B) * o.ld);
@@ -227,13 +226,13 @@ __device__ __forceinline__ V read_transposed(const char *tile, int width, int co
   return u.v;
 }
 
-template <int KB, class V>
+template <class V>
 __device__ __forceinline__ V read_row(const char *tile, int row, int chunk, int lane) {
-  return *reinterpret_cast<const V *>(tile + row * KB + ((chunk + lane / 16) ^ swizzle_row<KB>(row)) * 16);
+  return *reinterpret_cast<const V *>(tile + row * 128 + ((chunk + lane / 16) ^ swizzle_row(row)) * 16);
 }
 
-// What a step multiplies: 16-bit operands. In steps of 64 bytes the next step's fragments are on their
-// way from LDS while this one's are multiplied.
+// What a step multiplies: 16-bit operands. The fragments of the next 64 bytes are on their
+// way from LDS while these are multiplied.
 template <class S>
 struct PlainSteps {
   static constexpr bool kAhead = S::FC * S::FR >= 16;  // (small tiles wait for memory)
@@ -254,14 +253,14 @@ struct PlainSteps {
     if constexpr (S::XT)
       f.x[j] = read_transposed<V>(x, S::BR, at, ks, lane);
     else
-      f.x[j] = read_row<S::KB, V>(x, at + lane % 16, ks * 4, lane);
+      f.x[j] = read_row<V>(x, at + lane % 16, ks * 4, lane);
   }
   __device__ __forceinline__ void read_y(Held &f, const char *y, int ks, int i, int wc, int lane) const {
     const int at = (wc * S::FC + i) * 16;
     if constexpr (S::YT)
       f.y[i] = read_transposed<V>(y, S::BC, at, ks, lane);
     else
-      f.y[i] = read_row<S::KB, V>(y, at + lane % 16, ks * 4, lane);
+      f.y[i] = read_row<V>(y, at + lane % 16, ks * 4, lane);
   }
   // Part g of `of` of a fragment set, and of the products.
   __device__ __forceinline__ void read(Held &f, const char *y, int ks, int g, int of, int wc, int wr, int lane) const {
@@ -281,7 +280,7 @@ struct PlainSteps {
   }
   __device__ __forceinline__ void step(f32x4t (&acc)[S::FC][S::FR], const char *y, int, int wc, int wr, int lane) {
 #pragma unroll
-    for (int ks = 0; ks < S::KB / 64; ++ks) {
+    for (int ks = 0; ks < 2; ++ks) {
       Held f;
       read(f, y, ks, 0, 1, wc, wr, lane);
       multiply(acc, f, 0, 1);
@@ -353,7 +352,6 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
     // All stages on their way. Fragments are read 64 bytes of k ahead of their products; when the barrier
     // in a step's last half is passed, all waves hold that half in registers, so its stage is
     // free, and the next step has arrived.
-    constexpr int halves = S::KB / 64;
     typename Steps::Held f[2];
 #pragma unroll
     for (int s = 0; s < S::NS; ++s) load(s, nothing);
@@ -381,16 +379,9 @@ __global__ __launch_bounds__(S::kThreads, S::kWaves == 8 ? 2 : 1) void tile_kern
         __builtin_amdgcn_sched_barrier(0);
       });
     };
-    if constexpr (halves == 2) {
-      for (int k = from; k < to; ++k) {
-        first(f[0], f[1]);
-        last(f[1], f[0]);
-      }
-    } else {
-      for (int k = from; k < to; k += 2) {
-        last(f[0], f[1]);
-        if (k + 1 < to) last(f[1], f[0]);
-      }
+    for (int k = from; k < to; ++k) {
+      first(f[0], f[1]);
+      last(f[1], f[0]);
     }
   } else if constexpr (Steps::kStream) {
     // The classes' fragments go one by one, one ahead; the barrier is before the last one's products, when
