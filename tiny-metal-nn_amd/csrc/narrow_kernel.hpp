@@ -38,9 +38,10 @@ struct WalkArgs {
   int32_t part_tiles;        // tiles of y of one part
 };
 
-// Which 16 bytes of an item lie at a place in LDS: reads of 16 items' same chunk meet no bank twice.
-// (The transposing reads meet one twice, a third of LDS's busy time; an order without that was no faster, 65536 x 64 x
-// 1000 fp32 63 us and 63, and its addresses cost more, 4096 x 128 x 131072 bf16 326 and 375.)
+// Which 16 bytes of an item lie at a place in LDS: reads of 16 items' same chunk meet no bank twice. (The transposing
+// reads meet one twice, a third of LDS's busy time. An order without that, by the counters too, was no faster, 65536 x
+// 64 x 1000 fp32 62 us and 63, and its registers leave room for three waves where four were: 4096 x 128 x 131072
+// bf16 325 and 360.)
 template <int DP>
 __device__ __forceinline__ int walk_swizzle(int item) {
   return DP == 32 ? (item >> 2) & 3 : DP == 64 ? (item >> 1) & 7 : item & 15;
