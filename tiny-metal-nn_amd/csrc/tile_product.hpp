@@ -9,10 +9,12 @@
 // tile's width, read with the transposing LDS loads, so that no transposed copy of
 // it is ever made. Both lie swizzled: by the counters no two lanes of a read meet in a bank.
 //
-// What bounds it is the way of the operands from the L2 into LDS, 9 to 12 TB/s over the chip: a tile of 256 x 256
-// takes 64 KB for 8.4 MFLOP of 16-bit products. With two stages of that a unit is full; half steps of 64 bytes
-// in five stages were slower (half a cache line a row, a barrier for half the products). 16-bit products reach 1.2
-// to 1.3 PFLOP/s, 8-bit ones with scales 1.7 to 2.2.
+// 16-bit products reach 1.2 to 1.3 PFLOP/s, 8-bit ones with scales 1.7 to 1.9. A tile of 256 x 256 takes 64 KB for 8.4
+// MFLOP of 16-bit products, so 9 to 10 TB/s pass from the L2 into LDS over the chip, 1.7 us a step; with the loads
+// left out (and with them the data, which lowers the power too) the loop runs at 1.56 to 1.86 PFLOP/s. It is not their
+// latency: with a ring of five half stages, which gives a load one to two steps to arrive, the times were the same
+// (4096 x 2048 x 131072 bf16, all products 7.37 and 7.46 ms). Half steps of 64 bytes in five stages were slower: half a
+// cache line a row, and a barrier for half the products.
 //
 // Layout of a result: lane l of a 16 x 16 block holds row r = l % 16, columns
 // c = 4 (l / 16) .. + 3: y is the matrix instruction's first operand.
