@@ -795,7 +795,7 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
 
 /* ---- class head ------------------------------------------------------------------ */
 /* Operators over features [rows][dims] and a table [classes][dims], whose class
- * logits are z = features . table: a training loss that never keeps the logits, and the
+ * logits are z = features . table: a training loss that keeps no logits, and the
  * logits themselves from 8-bit operands. They take a tmnn_logits, as the operators above.
  *
  * Rows start at feature_stride, table_stride, ... elements (>= dims) from each other, at

@@ -430,3 +430,20 @@ def test_parts_of_few_sums(ops, n, d, v, dtype):
     again = ops.class_loss(h, w, labels, row_weights=weights)
     for name in NAMES:  # sums are added in one order
         assert torch.equal(got[name], again[name])
+
+
+# more classes than one piece of the logits' gradient holds, the last piece a short one; and as many as are kept
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n, v", [(1100, 130001), (1100, 60000)])
+def test_pieces_of_classes(ops, n, v, dtype):
+    d = 136
+    h, w, labels, weights = inputs(n, d, v, 5)
+    labels[:3] = torch.tensor([v - 1, 0, v // 2])
+    h, w = matrix(h, dtype), matrix(w, dtype)
+    got = ops.class_loss(h, w, labels, row_weights=weights)
+    want = ref.class_loss(h, w, labels, weights)
+    check_all(got, want, h, w, weights, dtype, 1.0)
+    # the backward call computes the logits again
+    plain = ops.class_loss(h, w, labels, gradient="none")
+    again = ops.class_loss_backward(h, w, labels, plain["stats"], weights)
+    check_all({"loss": got["loss"], **again}, want, h, w, weights, dtype, 1.0)

@@ -287,10 +287,11 @@ struct LossPlan {
   int64_t slab_ld;
   bool slabs_x, slabs_y;
   // features of up to 128 dims: parts of the walks
+  bool keep;                         // the logits, between the sums and d
   bool narrow, wide_t;
   int32_t blocks_r, tiles_r, parts_r, blocks_t, tiles_t, parts_t;
   int64_t at_part_sum, at_part_own, at_part_out;
-  int64_t at_exps, at_most, at_x, at_w, at_y, at_sums, at_own, at_stats, at_d, at_slab_x, at_slab_y, bytes;
+  int64_t at_exps, at_most, at_x, at_w, at_y, at_sums, at_own, at_stats, at_z, at_d, at_slab_x, at_slab_y, bytes;
 };
 
 // Rows up to which d of fp16 inputs goes in two terms. (rows x 1000 x 50000, a call with one term and with two, us:
@@ -396,6 +397,11 @@ LossPlan plan_loss(const tmnn_class_loss_args &a, bool back) {
     // channels of the caches: 2048 x 768 x 32768 fp32's d_features 285 -> 264 us, 4096 x 2048 x 131072 bf16's 440 -> 430)
     p.ld_d = p.k_d / 64 % 2 ? p.k_d : p.k_d + 64;
     p.t_d = choose(n, piece, p.k * 2, p.pairs, false, true, true, false);
+    // Logits of a call whose d is one piece are kept between the two, in fp32, rather than computed again (all
+    // kernels of a call, computed again and kept, us: 515 x 1000 x 50021 fp16 418 and 373, 2048 x 768 x 32768 fp32 1433
+    // and 1212, 512 x 4096 x 100000 bf16 2420 and 2070, 100 x 200 x 50 fp32 58 and 53).
+    p.keep = p.sums && piece == v && n * p.k_d * 4 <= 2 * kPieceBytes;
+    if (p.keep) p.at_z = room(n * p.k_d * 4);
     p.at_d = room(n * p.ld_d * 2 * p.planes_d);
     p.slab_ld = up(a.dims, 4);
     if (a.d_features) {
@@ -516,6 +522,19 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
   return run_reduce<T>(scale, a.d_table, a.d_table_stride, slabs, p.slab_ld, p.parts_t, v, dims, st);
 }
 
+int run_terms(const LossPlan &p, const RowInfo &row, float c, const float4 *stats, int64_t n, int64_t v, char *ws, _Float16 *d,
+              int64_t plane, hipStream_t st) {
+  TermsArgs t{row, c, stats, reinterpret_cast<const float *>(ws + p.at_z), static_cast<int32_t>(n), static_cast<int32_t>(v),
+              static_cast<int32_t>(p.k_d / 8), 1, 1, p.k_d, p.ld_d, p.planes_d, plane, d};
+  while (t.lanes < 256 && t.lanes < t.chunks) t.lanes *= 2;
+  const int64_t groups = parts_of(n, 256 / t.lanes);
+  // (two vectors a thread at least, and blocks for eight a unit)
+  t.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(parts_of(8 * kUnits, groups), t.chunks / (2 * t.lanes))));
+  hipLaunchKernelGGL(class_terms_kernel, dim3(static_cast<uint32_t>(groups * t.splits)), dim3(256), 0, st, t);
+  TMNN_HIP_TRY(hipGetLastError());
+  return TMNN_OK;
+}
+
 template <class T>
 int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, bool back, hipStream_t st) {
   const int device = h->ctx->device;
@@ -584,7 +603,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
 
   if (p.sums) {
     SumsEpilogue e{exps, row, c, reinterpret_cast<float2 *>(ws + p.at_sums),
-                   reinterpret_cast<float *>(ws + p.at_own)};
+                   reinterpret_cast<float *>(ws + p.at_own), p.keep ? reinterpret_cast<float *>(ws + p.at_z) : nullptr, p.k_d};
     const TileArgs t = tile_args(x, y, n, v, p.t_sums, p.pairs);
     int rc;
     if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16))
@@ -610,16 +629,20 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
     Operand yp = y;
     yp.base += first * y.ld;
     yp.rows = static_cast<int32_t>(count);
-    GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.k_d), p.ld_d, p.planes_d, d_plane, d};
-    // (columns up to d's padded width, so that those past the piece become 0)
-    TileArgs t = tile_args(x, yp, n, count, of_piece(p.t_d, p.k_d), p.pairs);
-    int rc = run_rows<F16>(t, p.t_d.shape, g, device, st);
+    int rc;
+    if (p.keep) {
+      rc = run_terms(p, row, c, stats, n, v, ws, d, d_plane, st);
+    } else {
+      GradEpilogue g{exps, row, c, stats, static_cast<int32_t>(first), static_cast<int32_t>(p.k_d), p.ld_d, p.planes_d, d_plane, d};
+      // (columns up to d's padded width, so that those past the piece become 0)
+      rc = run_rows<F16>(tile_args(x, yp, n, count, of_piece(p.t_d, p.k_d), p.pairs), p.t_d.shape, g, device, st);
+    }
     if (rc != TMNN_OK) return rc;
     if (a.d_features) {
       GradOut<T> o{by_row, static_cast<T *>(a.d_features), a.d_feature_stride,
                    p.slabs_x ? reinterpret_cast<float *>(ws + p.at_slab_x) : nullptr, static_cast<int32_t>(p.slab_ld),
                    first > 0};
-      t = tile_args(dop, yp, n, a.dims, p.t_x, p.pairs_d);
+      const TileArgs t = tile_args(dop, yp, n, a.dims, p.t_x, p.pairs_d);
       rc = run_grad<false>(t, p.t_x.shape, o, device, st);
       if (rc != TMNN_OK) return rc;
     }
@@ -629,7 +652,7 @@ int run_loss(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p, b
                    static_cast<int32_t>(p.slab_ld), 0};
       Tiles ty = p.t_y;
       ty.r = static_cast<int32_t>(parts_of(count, ty.br));
-      t = tile_args(dop, w, count, a.dims, ty, p.pairs_d);
+      const TileArgs t = tile_args(dop, w, count, a.dims, ty, p.pairs_d);
       rc = run_grad<true>(t, ty.shape, o, device, st);
       if (rc != TMNN_OK) return rc;
       if (p.slabs_y) {

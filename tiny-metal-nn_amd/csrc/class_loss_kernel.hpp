@@ -9,9 +9,9 @@
 // confident row is a difference of two numbers near 1.
 //
 // The logits are a tile product (tile_product.hpp) whose epilogue sums a tile up to (max, sum) per
-// row; a second kernel joins the tiles of a row. The backward pass computes the logits again, for a
-// piece of the classes at a time, writes d of the piece in 16 bits, and multiplies it with the table
-// (d_features) and with the features (d_table).
+// row; a second kernel joins the tiles of a row. The backward pass computes the logits again (or, of a call of
+// both, reads up to 512 MB of them back), for a piece of the classes at a time, writes d of the piece in
+// 16 bits, and multiplies it with the table (d_features) and with the features (d_table).
 //
 // Numbers in 16 bits. Products take fp16 operands wherever a gradient is formed, also of
 // bf16 inputs: a bf16 matrix times the power of two that brings its largest magnitude to 2^14 is
@@ -276,6 +276,8 @@ struct SumsEpilogue {
   float c;
   float2 *sums;           // [rows][tiles_c]
   float *own;             // [rows] the label's logit
+  float *z;               // [rows][z_ld] the logits, nullable
+  int64_t z_ld;
 
   template <class S>
   __device__ __forceinline__ void finish(const TileArgs &a, const TilePlace &p, f32x4t (&acc)[S::FC][S::FR],
@@ -289,16 +291,20 @@ struct SumsEpilogue {
       const int label = r < a.rows ? row.label(r) : -1;
       float m = -3.4e38f, s = 0.f;
 #pragma unroll
-      for (int i = 0; i < S::FC; ++i)
+      for (int i = 0; i < S::FC; ++i) {
+        const int four = c0 + i * 16 + g4;
+        acc[i][j] *= inv;
+        if (z && r < a.rows && four < z_ld) *reinterpret_cast<f32x4t *>(z + r * z_ld + four) = acc[i][j];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int col = c0 + i * 16 + g4 + e;
-          float z = acc[i][j][e] * inv;
-          if (col == label) own[r] = z;
-          z = col == label || col >= a.cols ? -__builtin_inff() : z;
-          acc[i][j][e] = z;
-          m = fmaxf(m, z);
+          const int col = four + e;
+          float v = acc[i][j][e];
+          if (col == label) own[r] = v;
+          v = col == label || col >= a.cols ? -__builtin_inff() : v;
+          acc[i][j][e] = v;
+          m = fmaxf(m, v);
         }
+      }
 #pragma unroll
       for (int i = 0; i < S::FC; ++i)
 #pragma unroll
@@ -381,6 +387,31 @@ __global__ __launch_bounds__(256) void class_join_kernel(JoinArgs a) {
   if (a.stats) a.stats[r] = float4{big, total, missing, 0.f};
 }
 
+// What a row's d is made of.
+struct GradRow {
+  int label;
+  bool used;
+  float big, share, mine;
+  __device__ __forceinline__ GradRow(const RowInfo &row, const float4 *stats, int r, int first) {
+    const float w = row.weight(r);
+    const int l = row.label(r);
+    label = l - first;
+    used = l >= 0 && w != 0.f;
+    const float4 st = stats[r];
+    float f = __builtin_isfinite(w) ? __builtin_amdgcn_frexp_mantf(w) * (2.f * (1 << kDTerm)) : w;
+    if (l == row.classes) f = __builtin_nanf("");
+    big = st.x;
+    share = f / st.y;
+    mine = -f * st.z;
+  }
+  // of the logit z of class `col` of `cols`
+  __device__ __forceinline__ float operator()(float z, int col, int cols, float c) const {
+    float v = __builtin_amdgcn_exp2f((z - big) * c) * share;
+    v = col == label ? mine : v;
+    return used && col < cols ? v : 0.f;
+  }
+};
+
 // The piece's d in fp16 terms, times 2^14, the weight's mantissa and T / w. A quarter of those classes, with 268 MB of
 // d written: 0.52 ms, 1.06 PFLOP/s.
 struct GradEpilogue {
@@ -404,13 +435,7 @@ struct GradEpilogue {
     for (int j = 0; j < S::FR; ++j) {
       const int r = r0 + j * 16 + lane % 16;
       if (r >= a.rows) continue;
-      const float w = row.weight(r);
-      const int label = row.label(r) - first;
-      const bool used = row.label(r) >= 0 && w != 0.f;
-      const float4 st = stats[r];
-      float f = __builtin_isfinite(w) ? __builtin_amdgcn_frexp_mantf(w) * (2.f * (1 << kDTerm)) : w;
-      if (row.label(r) == row.classes) f = __builtin_nanf("");
-      const float share = f / st.y, mine = -f * st.z;
+      const GradRow d_of(row, stats, r, first);
 #pragma unroll
       for (int i = 0; i < S::FC; ++i) {
         const int col = c0 + i * 16 + g4;
@@ -418,9 +443,7 @@ struct GradEpilogue {
         f16x4 high, low;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = __builtin_amdgcn_exp2f((acc[i][j][e] * inv - st.x) * c) * share;
-          v = col + e == label ? mine : v;
-          v = used && col + e < a.cols ? v : 0.f;
+          const float v = d_of(acc[i][j][e] * inv, col + e, a.cols, c);
           high[e] = static_cast<_Float16>(v);
           low[e] = static_cast<_Float16>(v - static_cast<float>(high[e]));
         }
@@ -431,6 +454,44 @@ struct GradEpilogue {
     }
   }
 };
+
+// The same from logits that the sums' pass kept: one pass, 515 x 50021 in 30 us (154 MB, 5.1 TB/s), which adds
+// 20 us to the sums' pass.
+struct TermsArgs {
+  RowInfo row;
+  float c;
+  const float4 *stats;
+  const float *z;      // [rows][ld]
+  int32_t rows, cols;
+  int32_t chunks;      // of 8 columns of a row, those past `cols` give 0
+  int32_t lanes, splits;  // threads that take a row together, a power of two; blocks that do
+  int64_t z_ld, ld;
+  int32_t planes;
+  int64_t plane;
+  _Float16 *d;
+};
+
+__global__ __launch_bounds__(256) void class_terms_kernel(TermsArgs a) {
+  const int r = static_cast<int>(blockIdx.x / a.splits) * (256 / a.lanes) + threadIdx.x / a.lanes;
+  if (r >= a.rows) return;
+  const GradRow d_of(a.row, a.stats, r, 0);
+  const float *z = a.z + r * a.z_ld;
+  _Float16 *d = a.d + r * a.ld;
+  for (int k = blockIdx.x % a.splits * a.lanes + threadIdx.x % a.lanes; k < a.chunks; k += a.splits * a.lanes) {
+    f32x4t in[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) in[h] = *reinterpret_cast<const f32x4t *>(z + k * 8 + 4 * h);
+    f16x8 high, low;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = d_of(in[i / 4][i % 4], k * 8 + i, a.cols, a.c);
+      high[i] = static_cast<_Float16>(v);
+      low[i] = static_cast<_Float16>(v - static_cast<float>(high[i]));
+    }
+    *reinterpret_cast<f16x8 *>(d + k * 8) = high;
+    if (a.planes == 2) *reinterpret_cast<f16x8 *>(d + a.plane + k * 8) = low;
+  }
+}
 
 // ---- the gradients' epilogues ----------------------------------------------------------------
 

@@ -114,8 +114,8 @@ class _HeadCalls:
 
         `out`: arrays to write to, by these names; it gets those that it lacks, and is
         returned. None may overlap the inputs. `workspace`: a uint8 tensor to work in; the call
-        takes memory of its stream otherwise (about as much as the inputs, 256 MB and, beyond 128
-        dims, rows * classes / 32 bytes)."""
+        takes memory of its stream otherwise (about as much as the inputs and, beyond 128 dims, up
+        to 256 MB for pieces of the logits' gradient, 512 MB for logits if they fit there, and rows * classes / 32 bytes)."""
         a = self._arrays(features, stream)
         if out is None:
             out = {}
