@@ -447,3 +447,39 @@ def test_pieces_of_classes(ops, n, v, dtype):
     plain = ops.class_loss(h, w, labels, gradient="none")
     again = ops.class_loss_backward(h, w, labels, plain["stats"], weights)
     check_all({"loss": got["loss"], **again}, want, h, w, weights, dtype, 1.0)
+
+
+@pytest.mark.parametrize("d", DIMS)
+def test_calls_of_several_threads(ops, d):
+    import threading
+
+    cases, got = [], [None] * 4
+    for i in range(4):
+        h, w, labels, weights = inputs(70 + 30 * i, d, 200 + 100 * i, i)
+        cases.append((matrix(h, "bf16"), matrix(w, "bf16"), labels, weights))
+    want = [ops.class_loss(h, w, labels, row_weights=weights) for h, w, labels, weights in cases]
+    torch.cuda.synchronize()
+
+    def work(i):
+        h, w, labels, weights = cases[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = ops.class_loss(h, w, labels, row_weights=weights)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        for name in NAMES:
+            assert torch.equal(a[name], b[name])
+
+
+@pytest.mark.parametrize("d", DIMS)
+def test_one_matrix_as_features_and_table(ops, d):
+    h, _, labels, weights = inputs(90, d, 90, 3)
+    h = matrix(h, "f32")
+    got = ops.class_loss(h, h, labels, row_weights=weights)
+    check_all(got, ref.class_loss(h, h, labels, weights), h, h, weights, "f32", 1.0)
