@@ -483,3 +483,22 @@ def test_one_matrix_as_features_and_table(ops, d):
     h = matrix(h, "f32")
     got = ops.class_loss(h, h, labels, row_weights=weights)
     check_all(got, ref.class_loss(h, h, labels, weights), h, h, weights, "f32", 1.0)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", DIMS)
+def test_large_values_in_rows_that_do_not_count(ops, d, dtype):
+    """What such rows hold does not cost the others their bits."""
+    n, v = 150, 70
+    h, w, labels, weights = inputs(n, d, v, 3)
+    labels[10], labels[149], weights[20] = -5, -1, 0.0
+    clean, w = matrix(h, dtype), matrix(w, dtype)
+    want = ref.class_loss(clean, w, labels, weights)
+    dirty = clean.clone()
+    for row in (10, 20, 149):
+        dirty[row] = 6e4 if dtype == "f16" else 1e38
+    got = ops.class_loss(dirty, w, labels, row_weights=weights)
+    check_all(got, want, clean, w, weights, dtype, 1.0)
+    plain = ops.class_loss(clean, w, labels, gradient="none")
+    back = ops.class_loss_backward(dirty, w, labels, plain["stats"], weights)
+    check_all({"loss": got["loss"], **back}, want, clean, w, weights, dtype, 1.0)

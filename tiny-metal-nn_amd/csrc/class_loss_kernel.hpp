@@ -50,6 +50,16 @@ struct RowInfo {  // of the rows of a call
     return l < 0 ? -1 : l < classes ? l : classes;
   }
   __device__ __forceinline__ float weight(int64_t r) const { return weights ? weights[r] : 1.f; }
+  // Whether a row counts, in two loads without a branch: a label's sign, and the weight or something in its place.
+  struct Counts {
+    int32_t sign;
+    float weight;
+  };
+  __device__ __forceinline__ Counts counts(int64_t r) const {
+    const float *w = weights ? weights : static_cast<const float *>(labels);
+    return {static_cast<const int32_t *>(labels)[wide ? 2 * r + 1 : r], w[r]};
+  }
+  __device__ __forceinline__ bool used(const Counts &v) const { return v.sign >= 0 && (!weights || v.weight != 0.f); }
 };
 
 // w = m 2^e with |m| in [1, 2); what is not finite keeps e = 0.
@@ -105,7 +115,8 @@ __device__ __forceinline__ uint32_t magnitude(T v) {  // its bits, 0 for what is
   return b < 0x7f800000u ? b : 0;
 }
 
-// The largest finite magnitude of each operand, one per block, and of the weights. One pass over both: 554 MB of
+// The largest finite magnitude of each operand, one per block, and of the weights. Rows that do not count may hold
+// anything and take no part. One pass over both: 554 MB of
 // 4096 x 2048 and 131072 x 2048 bf16 in 117 us, 4.7 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void class_scale_kernel(LayArgs a) {
@@ -119,34 +130,46 @@ __global__ __launch_bounds__(256) void class_scale_kernel(LayArgs a) {
     typedef T V __attribute__((ext_vector_type(8), aligned(sizeof(T))));
     const int chunks = (p.dims + 7) / 8, lanes = row_lanes(chunks), per = 256 / lanes;
     const int64_t step = static_cast<int64_t>(p.parts) * per;
+    auto used = [&](const RowInfo::Counts &v) { return which == 1 || a.row.used(v); };
+    // (of the table's rows, which all count, some row's)
+    auto counts = [&](int64_t r) { return a.row.counts(which == 1 ? 0 : r); };
     for (int c = threadIdx.x % lanes; c < chunks; c += lanes) {
       const T *at = static_cast<const T *>(p.in) + c * 8;
       int64_t r = static_cast<int64_t>(block) * per + threadIdx.x / lanes;
       if (c * 8 + 8 <= p.dims) {
         for (; r + 3 * step < p.rows; r += 4 * step) {  // four loads on their way
           V v[4];
+          RowInfo::Counts in[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const V *>(at + (r + u * step) * p.stride);
+          for (int u = 0; u < 4; ++u) {
+            v[u] = *reinterpret_cast<const V *>(at + (r + u * step) * p.stride);
+            in[u] = counts(r + u * step);
+          }
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+          for (int u = 0; u < 4; ++u) {
+            uint32_t top = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[u][i]));
+            for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[u][i]));
+            most = max(most, used(in[u]) ? top : 0);
+          }
         }
         for (; r < p.rows; r += step) {
           const V v = *reinterpret_cast<const V *>(at + r * p.stride);
+          const RowInfo::Counts in = counts(r);
+          uint32_t top = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[i]));
+          for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+          most = max(most, used(in) ? top : 0);
         }
       } else {
         for (; r < p.rows; r += step)
-          for (int i = 0; i < p.dims - c * 8; ++i) most = max(most, magnitude(at[r * p.stride + i]));
+          for (int i = 0; i < p.dims - c * 8 && used(counts(r)); ++i) most = max(most, magnitude(at[r * p.stride + i]));
       }
     }
   } else {
     // (exponents shifted by 1000, 0 being none)
     for (int64_t r = static_cast<int64_t>(block) * 256 + threadIdx.x; r < a.part[0].rows; r += 256ll * a.parts_w) {
-      const float w = a.row.weight(r);
-      if (a.row.label(r) >= 0 && w != 0.f) most = max(most, static_cast<uint32_t>(weight_exponent(w) + 1000));
+      if (a.row.used(a.row.counts(r))) most = max(most, static_cast<uint32_t>(weight_exponent(a.row.weight(r)) + 1000));
     }
   }
 #pragma unroll
