@@ -502,3 +502,15 @@ def test_large_values_in_rows_that_do_not_count(ops, d, dtype):
     plain = ops.class_loss(clean, w, labels, gradient="none")
     back = ops.class_loss_backward(dirty, w, labels, plain["stats"], weights)
     check_all({"loss": got["loss"], **back}, want, clean, w, weights, dtype, 1.0)
+
+
+# a walk over the table in a few parts and in many
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n, d, v", [(20001, 32, 700), (9000, 100, 3001), (4097, 50, 5000), (70, 64, 5000)])
+def test_parts_of_rows(ops, n, d, v, dtype):
+    h, w, labels, weights = inputs(n, d, v, 5)
+    h, w = matrix(h, dtype), matrix(w, dtype)
+    want = ref.class_loss(h, w, labels, weights)
+    for gradient in ("both", "features", "none"):
+        got = ops.class_loss(h, w, labels, row_weights=weights, gradient=gradient)
+        check_all(got, want, h, w, weights, dtype, 1.0, names=[name for name in NAMES[1:] if name in got])

@@ -304,7 +304,9 @@ constexpr int64_t kFewRows = 128;
 constexpr int64_t kNarrow = 128;
 
 // Parts of a walk's tiles, where the items of one side alone make too few blocks: four blocks a unit, and
-// four tiles a part at least.
+// four tiles a part at least. (Kernels of a call with both gradients, us. With two, four and eight blocks a unit: 512 x
+// 64 x 262144 fp16 191, 188 and 188. With two, four and eight tiles: 4096 x 16 x 64 fp32 27, 31 and 36, 64 x 128 x
+// 131072 bf16 84, 77 and 70, 1000 x 100 x 5000 fp32 79, 75 and 86.)
 int32_t walk_parts(int64_t blocks, int64_t tiles) {
   int64_t parts = std::max<int64_t>(1, std::min<int64_t>(4 * kUnits / blocks, tiles / 4));
   return static_cast<int32_t>(parts_of(tiles, parts_of(tiles, parts)));
@@ -493,7 +495,13 @@ int run_narrow(tmnn_logits *h, const tmnn_class_loss_args &a, const LossPlan &p,
     const int rc = out ? walk(RowsWalk<T, true>{}) : walk(RowsWalk<T, false>{});
     if (rc != TMNN_OK) return rc;
     if (p.parts_r > 1) {
-      hipLaunchKernelGGL((walk_join_kernel<T, DP>), dim3(static_cast<uint32_t>(n)), dim3(256), 0, st, g, n, p.parts_r, table, a.table_stride, out, a.d_feature_stride, dims);
+      const dim3 groups(static_cast<uint32_t>(parts_of(n, 256 / (DP / 4))));
+      if (p.parts_r <= kFewParts)
+        hipLaunchKernelGGL((walk_join_few_kernel<T, DP>), groups, dim3(256), 0, st, g, n, p.parts_r, table,
+                           a.table_stride, out, a.d_feature_stride, dims);
+      else
+        hipLaunchKernelGGL((walk_join_kernel<T, DP>), dim3(static_cast<uint32_t>(n)), dim3(256), 0, st, g, n, p.parts_r,
+                           table, a.table_stride, out, a.d_feature_stride, dims);
       TMNN_HIP_TRY(hipGetLastError());
     }
   }
