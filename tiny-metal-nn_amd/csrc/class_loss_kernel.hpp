@@ -135,36 +135,37 @@ __global__ __launch_bounds__(256) void class_scale_kernel(LayArgs a) {
     auto counts = [&](int64_t r) { return a.row.counts(which == 1 ? 0 : r); };
     for (int c = threadIdx.x % lanes; c < chunks; c += lanes) {
       const T *at = static_cast<const T *>(p.in) + c * 8;
-      int64_t r = static_cast<int64_t>(block) * per + threadIdx.x / lanes;
-      if (c * 8 + 8 <= p.dims) {
+      auto scan = [&](auto load) {
+        auto top_of = [&](const V &v, const RowInfo::Counts &in) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+          most = max(most, used(in) ? top : 0);
+        };
+        int64_t r = static_cast<int64_t>(block) * per + threadIdx.x / lanes;
         for (; r + 3 * step < p.rows; r += 4 * step) {  // four loads on their way
           V v[4];
           RowInfo::Counts in[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            v[u] = *reinterpret_cast<const V *>(at + (r + u * step) * p.stride);
+            v[u] = load(at + (r + u * step) * p.stride);
             in[u] = counts(r + u * step);
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[u][i]));
-            most = max(most, used(in[u]) ? top : 0);
-          }
+          for (int u = 0; u < 4; ++u) top_of(v[u], in[u]);
         }
-        for (; r < p.rows; r += step) {
-          const V v = *reinterpret_cast<const V *>(at + r * p.stride);
-          const RowInfo::Counts in = counts(r);
-          uint32_t top = 0;
+        for (; r < p.rows; r += step) top_of(load(at + r * p.stride), counts(r));
+      };
+      const int last = p.dims - 1 - c * 8;
+      if (last >= 7)
+        scan([](const T *x) { return *reinterpret_cast<const V *>(x); });
+      else  // (a row's end: its last value in place of those past it, without a branch)
+        scan([=](const T *x) {
+          V v;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
-          most = max(most, used(in) ? top : 0);
-        }
-      } else {
-        for (; r < p.rows; r += step)
-          for (int i = 0; i < p.dims - c * 8 && used(counts(r)); ++i) most = max(most, magnitude(at[r * p.stride + i]));
-      }
+          for (int i = 0; i < 8; ++i) v[i] = x[min(i, last)];
+          return v;
+        });
     }
   } else {
     // (exponents shifted by 1000, 0 being none)
