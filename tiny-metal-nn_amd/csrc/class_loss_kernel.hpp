@@ -23,11 +23,11 @@
 // exponent goes to the other factor or to the result, exactly, so rows of any weight keep their bits.
 #pragma once
 
+#include "head_plan.hpp"
 #include "tile_product.hpp"
 
 namespace tmnn_hip {
 
-constexpr int kScaleParts = 1024;  // most blocks that look for one operand's largest magnitude
 constexpr int kDTerm = 14;         // d is held times 2^14
 
 // Powers of two that the operands of the logits and the weighted features were multiplied with, and
@@ -35,6 +35,7 @@ constexpr int kDTerm = 14;         // d is held times 2^14
 struct Exponents {
   int32_t x, y, w, weighted;
 };
+static_assert(sizeof(Exponents) == kExponentBytes, "its place in the workspace");
 
 struct RowInfo {  // of the rows of a call
   const void *labels;

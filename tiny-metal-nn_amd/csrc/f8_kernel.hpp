@@ -18,11 +18,11 @@
 // scales, whose fma take the vector unit about as long as the instructions take the matrix unit.
 #pragma once
 
+#include "head_plan.hpp"
 #include "tile_product.hpp"
 
 namespace tmnn_hip {
 
-constexpr int kScaleBlock = 128;
 constexpr float kF8Largest = 448.f;
 
 struct F8Scales {

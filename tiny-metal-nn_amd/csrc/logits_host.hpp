@@ -10,6 +10,7 @@
 #include <new>
 #include <vector>
 
+#include "arg_types.hpp"
 #include "context.hpp"
 #include "tmnn_hip.h"
 
@@ -26,10 +27,6 @@ struct tmnn_logits {
 };
 
 namespace tmnn_hip {
-
-inline size_t dtype_size(int32_t dtype) { return dtype == TMNN_DTYPE_F32 ? 4 : 2; }
-
-inline bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 inline hipStream_t stream_of(tmnn_logits *h, void *stream) {
   return stream == TMNN_STREAM_CONTEXT ? h->ctx->stream : static_cast<hipStream_t>(stream);

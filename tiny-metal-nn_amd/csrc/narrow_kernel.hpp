@@ -23,8 +23,7 @@
 
 namespace tmnn_hip {
 
-constexpr int kWalkItems = 64;   // items of a tile in LDS
-constexpr int kWalkWaves = 4, kWalkThreads = kWalkWaves * 64;
+constexpr int kWalkThreads = kWalkWaves * 64;
 constexpr int kWalkStages = 2;
 
 constexpr float kLowest = -3.4e38f;  // a maximum of nothing

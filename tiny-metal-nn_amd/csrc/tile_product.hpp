@@ -23,6 +23,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "tile_args.hpp"
+
 namespace tmnn_hip {
 
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -33,25 +35,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4t __attribute__((ext_vector_type(4)));
 typedef int32_t i32x4t __attribute__((ext_vector_type(4)));
 typedef int32_t i32x8t __attribute__((ext_vector_type(8)));
-
-// One operand. Rows of it are the output's rows (x) or columns (y), or, of a transposed
-// one, the values of k. Everything of it that a tile reads starts at multiples of 16 bytes.
-struct Operand {
-  const char *base;
-  int64_t ld;      // bytes from row to row: below 2^23
-  int64_t plane;   // bytes from plane to plane (operands in two terms)
-  int32_t rows;    // rows that exist
-  int32_t bytes;   // bytes of a row that exist, a multiple of 16; what lies beyond counts as 0
-};
-
-struct TileArgs {
-  Operand x, y;
-  int32_t rows, cols;          // of the output
-  int32_t tiles_r, tiles_c, parts;
-  int32_t steps;               // of k, in one pair of planes
-  int32_t pairs;               // 1: one plane each; 2: and x low; 3: x high, y low first, x low then
-  int32_t part_steps;          // steps of one part, counted over all pairs
-};
 
 // A block's tile and part. Blocks go to the chip's eight dies in turn, each with an L2 of
 // its own: every die takes a contiguous eighth, in columns of four tiles.
@@ -120,8 +103,6 @@ __device__ __forceinline__ int swizzle_k(int k, int chunks) {
   return 2 * (((k & 3) | ((k >> 1) & 4)) & (chunks / 2 - 1));
 }
 
-constexpr uint32_t kOutside = 0x80000000u;  // an offset past the end of every buffer: loads give 0
-
 // One thread's loads of one operand's part of a stage: B rows (columns) of the tile. What changes from
 // step to step is in scalar registers: the base and how much of k is left.
 template <class S, int B, bool T, int Q>
@@ -147,7 +128,7 @@ struct TileLoad {
       place = 16 * ((lane % kChunks) ^ swizzle_row(row));
       at = static_cast<uint32_t>(row * o.ld) + place;
       // (rows past the last one lie past the buffer's end)
-      rsrc[2] = static_cast<int32_t>(min(o.rows - first, B) * o.ld);
+      rsrc[2] = tile_bytes(o, first, B);
     }
     each = static_cast<uint32_t>(kEach * o.ld);
     advance = T ? S::KN * o.ld : S::KB;
