@@ -1,5 +1,6 @@
 // Reads the class head's plans (csrc/head_plan.hpp) on the CPU: every tile that a call launches begins inside its
-// operands, no buffer that a tile loads from has a size that a load meant to give zeros falls into, laid-out operands lie
+// operands, no buffer that a tile loads from has a size that a load meant to give zeros falls into, rows that exist
+// are loaded from where they are and others from past the buffer's end, laid-out operands lie
 // in the workspace, and a launch's threads fit 32 bits. Prints the first plans that break this; returns how
 // many there are (up to 100).
 #include <math.h>
@@ -22,15 +23,34 @@ void fail(const char *what, const char *product, long long tile, long long value
   if (++bad <= 10) printf("%s: %s, %s from %lld on: %lld\n", now, what, product, tile, value);
 }
 
+// The rows that the tile from row `first` on loads, `each` rows from one load of a thread to its next.
+void rows_of(const char *product, const Operand &o, bool transposed, int64_t first, int64_t edge, int64_t waves) {
+  const int64_t each = waves * (transposed ? 64 / (edge / 8) : 8), rows = transposed ? 64 : edge;
+  const int64_t exist = transposed ? std::min<int64_t>(o.rows, 64) : std::min<int64_t>(o.rows - first, edge);
+  const uint32_t size = transposed ? 0x7fffffffu : static_cast<uint32_t>(tile_bytes(o, static_cast<int32_t>(first), static_cast<int32_t>(edge)));
+  for (const int64_t r : {int64_t{0}, each - 1, each, exist - 1, exist, (exist / each + 1) * each, 128 - each % 128, rows - 1}) {
+    if (r < 0 || r >= rows) continue;
+    const uint64_t whole = static_cast<uint64_t>(row_offset(o, static_cast<int32_t>(r % each))) +
+                           static_cast<uint64_t>(r / each) * load_step(o, static_cast<int32_t>(each));
+    if (r < exist && (whole != static_cast<uint64_t>(r * o.ld) || whole + 16 > size)) fail("an offset", product, first + r, static_cast<long long>(whole));
+    // (a transposed operand's rows that do not exist are left out by their number)
+    if (r >= exist && !transposed && whole < size) fail("a row that does not exist lies inside", product, first + r, static_cast<long long>(whole));
+    if (!transposed && whole + 128 >= 1ull << 32) fail("an offset past 32 bits", product, first + r, static_cast<long long>(whole));
+    if (transposed && r < exist && kOutside + static_cast<uint64_t>(r / each) * load_step(o, static_cast<int32_t>(each)) >= 1ull << 32)
+      fail("an offset past 32 bits", product, first + r, o.ld);
+  }
+}
+
 // One side of a product: tiles of `edge` rows, `count` of them, over `rows` of the output.
 void side(const char *product, const Operand &o, bool transposed, int64_t count, int64_t edge, int64_t rows, const char *ws,
-          int64_t ws_bytes, int planes) {
+          int64_t ws_bytes, int planes, int64_t waves) {
   if (count * edge < rows) fail("rows that no tile takes", product, count * edge, rows);
   if (count > 0 && (count - 1) * edge >= rows) fail("a tile past the output", product, (count - 1) * edge, rows);
   if (o.rows < 0 || o.bytes < 0 || o.bytes % 16) fail("rows or bytes", product, 0, o.bytes);
   for (int64_t t = 0; t < count; ++t) {
     const int64_t first = t * edge;
     ++tiles;
+    if (t == 0 || t == count - 1) rows_of(product, o, transposed, first, edge, waves);
     if (transposed) {
       if (first * 2 >= o.bytes) fail("a tile past the operand", product, first, o.bytes);
       continue;
@@ -51,9 +71,10 @@ void side(const char *product, const Operand &o, bool transposed, int64_t count,
 void product(const char *name, const TileArgs &t, const Tiles &s, bool xt, bool yt, const char *ws, int64_t ws_bytes,
              int x_planes, int y_planes) {
   if (t.tiles_r != s.r || t.tiles_c != s.c) fail("tiles", name, t.tiles_r, s.r);
-  side(name, t.x, xt, t.tiles_r, s.br, t.rows, ws, ws_bytes, x_planes);
-  side(name, t.y, yt, t.tiles_c, s.bc, t.cols, ws, ws_bytes, y_planes);
-  const long long threads = 1ll * t.tiles_r * t.tiles_c * t.parts * (s.shape <= kWide ? 512 : 256);
+  const int64_t waves = s.shape <= kWide ? 8 : 4;
+  side(name, t.x, xt, t.tiles_r, s.br, t.rows, ws, ws_bytes, x_planes, waves);
+  side(name, t.y, yt, t.tiles_c, s.bc, t.cols, ws, ws_bytes, y_planes, waves);
+  const long long threads = 64ll * waves * t.tiles_r * t.tiles_c * t.parts;
   if (threads >= 1ll << 32) fail("threads of a launch", name, 0, threads);
   if (t.parts < 1 || (t.parts - 1ll) * t.part_steps >= 1ll * t.steps * t.pairs ||
       1ll * t.parts * t.part_steps < 1ll * t.steps * t.pairs)
@@ -131,6 +152,10 @@ int main(int argc, char **argv) {
         for (int64_t d : dims)
           for (int back = 0; back < 2; ++back)
             for (int gradient = back; gradient < 4; ++gradient) loss(dtype, n, v, d, d % 8 ? 3 : 0, gradient, back);
+  for (int32_t dtype = 0; dtype < 3; ++dtype)  // few rows of very many classes: rows of d far apart
+    for (int64_t n : {1, 2, 3, 7, 15, 16, 31, 33, 64})
+      for (int64_t v : {1ll << 20, (1ll << 22) - 64, 1ll << 22, (1ll << 22) + 1, 5000001ll, 1ll << 23, (1ll << 24) - 1, 1ll << 24})
+        for (int gradient = 0; gradient < 4; ++gradient) loss(dtype, n, v, 136, 0, gradient, false);
   std::mt19937_64 g(1);
   auto between = [&](double low, double high) {  // over the logarithm
     return static_cast<int64_t>(exp2(std::uniform_real_distribution<double>(log2(low), log2(high))(g)));

@@ -16,7 +16,8 @@ namespace tmnn_hip {
 // one, the values of k. Everything of it that a tile reads starts at multiples of 16 bytes.
 struct Operand {
   const char *base;
-  int64_t ld;      // bytes from row to row: below 2^23
+  int64_t ld;      // bytes from row to row: below 2^23, or, of d of few rows, up to 2^25 and 256; the rows of a
+                   // tile, those that do not exist too, lie within 32 bits (d's tiles of up to 128 rows are 128 high)
   int64_t plane;   // bytes from plane to plane (operands in two terms)
   int32_t rows;    // rows that exist
   int32_t bytes;   // bytes of a row that exist, a multiple of 16; what lies beyond counts as 0
@@ -39,5 +40,10 @@ TMNN_BOTH int32_t tile_bytes(const Operand &o, int32_t first, int32_t tile) {
   const int32_t left = o.rows - first;
   return left <= 0 ? 0 : static_cast<int32_t>((left < tile ? left : tile) * o.ld);
 }
+
+// Byte offset of a tile's row, and from one load of a thread to its next, `rows` rows on. (32 bits: a row that does
+// not exist lies past the buffer's end, never back inside it.)
+TMNN_BOTH uint32_t row_offset(const Operand &o, int32_t row) { return static_cast<uint32_t>(row * o.ld); }
+TMNN_BOTH uint32_t load_step(const Operand &o, int32_t rows) { return static_cast<uint32_t>(rows * o.ld); }
 
 }  // namespace tmnn_hip

@@ -122,15 +122,15 @@ struct TileLoad {
     if constexpr (T) {
       const int c = 16 * ((lane % kChunks) ^ swizzle_k(row, kChunks));
       place = row;
-      at = first * 2 + c < o.bytes ? static_cast<uint32_t>(row * o.ld) + c : kOutside;
+      at = first * 2 + c < o.bytes ? row_offset(o, row) + c : kOutside;
       rsrc[2] = 0x7fffffff;
     } else {
       place = 16 * ((lane % kChunks) ^ swizzle_row(row));
-      at = static_cast<uint32_t>(row * o.ld) + place;
+      at = row_offset(o, row) + place;
       // (rows past the last one lie past the buffer's end)
       rsrc[2] = tile_bytes(o, first, B);
     }
-    each = static_cast<uint32_t>(kEach * o.ld);
+    each = load_step(o, kEach);
     advance = T ? S::KN * o.ld : S::KB;
     rsrc[3] = 0x00020000;
   }
