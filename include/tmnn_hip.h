@@ -816,7 +816,8 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
  *   d_features, d_table  the gradients of sum_row loss[row], null where not wanted
  * A negative label marks a row without one: loss and gradients 0. So do rows of weight 0,
  * whatever they hold (the stats of both sorts hold where their features are no larger than the other
- * rows'). A label >= classes makes its loss and gradients NaN, as logits that are not finite do. The backward call takes the stats of a call with the same features, table,
+ * rows'). A label >= classes makes its row's loss and gradients NaN. So do logits that are NaN or +infinity and a label's
+ * of -infinity; another class's of -infinity has no probability. The backward call takes the stats of a call with the same features, table,
  * labels and temperature, and the loss's gradient as row_weights; it writes the gradients. All
  * sums in fp32; gradients are rounded once at the end. Products of gradients take the inputs as they are
  * (16 bits; bf16 below 2^-32 of a tensor's largest loses bits) or with 22 bits (fp32, of values from 2^-16 of a

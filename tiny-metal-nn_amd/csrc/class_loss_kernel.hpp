@@ -370,6 +370,12 @@ struct JoinArgs {
   float4 *stats;               // (m, S, R / S, 0)
 };
 
+// The label's logit in a row's end: NaN without such a class, and where it is not finite, so that all that comes
+// of it is NaN too. (An infinite one would end as a loss of 0 or infinity beside sums that look sound.)
+__device__ __forceinline__ float own_logit(float z, int label, int classes) {
+  return label < classes && __builtin_isfinite(z) ? z : __builtin_nanf("");
+}
+
 __global__ __launch_bounds__(256) void class_join_kernel(JoinArgs a) {
   const int lane = threadIdx.x % a.lanes;
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / a.lanes) + threadIdx.x / a.lanes;
@@ -399,7 +405,7 @@ __global__ __launch_bounds__(256) void class_join_kernel(JoinArgs a) {
   if (!here || lane != 0) return;
   float loss = 0.f, big = m, total = s, missing = 1.f;
   if (label >= 0) {
-    const float z = label < a.row.classes ? a.own[r] : __builtin_nanf("");
+    const float z = own_logit(a.own[r], label, a.row.classes);
     big = fmaxf(m, z);
     s *= __builtin_amdgcn_exp2f((m - big) * a.c);
     total = s + __builtin_amdgcn_exp2f((z - big) * a.c);

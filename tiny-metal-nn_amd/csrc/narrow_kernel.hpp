@@ -290,7 +290,7 @@ __device__ __forceinline__ RowEnd end_row(float m, float s, float z, int label, 
                                           float inv_t) {
   RowEnd e{0.f, m, s, 1.f, 0.f};
   if (label >= 0) {
-    if (label >= classes) z = __builtin_nanf("");
+    z = own_logit(z, label, classes);
     e.big = fmaxf(m, z);
     e.scale = __builtin_amdgcn_exp2f((m - e.big) * c);
     s *= e.scale;
