@@ -283,7 +283,8 @@ __device__ __forceinline__ float f8_scale(float most) {
 }
 
 // x / s rounded to the nearest e4m3 (ties to even) of the exact quotient: the fp32 quotient is
-// made odd where it is not exact, so that it never lies on a border that the exact one is beside.
+// made odd where it is not exact, so that it never lies on a border that the exact one is beside. (s: 2^-64 or more, so
+// that what a division leaves over is an ordinary number.)
 template <bool POWER>
 __device__ __forceinline__ float f8_quotient(float x, float s, float inv) {
   if constexpr (POWER) return x * inv;  // (inv is exact)
@@ -325,8 +326,16 @@ template <bool POWER>
 __device__ __forceinline__ void f8_store8(uint8_t *row, int c, int dims, const float (&v)[8], float s, float inv) {
   float y[8];
 #pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = v[i];
+  if (!POWER && s < 0x1p-64f) {  // blocks of tiny values are divided 2^64 larger, exactly
+    s *= 0x1p64f;
+    inv *= 0x1p-64f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] *= 0x1p64f;
+  }
+#pragma unroll
   for (int i = 0; i < 8; ++i)
-    y[i] = fabsf(v[i]) < __builtin_inff() ? f8_quotient<POWER>(v[i], s, inv) : __builtin_nanf("");
+    y[i] = fabsf(y[i]) < __builtin_inff() ? f8_quotient<POWER>(y[i], s, inv) : __builtin_nanf("");
   int32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
