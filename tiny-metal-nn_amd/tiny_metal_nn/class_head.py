@@ -59,6 +59,8 @@ class _HeadCalls:
         """A call whose args are `head` and a workspace: on the device one of the caller's, or memory
         that belongs to the call's stream."""
         if a.device is None:
+            if workspace is not None:
+                raise ValueError("workspace goes with torch tensors")
             self._run(a, on_host, on_device, head + _NO_WORKSPACE, stream)
             return
         if workspace is None:
