@@ -1,6 +1,6 @@
 """A field whose 16 outputs are features, compared with a table of labels: it learns
-the labels of a scene and the table together with LogitOps.class_loss (whose logits are
-never kept as a tensor), then answers from features and a table in 8 bits with
+the labels of a scene and the table together with LogitOps.class_loss (which needs no
+tensor of logits), then answers from features and a table in 8 bits with
 LogitOps.class_logits_f8 and LogitOps.token_logprobs.
 
 The scene labels the unit cube by 500 sites, each point by its nearest. Run:

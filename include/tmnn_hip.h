@@ -94,7 +94,7 @@ typedef struct tmnn_model_desc {
   /* network */
   int32_t hidden_dim;         /* 1..64; 128 (fp16 training, 16x2 inputs) */
   int32_t num_hidden_layers;  /* 1..8 */
-  int32_t num_outputs;        /* 1..16 in this build */
+  int32_t num_outputs;        /* 1 or more (above 16 by the layer-wise kernels) */
   /* loss */
   int32_t loss_kind;          /* TMNN_LOSS_* */
   float huber_delta;
@@ -795,7 +795,7 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
 
 /* ---- class head ------------------------------------------------------------------ */
 /* Operators over features [rows][dims] and a table [classes][dims], whose class
- * logits are z = features . table: a training loss that keeps no logits, and the
+ * logits are z = features . table: a training loss that needs no tensor of logits, and the
  * logits themselves from 8-bit operands. They take a tmnn_logits, as the operators above.
  *
  * Rows start at feature_stride, table_stride, ... elements (>= dims) from each other, at
@@ -817,16 +817,21 @@ int tmnn_distill_backward_device(tmnn_logits *h, const tmnn_distill_args *args, 
  * A negative label marks a row without one: loss and gradients 0. So do rows of weight 0,
  * whatever they hold (the stats of both sorts hold where their features are no larger than the other
  * rows'). A label >= classes makes its row's loss and gradients NaN. So do logits that are NaN or +infinity and a label's
- * of -infinity; another class's of -infinity has no probability. The backward call takes the stats of a call with the same features, table,
+ * of -infinity; another class's of -infinity has no probability (of 16-bit inputs: what an infinity among fp32 inputs
+ * enters is NaN). The workspace of a call of loss and gradients may hold logits, up to 512 MB of them. The backward call takes the stats of a call with the same features, table,
  * labels and temperature, and the loss's gradient as row_weights; it writes the gradients. All
  * sums in fp32; gradients are rounded once at the end. Products of gradients take the inputs as they are
  * (16 bits; bf16 below 2^-32 of a tensor's largest loses bits) or with 22 bits (fp32, of values from 2^-16 of a
- * tensor's largest on), and d loss / d z with 11 bits (bf16, and fp16 of many rows) or 22. */
+ * tensor's largest on), and d loss / d z of a class of probability p with 11 bits (bf16, and fp16 of more than 128 rows
+ * and 128 dims) or 22, but never more than 39 + log2 p: classes below 2^-28, or 2^-17, have fewer, and below 2^-39
+ * none, their part in the gradients being 0. (The label's counts by 1 - p. With up to 128 dims d_features counts p relative to the row's
+ * best other class.) In d_table rows are held relative to the largest row weight: those far below it lose as
+ * many bits of one of the two factors, d (up to 128 dims) or the features. */
 typedef struct tmnn_class_loss_args {
   uint32_t struct_size;       /* sizeof(tmnn_class_loss_args) */
   int32_t dtype;              /* TMNN_DTYPE_* of features, table and their gradients */
   int32_t index_dtype;        /* TMNN_INDEX_* of labels */
-  float temperature;          /* > 0 */
+  float temperature;          /* 1e-6..1e6 */
   int64_t rows;               /* 0..TMNN_HEAD_MAX_ROWS */
   int64_t classes;            /* 1..TMNN_LOGITS_MAX_CLASSES */
   int64_t dims;               /* 1..TMNN_HEAD_MAX_DIMS */
@@ -861,7 +866,8 @@ int tmnn_class_loss_backward_device(tmnn_logits *h, const tmnn_class_loss_args *
  * w = table[class][k] table_scales[class / 128][k / 128]; values are e4m3 (OCP; no
  * infinities), sums fp32, rounded once to the logits' type. On the way to 16-bit logits the matrix
  * instructions may cut each product to 2^-13 of the largest of the eight that they add. A NaN among values or scales makes
- * the logits that it enters NaN. */
+ * the logits that it enters NaN. The product of a feature's and a table's scale is taken in fp32: it should be finite, and loses
+ * bits below 2^-126. Rows read in place are read in whole 16 bytes; what lies behind their end has no part in the result. */
 typedef struct tmnn_class_logits_f8_args {
   uint32_t struct_size;       /* sizeof(tmnn_class_logits_f8_args) */
   int32_t dtype;              /* TMNN_DTYPE_* of logits */

@@ -1,5 +1,5 @@
 // class_loss_kernel.hpp -- softmax cross entropy of features against a table of
-// classes, without keeping the logits, and its gradients.
+// classes, without a tensor of logits of the caller's, and its gradients.
 //
 // Of a row h with label l, logits z_v = h . W_v, c = log2(e) / T, m = max z:
 //   R = sum_{v != l} 2^(c (z_v - m)),  e = 2^(c (z_l - m)),  S = R + e
@@ -20,7 +20,10 @@
 // fp16 terms, 22 bits, and three products, at a third of the rate of fp16, three times that of the fp32 matrix
 // instructions (154 TFLOP/s in a large product). fp16 inputs of few rows, or of few dims, have d in two terms:
 // there its 11 bits would show beside those of the results. d is held as 2^14 m d T / w, m in [1, 2) being w's mantissa: its
-// exponent goes to the other factor or to the result, exactly, so rows of any weight keep their bits.
+// exponent goes to the result (d_features: exactly, rows of any weight keep their bits) or to the features (d_table: rows of
+// weights far below the largest lose bits of theirs, as small features do).
+// A fixed point of 2^14 means that d ends at 2^-39: a class of probability p has at most 39 + log2 p bits, in one term
+// 11 of them from 2^-28 on, in two 22 from 2^-17 on.
 #pragma once
 
 #include "head_plan.hpp"

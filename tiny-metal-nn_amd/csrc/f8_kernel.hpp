@@ -13,9 +13,11 @@
 //     the instruction; fp32 ones multiply its result, four fma an instruction.
 //   fp32 logits, and calls of few rows, which wait for memory anyway: values widened to fp16 (exact) and four
 //     16 x 16 x 32 instructions, whose products are exact and whose sums are fp32.
-// One row is bound by reading the table: 131072 x 4096 in 111 us, 4.8 TB/s. 4096 x 4096 x 65536 to bf16, 2.2 TFLOP, is
-// bound by the way into LDS and by the scales: 1.14 ms (1.93 PFLOP/s) with powers of two, 1.28 (1.72) with fp32
-// scales, whose fma take the vector unit about as long as the instructions take the matrix unit.
+// One row is bound by reading the table: 131072 x 4096 in 111 us, 4.8 TB/s. 4096 x 4096 x 65536 to bf16, 2.2 TFLOP, takes
+// 1.14 ms (1.93 PFLOP/s) with powers of two, 1.28 (1.72) with fp32 scales, which cost four fma an instruction. By the
+// counters neither unit is full then (matrix 0.37, vector 0.35 of the time), and 8.6 GB pass into LDS at 6.7 to
+// 7.5 TB/s, where 16-bit products reach 9 to 10: waves wait. A step's loads go out in a row here, not between products as the
+// 16-bit loop's do; whether that is the wait is not measured.
 #pragma once
 
 #include "head_plan.hpp"

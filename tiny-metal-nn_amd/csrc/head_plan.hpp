@@ -33,7 +33,7 @@ struct Tiles {
 constexpr int kUnits = 256;  // compute units
 
 // What a tile's step of 128 bytes of k takes, in us, with one block on a unit and with two, and what a tile
-// takes besides. All shapes are bound by the way from the L2 into LDS, 9 to 12 TB/s over the chip, so
+// takes besides. All shapes of 16 bits are bound by the way from the L2 into LDS, 9 to 12 TB/s over the chip, so
 // the larger the tile the less a product takes, and the smaller the less is left over at the edges. Measured
 // (us): 515 x 1000 x 50021 fp16, logits and sums, Large 84 (588 tiles, 3 rounds), Wide 98 (980, 4), Middle 102
 // (1955, 4), Flat 116 (3519, 7), Small 176 (6647, 13); 64 x 1024 x 32768 Wide 20, Middle 22, Flat 15, Small 15;

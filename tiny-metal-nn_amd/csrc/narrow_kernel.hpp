@@ -13,8 +13,12 @@
 // 128 dims they fit beside the rest. The walk over the table keeps a running maximum, as an online
 // softmax does, and the label's class out of its sums.
 //
-// Products and exponentials take turns on a unit. 4096 x 128 x 131072 bf16, 275 GFLOP a walk: 327 us for loss and
-// d_features (0.84 PFLOP/s), 352 for d_table; 262144 x 64 x 1000 bf16, 67 GFLOP a walk: 125 and 144 us (0.5).
+// The walk over the table holds a class's part relative to the row's best other class, the walk over the rows p itself
+// times 2^14 and the row's weight over the largest one's power of two: there a class has at most 39 + log2 p bits, and
+// rows of smaller weights as many fewer.
+//
+// Products and exponentials take turns on a unit. 4096 x 128 x 131072 bf16, 275 GFLOP a walk: 328 to 336 us for loss and
+// d_features (0.83 PFLOP/s), 352 for d_table; 262144 x 64 x 1000 bf16, 67 GFLOP a walk: 123 and 144 us (0.5).
 #pragma once
 
 #include <type_traits>

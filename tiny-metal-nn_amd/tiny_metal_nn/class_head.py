@@ -1,6 +1,6 @@
 """The class head's calls of LogitOps (include/tmnn_hip.h, class head): operators over
 features [rows, dims] and a table of classes [classes, dims], whose class logits are their
-products: cross entropy without the logits and its gradients, logits from 8-bit
+products: cross entropy without a tensor of logits and its gradients, logits from 8-bit
 operands, and the quantisation that makes these. No counterpart in the reference.
 
 Arrays are looked at as in logits.py: numpy arrays or torch tensors, all of one sort, unit
@@ -108,16 +108,20 @@ class _HeadCalls:
 
     def class_loss(self, features, table, labels, *, temperature: float = 1.0, row_weights=None,
                    gradient: str = "both", out: dict | None = None, workspace=None, stream=None) -> dict:
-        """Softmax cross entropy of the logits features . table / temperature without keeping
-        them: `loss` [rows] = -row_weights ln p(label) and, by `gradient` ("both", "features",
+        """Softmax cross entropy of the logits features . table / temperature without a tensor
+        of them: `loss` [rows] = -row_weights ln p(label) and, by `gradient` ("both", "features",
         "table", "none"), `d_features` and `d_table`, the gradients of its sum. A negative label
         marks a row without one; such rows and those of weight 0 give 0, whatever they hold. A
-        label >= classes gives NaN. `stats` [rows, 4] is what class_loss_backward takes.
+        label >= classes gives NaN, as do logits that are NaN or +inf and a label's of -inf.
+        Classes of probability p have at most 39 + log2 p bits in the gradients (tmnn_hip.h).
+        `stats` [rows, 4] is what class_loss_backward takes. temperature: 1e-6 to 1e6.
 
         `out`: arrays to write to, by these names; it gets those that it lacks, and is
-        returned. None may overlap the inputs. `workspace`: a uint8 tensor to work in; the call
-        takes memory of its stream otherwise (about as much as the inputs and, beyond 128 dims, up
-        to 256 MB for pieces of the logits' gradient, 512 MB for logits if they fit there, and rows * classes / 32 bytes)."""
+        returned. None may overlap the inputs. `workspace`: a uint8 tensor to work in (with torch
+        tensors); the call takes memory of its stream otherwise: about as much as the inputs, up to 256 MB
+        of sums in parts for each gradient, and beyond 128 dims 256 MB for a piece of the logits' gradient (or what 256
+        classes of all rows take, if that is more), 512 MB for logits if they fit there, and rows * classes / 32
+        bytes (/ 16 for few rows)."""
         a = self._arrays(features, stream)
         if out is None:
             out = {}
